@@ -154,6 +154,62 @@ typedef struct nvq_attention_prompt_desc {
     int32_t causal;
 } nvq_attention_prompt_desc;
 
+/* Rotary positions of heads, with or without a norm over each head: up to two operands (queries and keys) of
+ * [batch, heads, length, head_dim] in one launch, any strides but consecutive values of a head.
+ *   table f32 [table_rows, rotary_dims / 2, 2]: (cosine, sine) of every position (nvq_rotation_table);
+ *   the position of element l of batch b is `offset + l` with offsets NULL, offsets[b] + l, or (per_position) offsets[b * length + l]. */
+typedef struct nvq_head_rope_desc {
+    int32_t dtype;       /* NVQ_F16 / NVQ_BF16 / NVQ_F32: x, weights, y */
+    int32_t head_dim;    /* 1 .. 512 */
+    int32_t rotary_dims; /* even, 0 .. head_dim: the values that turn, the first ones (0: none, no table) */
+    int32_t interleaved; /* 1: pairs (2 i, 2 i + 1); 0: (i, i + rotary_dims / 2) */
+    int32_t per_position;
+    int64_t table_rows, batch, length, offset;
+    int64_t heads[2];        /* of each operand; 0: absent */
+    int64_t x_strides[2][3]; /* elements between batches, heads, positions */
+    int64_t y_strides[2][3];
+    double eps;              /* of the norm of operands with a weight */
+} nvq_head_rope_desc;
+
+/* A paged, affine-quantized key / value cache: a pool of pages [pages, key_heads, page_size, ...] for each of
+ *   k_w, v_w u32 [.., head_dim*bits/32];  k_s, k_b, v_s, v_b dtype [.., head_dim/group_size], all contiguous,
+ * and page_table i32 [sequences, columns] (rows table_stride apart): position p of a sequence lies in page
+ * page_table[sequence][p / page_size], at place p % page_size. */
+typedef struct nvq_paged_desc {
+    int32_t dtype;      /* NVQ_F16 / NVQ_BF16 / NVQ_F32: scales, biases and the values beside them */
+    int32_t bits;       /* 4 or 8 */
+    int32_t group_size; /* 32, 64 or 128, dividing head_dim */
+    int32_t head_dim;   /* 64 or 128 */
+    int64_t pages, page_size; /* page_size: a power of two, 16 .. 1024 */
+    int64_t key_heads;
+    int64_t sequences, columns, table_stride;
+} nvq_paged_desc;
+
+/* New rows of a paged cache: token t is position positions[t] of sequence sequences[t] (NULL: t).
+ *   k, v dtype [tokens, key_heads, head_dim], q dtype [tokens, query_heads, head_dim] or NULL, strides as given, values of a head
+ *   consecutive; q_out contiguous. */
+typedef struct nvq_paged_append_desc {
+    nvq_paged_desc cache;
+    int64_t tokens, query_heads;
+    int32_t rotary_dims, interleaved; /* of keys and queries, as nvq_head_rope_desc */
+    int64_t table_rows;
+    int64_t q_strides[2], k_strides[2], v_strides[2]; /* elements between tokens, heads */
+    double eps;
+} nvq_paged_append_desc;
+
+/* Attention over a paged cache: rows q dtype [rows, query_heads, head_dim].  Sequence b has rows query_starts[b] ..
+ * query_starts[b + 1] - 1 (NULL: row b alone), the last of its lengths[b] positions: row i of n sees keys up to
+ * lengths[b] - n + i, with `window` > 0 the last `window` of those alone. */
+typedef struct nvq_paged_attention_desc {
+    nvq_paged_desc cache;
+    int64_t rows, query_heads;
+    int64_t max_queries;                /* rows of a sequence that the launch is sized for; more are right, but slower */
+    int64_t q_strides[2], out_strides[2]; /* elements between rows, heads */
+    int64_t window;
+    int32_t causal;                     /* 0: every row of a sequence sees all its positions (window must be 0) */
+    float scale;
+} nvq_paged_attention_desc;
+
 /* ── runtime ─────────────────────────────────────────────────────────────────────── */
 
 /* Binds the library to HIP device `device` (idempotent; the process-wide device record,
@@ -310,6 +366,38 @@ NVQ_API size_t nvq_quantized_attention_prompt_f32_workspace_bytes(const nvq_atte
 NVQ_API int32_t nvq_quantized_attention_prompt_f32(const nvq_attention_prompt_desc *desc, const void *q, const void *k_w, const void *k_s,
                                 const void *k_b, const void *v_w, const void *v_s, const void *v_b, const void *sinks,
                                 void *out, void *workspace, void *stream);
+
+/* Angles of positions 0 .. rows - 1: table f32 [rows, dims / 2, 2] = magnitude * (cos, sin)(scale * position / f_i), with f_i = freqs[i]
+ * (f32 [dims / 2]) or, with freqs NULL, base^(2 i / dims); the angles in 64 bits. */
+NVQ_API int32_t nvq_rotation_table(const float *freqs, int32_t dims, int64_t rows, double base, double scale, double magnitude, float *table,
+                           void *stream);
+
+/* y = rotate(norm(x)): float32 throughout, rounded once.  x1 NULL: one operand; a weight ([head_dim] dtype) NULL: that operand is not
+ * normed; table NULL (rotary_dims 0): not rotated.  y may be x itself.  Positions outside the table are clamped to it. */
+NVQ_API int32_t nvq_head_norm_rope(const nvq_head_rope_desc *desc, const float *table, const int32_t *offsets, const void *x0, const void *weight0,
+                           void *y0, const void *x1, const void *weight1, void *y1, void *stream);
+
+/* New keys (normed where k_weight, rotated where rotary_dims) and values quantized into the cache, and q_out = rotate(norm(q)) beside
+ * them.  Codes are made from float32 results, each the nearest to the scale and bias as they are stored.  A token whose position is
+ * negative (padding) or outside the table, the cache or the sequences writes no row of the cache; its queries are computed all the same.
+ * Two tokens of one position: either's codes and scales may stay. */
+NVQ_API int32_t nvq_append_paged(const nvq_paged_append_desc *desc, const int32_t *page_table, const int32_t *sequences, const int32_t *positions,
+                         const float *table, const void *q, const void *q_weight, void *q_out, const void *k, const void *k_weight, const void *v,
+                         uint32_t *k_w, void *k_s, void *k_b, uint32_t *v_w, void *v_s, void *v_b, void *stream);
+
+/* Rows of the cache as values, code * scale + bias rounded once: keys, values dtype [tokens, key_heads, head_dim], contiguous; zeros for
+ * a token that lies outside the cache. */
+NVQ_API int32_t nvq_read_paged(const nvq_paged_desc *desc, int64_t tokens, const int32_t *page_table, const int32_t *sequences,
+                       const int32_t *positions, const uint32_t *k_w, const void *k_s, const void *k_b, const uint32_t *v_w, const void *v_s,
+                       const void *v_b, void *keys, void *values, void *stream);
+
+/* softmax(scale * q . K^T [, sinks]) . V of every row over its sequence's pages; a row that sees no key is zeros.  Rows outside every
+ * sequence are left as they were.  lengths beyond the table's columns count as those; pages outside the pool are the caller's error (another page
+ * is read).  `workspace`: the size query's bytes (float32 states of the splits of the positions), NULL where it says 0. */
+NVQ_API size_t nvq_paged_attention_workspace_bytes(const nvq_paged_attention_desc *desc);
+NVQ_API int32_t nvq_paged_attention(const nvq_paged_attention_desc *desc, const void *q, const uint32_t *k_w, const void *k_s, const void *k_b,
+                            const uint32_t *v_w, const void *v_s, const void *v_b, const int32_t *page_table, const int32_t *lengths,
+                            const int32_t *query_starts, const void *sinks, void *out, void *workspace, void *stream);
 
 /* GpuEval::sorted_offsets (gpu.rs:6732-6756); kernels::sorted_offsets (kernels.rs:873-892):
  * per row of `indices` u32[rows, m], offsets[row, g] = first position whose value is >= g. */

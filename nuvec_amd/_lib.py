@@ -60,6 +60,27 @@ class AttentionDescC(C.Structure):
                 ("scale", C.c_float)]
 
 
+class HeadRopeDescC(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("head_dim", C.c_int32), ("rotary_dims", C.c_int32), ("interleaved", C.c_int32), ("per_position", C.c_int32),
+                ("table_rows", C.c_int64), ("batch", C.c_int64), ("length", C.c_int64), ("offset", C.c_int64), ("heads", C.c_int64 * 2),
+                ("x_strides", C.c_int64 * 3 * 2), ("y_strides", C.c_int64 * 3 * 2), ("eps", C.c_double)]
+
+
+class PagedDescC(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("bits", C.c_int32), ("group_size", C.c_int32), ("head_dim", C.c_int32), ("pages", C.c_int64),
+                ("page_size", C.c_int64), ("key_heads", C.c_int64), ("sequences", C.c_int64), ("columns", C.c_int64), ("table_stride", C.c_int64)]
+
+
+class PagedAppendDescC(C.Structure):
+    _fields_ = [("cache", PagedDescC), ("tokens", C.c_int64), ("query_heads", C.c_int64), ("rotary_dims", C.c_int32), ("interleaved", C.c_int32),
+                ("table_rows", C.c_int64), ("q_strides", C.c_int64 * 2), ("k_strides", C.c_int64 * 2), ("v_strides", C.c_int64 * 2), ("eps", C.c_double)]
+
+
+class PagedAttentionDescC(C.Structure):
+    _fields_ = [("cache", PagedDescC), ("rows", C.c_int64), ("query_heads", C.c_int64), ("max_queries", C.c_int64), ("q_strides", C.c_int64 * 2),
+                ("out_strides", C.c_int64 * 2), ("window", C.c_int64), ("causal", C.c_int32), ("scale", C.c_float)]
+
+
 class AttentionPromptDescC(C.Structure):
     _fields_ = [("cache", AttentionDescC), ("queries", C.c_int64), ("causal", C.c_int32)]
 
@@ -109,6 +130,12 @@ SIGNATURES = {
     "nvq_quantized_attention_prompt": (C.c_int32, [C.POINTER(AttentionPromptDescC)] + [C.c_void_p] * 11),
     "nvq_quantized_attention_prompt_f32_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionPromptDescC)]),
     "nvq_quantized_attention_prompt_f32": (C.c_int32, [C.POINTER(AttentionPromptDescC)] + [C.c_void_p] * 11),
+    "nvq_rotation_table": (C.c_int32, [C.c_void_p, C.c_int32, C.c_int64, C.c_double, C.c_double, C.c_double, C.c_void_p, C.c_void_p]),
+    "nvq_head_norm_rope": (C.c_int32, [C.POINTER(HeadRopeDescC)] + [C.c_void_p] * 9),
+    "nvq_append_paged": (C.c_int32, [C.POINTER(PagedAppendDescC)] + [C.c_void_p] * 17),
+    "nvq_read_paged": (C.c_int32, [C.POINTER(PagedDescC), C.c_int64] + [C.c_void_p] * 12),
+    "nvq_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedAttentionDescC)]),
+    "nvq_paged_attention": (C.c_int32, [C.POINTER(PagedAttentionDescC)] + [C.c_void_p] * 14),
     "nvq_sorted_offsets": (C.c_int32, [C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p]),
     "nvq_quantize_scaled": (C.c_int32, [C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "nvq_dequantize_scaled": (C.c_int32, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]),

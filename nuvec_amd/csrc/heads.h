@@ -1,0 +1,173 @@
+// Eight consecutive values of a head a lane: loads and stores, the norm over a head, the rotation of its positions, the affine
+// codes of its groups.  P lanes (a power of two, 8 .. 64) hold a head of at most 8 P values.
+#pragma once
+
+#include "nvq_device.h"
+
+namespace nvq {
+namespace {
+
+constexpr int kHeadBlock = 256;
+
+template <typename T>
+__device__ __forceinline__ void load_run(const T *p, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+        const uint4 w = *reinterpret_cast<const uint4 *>(p);
+        T t[8];
+        __builtin_memcpy(t, &w, 16);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = Elem<T>::load(t, i);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_run(T *p, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        uint4 w;
+        if constexpr (Elem<T>::code == NVQ_BF16) {
+            w = make_uint4(f32_to_bf16_pair(v[0], v[1]), f32_to_bf16_pair(v[2], v[3]), f32_to_bf16_pair(v[4], v[5]), f32_to_bf16_pair(v[6], v[7]));
+        } else {
+            T t[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) Elem<T>::store(t, i, v[i]);
+            __builtin_memcpy(&w, t, 16);
+        }
+        *reinterpret_cast<uint4 *>(p) = w;
+    }
+}
+
+// Values across the lanes of a head.  Within 16 lanes by data-parallel moves: pairs, quads, then mirrors, which meet another quad or
+// half each time, so that after a step all lanes that have met hold the same bits (addition and the extremes commute).
+template <int CTRL> __device__ __forceinline__ float moved(float v) {
+    return u2f((uint32_t)__builtin_amdgcn_mov_dpp((int)f2u(v), CTRL, 0xF, 0xF, true));
+}
+template <int CTRL> __device__ __forceinline__ double moved(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, CTRL, 0xF, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)lo | (uint64_t)hi << 32);
+}
+constexpr int kPairs = 0xB1, kQuads = 0x4E, kHalfRow = 0x141, kRow = 0x140;
+template <int LANES, typename V, typename F>
+__device__ __forceinline__ V across(V v, F f) {
+    v = f(v, moved<kPairs>(v));
+    v = f(v, moved<kQuads>(v));
+    if constexpr (LANES >= 8) v = f(v, moved<kHalfRow>(v));
+    if constexpr (LANES >= 16) v = f(v, moved<kRow>(v));
+    if constexpr (LANES >= 32) v = f(v, __shfl_xor(v, 16));
+    if constexpr (LANES >= 64) v = f(v, __shfl_xor(v, 32));
+    return v;
+}
+
+// 1 / sqrt(mean of squares + eps) of the head whose values lie in P lanes, 0 where a lane has none.  The sum is 64 bits wide and so
+// the factor is the correctly rounded one for any order of the sum: a cache's codes turn over on its last bit.
+template <int P>
+__device__ __forceinline__ float norm_factor(const float (&v)[8], int dim, double eps) {
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) sum = __builtin_fma((double)v[i], (double)v[i], sum);
+    sum = across<P>(sum, [](double a, double b) { return a + b; });
+    const double x = sum / (double)dim + eps;
+    double y = __builtin_amdgcn_rsq(x);  // (half its digits; each step doubles them)
+#pragma unroll
+    for (int i = 0; i < 2; i++) y = y * __builtin_fma(-0.5 * x * y, y, 1.5);
+    return (float)y;
+}
+
+// Which values of a head the rotation turns and with which others, for the lane's run of eight.
+struct Turn {
+    float c[8], n[8];  // cosine, and sine with the sign of the partner's share; 1 and 0 where nothing turns
+};
+// WIDE: whole runs of eight turn or stay, and their partners are one run (half layout) or in the same run (interleaved).
+template <bool WIDE>
+__device__ __forceinline__ Turn read_turn(const float2 *__restrict__ angles, int j0, int half, bool interleaved) {
+    Turn t;
+    if (WIDE) {
+        const bool turns = j0 < 2 * half, second = !interleaved && j0 >= half;
+        if (turns) {
+            if (interleaved) {
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    const float4 a = *reinterpret_cast<const float4 *>(angles + (j0 >> 1) + i);
+                    t.c[2 * i] = t.c[2 * i + 1] = a.x, t.n[2 * i] = -a.y, t.n[2 * i + 1] = a.y;
+                    t.c[2 * i + 2] = t.c[2 * i + 3] = a.z, t.n[2 * i + 2] = -a.w, t.n[2 * i + 3] = a.w;
+                }
+            } else {
+                const float2 *from = angles + (second ? j0 - half : j0);
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const float4 a = *reinterpret_cast<const float4 *>(from + i);
+                    t.c[i] = a.x, t.n[i] = second ? a.y : -a.y;
+                    t.c[i + 1] = a.z, t.n[i + 1] = second ? a.w : -a.w;
+                }
+            }
+            return t;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) t.c[i] = 1.0f, t.n[i] = 0.0f;
+        return t;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int j = j0 + i;
+        t.c[i] = 1.0f, t.n[i] = 0.0f;
+        if (j < 2 * half) {
+            const float2 a = angles[interleaved ? j >> 1 : j < half ? j : j - half];
+            const bool second = interleaved ? (j & 1) != 0 : j >= half;
+            t.c[i] = a.x, t.n[i] = second ? a.y : -a.y;
+        }
+    }
+    return t;
+}
+
+// The lane's values of a head and those that the rotation mixes into them.
+template <typename T, bool WIDE>
+struct HeadRun {
+    float v[8], p[8];
+    __device__ __forceinline__ void load(const T *row, int j0, int dim, int half, bool interleaved) {
+        if (WIDE) {
+            if (j0 < dim) {
+                load_run(row + j0, v);
+                if (!interleaved && j0 < 2 * half) load_run(row + (j0 < half ? j0 + half : j0 - half), p);
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int j = j0 + i;
+            v[i] = j < dim ? Elem<T>::load(row, j) : 0.0f;
+            p[i] = j < 2 * half ? Elem<T>::load(row, interleaved ? j ^ 1 : j < half ? j + half : j - half) : 0.0f;
+        }
+    }
+    // times the factor and the weight: two roundings in float32, those of the partners likewise
+    __device__ __forceinline__ void scale(float r, const T *__restrict__ weight, int j0, int dim, int half, bool interleaved) {
+        HeadRun<T, WIDE> w;
+        w.load(weight, j0, dim, half, interleaved);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = v[i] * r * w.v[i], p[i] = p[i] * r * w.p[i];
+    }
+    __device__ __forceinline__ void turn(const Turn &t, int j0, int half, bool interleaved) {
+        if (j0 >= 2 * half) return;  // (nothing of this run; not times 1 plus times 0, which an infinite partner would spoil)
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float other = WIDE && interleaved ? v[i ^ 1] : p[i];
+            const float turned = v[i] * t.c[i] + other * t.n[i];
+            y[i] = WIDE || j0 + i < 2 * half ? turned : v[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = y[i];
+    }
+};
+
+// Whether a head's runs of eight can be read as such (the pointers' and strides' alignment aside).
+inline bool whole_runs(int dim, int half, bool interleaved) { return dim % 8 == 0 && (interleaved ? half % 4 == 0 : half % 8 == 0); }
+
+}  // namespace
+}  // namespace nvq

@@ -111,6 +111,21 @@ int32_t check_quant(const nvq_quant *q, const char *op) {
     return NVQ_OK;
 }
 
+int32_t check_float(const char *op, int32_t dtype) {
+    if (!float_dtype(dtype)) return fail(NVQ_INVALID_ARGUMENT, "%s: unsupported dtype %s", op, dtype_name(dtype));
+    return NVQ_OK;
+}
+
+// The kernels use 16-byte vector accesses on x, the packed weights, y and the workspace; allocations from
+// hipMalloc (and any sub-buffer at a multiple of 16 bytes) satisfy this.  Scales and biases are read at element
+// granularity (the kernels that fetch them in wider pieces start at the enclosing aligned piece), so they need
+// only the alignment of their element type.
+int32_t check_aligned(const char *op, const char *what, const void *p, size_t to) {
+    if (p != nullptr && !aligned(p, to))
+        return fail(NVQ_UNSUPPORTED, "%s: %s is not %zu-byte aligned", op, what, to);
+    return NVQ_OK;
+}
+
 namespace {
 
 // check_groups (quantized.rs:363-379) as far as pointers can tell: affine needs biases, the
@@ -123,32 +138,12 @@ int32_t check_groups(const char *op, int32_t mode, const void *biases) {
     return NVQ_OK;
 }
 
-int32_t check_float(const char *op, int32_t dtype) {
-    if (!float_dtype(dtype)) return fail(NVQ_INVALID_ARGUMENT, "%s: unsupported dtype %s", op, dtype_name(dtype));
-    return NVQ_OK;
-}
-
-// The kernels use 16-byte vector accesses on x, the packed weights, y and the workspace; allocations from
-// hipMalloc (and any sub-buffer at a multiple of 16 bytes) satisfy this.  Scales and biases are read at element
-// granularity (the kernels that fetch them in wider pieces start at the enclosing aligned piece), so they need
-// only the alignment of their element type.
-int32_t check_aligned(const char *op, const char *what, const void *p, size_t to = 16) {
-    if (p != nullptr && !aligned(p, to))
-        return fail(NVQ_UNSUPPORTED, "%s: %s is not %zu-byte aligned", op, what, to);
-    return NVQ_OK;
-}
-
 int32_t check_groups_aligned(const char *op, const nvq_quant &q, int32_t dtype, const void *scales, const void *biases) {
     const size_t to = q.mode == NVQ_AFFINE ? (size_t)dtype_size(dtype) : 1;
     int32_t rc = check_aligned(op, "scales", scales, to);
     return rc != NVQ_OK ? rc : check_aligned(op, "biases", biases, to);
 }
 
-#define NVQ_TRY(expr)                     \
-    do {                                  \
-        int32_t nvq_rc_ = (expr);         \
-        if (nvq_rc_ != NVQ_OK) return nvq_rc_; \
-    } while (0)
 
 // The product's argument checks (primitive.rs:1279-1320 after quantized_columns,
 // primitive.rs:1412-1460): K must be whole groups and whole packed words.

@@ -31,6 +31,13 @@ int32_t fail(int32_t status, const char *fmt, ...) __attribute__((format(printf,
             return ::nvq::fail(NVQ_BACKEND, "%s launch: %s", what, hipGetErrorString(nvq_e_));   \
     } while (0)
 
+// For the entry points: the first status that is not NVQ_OK is the call's.
+#define NVQ_TRY(expr)                     \
+    do {                                  \
+        int32_t nvq_rc_ = (expr);         \
+        if (nvq_rc_ != NVQ_OK) return nvq_rc_; \
+    } while (0)
+
 int32_t require_device();          // NVQ_OK once nvq_init succeeded
 int32_t compute_units();           // of the bound device
 int32_t check_quant(const nvq_quant *q, const char *op);
@@ -38,6 +45,8 @@ inline bool float_dtype(int32_t d) { return d == NVQ_F16 || d == NVQ_BF16 || d =
 inline int dtype_size(int32_t d) { return d == NVQ_F32 ? 4 : (d == NVQ_U8 ? 1 : (d == NVQ_U32 || d == NVQ_I32 ? 4 : 2)); }
 const char *dtype_name(int32_t d);
 const char *mode_name(int32_t m);
+int32_t check_float(const char *op, int32_t dtype);
+int32_t check_aligned(const char *op, const char *what, const void *p, size_t to = 16);
 
 // ── kernel launchers (each validates nothing: the entry points did) ─────────────────────
 int32_t launch_affine_quantize(int32_t dtype, int group, int bits, const void *w, int64_t n_values,
@@ -196,6 +205,25 @@ size_t attention_prompt_f32_workspace_bytes(const nvq_attention_prompt_desc &d);
 int32_t launch_attention_prompt_f32(const nvq_attention_prompt_desc &d, const void *q, const void *kw, const void *ks, const void *kb,
                                     const void *vw, const void *vs, const void *vb, const void *sinks, void *out, void *workspace,
                                     hipStream_t s);
+// Heads and the paged cache.
+struct PagedAppendOperands {
+    const int32_t *page_table, *sequences, *positions;
+    const float *table;
+    const void *q, *q_weight, *k, *k_weight, *v;
+    void *q_out, *kw, *ks, *kb, *vw, *vs, *vb;
+};
+struct PagedAttentionOperands {
+    const void *q, *kw, *ks, *kb, *vw, *vs, *vb, *sinks;
+    const int32_t *page_table, *lengths, *starts;
+    void *out, *workspace;
+};
+int32_t launch_rotation_table(const float *freqs, int half, int64_t rows, double base, double scale, double magnitude, float *table, hipStream_t s);
+int32_t launch_head_rope(const nvq_head_rope_desc &d, const float *table, const int32_t *offsets, const void *const (&x)[2],
+                         const void *const (&w)[2], void *const (&y)[2], hipStream_t s);
+int32_t launch_append_paged(const nvq_paged_append_desc &d, const PagedAppendOperands &o, hipStream_t s);
+int32_t launch_read_paged(const nvq_paged_desc &c, int64_t tokens, const PagedAppendOperands &o, void *keys, void *values, hipStream_t s);
+size_t paged_attention_workspace_bytes(const nvq_paged_attention_desc &d);
+int32_t launch_paged_attention(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, hipStream_t s);
 int32_t launch_calibrate(int32_t kind, const void *buffer, int64_t bytes, int32_t iters, void *sink, int64_t *work, hipStream_t s);
 // Products with the weights stored [K, N] (transpose = false); K is split over the grid through a float32 workspace.
 int qvm_splits(const ProductArgs &a);

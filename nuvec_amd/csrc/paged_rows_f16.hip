@@ -1,0 +1,12 @@
+// Attention of few lines over a paged cache, float16.
+#include "paged_rows_kernel.h"
+
+namespace nvq {
+namespace paged {
+
+int32_t launch_rows_f16(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const RowsLaunch &r, hipStream_t s) {
+    return launch_rows<f16_t>(d, o, r, s);
+}
+
+}  // namespace paged
+}  // namespace nvq

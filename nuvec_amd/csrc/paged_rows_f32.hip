@@ -1,0 +1,12 @@
+// Attention of few lines over a paged cache, float32.
+#include "paged_rows_kernel.h"
+
+namespace nvq {
+namespace paged {
+
+int32_t launch_rows_f32(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const RowsLaunch &r, hipStream_t s) {
+    return launch_rows<float>(d, o, r, s);
+}
+
+}  // namespace paged
+}  // namespace nvq
