@@ -15,6 +15,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <ATen/ExpandUtils.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/core/Tensor.h>
 #include <c10/hip/HIPFunctions.h>
@@ -33,6 +34,7 @@ using at::Tensor;
 struct Names {
     PyObject *mode, *group_size, *bits, *weight, *scales, *biases, *bias, *quant, *global_scale;
     PyObject *gate_proj, *up_proj, *down_proj, *gate_up_proj, *geglu;
+    PyObject *keys, *values, *table, *interleaved;
     PyObject *gate, *switch_mlp, *experts_per_token, *norm_topk_prob, *gate_up_paired, *activation, *alpha, *limit;
 } names;
 
@@ -721,6 +723,247 @@ PyObject *py_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
+// ── heads and the paged cache (paged.py) ────────────────────────────────────────────────────────────────────────────
+// A rotation's table of angles, or none at all; nothing here is looked up of a class, so any object with the attributes will do.
+struct Angles {
+    Tensor table;
+    bool interleaved = false;
+    int32_t dims() const { return table.defined() ? (int32_t)(2 * table.size(1)) : 0; }
+    int64_t rows() const { return table.defined() ? table.size(0) : 0; }
+    bool fits(const Place &at, int64_t dim) const {
+        return !table.defined() || (table.scalar_type() == at::kFloat && table.dim() == 3 && table.size(2) == 2 && table.size(0) > 0 && table.size(1) > 0 &&
+                                    2 * table.size(1) <= dim && at.holds(table));
+    }
+};
+bool read_angles(PyObject *o, Angles &a) {
+    return o == Py_None || (read_tensor(o, names.table, a.table) && a.table.defined() && read_truth(o, names.interleaved, a.interleaved));
+}
+
+bool weight_fits(const Tensor &w, const Place &at, at::ScalarType type, int64_t dim) {
+    return !w.defined() || (w.scalar_type() == type && w.dim() == 1 && w.size(0) == dim && at.holds(w));
+}
+
+bool is_index(const Tensor &t, const Place &at, int64_t n) { return t.defined() && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && at.holds(t); }
+
+// Heads [batch, heads, length, dim] with consecutive values, on the device.
+bool is_heads(const Tensor &x, const Place &at, at::ScalarType type) {
+    return x.defined() && x.dim() == 4 && x.numel() > 0 && x.device() == at.device && x.scalar_type() == type && x.stride(3) == 1 && x.size(3) <= 512;
+}
+
+// Operands of one call (queries and keys, or one alone) rotated into dense outputs of their strides' order, or `out` of the first.
+bool rotate(const Place &at, const Tensor *xs, const Tensor *weights, int count, const Angles &angles, const Tensor &offsets, int64_t offset, double eps,
+            Tensor *ys) {
+    const Tensor &x = xs[0];
+    nvq_head_rope_desc d{};
+    d.dtype = code_of(x.scalar_type()), d.head_dim = (int32_t)x.size(3), d.rotary_dims = angles.dims(), d.interleaved = angles.interleaved;
+    d.table_rows = angles.rows(), d.batch = x.size(0), d.length = x.size(2), d.eps = eps;
+    if (offsets.defined()) {
+        d.per_position = offsets.dim() == 2;
+        if (offsets.scalar_type() != at::kInt || !at.holds(offsets) || offsets.dim() < 1 || offsets.dim() > 2 || offsets.size(0) != d.batch ||
+            (d.per_position && offsets.size(1) != d.length))
+            return false;
+    } else {
+        d.offset = offset;
+        if (angles.table.defined() && (offset < 0 || offset + d.length > d.table_rows)) return false;
+    }
+    for (int i = 0; i < count; i++) {
+        if (!ys[i].defined()) {
+            const auto strides = at::infer_dense_strides(xs[i].sizes(), xs[i].strides());
+            ys[i] = at::detail::empty_strided_cuda(xs[i].sizes(), strides, xs[i].scalar_type(), at.device);
+        } else if (!is_heads(ys[i], at, x.scalar_type()) || ys[i].sizes() != xs[i].sizes()) {
+            return false;
+        }
+        d.heads[i] = xs[i].size(1);
+        for (int k = 0; k < 3; k++) d.x_strides[i][k] = xs[i].stride(k), d.y_strides[i][k] = ys[i].stride(k);
+    }
+    const bool two = count == 2;
+    return nvq_head_norm_rope(&d, (const float *)ptr(angles.table), (const int32_t *)ptr(offsets), ptr(xs[0]), ptr(weights[0]), ys[0].mutable_data_ptr(),
+                              two ? ptr(xs[1]) : nullptr, two ? ptr(weights[1]) : nullptr, two ? ys[1].mutable_data_ptr() : nullptr,
+                              at.stream()) == NVQ_OK;
+}
+
+// An offset: a tensor, or an int.
+bool read_offset(PyObject *o, Tensor &offsets, int64_t &offset) {
+    if (THPVariable_Check(o)) return as_tensor(o, offsets);
+    if (!PyLong_Check(o)) return false;
+    offset = PyLong_AsLongLong(o);
+    return offset != -1 || !PyErr_Occurred() || declined();
+}
+
+// rope(x, rotation, offset, out or None)
+PyObject *py_rope(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        Tensor x, y, offsets;
+        const Tensor no_weight;
+        Angles angles;
+        int64_t offset = 0;
+        if (n != 4 || !as_tensor(args[0], x) || !read_angles(args[1], angles) || !angles.table.defined() || !read_offset(args[2], offsets, offset) ||
+            !as_tensor(args[3], y))
+            return none();
+        const Place at(x);
+        if (!at.usable() || code_of(x.scalar_type()) < 0 || !is_heads(x, at, x.scalar_type()) || !angles.fits(at, x.size(3))) return none();
+        return wrap(unlocked([&] { return rotate(at, &x, &no_weight, 1, angles, offsets, offset, 0.0, &y); }), y);
+    });
+}
+
+// head_norm_rope(q, k, q weight, k weight, rotation or None, offset, eps)
+PyObject *py_head_norm_rope(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        Tensor xs[2], ys[2], weights[2], offsets;
+        Angles angles;
+        int64_t offset = 0;
+        if (n != 7 || !as_tensor(args[0], xs[0]) || !as_tensor(args[1], xs[1]) || !as_tensor(args[2], weights[0]) || !as_tensor(args[3], weights[1]) ||
+            !read_angles(args[4], angles) || !read_offset(args[5], offsets, offset))
+            return none();
+        const double eps = PyFloat_AsDouble(args[6]);
+        if (eps == -1.0 && PyErr_Occurred()) return declined(), none();
+        const Place at(xs[0]);
+        if (!at.usable() || code_of(xs[0].scalar_type()) < 0) return none();
+        const at::ScalarType type = xs[0].scalar_type();
+        for (int i = 0; i < 2; i++)
+            if (!is_heads(xs[i], at, type) || !weight_fits(weights[i], at, type, xs[0].size(3))) return none();
+        if (xs[1].size(0) != xs[0].size(0) || xs[1].size(2) != xs[0].size(2) || xs[1].size(3) != xs[0].size(3) || !angles.fits(at, xs[0].size(3))) return none();
+        if (!unlocked([&] { return rotate(at, xs, weights, 2, angles, offsets, offset, eps, ys); })) return none();
+        Ref q(THPVariable_Wrap(std::move(ys[0]))), k(THPVariable_Wrap(std::move(ys[1])));
+        return q.p && k.p ? PyTuple_Pack(2, q.p, k.p) : nullptr;
+    });
+}
+
+struct Paged {
+    Packed k, v;
+    Tensor table;  // of pages
+    nvq_paged_desc d{};
+
+    bool fits(const Place &at, at::ScalarType type) {
+        int64_t dim, same;
+        const auto apart = [](const Tensor &t) { return t.dim() == 2 && (t.numel() == 0 || (t.stride(1) == 1 && t.stride(0) >= t.size(1))); };
+        if (code_of(type) < 0 || k.q.mode != NVQ_AFFINE || k.q.bits != v.q.bits || k.q.group_size != v.q.group_size || v.q.mode != NVQ_AFFINE ||
+            !k.fits(at, type, 4, dim) || !v.fits(at, type, 4, same) || k.w.sizes() != v.w.sizes() || !table.defined() || table.scalar_type() != at::kInt ||
+            table.device() != at.device || !apart(table) || k.w.numel() == 0)
+            return false;
+        d = nvq_paged_desc{code_of(type), k.q.bits, k.q.group_size, (int32_t)dim, k.w.size(0), k.w.size(2), k.w.size(1), table.size(0), table.size(1),
+                           std::max(table.stride(0), table.size(1))};
+        return true;
+    }
+};
+bool read_pages(PyObject *o, PyObject *name, Packed &p) {
+    Ref a(PyObject_GetAttr(o, name));
+    if (a.p == nullptr) return declined();
+    Ref q(PyObject_GetAttr(a.p, names.quant));
+    return q.p == nullptr ? declined() : read_quant(q.p, p.q) && read_tensor(a.p, names.weight, p.w) && read_tensor(a.p, names.scales, p.s) && read_tensor(a.p, names.biases, p.b);
+}
+bool read_paged(PyObject *cache, PyObject *table, Paged &p) { return read_pages(cache, names.keys, p.k) && read_pages(cache, names.values, p.v) && as_tensor(table, p.table); }
+
+// Rows [tokens, heads, dim] with consecutive values.
+bool is_rows(const Tensor &x, const Place &at, at::ScalarType type, int64_t tokens, int64_t dim) {
+    return x.defined() && x.dim() == 3 && x.numel() > 0 && x.device() == at.device && x.scalar_type() == type && x.size(0) == tokens && x.size(2) == dim &&
+           x.stride(2) == 1;
+}
+
+// append_paged(cache, k, v, page table, positions, sequences, rotation, k weight, q, q weight, eps): the queries, or True without any
+PyObject *py_append_paged(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        Paged p;
+        Angles angles;
+        Tensor k, v, positions, sequences, k_weight, q, q_weight, y;
+        if (n != 11 || !as_tensor(args[1], k) || !as_tensor(args[2], v) || !read_paged(args[0], args[3], p) || !as_tensor(args[4], positions) ||
+            !as_tensor(args[5], sequences) || !read_angles(args[6], angles) || !as_tensor(args[7], k_weight) || !as_tensor(args[8], q) ||
+            !as_tensor(args[9], q_weight))
+            return none();
+        const double eps = PyFloat_AsDouble(args[10]);
+        if (eps == -1.0 && PyErr_Occurred()) return declined(), none();
+        const Place at(k);
+        if (!at.usable() || k.dim() != 3) return none();
+        const at::ScalarType type = k.scalar_type();
+        const int64_t tokens = k.size(0), dim = k.size(2);
+        if (!p.fits(at, type) || p.d.head_dim != dim || !is_rows(k, at, type, tokens, dim) || !is_rows(v, at, type, tokens, dim) ||
+            k.size(1) != p.d.key_heads || v.size(1) != p.d.key_heads || !is_index(positions, at, tokens) ||
+            (sequences.defined() ? !is_index(sequences, at, tokens) : p.d.sequences != tokens) || !angles.fits(at, dim) ||
+            !weight_fits(k_weight, at, type, dim) || (q.defined() && (!is_rows(q, at, type, tokens, dim) || !weight_fits(q_weight, at, type, dim))))
+            return none();
+        nvq_paged_append_desc d{};
+        d.cache = p.d, d.tokens = tokens, d.rotary_dims = angles.dims(), d.interleaved = angles.interleaved, d.table_rows = angles.rows(), d.eps = eps;
+        d.query_heads = q.defined() ? q.size(1) : 0;
+        for (int i = 0; i < 2; i++) {
+            d.k_strides[i] = k.stride(i), d.v_strides[i] = v.stride(i);
+            if (q.defined()) d.q_strides[i] = q.stride(i);
+        }
+        const bool done = unlocked([&] {
+            if (q.defined()) y = at.empty(q.sizes(), type);
+            return nvq_append_paged(&d, (const int32_t *)ptr(p.table), (const int32_t *)ptr(sequences), (const int32_t *)ptr(positions),
+                                    (const float *)ptr(angles.table), ptr(q), q.defined() ? ptr(q_weight) : nullptr,
+                                    q.defined() ? y.mutable_data_ptr() : nullptr, ptr(k), ptr(k_weight), ptr(v), (uint32_t *)p.k.w.mutable_data_ptr(),
+                                    p.k.s.mutable_data_ptr(), p.k.b.mutable_data_ptr(), (uint32_t *)p.v.w.mutable_data_ptr(), p.v.s.mutable_data_ptr(),
+                                    p.v.b.mutable_data_ptr(), at.stream()) == NVQ_OK;
+        });
+        if (done && !q.defined()) Py_RETURN_TRUE;
+        return wrap(done, y);
+    });
+}
+
+// read_paged(cache, page table, positions, sequences)
+PyObject *py_read_paged(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        Paged p;
+        Tensor positions, sequences, keys, values;
+        if (n != 4 || !read_paged(args[0], args[1], p) || !as_tensor(args[2], positions) || !as_tensor(args[3], sequences) || !p.k.s.defined()) return none();
+        const Place at(p.k.w);
+        const at::ScalarType type = p.k.s.scalar_type();
+        if (!at.usable() || !p.fits(at, type) || !positions.defined() || positions.dim() != 1 || positions.size(0) == 0) return none();
+        const int64_t tokens = positions.size(0);
+        if (!is_index(positions, at, tokens) || (sequences.defined() ? !is_index(sequences, at, tokens) : p.d.sequences != tokens)) return none();
+        const bool done = unlocked([&] {
+            keys = at.empty({tokens, p.d.key_heads, p.d.head_dim}, type), values = at.empty({tokens, p.d.key_heads, p.d.head_dim}, type);
+            return nvq_read_paged(&p.d, tokens, (const int32_t *)ptr(p.table), (const int32_t *)ptr(sequences), (const int32_t *)ptr(positions),
+                                  (const uint32_t *)ptr(p.k.w), ptr(p.k.s), ptr(p.k.b), (const uint32_t *)ptr(p.v.w), ptr(p.v.s), ptr(p.v.b),
+                                  keys.mutable_data_ptr(), values.mutable_data_ptr(), at.stream()) == NVQ_OK;
+        });
+        if (!done) return none();
+        Ref k(THPVariable_Wrap(std::move(keys))), v(THPVariable_Wrap(std::move(values)));
+        return k.p && v.p ? PyTuple_Pack(2, k.p, v.p) : nullptr;
+    });
+}
+
+// paged_attention(q, cache, page table, lengths, scale, query starts, max queries or None, sinks, causal, window, out or None)
+PyObject *py_paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        Paged p;
+        Tensor q, lengths, starts, sinks, y;
+        if (n != 11 || !as_tensor(args[0], q) || !read_paged(args[1], args[2], p) || !as_tensor(args[3], lengths) || !as_tensor(args[5], starts) ||
+            !as_tensor(args[7], sinks) || !as_tensor(args[10], y) || !PyLong_Check(args[9]))
+            return none();
+        const double scale = PyFloat_AsDouble(args[4]);
+        if (scale == -1.0 && PyErr_Occurred()) return declined(), none();
+        const int64_t window = PyLong_AsLongLong(args[9]);
+        int64_t most = args[6] == Py_None ? INT64_MAX : PyLong_Check(args[6]) ? PyLong_AsLongLong(args[6]) : -1;
+        if (PyErr_Occurred()) return declined(), none();
+        const int causal = PyObject_IsTrue(args[8]);
+        if (causal < 0) return nullptr;
+        const Place at(q);
+        if (!at.usable() || q.dim() != 3 || window < 0 || most < 0) return none();
+        const at::ScalarType type = q.scalar_type();
+        const int64_t rows = q.size(0), heads = q.size(1), dim = q.size(2);
+        if (!p.fits(at, type) || p.d.head_dim != dim || !is_rows(q, at, type, rows, dim) || !is_index(lengths, at, p.d.sequences) ||
+            (starts.defined() ? !is_index(starts, at, p.d.sequences + 1) : p.d.sequences != rows) || !bias_fits(sinks, at, type, heads) ||
+            (y.defined() && (!is_rows(y, at, type, rows, dim) || y.size(1) != heads)))
+            return none();
+        nvq_paged_attention_desc d{};
+        d.cache = p.d, d.rows = rows, d.query_heads = heads, d.max_queries = !starts.defined() ? 1 : most < 1 ? 1 : most < rows ? most : rows;
+        d.window = window, d.causal = causal, d.scale = (float)scale;
+        const bool done = unlocked([&] {
+            if (!y.defined()) y = at.empty(q.sizes(), type);
+            for (int i = 0; i < 2; i++) d.q_strides[i] = q.stride(i), d.out_strides[i] = y.stride(i);
+            const size_t need = nvq_paged_attention_workspace_bytes(&d);
+            Tensor workspace;
+            if (need > 0) workspace = at.empty({(int64_t)need}, at::kByte);
+            return nvq_paged_attention(&d, ptr(q), (const uint32_t *)ptr(p.k.w), ptr(p.k.s), ptr(p.k.b), (const uint32_t *)ptr(p.v.w), ptr(p.v.s),
+                                       ptr(p.v.b), (const int32_t *)ptr(p.table), (const int32_t *)ptr(lengths), (const int32_t *)ptr(starts), ptr(sinks),
+                                       y.mutable_data_ptr(), need > 0 ? workspace.mutable_data_ptr() : nullptr, at.stream()) == NVQ_OK;
+        });
+        return wrap(done, y);
+    });
+}
+
 // register((type, {name: function}), ...): QuantizedLinear, SwitchProjection, SwitchGlu and MoeMlp with their own methods
 PyObject *py_register(PyObject *, PyObject *const *args, Py_ssize_t n) {
     Kind *const kinds[] = {&linear_kind, &projection_kind, &switch_glu_kind, &moe_kind};
@@ -761,6 +1004,11 @@ PyMethodDef methods[] = {
     {"dequantize", NVQ_FAST(py_dequantize), nullptr},
     {"embedding", NVQ_FAST(py_embedding), nullptr},
     {"attention", NVQ_FAST(py_attention), nullptr},
+    {"rope", NVQ_FAST(py_rope), nullptr},
+    {"head_norm_rope", NVQ_FAST(py_head_norm_rope), nullptr},
+    {"append_paged", NVQ_FAST(py_append_paged), nullptr},
+    {"read_paged", NVQ_FAST(py_read_paged), nullptr},
+    {"paged_attention", NVQ_FAST(py_paged_attention), nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
@@ -775,7 +1023,8 @@ extern "C" __attribute__((visibility("default"))) PyObject *PyInit__native(void)
         {&names.down_proj, "down_proj"}, {&names.gate_up_proj, "gate_up_proj"}, {&names.geglu, "geglu"},
         {&names.gate, "gate"}, {&names.switch_mlp, "switch_mlp"}, {&names.experts_per_token, "experts_per_token"},
         {&names.norm_topk_prob, "norm_topk_prob"}, {&names.gate_up_paired, "gate_up_paired"}, {&names.activation, "activation"},
-        {&names.alpha, "alpha"}, {&names.limit, "limit"},
+        {&names.alpha, "alpha"}, {&names.limit, "limit"}, {&names.keys, "keys"}, {&names.values, "values"},
+        {&names.table, "table"}, {&names.interleaved, "interleaved"},
     };
     for (auto &n : all) {
         *n.at = PyUnicode_InternFromString(n.text);

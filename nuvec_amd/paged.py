@@ -169,6 +169,9 @@ def rope(x: torch.Tensor, rotation: Rotation, offset: Union[int, torch.Tensor] =
     """Rotary positions of `x` `[batch, heads, length, dim]` (any strides with consecutive values of a head; MLX's `fast.rope`): the first
     `rotation.dims` values of a head turn, the others stay.  Element l is at position `offset + l`; `offset` is an int, int32 `[batch]`, or int32
     `[batch, length]` for positions one by one.  Positions on the device outside the table are clamped to it.  `out` may be `x` itself."""
+    y = (_lib._native or _lib.native()).rope(x, rotation, offset, out)
+    if y is not None:
+        return y if out is None else out
     return _rotate("rope", (_heads("rope", x),), (None,), (out,), rotation, offset, 0.0)[0]
 
 
@@ -176,6 +179,9 @@ def head_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
                    rotation: Optional[Rotation] = None, offset: Union[int, torch.Tensor] = 0, eps: float = 1e-6):
     """The RMS norms over each head of queries and keys (`[batch, heads, length, dim]`, their own numbers of heads; weights `[dim]`, None: not
     normed) and their rotation, in one pass over both: `(q, k)`, rounded once.  `offset` as in `rope`."""
+    done = (_lib._native or _lib.native()).head_norm_rope(q, k, q_weight, k_weight, rotation, offset, eps)
+    if done is not None:
+        return done
     op = "head_norm_rope"
     q, k = _heads(op, q), _heads(op, k)
     if k.dtype != q.dtype or (k.shape[0], k.shape[2], k.shape[3]) != (q.shape[0], q.shape[2], q.shape[3]):
@@ -267,6 +273,9 @@ def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table
     A token with a negative position is padding: nothing is written.  Neither is one whose position lies outside the rotation's table or the page
     table, or whose page is not in the pool.  Two tokens of one position are the caller's error.  (Codes are the nearest to the scale and bias as
     stored, those of `quantize` to the unrounded ones.)"""
+    done = (_lib._native or _lib.native()).append_paged(cache, k, v, page_table, positions, sequences, rotation, k_weight, q, q_weight, eps)
+    if done is not None:
+        return None if done is True else done
     op = "append_paged"
     if k.ndim != 3 or k.dtype not in _FLOATS:
         raise InvalidArgument(f"{op}: keys must be [tokens, key heads, dim] of a float type, got {_name(k.dtype)} {list(k.shape)}")
@@ -304,6 +313,9 @@ def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table
 def read_paged(cache: PagedCache, page_table: torch.Tensor, positions: torch.Tensor, sequences: Optional[torch.Tensor] = None):
     """Positions of the cache as values: `(keys, values)`, each `[tokens, key_heads, dim]` in the scales' type, code * scale + bias rounded once;
     row t is position `positions[t]` of sequence `sequences[t]` (int32; None: t), zeros where `append_paged` would write nothing."""
+    done = (_lib._native or _lib.native()).read_paged(cache, page_table, positions, sequences)
+    if done is not None:
+        return done
     op = "read_paged"
     cd, page_table, pool = _paged(op, cache, None, None, page_table)
     if positions.ndim != 1:
@@ -333,6 +345,9 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
 
     The keys' and values' codes are exact operands; the softmax's weights, times the values' scales, are rounded to the precision of the element type,
     everything else is float32."""
+    y = (_lib._native or _lib.native()).paged_attention(q, cache, page_table, lengths, scale, query_starts, max_queries, sinks, causal, window, out)
+    if y is not None:
+        return y if out is None else out
     op = "paged_attention"
     if q.ndim != 3 or q.dtype not in _FLOATS:
         raise InvalidArgument(f"{op}: queries must be [rows, query heads, dim] of a float type, got {_name(q.dtype)} {list(q.shape)}")
