@@ -1,4 +1,4 @@
-// The launches of attention over a paged cache, one translation unit per element type.
+// The launches of attention over a paged cache, one translation unit per element type and kernel.
 #pragma once
 
 #include "nvq_internal.h"
@@ -7,13 +7,18 @@
 namespace nvq {
 namespace paged {
 
-struct RowsLaunch {
+struct PagedLaunch {
     PagedBatch batch;
+    size_t states;                            // where in the workspace the kernel's states lie
     uint32_t grid, merge_units, merge_lines;  // merge_units 0: no sequence can be split
 };
-int32_t launch_rows_f32(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const RowsLaunch &r, hipStream_t s);
-int32_t launch_rows_bf16(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const RowsLaunch &r, hipStream_t s);
-int32_t launch_rows_f16(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const RowsLaunch &r, hipStream_t s);
+// few lines: query rows x query heads of a key head
+int32_t launch_rows_f32(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const PagedLaunch &r, hipStream_t s);
+int32_t launch_rows_bf16(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const PagedLaunch &r, hipStream_t s);
+int32_t launch_rows_f16(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const PagedLaunch &r, hipStream_t s);
+// many
+int32_t launch_prompt_bf16(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const PagedLaunch &r, hipStream_t s);
+int32_t launch_prompt_f16(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const PagedLaunch &r, hipStream_t s);
 
 }  // namespace paged
 }  // namespace nvq

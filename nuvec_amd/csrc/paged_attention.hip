@@ -22,42 +22,68 @@ PagedBatch batch_of(const nvq_paged_attention_desc &d, const PagedAttentionOpera
 
 namespace {
 
-// Blocks of the kernel of few lines that the chip holds at once.
-int32_t rows_target(const nvq_paged_attention_desc &d) {
-    return (d.cache.dtype == NVQ_F32 || d.cache.head_dim / d.cache.group_size == 4 ? 2 : 3) * compute_units();
+// Lines of a sequence that the kernel of few lines takes, where the other kernel has the type.
+constexpr int32_t kFewLines = 32;
+constexpr int64_t kPromptLines = 128;
+
+struct Kernel {
+    int64_t lines;   // of a unit
+    int32_t target;  // blocks that the chip holds at once
+    size_t bytes;    // of its states
+};
+// States of every item of the sequences that are split: at most twice the target (paged_schedule.h: each of their splits but the last is a
+// whole item).
+Kernel kernel_of(const nvq_paged_attention_desc &d, bool many) {
+    const int groups = d.cache.head_dim / d.cache.group_size;
+    Kernel k;
+    k.lines = many ? kPromptLines : 16 / groups;
+    k.target = (many || d.cache.dtype == NVQ_F32 || groups == 4 ? 2 : 3) * compute_units();
+    k.bytes = (size_t)(2 * (int64_t)k.target * k.lines * (d.cache.head_dim + 2)) * sizeof(float);
+    return k;
 }
 
 // (the device decides by the lengths, which are at most the table's columns)
-bool may_split(const nvq_paged_attention_desc &d) { return d.cache.columns * d.cache.page_size > 32 * 8; }
+bool may_split(const nvq_paged_attention_desc &d) { return d.cache.columns * d.cache.page_size > kScheduleKeys * kScheduleTiles; }
+// Whether a sequence may have more lines than the kernel of few takes.
+bool takes_many(const nvq_paged_attention_desc &d, bool starts) {
+    const int64_t most = d.max_queries < d.rows ? d.max_queries : d.rows;
+    return starts && d.cache.dtype != NVQ_F32 && most * (d.query_heads / d.cache.key_heads) > kFewLines;
+}
 
 }  // namespace
 
-// States of every item of the sequences that are split: at most twice the target (paged_schedule.h: each of their splits but the last
-// is a whole item).
 size_t paged_attention_workspace_bytes(const nvq_paged_attention_desc &d) {
     if (!may_split(d) || d.rows == 0) return 0;
-    const int64_t lines = 16 / (d.cache.head_dim / d.cache.group_size);
-    return (size_t)(2 * (int64_t)rows_target(d) * lines * (d.cache.head_dim + 2)) * sizeof(float);
+    return kernel_of(d, false).bytes + (takes_many(d, true) ? kernel_of(d, true).bytes : 0);
 }
 
 int32_t launch_paged_attention(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, hipStream_t s) {
-    paged::RowsLaunch r{};
     const nvq_paged_desc &c = d.cache;
-    r.batch = paged::batch_of(d, o);
-    r.batch.target = rows_target(d);
-    const int64_t lines = 16 / (c.head_dim / c.group_size), rep = r.batch.rep;
-    // At most so many units and items, whatever the lengths and starts on the device say (paged_schedule.h).
-    const int64_t most = c.key_heads * (o.starts == nullptr ? c.sequences * ((rep + lines - 1) / lines) : (d.rows * rep + lines - 1) / lines + c.sequences);
-    const int64_t splits = (c.columns * c.page_size + 255) / 256, full = r.batch.target, spare = full / 2 + most;
-    const int64_t items = full > spare ? full : spare;
-    r.grid = (uint32_t)(most * splits < items ? most * splits : items);
-    r.merge_units = may_split(d) ? (uint32_t)(most < full ? most : full) : 0;
-    r.merge_lines = (uint32_t)(o.starts == nullptr && rep < lines ? rep : lines);
-    switch (c.dtype) {
-    case NVQ_F32: return paged::launch_rows_f32(d, o, r, s);
-    case NVQ_BF16: return paged::launch_rows_bf16(d, o, r, s);
-    default: return paged::launch_rows_f16(d, o, r, s);
-    }
+    const bool starts = o.starts != nullptr, many = takes_many(d, starts);
+    auto launch_of = [&](bool of_many) {
+        const Kernel k = kernel_of(d, of_many);
+        paged::PagedLaunch r{};
+        r.batch = paged::batch_of(d, o);
+        r.batch.few = many ? kFewLines : INT32_MAX, r.batch.target = k.target;
+        const int64_t rep = r.batch.rep;
+        // At most so many units and items, whatever the lengths and starts on the device say (paged_schedule.h).
+        const int64_t each = many && !of_many ? (kFewLines + k.lines - 1) / k.lines : (rep + k.lines - 1) / k.lines;
+        int64_t units = c.sequences * each;
+        if (starts) units = of_many ? d.rows * rep / k.lines + c.sequences : (d.rows * rep + k.lines - 1) / k.lines + c.sequences;
+        if (many && !of_many && units > c.sequences * each) units = c.sequences * each;
+        units *= c.key_heads;
+        const int64_t splits = (c.columns * c.page_size + kScheduleKeys * kScheduleTiles - 1) / (kScheduleKeys * kScheduleTiles), full = k.target, spare = full / 2 + units;
+        const int64_t items = full > spare ? full : spare;
+        r.grid = (uint32_t)(units * splits < items ? units * splits : items);
+        r.merge_units = may_split(d) ? (uint32_t)(units < full ? units : full) : 0;
+        r.merge_lines = (uint32_t)(!starts && rep < k.lines ? rep : k.lines);
+        r.states = of_many ? kernel_of(d, false).bytes : 0;
+        return r;
+    };
+    const paged::PagedLaunch few = launch_of(false);
+    const int32_t rc = c.dtype == NVQ_F32 ? paged::launch_rows_f32(d, o, few, s) : c.dtype == NVQ_BF16 ? paged::launch_rows_bf16(d, o, few, s) : paged::launch_rows_f16(d, o, few, s);
+    if (rc != NVQ_OK || !many) return rc;
+    return c.dtype == NVQ_BF16 ? paged::launch_prompt_bf16(d, o, launch_of(true), s) : paged::launch_prompt_f16(d, o, launch_of(true), s);
 }
 
 }  // namespace nvq

@@ -1,0 +1,12 @@
+// Attention of many lines over a paged cache, bfloat16.
+#include "paged_prompt_kernel.h"
+
+namespace nvq {
+namespace paged {
+
+int32_t launch_prompt_bf16(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const PagedLaunch &r, hipStream_t s) {
+    return launch_prompt<bf16_t>(d, o, r, s);
+}
+
+}  // namespace paged
+}  // namespace nvq

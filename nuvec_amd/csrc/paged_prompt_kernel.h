@@ -1,0 +1,360 @@
+// Attention of many lines (query rows x query heads of a key head) over a paged, affine-quantized key / value cache, float16 and bfloat16.
+//
+// The products run on the matrix cores over the codes, as for few lines (paged_rows_kernel.h): scale and bias of a key's groups
+// are applied to the float32 scores, those of a value's to the softmax's weights, so that no key or value is rounded.
+// A block has 128 lines, a wavefront 32 of them: S^T = K . Q^T with v_mfma_f32_32x32x16, a group of the head at a time, leaves a lane
+// with 16 of 32 keys of ONE line; its maximum and sum are in-lane but for one exchange, and its weights are already the operand of
+// O^T = V^T . P^T, whose keys are stored in the order in which the lanes hold them.
+//
+// 64 keys at a time become operands in LDS, once for the block: expanded by each wavefront for itself they would cost it three times
+// the instructions, which are what bounds the kernel.  The next 64 keys' codes are requested before, and expanded after, this
+// tile's products; two buffers, one barrier a tile.  A code becomes an element in two instructions for two of them (16 + code in the
+// mantissa; 8 bits through float32); the 16, and for V the middle of the codes' range, are taken off the sums: the scores' by the
+// bias, the outputs' by the sum of the rounded weights.
+//
+// Terms: queries are exact in their own type.  Weights x scale are rounded to bfloat16, to two terms of it where the element type is float16.
+#pragma once
+
+#include "paged_rows_kernel.h"
+
+namespace nvq {
+namespace paged {
+namespace {
+
+using qmf::floatx16_t;
+constexpr int kPromptLines = 128, kStageKeys = 64;
+
+// Eight codes of a row as an operand of the element type, value code_at<BITS>(j) of them in place j, each plus key_offset.
+template <typename T, int BITS> constexpr float key_offset = BITS == 4 ? 16.0f : Elem<T>::code == NVQ_BF16 ? 0.0f : 1024.0f;
+template <typename T, int BITS>
+__device__ __forceinline__ uint4 key_codes(const CodeConstants<BITS == 8 ? 4 : BITS> &c, uint32_t w0, uint32_t w1) {
+    if constexpr (BITS == 8 && Elem<T>::code == NVQ_BF16) {
+        return make_uint4(pack_exact(qmf::ubyte_to_float<0>(w0), qmf::ubyte_to_float<1>(w0)), pack_exact(qmf::ubyte_to_float<2>(w0), qmf::ubyte_to_float<3>(w0)),
+                          pack_exact(qmf::ubyte_to_float<0>(w1), qmf::ubyte_to_float<1>(w1)), pack_exact(qmf::ubyte_to_float<2>(w1), qmf::ubyte_to_float<3>(w1)));
+    } else if constexpr (BITS == 8) {  // 1024 + code: the low bits of the mantissa
+        auto two = [](uint32_t w, bool high) { return __builtin_amdgcn_perm(0u, w, high ? 0x0C030C02u : 0x0C010C00u) | 0x64006400u; };
+        return make_uint4(two(w0, false), two(w0, true), two(w1, false), two(w1, true));
+    } else if constexpr (Elem<T>::code == NVQ_BF16) {
+        return make_uint4(two_codes(c, w0, 0), two_codes(c, w0, 4), two_codes(c, w0, 8), two_codes(c, w0, 12));
+    } else {  // 16 + code, in float16 at bit 6
+        auto two = [](uint32_t z, int at) { return ((at >= 6 ? z >> (at - 6) : z << (6 - at)) & 0x03C003C0u) | 0x4C004C00u; };
+        return make_uint4(two(w0, 0), two(w0, 4), two(w0, 8), two(w0, 12));
+    }
+}
+
+template <typename T, int BITS, int D, int G>
+__global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const RowsArgs<T> a, const int32_t *__restrict__ table) {
+    constexpr int TP = Elem<T>::code == NVQ_BF16 ? 1 : 2;
+    constexpr int KS = D / 16, DB = D / 32, GS = KS / G, GB = DB / G > 0 ? DB / G : 1;  // steps of K, blocks of D; of a group
+    constexpr int kRowBytes = D * BITS / 8, kPart = kRowBytes / 4;     // a row; a quarter of one, a thread's share of the keys' codes
+    constexpr int kChunks = D / 32, kVals = D / 16, kSlot = BITS * kVals;  // eight-code chunks of a quarter; values of a sixteenth and its bits
+    constexpr float kOff = key_offset<T, BITS>, kValueOff = BITS == 4 ? 16.0f : 0.0f, kMiddle = 1 << (BITS - 1);
+    struct Stage {
+        uint4 keys[2][KS][64];          // [half of the tile][step][half of the step x key]
+        uint4 values[4][DB][64];        // [16 keys][block][half of the keys x value]
+        float scale[4][G][kStageKeys];  // of keys and what goes with it, of values and what goes with it (expand)
+    };
+    __shared__ Stage stages[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
+    PagedItem item;
+    if (!paged_item<kPromptLines, 1, false>(a.batch, lane, blockIdx.x, item)) return;
+    const int rep = a.batch.rep, hk = item.head, S = item.s.length, n = item.s.rows;
+    const int part = item.s.parts - 1 - item.part;  // (the lines that see most first)
+    const int lines = n * rep;
+    const int window = (int)(a.batch.window < S + 1 ? a.batch.window : S + 1);
+    auto last_of = [&](int i) { return a.batch.causal ? S - n + i : S - 1; };
+    auto first_of = [&](int i) { return window > 0 && a.batch.causal ? last_of(i) - window + 1 : 0; };
+    // the block's keys
+    const int b_first = part * kPromptLines / rep, b_end = (part + 1) * kPromptLines < lines ? (part + 1) * kPromptLines : lines, b_last = (b_end - 1) / rep;
+    const int split_begin = item.s.base + item.split * item.per * kTile;
+    int s_begin = split_begin, s_end = item.splits == 1 ? S : split_begin + item.per * kTile < S ? split_begin + item.per * kTile : S;
+    if (last_of(b_last) + 1 < s_end) s_end = last_of(b_last) + 1;
+    if (first_of(b_first) / kTile * kTile > s_begin) s_begin = first_of(b_first) / kTile * kTile;
+    // the wavefront's lines
+    const int r0 = part * kPromptLines + wave * 32, r = r0 + col;
+    const bool live = r < lines;
+    const int my_row = (live ? r : lines - 1) / rep, my_head = hk * rep + (live ? r % rep : 0);
+    const int my_last = last_of(my_row), my_first = first_of(my_row);
+    const int w_first = (r0 < lines ? r0 : lines - 1) / rep, w_last = (r0 + 31 < lines ? r0 + 31 : lines - 1) / rep;
+    const int all_last = last_of(w_first), all_first = first_of(w_last);                       // keys up to / from which all of them see
+    const int any_last = r0 < lines ? last_of(w_last) : -1, any_first = first_of(w_first);  // and any does
+
+    uint4 qf[KS];
+    float qsum[G];
+#pragma unroll
+    for (int g = 0; g < G; g++) qsum[g] = 0.0f;
+    const T *query = a.q + (int64_t)(item.s.start + my_row) * a.q_strides[0] + (int64_t)my_head * a.q_strides[1];
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+        const uint4 w = load_any<uint4>(query + 16 * s + 8 * half);
+        T t[8], to[8];
+        __builtin_memcpy(t, &w, 16);
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) to[j] = t[code_at<BITS>(j)], sum += Elem<T>::load(t, j);
+        __builtin_memcpy(&qf[s], to, 16);
+        qsum[s / GS] += sum;
+    }
+#pragma unroll
+    for (int g = 0; g < G; g++) qsum[g] += __shfl_xor(qsum[g], 32);
+
+    // ── staging ──
+    const CodeConstants<4> constants;
+    const float scale = a.scale * kLog2e;
+    const int shift = a.batch.place.page_shift, last_column = S > 0 ? (S - 1) >> shift : 0;
+    const int32_t *columns = table + item.b * a.batch.place.stride;
+    // The row (of all pages and heads) of position `at`, which lies in a page of the sequence or behind its end.
+    auto row_of = [&](int at) __attribute__((always_inline)) {
+        const int column = at >> shift;
+        const int64_t id = columns[column < last_column ? column : last_column], pages = a.batch.place.pages;
+        const int64_t page = id < 0 ? 0 : id < pages ? id : pages - 1;
+        return ((page * a.batch.key_heads + hk) << shift) + (at & ((1 << shift) - 1));
+    };
+    // Of 64 keys this thread's: a quarter of a key's codes; a sixteenth of four values' codes; in two wavefronts a key's or value's scales.
+    const int k_key = tid >> 2, k_part = tid & 3;
+    const int v_slot = tid & 15, v_run = tid >> 4;  // run: keys 4 v_run .. + 3, that is 16 t + 8 high + 4 half + 0 .. 3
+    const int v_t = v_run >> 2, v_high = v_run >> 1 & 1, v_half = v_run & 1;
+    const int s_key = tid & 63;
+    uint32_t kc[kPart / 4], vc[4][(kSlot + 31) / 32];
+    struct __attribute__((packed)) Groups { T v[G]; } sc, bc;
+    bool s_real;
+    auto request = [&](int s0) __attribute__((always_inline)) {
+        struct Words { uint32_t w[kPart / 4]; };
+        const Words w = *reinterpret_cast<const Words *>(reinterpret_cast<const uint8_t *>(a.kw) + row_of(s0 + k_key) * kRowBytes + k_part * kPart);
+#pragma unroll
+        for (int i = 0; i < kPart / 4; i++) kc[i] = w.w[i];
+        const uint8_t *rows = reinterpret_cast<const uint8_t *>(a.vw) + row_of(s0 + 4 * v_run) * kRowBytes;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if constexpr (kSlot == 64) {
+                const uint2 v = *reinterpret_cast<const uint2 *>(rows + j * kRowBytes + 8 * v_slot);
+                vc[j][0] = v.x, vc[j][1] = v.y;
+            } else if constexpr (kSlot == 32) {
+                vc[j][0] = *reinterpret_cast<const uint32_t *>(rows + j * kRowBytes + 4 * v_slot);
+            } else {
+                vc[j][0] = *reinterpret_cast<const uint16_t *>(rows + j * kRowBytes + 2 * v_slot);
+            }
+        }
+        if (wave < 2) {
+            const int64_t row = row_of(s0 + s_key) * G;
+            sc = *reinterpret_cast<const Groups *>((wave == 0 ? a.ks : a.vs) + row);
+            bc = *reinterpret_cast<const Groups *>((wave == 0 ? a.kb : a.vb) + row);
+            s_real = s0 + s_key < S;
+        }
+    };
+    // 16-byte places are exchanged within their kilobyte so that neither side meets its own banks: a quarter's key with the quarter, a
+    // value's row with its block and the upper half of the rows.
+    auto expand = [&](Stage &to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < kChunks; j++) {
+            const int c = kChunks * k_part + j;  // (step c / 2, half c % 2)
+            const uint4 v = key_codes<T, BITS>(constants, kc[BITS == 8 ? 2 * j : j], BITS == 8 ? kc[2 * j + 1] : 0u);
+            to.keys[k_key >> 5][c >> 1][(c & 1) * 32 + ((k_key & 31) ^ (k_part << 1))] = v;
+        }
+#pragma unroll
+        for (int i = 0; i < kVals; i++) {
+            const int d = kVals * v_slot + i, row = (d & 31) ^ ((d >> 5) | (d >> 4 & 1) * DB);
+            uint32_t p[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                if constexpr (BITS == 8) {
+                    const uint32_t x = vc[2 * j][i / 4] >> (8 * (i % 4)), y = vc[2 * j + 1][i / 4] >> (8 * (i % 4));
+                    p[j] = pack_exact((float)(x & 0xFFu), (float)(y & 0xFFu));
+                } else {
+                    const uint32_t both = __builtin_amdgcn_perm(vc[2 * j + 1][0], vc[2 * j][0], i >= 4 ? 0x07060302u : 0x05040100u);
+                    p[j] = two_codes(constants, both, 4 * (i & 3));
+                }
+            }
+            reinterpret_cast<uint2 *>(&to.values[v_t][d >> 5][v_half * 32 + row])[v_high] = make_uint2(p[0], p[1]);
+        }
+        // Keys: both with the softmax's scale, the bias without the codes' offset; values: the bias from the middle of the codes' range.  What lies
+        // behind the sequence's end may hold anything: zeros.
+        if (wave < 2) {
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                const float v = Elem<T>::load(sc.v, g), b = Elem<T>::load(bc.v, g);
+                to.scale[2 * wave][g][s_key] = !s_real ? 0.0f : wave == 0 ? v * scale : v;
+                to.scale[2 * wave + 1][g][s_key] = !s_real ? 0.0f : wave == 0 ? __builtin_fmaf(-kOff, v, b) * scale : __builtin_fmaf(kMiddle, v, b);
+            }
+        }
+    };
+
+    floatx16_t o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
+    float m = -1.0e30f, l = 0.0f, ones[G], accb[G];
+#pragma unroll
+    for (int g = 0; g < G; g++) ones[g] = accb[g] = 0.0f;
+
+    // 32 keys from s0 on, half `sub` of the stage.  MASKED: not all lines see all of them.
+    auto tile = [&](const Stage &from, int s0, int sub, auto masked_of) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked_of)::value;
+        const int base = 32 * sub + 4 * half;  // register e: key 8 (e / 4) + e % 4 from there
+        float x[16];
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            floatx16_t s;
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[e] = 0.0f;
+#pragma unroll
+            for (int k = g * GS; k < (g + 1) * GS; k++) s = qmf::Ops<T>::mfma(from.keys[sub][k][half * 32 + (col ^ (k * 2 / kChunks << 1))], qf[k], s);
+            const float sum = qsum[g];
+#pragma unroll
+            for (int q4 = 0; q4 < 4; q4++) {
+                const float4 sk = *reinterpret_cast<const float4 *>(&from.scale[0][g][base + 8 * q4]), bk = *reinterpret_cast<const float4 *>(&from.scale[1][g][base + 8 * q4]);
+                auto one = [&](int i, float ss, float bb) __attribute__((always_inline)) {
+                    const int e = 4 * q4 + i;
+                    const float v = g == 0 ? bb * sum : __builtin_fmaf(bb, sum, x[e]);
+                    x[e] = __builtin_fmaf(ss, s[e], v);
+                };
+                one(0, sk.x, bk.x), one(1, sk.y, bk.y), one(2, sk.z, bk.z), one(3, sk.w, bk.w);
+            }
+        }
+        uint32_t hidden = 0;
+        if constexpr (MASKED) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int key = s0 + 4 * half + 8 * (e >> 2) + (e & 3);
+                if (key > my_last || key < my_first) x[e] = -INFINITY, hidden |= 1u << e;
+            }
+        }
+        float top = x[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) top = fmaxf(top, x[e]);
+        // Rescaled only when a maximum has grown by more than 2^8: until then the weights are at most 2^8.
+        if (__any(top > m + 8.0f)) {
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float m_new = fmaxf(m, top), f = exp2f(m - m_new);
+            m = m_new, l *= f;
+#pragma unroll
+            for (int g = 0; g < G; g++) ones[g] *= f, accb[g] *= f;
+#pragma unroll
+            for (int d = 0; d < DB; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[d][e] *= f;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[e] = __builtin_amdgcn_exp2f(x[e] - m), l += x[e];
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            uint32_t p[TP][8];
+#pragma unroll
+            for (int q4 = 0; q4 < 4; q4++) {
+                float4 sv = *reinterpret_cast<const float4 *>(&from.scale[2][g][base + 8 * q4]), bv = *reinterpret_cast<const float4 *>(&from.scale[3][g][base + 8 * q4]);
+                auto one = [&](int i, float &ss, float bb) __attribute__((always_inline)) {
+                    const int e = 4 * q4 + i;
+                    if (MASKED && (hidden >> e & 1) != 0) ss = bb = 0.0f;
+                    accb[g] = __builtin_fmaf(x[e], bb, accb[g]);
+                    ss *= x[e];
+                };
+                one(0, sv.x, bv.x), one(1, sv.y, bv.y), one(2, sv.z, bv.z), one(3, sv.w, bv.w);
+                uint32_t t[TP];
+                split_pair<TP>(sv.x, sv.y, t);
+#pragma unroll
+                for (int i = 0; i < TP; i++) p[i][2 * q4] = t[i];
+                split_pair<TP>(sv.z, sv.w, t);
+#pragma unroll
+                for (int i = 0; i < TP; i++) p[i][2 * q4 + 1] = t[i];
+            }
+            typedef __bf16 pair_t __attribute__((ext_vector_type(2)));
+            const pair_t one2 = {(__bf16)1.0f, (__bf16)1.0f};
+#pragma unroll
+            for (int i = 0; i < TP; i++)
+#pragma unroll
+                for (int w = 0; w < 8; w++) ones[g] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair_t, p[i][w]), one2, ones[g], false);
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int d = g * DB / G; d < g * DB / G + GB; d++) {
+                    const uint4 v = from.values[2 * sub + t][d][half * 32 + (col ^ (d | (col >> 4) * DB))];
+#pragma unroll
+                    for (int i = 0; i < TP; i++) o[d] = qmf::Ops<bf16_t>::mfma(v, make_uint4(p[i][4 * t], p[i][4 * t + 1], p[i][4 * t + 2], p[i][4 * t + 3]), o[d]);
+                }
+        }
+    };
+
+    if (s_begin < s_end) {
+        request(s_begin);
+        expand(stages[0]);
+    }
+    __syncthreads();
+    int at = 0;
+    for (int s0 = s_begin; s0 < s_end; s0 += kStageKeys) {
+        const bool more = s0 + kStageKeys < s_end;
+        if (more) request(s0 + kStageKeys);
+#pragma unroll
+        for (int sub = 0; sub < 2; sub++) {
+            const int k0 = s0 + 32 * sub;
+            if (k0 > any_last || k0 >= s_end || k0 + 31 < any_first) continue;  // (uniform in the wavefront)
+            if (k0 + 31 > all_last || k0 < all_first || k0 + 31 >= S) tile(stages[at], k0, sub, std::true_type{});
+            else tile(stages[at], k0, sub, std::false_type{});
+        }
+        if (more) expand(stages[at ^ 1]);
+        __syncthreads();
+        at ^= 1;
+    }
+    l += __shfl_xor(l, 32);
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        ones[g] += __shfl_xor(ones[g], 32), accb[g] += __shfl_xor(accb[g], 32);
+        accb[g] = __builtin_fmaf(-(kValueOff + kMiddle), ones[g], accb[g]);  // (the operands and kValueOff + kMiddle went through the same weights)
+    }
+    if (!live) return;
+    const bool whole = item.splits == 1;
+    float inv = 1.0f;
+    float *state = nullptr;  // of this line and split: maximum, denominator, weighted sums
+    if (whole) {
+        float denom = l, f = 1.0f;
+        if (a.sinks != nullptr) {
+            const float sink = Elem<T>::load(a.sinks, my_head) * kLog2e, top = fmaxf(m, sink);
+            f = exp2f(m - top), denom = denom * f + exp2f(sink - top);
+        }
+        inv = denom == 0.0f ? 0.0f : f / denom;  // (a row that sees nothing: zeros)
+    } else {
+        state = a.states + ((int64_t)item.slot * kPromptLines + wave * 32 + col) * (D + 2);
+        if (half == 0) *reinterpret_cast<float2 *>(state) = make_float2(m, l);
+    }
+    T *out = a.out + (int64_t)(item.s.start + my_row) * a.out_strides[0] + (int64_t)my_head * a.out_strides[1];
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; q4++) {
+            const int c = 32 * d + 8 * q4 + 4 * half;
+            const float b = accb[d * G / DB];
+            const float v0 = o[d][4 * q4] + b, v1 = o[d][4 * q4 + 1] + b, v2 = o[d][4 * q4 + 2] + b, v3 = o[d][4 * q4 + 3] + b;
+            if (whole) {
+                struct __attribute__((packed)) Four { uint32_t w[2]; };
+                *reinterpret_cast<Four *>(out + c) = Four{{qmf::Ops<T>::pack(v0 * inv, v1 * inv), qmf::Ops<T>::pack(v2 * inv, v3 * inv)}};
+            } else {
+                *reinterpret_cast<float2 *>(state + 2 + c) = make_float2(v0, v1);
+                *reinterpret_cast<float2 *>(state + 4 + c) = make_float2(v2, v3);
+            }
+        }
+}
+
+template <typename T, int BITS>
+int32_t launch_prompt_bits(const RowsArgs<T> &a, const nvq_paged_desc &c, uint32_t grid, hipStream_t s) {
+#define NVQ_PROMPT(D, G) hipLaunchKernelGGL((paged_prompt_kernel<T, BITS, D, G>), dim3(grid), dim3(64 * kWaves), 0, s, a, a.batch.place.table)
+    if (c.head_dim == 64 && c.group_size == 32) NVQ_PROMPT(64, 2);
+    else if (c.head_dim == 64) NVQ_PROMPT(64, 1);
+    else if (c.group_size == 32) NVQ_PROMPT(128, 4);
+    else if (c.group_size == 64) NVQ_PROMPT(128, 2);
+    else NVQ_PROMPT(128, 1);
+#undef NVQ_PROMPT
+    NVQ_LAUNCH_CHECK("paged_attention");
+    return NVQ_OK;
+}
+
+template <typename T>
+int32_t launch_prompt(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const PagedLaunch &r, hipStream_t s) {
+    const RowsArgs<T> a = rows_args<T>(d, o, r);
+    const int32_t rc = d.cache.bits == 4 ? launch_prompt_bits<T, 4>(a, d.cache, r.grid, s) : launch_prompt_bits<T, 8>(a, d.cache, r.grid, s);
+    if (rc != NVQ_OK || r.merge_units == 0) return rc;
+    return d.cache.head_dim == 64 ? launch_merge<T, 64, kPromptLines, 1, 1>(a, r, s) : launch_merge<T, 128, kPromptLines, 1, 1>(a, r, s);
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace nvq

@@ -4,7 +4,7 @@
 namespace nvq {
 namespace paged {
 
-int32_t launch_rows_bf16(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const RowsLaunch &r, hipStream_t s) {
+int32_t launch_rows_bf16(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const PagedLaunch &r, hipStream_t s) {
     return launch_rows<bf16_t>(d, o, r, s);
 }
 

@@ -356,26 +356,27 @@ __global__ void __launch_bounds__(64 * kWaves, (rows_blocks<T, G>())) paged_rows
     }
 }
 
-// The splits of a line merged.  Block: a line of a unit; its wavefronts take the splits in turn, eight loads under way at a time, and
-// add up through LDS.
-template <typename T, int D, int R>
+// The splits of a line merged, by WAVES wavefronts, which take them in turn, eight loads under way at a time, and add up through LDS.  Block:
+// 4 / WAVES lines of a unit.
+template <typename T, int D, int LINES, int KIND, int WAVES>
 __global__ void __launch_bounds__(64 * kWaves) paged_merge_kernel(const RowsArgs<T> a) {
     constexpr int V = D / 64;
     __shared__ float sums[kWaves][D], tops[kWaves], totals[kWaves];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), first = wave / WAVES * WAVES;
     PagedItem item;
-    if (!paged_item<R, 0, true>(a.batch, lane, blockIdx.x, item)) return;
-    const int rep = a.batch.rep, ln = blockIdx.y, rr = item.part * R + ln;
-    if (rr >= item.s.rows * rep) return;
-    {
-        const int64_t stride = (int64_t)a.batch.key_heads * R * (D + 2);  // of a split's states
-        const float *src = a.states + ((int64_t)item.slot * R + ln) * (D + 2);
-        float top = -1.0e30f, total = 0.0f, sum[V] = {};
-        for (int z0 = wave; z0 < item.splits; z0 += 8 * kWaves) {
+    if (!paged_item<LINES, KIND, true>(a.batch, lane, blockIdx.x, item)) return;
+    const int rep = a.batch.rep, ln = blockIdx.y * (kWaves / WAVES) + wave / WAVES;
+    const int part = KIND == 0 ? item.part : item.s.parts - 1 - item.part, line = part * LINES + ln;  // (the kernel of many lines counts from the last)
+    const bool real = ln < LINES && line < item.s.rows * rep;
+    float top = -1.0e30f, total = 0.0f, sum[V] = {};
+    if (real) {
+        const int64_t stride = (int64_t)a.batch.key_heads * LINES * (D + 2);  // of a split's states
+        const float *src = a.states + ((int64_t)item.slot * LINES + ln) * (D + 2);
+        for (int z0 = wave - first; z0 < item.splits; z0 += 8 * WAVES) {
             float m[8], d[8], v[8][V];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const int z = z0 + kWaves * i < item.splits ? z0 + kWaves * i : z0;
+                const int z = z0 + WAVES * i < item.splits ? z0 + WAVES * i : z0;
                 const float *state = src + z * stride;
                 m[i] = state[0], d[i] = state[1];
 #pragma unroll
@@ -390,60 +391,82 @@ __global__ void __launch_bounds__(64 * kWaves) paged_merge_kernel(const RowsArgs
             for (int e = 0; e < V; e++) sum[e] *= f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float w = z0 + kWaves * i < item.splits ? exp2f(m[i] - top) : 0.0f;
+                const float w = z0 + WAVES * i < item.splits ? exp2f(m[i] - top) : 0.0f;
                 total = __builtin_fmaf(d[i], w, total);
 #pragma unroll
                 for (int e = 0; e < V; e++) sum[e] = __builtin_fmaf(v[i][e], w, sum[e]);
             }
         }
+    }
+    if constexpr (WAVES > 1) {
         tops[wave] = top, totals[wave] = total;
 #pragma unroll
         for (int e = 0; e < V; e++) sums[wave][V * lane + e] = sum[e];
-    }
-    __syncthreads();
-    if (tid < D) {
-        const int head = item.head * rep + rr % rep;
-        float top = -1.0e30f, total = 0.0f, sum = 0.0f;
+        __syncthreads();
+        if (wave != first) return;
+        float most = top;
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) top = fmaxf(top, tops[w]);
-        const float sink = a.sinks != nullptr ? Elem<T>::load(a.sinks, head) * kLog2e : -INFINITY;
-        top = fmaxf(top, sink);
+        for (int w = 0; w < WAVES; w++) most = fmaxf(most, tops[first + w]);
+        const float f = exp2f(top - most);
+        top = most, total *= f;
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            const float f = exp2f(tops[w] - top);
-            total = __builtin_fmaf(totals[w], f, total), sum = __builtin_fmaf(sums[w][tid], f, sum);
+        for (int e = 0; e < V; e++) sum[e] *= f;
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) {
+            const float g = exp2f(tops[first + w] - top);
+            total = __builtin_fmaf(totals[first + w], g, total);
+#pragma unroll
+            for (int e = 0; e < V; e++) sum[e] = __builtin_fmaf(sums[first + w][V * lane + e], g, sum[e]);
         }
-        total += exp2f(sink - top);
-        Elem<T>::store(a.out + (int64_t)(item.s.start + rr / rep) * a.out_strides[0] + (int64_t)head * a.out_strides[1], tid, total == 0.0f ? 0.0f : sum / total);
     }
+    if (!real) return;
+    const int head = item.head * rep + line % rep;
+    if (a.sinks != nullptr) {
+        const float sink = Elem<T>::load(a.sinks, head) * kLog2e, most = fmaxf(top, sink), f = exp2f(top - most);
+        total = __builtin_fmaf(total, f, exp2f(sink - most));
+#pragma unroll
+        for (int e = 0; e < V; e++) sum[e] *= f;
+    }
+    T *out = a.out + (int64_t)(item.s.start + line / rep) * a.out_strides[0] + (int64_t)head * a.out_strides[1];
+#pragma unroll
+    for (int e = 0; e < V; e++) Elem<T>::store(out, V * lane + e, total == 0.0f ? 0.0f : sum[e] / total);
 }
 
-template <typename T, int BITS, int D, int G>
-int32_t launch_rows_sized(const RowsArgs<T> &a, const RowsLaunch &r, hipStream_t s) {
-    hipLaunchKernelGGL((paged_rows_kernel<T, BITS, D, G>), dim3(r.grid), dim3(64 * kWaves), 0, s, a, a.batch.place.table);
-    NVQ_LAUNCH_CHECK("paged_attention");
-    if (r.merge_units > 0) {
-        hipLaunchKernelGGL((paged_merge_kernel<T, D, 16 / G>), dim3(r.merge_units, r.merge_lines), dim3(64 * kWaves), 0, s, a);
-        NVQ_LAUNCH_CHECK("paged_attention merge");
-    }
+template <typename T, int D, int LINES, int KIND, int WAVES>
+int32_t launch_merge(const RowsArgs<T> &a, const PagedLaunch &r, hipStream_t s) {
+    hipLaunchKernelGGL((paged_merge_kernel<T, D, LINES, KIND, WAVES>), dim3(r.merge_units, (r.merge_lines * WAVES + kWaves - 1) / kWaves), dim3(64 * kWaves), 0, s, a);
+    NVQ_LAUNCH_CHECK("paged_attention merge");
     return NVQ_OK;
 }
 
+template <typename T, int BITS, int D, int G>
+int32_t launch_rows_sized(const RowsArgs<T> &a, const PagedLaunch &r, hipStream_t s) {
+    hipLaunchKernelGGL((paged_rows_kernel<T, BITS, D, G>), dim3(r.grid), dim3(64 * kWaves), 0, s, a, a.batch.place.table);
+    NVQ_LAUNCH_CHECK("paged_attention");
+    return r.merge_units == 0 ? NVQ_OK : launch_merge<T, D, 16 / G, 0, kWaves>(a, r, s);
+}
+
 template <typename T, int BITS>
-int32_t launch_rows_bits(const RowsArgs<T> &a, const nvq_paged_desc &c, const RowsLaunch &r, hipStream_t s) {
+int32_t launch_rows_bits(const RowsArgs<T> &a, const nvq_paged_desc &c, const PagedLaunch &r, hipStream_t s) {
     if (c.head_dim == 64) return c.group_size == 32 ? launch_rows_sized<T, BITS, 64, 2>(a, r, s) : launch_rows_sized<T, BITS, 64, 1>(a, r, s);
     if (c.group_size == 32) return launch_rows_sized<T, BITS, 128, 4>(a, r, s);
     return c.group_size == 64 ? launch_rows_sized<T, BITS, 128, 2>(a, r, s) : launch_rows_sized<T, BITS, 128, 1>(a, r, s);
 }
 
 template <typename T>
-int32_t launch_rows(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const RowsLaunch &r, hipStream_t s) {
+RowsArgs<T> rows_args(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const PagedLaunch &r) {
     RowsArgs<T> a{};
     a.batch = r.batch;
     a.q = (const T *)o.q, a.ks = (const T *)o.ks, a.kb = (const T *)o.kb, a.vs = (const T *)o.vs, a.vb = (const T *)o.vb, a.sinks = (const T *)o.sinks;
-    a.kw = (const uint32_t *)o.kw, a.vw = (const uint32_t *)o.vw, a.out = (T *)o.out, a.states = (float *)o.workspace;
+    a.kw = (const uint32_t *)o.kw, a.vw = (const uint32_t *)o.vw, a.out = (T *)o.out, a.states = (float *)((char *)o.workspace + r.states);
     for (int i = 0; i < 2; i++) a.q_strides[i] = d.q_strides[i], a.out_strides[i] = d.out_strides[i];
     a.scale = d.scale;
+    return a;
+}
+
+template <typename T>
+int32_t launch_rows(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const PagedLaunch &r, hipStream_t s) {
+    const RowsArgs<T> a = rows_args<T>(d, o, r);
     return d.cache.bits == 4 ? launch_rows_bits<T, 4>(a, d.cache, r, s) : launch_rows_bits<T, 8>(a, d.cache, r, s);
 }
 

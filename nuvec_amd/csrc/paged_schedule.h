@@ -76,18 +76,22 @@ __device__ __forceinline__ PagedPlan paged_plan(const PagedBatch &a, int lane, c
         units += u, total += u * s.tiles;
     }
     units = wave_total(units), total = wave_total(total);
-    // (every unit's last item may be short: `units` of the target are left for them, half of it at most)
-    const int64_t left = a.target - units > a.target / 2 ? a.target - units : a.target / 2;
-    PagedPlan p;
-    const int64_t per = (total + left - 1) / left;
-    p.per = (int32_t)(per < kScheduleTiles ? kScheduleTiles : per < (1 << 26) ? per : 1 << 26);
-    p.items = 0;
+    // Every unit's last item may be short.  The shortest items of three whose number is within the target: none, half an item, or one of
+    // every unit left for that, half of the target at most.
+    PagedPlan p[3];
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+        const int64_t left = a.target - units * i / 2 > a.target / 2 ? a.target - units * i / 2 : a.target / 2, per = (total + left - 1) / left;
+        p[i].per = (int32_t)(per < kScheduleTiles ? kScheduleTiles : per < (1 << 26) ? per : 1 << 26), p[i].items = 0;
+    }
     for (int b0 = 0; b0 < a.sequences; b0 += 64) {
         const PagedSequence s = b0 == 0 ? first : paged_sequence<LINES, KIND>(a, b0 + lane);
-        p.items += s.parts * p.splits(s) * a.key_heads;
+#pragma unroll
+        for (int i = 0; i < 3; i++) p[i].items += s.parts * p[i].splits(s) * a.key_heads;
     }
-    p.items = wave_total(p.items);
-    return p;
+#pragma unroll
+    for (int i = 0; i < 3; i++) p[i].items = wave_total(p[i].items);
+    return p[0].items <= a.target ? p[0] : p[1].items <= a.target ? p[1] : p[2];
 }
 
 struct PagedItem {
