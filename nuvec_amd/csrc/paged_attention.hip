@@ -38,7 +38,7 @@ Kernel kernel_of(const nvq_paged_attention_desc &d, bool many) {
     Kernel k;
     k.lines = many ? kPromptLines : 16 / groups;
     k.target = (many || d.cache.dtype == NVQ_F32 || groups == 4 ? 2 : 3) * compute_units();
-    k.bytes = (size_t)(2 * (int64_t)k.target * k.lines * (d.cache.head_dim + 2)) * sizeof(float);
+    k.bytes = (size_t)(2 * (int64_t)k.target * k.lines * (d.cache.head_dim + 4)) * sizeof(float);
     return k;
 }
 

@@ -49,10 +49,13 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
     constexpr int kRowBytes = D * BITS / 8, kPart = kRowBytes / 4;     // a row; a quarter of one, a thread's share of the keys' codes
     constexpr int kChunks = D / 32, kVals = D / 16, kSlot = BITS * kVals;  // eight-code chunks of a quarter; values of a sixteenth and its bits
     constexpr float kOff = key_offset<T, BITS>, kValueOff = BITS == 4 ? 16.0f : 0.0f, kMiddle = 1 << (BITS - 1);
+    // Operands, 16 bytes a lane, with gaps: those that a quarter-wavefront writes at once, 2 keys of four pairs of steps, 16 sixteenths of a row's
+    // values, fall on different banks, and every address is one register and a constant.
     struct Stage {
-        uint4 keys[2][KS][64];          // [half of the tile][step][half of the step x key]
-        uint4 values[4][DB][64];        // [16 keys][block][half of the keys x value]
+        uint4 keys[2][KS][64 + 1];      // [half of the tile][step][half of the step x key]
+        uint4 values[4][DB][2 * 36 + 1];  // [16 keys][block][half of the keys: value, four places after the sixteenth]
         float scale[4][G][kStageKeys];  // of keys and what goes with it, of values and what goes with it (expand)
+        uint16_t wild[2][G][2];         // a bit for every key whose value's scale or bias is not finite
     };
     __shared__ Stage stages[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
@@ -70,14 +73,15 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
     int s_begin = split_begin, s_end = item.splits == 1 ? S : split_begin + item.per * kTile < S ? split_begin + item.per * kTile : S;
     if (last_of(b_last) + 1 < s_end) s_end = last_of(b_last) + 1;
     if (first_of(b_first) / kTile * kTile > s_begin) s_begin = first_of(b_first) / kTile * kTile;
+    s_begin = uniform(s_begin), s_end = uniform(s_end);
     // the wavefront's lines
     const int r0 = part * kPromptLines + wave * 32, r = r0 + col;
     const bool live = r < lines;
     const int my_row = (live ? r : lines - 1) / rep, my_head = hk * rep + (live ? r % rep : 0);
     const int my_last = last_of(my_row), my_first = first_of(my_row);
     const int w_first = (r0 < lines ? r0 : lines - 1) / rep, w_last = (r0 + 31 < lines ? r0 + 31 : lines - 1) / rep;
-    const int all_last = last_of(w_first), all_first = first_of(w_last);                       // keys up to / from which all of them see
-    const int any_last = r0 < lines ? last_of(w_last) : -1, any_first = first_of(w_first);  // and any does
+    const int all_last = uniform(last_of(w_first)), all_first = uniform(first_of(w_last));                       // keys up to / from which all of them see
+    const int any_last = uniform(r0 < lines ? last_of(w_last) : -1), any_first = uniform(first_of(w_first));  // and any does
 
     uint4 qf[KS];
     float qsum[G];
@@ -101,59 +105,56 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
     // ── staging ──
     const CodeConstants<4> constants;
     const float scale = a.scale * kLog2e;
-    const int shift = a.batch.place.page_shift, last_column = S > 0 ? (S - 1) >> shift : 0;
-    const int32_t *columns = table + item.b * a.batch.place.stride;
-    // The row (of all pages and heads) of position `at`, which lies in a page of the sequence or behind its end.
-    auto row_of = [&](int at) __attribute__((always_inline)) {
-        const int column = at >> shift;
-        const int64_t id = columns[column < last_column ? column : last_column], pages = a.batch.place.pages;
-        const int64_t page = id < 0 ? 0 : id < pages ? id : pages - 1;
-        return ((page * a.batch.key_heads + hk) << shift) + (at & ((1 << shift) - 1));
+    // A wavefront's 16 of the tile's 64 keys lie in one page: its place is a scalar, whose page is looked up a tile ahead.
+    const int shift = a.batch.place.page_shift, last_column = S > 0 ? (S - 1) >> shift : 0, pages = (int)a.batch.place.pages;
+    typedef const int32_t __attribute__((address_space(4))) *Columns;  // (constant memory: scalar loads)
+    const Columns columns = (Columns)(uintptr_t)table + item.b * a.batch.place.stride;
+    auto look_up = [&](int s0) __attribute__((always_inline)) {
+        const int column = (s0 + 16 * wave) >> shift;
+        return columns[uniform(column < last_column ? column : last_column)];  // (a tile behind the end reads the last page)
     };
-    // Of 64 keys this thread's: a quarter of a key's codes; a sixteenth of four values' codes; in two wavefronts a key's or value's scales.
-    const int k_key = tid >> 2, k_part = tid & 3;
-    const int v_slot = tid & 15, v_run = tid >> 4;  // run: keys 4 v_run .. + 3, that is 16 t + 8 high + 4 half + 0 .. 3
-    const int v_t = v_run >> 2, v_high = v_run >> 1 & 1, v_half = v_run & 1;
-    const int s_key = tid & 63;
+    // This lane's: a quarter of a key's codes; a sixteenth of four values' codes (keys 8 high + 4 half + 0 .. 3 of the sixteen); half of the lanes: the
+    // scales and biases of a key or of a value.
+    const int k_key = lane >> 2, k_part = lane & 3;
+    const int v_slot = lane & 15, v_run = lane >> 4, v_high = v_run >> 1, v_half = v_run & 1;
+    const int s_key = lane & 15, s_values = lane >> 4 & 1;
     uint32_t kc[kPart / 4], vc[4][(kSlot + 31) / 32];
     struct __attribute__((packed)) Groups { T v[G]; } sc, bc;
     bool s_real;
-    auto request = [&](int s0) __attribute__((always_inline)) {
+    auto request = [&](int32_t id, int s0) __attribute__((always_inline)) {
+        const int32_t page = id < 0 ? 0 : id < pages ? id : pages - 1;
+        const int64_t row = (((int64_t)page * a.batch.key_heads + hk) << shift) + ((s0 + 16 * wave) & ((1 << shift) - 1));
         struct Words { uint32_t w[kPart / 4]; };
-        const Words w = *reinterpret_cast<const Words *>(reinterpret_cast<const uint8_t *>(a.kw) + row_of(s0 + k_key) * kRowBytes + k_part * kPart);
+        const Words w = *reinterpret_cast<const Words *>(reinterpret_cast<const uint8_t *>(a.kw) + row * kRowBytes + (uint32_t)(lane * kPart));
 #pragma unroll
         for (int i = 0; i < kPart / 4; i++) kc[i] = w.w[i];
-        const uint8_t *rows = reinterpret_cast<const uint8_t *>(a.vw) + row_of(s0 + 4 * v_run) * kRowBytes;
+        const uint8_t *rows = reinterpret_cast<const uint8_t *>(a.vw) + row * kRowBytes;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
+            const uint8_t *at = rows + (uint32_t)(4 * v_run * kRowBytes + kSlot / 8 * v_slot) + j * kRowBytes;
             if constexpr (kSlot == 64) {
-                const uint2 v = *reinterpret_cast<const uint2 *>(rows + j * kRowBytes + 8 * v_slot);
+                const uint2 v = *reinterpret_cast<const uint2 *>(at);
                 vc[j][0] = v.x, vc[j][1] = v.y;
             } else if constexpr (kSlot == 32) {
-                vc[j][0] = *reinterpret_cast<const uint32_t *>(rows + j * kRowBytes + 4 * v_slot);
+                vc[j][0] = *reinterpret_cast<const uint32_t *>(at);
             } else {
-                vc[j][0] = *reinterpret_cast<const uint16_t *>(rows + j * kRowBytes + 2 * v_slot);
+                vc[j][0] = *reinterpret_cast<const uint16_t *>(at);
             }
         }
-        if (wave < 2) {
-            const int64_t row = row_of(s0 + s_key) * G;
-            sc = *reinterpret_cast<const Groups *>((wave == 0 ? a.ks : a.vs) + row);
-            bc = *reinterpret_cast<const Groups *>((wave == 0 ? a.kb : a.vb) + row);
-            s_real = s0 + s_key < S;
-        }
+        const T *ss = s_values != 0 ? a.vs : a.ks, *bb = s_values != 0 ? a.vb : a.kb;
+        sc = *reinterpret_cast<const Groups *>(ss + row * G + s_key * G), bc = *reinterpret_cast<const Groups *>(bb + row * G + s_key * G);
+        s_real = s0 + 16 * wave + s_key < S;
     };
-    // 16-byte places are exchanged within their kilobyte so that neither side meets its own banks: a quarter's key with the quarter, a
-    // value's row with its block and the upper half of the rows.
     auto expand = [&](Stage &to) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < kChunks; j++) {
             const int c = kChunks * k_part + j;  // (step c / 2, half c % 2)
             const uint4 v = key_codes<T, BITS>(constants, kc[BITS == 8 ? 2 * j : j], BITS == 8 ? kc[2 * j + 1] : 0u);
-            to.keys[k_key >> 5][c >> 1][(c & 1) * 32 + ((k_key & 31) ^ (k_part << 1))] = v;
+            to.keys[wave >> 1][c >> 1][(c & 1) * 32 + 16 * (wave & 1) + k_key] = v;
         }
 #pragma unroll
         for (int i = 0; i < kVals; i++) {
-            const int d = kVals * v_slot + i, row = (d & 31) ^ ((d >> 5) | (d >> 4 & 1) * DB);
+            const int d = kVals * v_slot + i, row = (d & 31) + (d >> 2 & 4);
             uint32_t p[2];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
@@ -165,16 +166,20 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
                     p[j] = two_codes(constants, both, 4 * (i & 3));
                 }
             }
-            reinterpret_cast<uint2 *>(&to.values[v_t][d >> 5][v_half * 32 + row])[v_high] = make_uint2(p[0], p[1]);
+            reinterpret_cast<uint2 *>(&to.values[wave][d >> 5][v_half * 36 + row])[v_high] = make_uint2(p[0], p[1]);
         }
         // Keys: both with the softmax's scale, the bias without the codes' offset; values: the bias from the middle of the codes' range.  What lies
         // behind the sequence's end may hold anything: zeros.
-        if (wave < 2) {
+        if (lane < 32) {
 #pragma unroll
             for (int g = 0; g < G; g++) {
                 const float v = Elem<T>::load(sc.v, g), b = Elem<T>::load(bc.v, g);
-                to.scale[2 * wave][g][s_key] = !s_real ? 0.0f : wave == 0 ? v * scale : v;
-                to.scale[2 * wave + 1][g][s_key] = !s_real ? 0.0f : wave == 0 ? __builtin_fmaf(-kOff, v, b) * scale : __builtin_fmaf(kMiddle, v, b);
+                const float own = s_values != 0 ? v : v * scale, with = s_values != 0 ? __builtin_fmaf(kMiddle, v, b) : __builtin_fmaf(-kOff, v, b) * scale;
+                const bool wild = s_values != 0 && !(fabsf(with) < INFINITY && fabsf(own) < INFINITY), used = s_real && !wild;
+                to.scale[2 * s_values][g][16 * wave + s_key] = used ? own : 0.0f;
+                to.scale[2 * s_values + 1][g][16 * wave + s_key] = used ? with : 0.0f;
+                const uint64_t all = __ballot(wild && s_real);
+                if (lane == 0) to.wild[wave >> 1][g][wave & 1] = (uint16_t)(all >> 16);
             }
         }
     };
@@ -188,9 +193,8 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
 #pragma unroll
     for (int g = 0; g < G; g++) ones[g] = accb[g] = 0.0f;
 
-    // 32 keys from s0 on, half `sub` of the stage.  MASKED: not all lines see all of them.
-    auto tile = [&](const Stage &from, int s0, int sub, auto masked_of) __attribute__((always_inline)) {
-        constexpr bool MASKED = decltype(masked_of)::value;
+    // 32 keys from s0 on, half `sub` of the stage.  (One piece of code: a second for masked tiles cost forty registers, which there are not.)
+    auto tile = [&](const Stage &from, int s0, int sub, bool masked) __attribute__((always_inline)) {
         const int base = 32 * sub + 4 * half;  // register e: key 8 (e / 4) + e % 4 from there
         float x[16];
 #pragma unroll
@@ -199,7 +203,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
 #pragma unroll
             for (int e = 0; e < 16; e++) s[e] = 0.0f;
 #pragma unroll
-            for (int k = g * GS; k < (g + 1) * GS; k++) s = qmf::Ops<T>::mfma(from.keys[sub][k][half * 32 + (col ^ (k * 2 / kChunks << 1))], qf[k], s);
+            for (int k = g * GS; k < (g + 1) * GS; k++) s = qmf::Ops<T>::mfma(from.keys[sub][k][lane], qf[k], s);
             const float sum = qsum[g];
 #pragma unroll
             for (int q4 = 0; q4 < 4; q4++) {
@@ -212,12 +216,12 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
                 one(0, sk.x, bk.x), one(1, sk.y, bk.y), one(2, sk.z, bk.z), one(3, sk.w, bk.w);
             }
         }
-        uint32_t hidden = 0;
-        if constexpr (MASKED) {
+        if (masked) {
+            asm volatile("");  // (a branch: as selects it would cost every tile)
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 const int key = s0 + 4 * half + 8 * (e >> 2) + (e & 3);
-                if (key > my_last || key < my_first) x[e] = -INFINITY, hidden |= 1u << e;
+                if (key > my_last || key < my_first || key >= S) x[e] = -INFINITY;
             }
         }
         float top = x[0];
@@ -237,6 +241,18 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
         }
 #pragma unroll
         for (int e = 0; e < 16; e++) x[e] = __builtin_amdgcn_exp2f(x[e] - m), l += x[e];
+        // Values whose scales are not finite were made zeros, so that lines that do not see them stay clean: those that do get a NaN.
+        uint32_t wild[G], any = 0;
+#pragma unroll
+        for (int g = 0; g < G; g++) wild[g] = *reinterpret_cast<const uint32_t *>(from.wild[sub][g]), any |= wild[g];
+        if (uniform((int32_t)any) != 0) {
+            asm volatile("");
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if (x[e] != 0.0f && (wild[g] >> (4 * half + 8 * (e >> 2) + (e & 3)) & 1) != 0) accb[g] = NAN;
+        }
 #pragma unroll
         for (int g = 0; g < G; g++) {
             uint32_t p[TP][8];
@@ -245,7 +261,6 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
                 float4 sv = *reinterpret_cast<const float4 *>(&from.scale[2][g][base + 8 * q4]), bv = *reinterpret_cast<const float4 *>(&from.scale[3][g][base + 8 * q4]);
                 auto one = [&](int i, float &ss, float bb) __attribute__((always_inline)) {
                     const int e = 4 * q4 + i;
-                    if (MASKED && (hidden >> e & 1) != 0) ss = bb = 0.0f;
                     accb[g] = __builtin_fmaf(x[e], bb, accb[g]);
                     ss *= x[e];
                 };
@@ -268,28 +283,31 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int d = g * DB / G; d < g * DB / G + GB; d++) {
-                    const uint4 v = from.values[2 * sub + t][d][half * 32 + (col ^ (d | (col >> 4) * DB))];
+                    const uint4 v = from.values[2 * sub + t][d][half * 36 + col + (col >> 2 & 4)];
 #pragma unroll
                     for (int i = 0; i < TP; i++) o[d] = qmf::Ops<bf16_t>::mfma(v, make_uint4(p[i][4 * t], p[i][4 * t + 1], p[i][4 * t + 2], p[i][4 * t + 3]), o[d]);
                 }
         }
     };
 
+    int32_t next = 0;
     if (s_begin < s_end) {
-        request(s_begin);
+        const int32_t first = look_up(s_begin);
+        next = look_up(s_begin + kStageKeys);
+        request(first, s_begin);
         expand(stages[0]);
     }
     __syncthreads();
     int at = 0;
     for (int s0 = s_begin; s0 < s_end; s0 += kStageKeys) {
         const bool more = s0 + kStageKeys < s_end;
-        if (more) request(s0 + kStageKeys);
-#pragma unroll
+        if (more) request(next, s0 + kStageKeys);
+        next = look_up(s0 + 2 * kStageKeys);
+#pragma unroll 1
         for (int sub = 0; sub < 2; sub++) {
             const int k0 = s0 + 32 * sub;
             if (k0 > any_last || k0 >= s_end || k0 + 31 < any_first) continue;  // (uniform in the wavefront)
-            if (k0 + 31 > all_last || k0 < all_first || k0 + 31 >= S) tile(stages[at], k0, sub, std::true_type{});
-            else tile(stages[at], k0, sub, std::false_type{});
+            tile(stages[at], k0, sub, k0 + 31 > all_last || k0 < all_first || k0 + 31 >= S);
         }
         if (more) expand(stages[at ^ 1]);
         __syncthreads();
@@ -313,7 +331,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
         }
         inv = denom == 0.0f ? 0.0f : f / denom;  // (a row that sees nothing: zeros)
     } else {
-        state = a.states + ((int64_t)item.slot * kPromptLines + wave * 32 + col) * (D + 2);
+        state = a.states + ((int64_t)item.slot * kPromptLines + wave * 32 + col) * kState<D>;
         if (half == 0) *reinterpret_cast<float2 *>(state) = make_float2(m, l);
     }
     T *out = a.out + (int64_t)(item.s.start + my_row) * a.out_strides[0] + (int64_t)my_head * a.out_strides[1];
@@ -328,10 +346,63 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
                 struct __attribute__((packed)) Four { uint32_t w[2]; };
                 *reinterpret_cast<Four *>(out + c) = Four{{qmf::Ops<T>::pack(v0 * inv, v1 * inv), qmf::Ops<T>::pack(v2 * inv, v3 * inv)}};
             } else {
-                *reinterpret_cast<float2 *>(state + 2 + c) = make_float2(v0, v1);
-                *reinterpret_cast<float2 *>(state + 4 + c) = make_float2(v2, v3);
+                *reinterpret_cast<float4 *>(state + 4 + c) = make_float4(v0, v1, v2, v3);
             }
         }
+}
+
+// The splits of many lines merged: D / 4 threads a line, four splits' loads under way at a time.
+template <typename T, int D>
+__global__ void __launch_bounds__(64 * kWaves) paged_merge_many_kernel(const RowsArgs<T> a) {
+    constexpr int kThreads = D / 4, kLines = 64 * kWaves / kThreads;
+    PagedItem item;
+    if (!paged_item<kPromptLines, 1, true>(a.batch, threadIdx.x & 63, blockIdx.x, item)) return;
+    const int rep = a.batch.rep, ln = blockIdx.y * kLines + (int)threadIdx.x / kThreads, at = (int)threadIdx.x % kThreads * 4;
+    const int line = (item.s.parts - 1 - item.part) * kPromptLines + ln;  // (items count the parts from the last)
+    if (line >= item.s.rows * rep) return;
+    const int64_t stride = (int64_t)a.batch.key_heads * kPromptLines * kState<D>;  // of a split's states
+    const float *src = a.states + ((int64_t)item.slot * kPromptLines + ln) * kState<D>;
+    float top = -1.0e30f, total = 0.0f;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int z0 = 0; z0 < item.splits; z0 += 4) {
+        float2 m[4];
+        float4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float *state = src + (z0 + i < item.splits ? z0 + i : z0) * stride;
+            m[i] = *reinterpret_cast<const float2 *>(state), v[i] = *reinterpret_cast<const float4 *>(state + 4 + at);
+        }
+        float most = top;
+#pragma unroll
+        for (int i = 0; i < 4; i++) most = fmaxf(most, m[i].x);
+        const float f = exp2f(top - most);
+        top = most, total *= f, sum.x *= f, sum.y *= f, sum.z *= f, sum.w *= f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float w = z0 + i < item.splits ? exp2f(m[i].x - top) : 0.0f;
+            total = __builtin_fmaf(m[i].y, w, total);
+            sum.x = __builtin_fmaf(v[i].x, w, sum.x), sum.y = __builtin_fmaf(v[i].y, w, sum.y);
+            sum.z = __builtin_fmaf(v[i].z, w, sum.z), sum.w = __builtin_fmaf(v[i].w, w, sum.w);
+        }
+    }
+    const int head = item.head * rep + line % rep;
+    float inv = 1.0f;
+    if (a.sinks != nullptr) {
+        const float sink = Elem<T>::load(a.sinks, head) * kLog2e, most = fmaxf(top, sink);
+        inv = exp2f(top - most), total = __builtin_fmaf(total, inv, exp2f(sink - most));
+    }
+    inv = total == 0.0f ? 0.0f : inv / total;
+    struct __attribute__((packed)) Four { uint32_t w[2]; };
+    *reinterpret_cast<Four *>(a.out + (int64_t)(item.s.start + line / rep) * a.out_strides[0] + (int64_t)head * a.out_strides[1] + at) =
+        Four{{qmf::Ops<T>::pack(sum.x * inv, sum.y * inv), qmf::Ops<T>::pack(sum.z * inv, sum.w * inv)}};
+}
+
+template <typename T, int D>
+int32_t launch_merge_many(const RowsArgs<T> &a, const PagedLaunch &r, hipStream_t s) {
+    constexpr int kLines = 64 * kWaves / (D / 4);
+    hipLaunchKernelGGL((paged_merge_many_kernel<T, D>), dim3(r.merge_units, (r.merge_lines + kLines - 1) / kLines), dim3(64 * kWaves), 0, s, a);
+    NVQ_LAUNCH_CHECK("paged_attention merge");
+    return NVQ_OK;
 }
 
 template <typename T, int BITS>
@@ -352,7 +423,7 @@ int32_t launch_prompt(const nvq_paged_attention_desc &d, const PagedAttentionOpe
     const RowsArgs<T> a = rows_args<T>(d, o, r);
     const int32_t rc = d.cache.bits == 4 ? launch_prompt_bits<T, 4>(a, d.cache, r.grid, s) : launch_prompt_bits<T, 8>(a, d.cache, r.grid, s);
     if (rc != NVQ_OK || r.merge_units == 0) return rc;
-    return d.cache.head_dim == 64 ? launch_merge<T, 64, kPromptLines, 1, 1>(a, r, s) : launch_merge<T, 128, kPromptLines, 1, 1>(a, r, s);
+    return d.cache.head_dim == 64 ? launch_merge_many<T, 64>(a, r, s) : launch_merge_many<T, 128>(a, r, s);
 }
 
 }  // namespace

@@ -35,20 +35,18 @@ struct RowsArgs {
     const T *q, *ks, *kb, *vs, *vb, *sinks;
     const uint32_t *kw, *vw;
     T *out;
-    float *states;  // [slots][LINES][D + 2]: maximum of the base-2 scores, denominator, D weighted sums
+    float *states;  // [slots][LINES][kState<D>]: maximum of the base-2 scores, denominator, two unused, D weighted sums
     int64_t q_strides[2], out_strides[2];
     float scale;
 };
 
 namespace {
 
-// Blocks on a compute unit.
+template <int D> constexpr int kState = D + 4;  // (rows of 16 bytes)
+
+// Blocks on a compute unit.  Three need 168 registers at most: heads of 128 read their queries from LDS in every tile there.
 template <typename T, int G> constexpr int rows_blocks() { return sizeof(T) == 4 || G == 4 ? 2 : 3; }
-template <typename T, int BITS, int D, int G>
-constexpr bool rows_queries_in_lds() {
-    constexpr bool f16 = Elem<T>::code != 10;
-    return rows_blocks<T, G>() == 3 && D == 128 && (G == 2 ? BITS == 8 || f16 : BITS == 8 && f16);
-}
+template <typename T, int D, int G> constexpr bool rows_queries_in_lds() { return rows_blocks<T, G>() == 3 && D == 128; }
 template <typename T> constexpr int weight_terms() { return sizeof(T) == 4 ? 3 : Elem<T>::code == NVQ_BF16 ? 1 : 2; }
 
 template <typename T, int BITS, int D, int G>
@@ -61,7 +59,7 @@ __global__ void __launch_bounds__(64 * kWaves, (rows_blocks<T, G>())) paged_rows
     constexpr uint32_t kOne = BITS == 8 ? 0x43004300u : 0x41C041C0u;  // two of kOff + kMiddle: 128, 24 (at 8 and 4 bits)
     __shared__ float part[kWaves][R][D + 1];
     __shared__ float wave_m[kWaves][R], wave_l[kWaves][R];
-    constexpr bool kLdsQueries = rows_queries_in_lds<T, BITS, D, G>();
+    constexpr bool kLdsQueries = rows_queries_in_lds<T, D, G>();
     __shared__ uint4 queries[kLdsQueries ? KS * TQ : 1][64];  // (the same in all wavefronts)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l = lane & 15, quarter = lane >> 4, g = l / R, line = l % R;
@@ -79,39 +77,15 @@ __global__ void __launch_bounds__(64 * kWaves, (rows_blocks<T, G>())) paged_rows
     const bool real = line < lines;
     const int r = item.part * R + (real ? line : 0), my_row = r / rep, my_head = hk * rep + r % rep;
     const int my_last = real ? last_of(my_row) : -1, my_first = first_of(my_row);
-    const int all_last = last_of(i_first), all_first = first_of(i_last);  // keys up to / from which all lines see
+    const int all_last = uniform(last_of(i_first)), all_first = uniform(first_of(i_last));  // keys up to / from which all lines see
     const int split_begin = item.s.base + item.split * item.per * kTile;
     int s_begin = split_begin, s_end = item.splits == 1 ? S : split_begin + item.per * kTile < S ? split_begin + item.per * kTile : S;
     if (last_of(i_last) + 1 < s_end) s_end = last_of(i_last) + 1;
     if (first_of(i_first) / kTile * kTile > s_begin) s_begin = first_of(i_first) / kTile * kTile;
+    s_begin = uniform(s_begin), s_end = uniform(s_end);
 
-    // The queries' operands: column (g, line), zeros outside the group; their sums per column.
-    uint4 qf[KS][TQ];
-    float qsum = 0.0f;
-    const T *query = a.q + (int64_t)(item.s.start + my_row) * a.q_strides[0] + (int64_t)my_head * a.q_strides[1];
-#pragma unroll
-    for (int s = 0; s < KS; s++) {
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int at = quarter * (D / 4) + 8 * s + code_at<BITS>(j);
-            v[j] = real && at / (D / G) == g ? Elem<T>::load(query, at) : 0.0f;
-            qsum += v[j];
-        }
-        uint32_t t[4][TQ];
-#pragma unroll
-        for (int j = 0; j < 4; j++) split_pair<TQ>(v[2 * j], v[2 * j + 1], t[j]);
-#pragma unroll
-        for (int i = 0; i < TQ; i++) {
-            qf[s][i] = make_uint4(t[0][i], t[1][i], t[2][i], t[3][i]);
-            if (kLdsQueries && wave == 0) queries[s * TQ + i][lane] = qf[s][i];
-        }
-    }
-    if (kLdsQueries) __syncthreads();
-    qsum += __shfl_xor(qsum, 16);
-    qsum += __shfl_xor(qsum, 32);
-
-    // What a tile of 32 keys reads; the next tile's keys are requested when this one's have become operands, its values likewise.
+    // What a tile of 32 keys reads; the next tile's keys are requested when this one's have become operands, its values likewise.  Behind
+    // the last tile an earlier one is requested again: under a condition the wait for this tile's values would be one for all requests.
     constexpr int kRun = G * (int)sizeof(T);  // bytes of a key's scales
     constexpr bool kOwn = kRun == 16;         // float32, four groups: the lane's own group alone
     struct Quad { uint32_t w[kOwn ? 4 : kRun]; };  // of four consecutive keys
@@ -123,18 +97,27 @@ __global__ void __launch_bounds__(64 * kWaves, (rows_blocks<T, G>())) paged_rows
         uint32_t c[8][(kSlot + 31) / 32];
         Quad s[2], b[2];
     } vt;
-    // The rows (of all pages and heads) at which the halves of the tile at s0 lie.  A half behind the end reads the last page.
+    // The rows (of all pages and heads) at which the halves of the tile at s0 lie, and the pages' ids before that, which are requested an
+    // iteration ahead.  A half behind the end reads the last page.
     struct Halves { int64_t row[2]; };
-    const int shift = a.batch.place.page_shift, last_column = S > 0 ? (S - 1) >> shift : 0;
-    const int32_t *columns = table + item.b * a.batch.place.stride;
+    struct Ids { int32_t id[2], s0; };
+    const int shift = a.batch.place.page_shift, last_column = S > 0 ? (S - 1) >> shift : 0, pages = (int)a.batch.place.pages;
+    // (constant memory: the page table's entries are scalar loads, and the addresses that follow from them scalar)
+    typedef const int32_t __attribute__((address_space(4))) *Columns;
+    const Columns columns = (Columns)(uintptr_t)table + item.b * a.batch.place.stride;
     auto look_up = [&](int s0) __attribute__((always_inline)) {
+        Ids o;
+#pragma unroll
+        for (int h = 0; h < 2; h++) o.id[h] = columns[uniform((s0 + 16 * h) >> shift < last_column ? (s0 + 16 * h) >> shift : last_column)];
+        o.s0 = s0;
+        return o;
+    };
+    auto place = [&](const Ids &of) __attribute__((always_inline)) {
         Halves o;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int at = s0 + 16 * h, column = at >> shift;
-            const int64_t id = columns[column < last_column ? column : last_column], pages = a.batch.place.pages;
-            const int64_t page = id < 0 ? 0 : id < pages ? id : pages - 1;
-            o.row[h] = ((page * a.batch.key_heads + hk) << shift) + (at & ((1 << shift) - 1));
+            const int32_t id = of.id[h], page = id < 0 ? 0 : id < pages ? id : pages - 1;
+            o.row[h] = (((int64_t)page * a.batch.key_heads + hk) << shift) + ((of.s0 + 16 * h) & ((1 << shift) - 1));
         }
         return o;
     };
@@ -176,6 +159,12 @@ __global__ void __launch_bounds__(64 * kWaves, (rows_blocks<T, G>())) paged_rows
 #pragma unroll
         for (int h = 0; h < 2; h++) vt.s[h] = four(a.vs, of, h), vt.b[h] = four(a.vb, of, h);
     };
+    // Zeros for key i.
+    auto clear = [](Quad &o, int i) {
+        if constexpr (kRun == 2) o.w[i >> 1] &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+#pragma unroll
+        for (int w = 0; w < (kOwn ? 1 : kRun / 4); w++) o.w[(kOwn ? 1 : kRun / 4) * i + w] = 0;
+    };
     // The lane's own group of key i.
     const int down = 16 * (g & 1);
     const uint32_t half_of = g & 1 ? 0x03020C0Cu : 0x01000C0Cu;  // (its 16 bits above zeros: one byte permutation)
@@ -207,12 +196,40 @@ __global__ void __launch_bounds__(64 * kWaves, (rows_blocks<T, G>())) paged_rows
     const int s_wave = s_begin + wave * kTile;
     Halves next{};
     if (s_wave < s_end) {
-        const Halves here = look_up(s_wave);
+        const Ids first = look_up(s_wave), second = look_up(s_wave + step < s_end ? s_wave + step : s_wave);
+        const Halves here = place(first);
         fetch_keys(here);
         fetch_values(here);
-        next = look_up(s_wave + step);
+        next = place(second);
     }
+    // The queries' operands: column (g, line), zeros outside the group; their sums per column.
+    uint4 qf[KS][TQ];
+    float qsum = 0.0f;
+    const T *query = a.q + (int64_t)(item.s.start + my_row) * a.q_strides[0] + (int64_t)my_head * a.q_strides[1];
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+        const int at = quarter * (D / 4) + 8 * s;  // (eight values of one group)
+        struct __attribute__((packed)) Eight { T v[8]; };
+        const Eight eight = *reinterpret_cast<const Eight *>(query + at);
+        const bool mine = real && at / (D / G) == g;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = mine ? Elem<T>::load(eight.v, code_at<BITS>(j)) : 0.0f, qsum += v[j];
+        uint32_t t[4][TQ];
+#pragma unroll
+        for (int j = 0; j < 4; j++) split_pair<TQ>(v[2 * j], v[2 * j + 1], t[j]);
+#pragma unroll
+        for (int i = 0; i < TQ; i++) {
+            qf[s][i] = make_uint4(t[0][i], t[1][i], t[2][i], t[3][i]);
+            if (kLdsQueries && wave == 0) queries[s * TQ + i][lane] = qf[s][i];
+        }
+    }
+    if (kLdsQueries) __syncthreads();
+    qsum += __shfl_xor(qsum, 16);
+    qsum += __shfl_xor(qsum, 32);
+
     for (int s0 = s_wave; s0 < s_end; s0 += step) {
+        const Ids behind = look_up(s0 + 2 * step < s_end ? s0 + 2 * step : s0);
         float score[8];
         if constexpr (kLdsQueries) {
             asm volatile("" ::: "memory");  // (not kept from the tile before)
@@ -240,17 +257,18 @@ __global__ void __launch_bounds__(64 * kWaves, (rows_blocks<T, G>())) paged_rows
                 score[4 * h + r4] = v * scale;
             }
         }
-        const bool masked = s0 + kTile - 1 > all_last || s0 < all_first || s0 + kTile > S;
-        uint32_t hidden = 0;  // of the lane's eight keys
-        if (masked) {
+        if (s0 + kTile - 1 > all_last || s0 < all_first || s0 + kTile > S) {
+            asm volatile("");  // (a branch: as selects it would cost every tile)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int key = s0 + 16 * (j >> 2) + 4 * quarter + (j & 3);
-                if (key > my_last || key < my_first || key >= S) score[j] = -INFINITY, hidden |= 1u << j;
+                if (key > my_last || key < my_first || key >= S) {
+                    score[j] = -INFINITY;
+                    clear(vt.s[j >> 2], j & 3), clear(vt.b[j >> 2], j & 3);
+                }
             }
         }
-        const bool more = s0 + step < s_end;
-        if (more) fetch_keys(next);
+        fetch_keys(next);
         float top = score[0];
 #pragma unroll
         for (int j = 1; j < 8; j++) top = fmaxf(top, score[j]);
@@ -272,8 +290,7 @@ __global__ void __launch_bounds__(64 * kWaves, (rows_blocks<T, G>())) paged_rows
         for (int j = 0; j < 8; j++) {
             const float p = __builtin_amdgcn_exp2f(score[j] - m);
             denom += p;
-            float sv = pick(vt.s[j >> 2], j & 3), bv = pick(vt.b[j >> 2], j & 3);
-            if (masked && (hidden >> j & 1) != 0) sv = bv = 0.0f;
+            const float sv = pick(vt.s[j >> 2], j & 3), bv = pick(vt.b[j >> 2], j & 3);
             accb = __builtin_fmaf(p, __builtin_fmaf(kMiddle, sv, bv), accb);
             w[j] = p * sv;
         }
@@ -310,10 +327,8 @@ __global__ void __launch_bounds__(64 * kWaves, (rows_blocks<T, G>())) paged_rows
 #pragma unroll
             for (int e = 0; e < TP; e++) acc[i] = mfma16(vf, pf[e], acc[i]);
         }
-        if (more) {
-            fetch_values(next);
-            next = look_up(s0 + 2 * step);
-        }
+        fetch_values(next);
+        next = place(behind);
     }
 
     // merge: the block's maximum, every wavefront scaled to it, the wavefronts added up
@@ -349,77 +364,68 @@ __global__ void __launch_bounds__(64 * kWaves, (rows_blocks<T, G>())) paged_rows
             // (a row that sees nothing: zeros)
             Elem<T>::store(a.out + (int64_t)(item.s.start + rr / rep) * a.out_strides[0] + (int64_t)head * a.out_strides[1], at, total == 0.0f ? 0.0f : sum / total);
         } else {
-            float *dst = a.states + ((int64_t)item.slot * R + ln) * (D + 2);
+            float *dst = a.states + ((int64_t)item.slot * R + ln) * kState<D>;
             if (at == 0) dst[0] = top, dst[1] = total;
-            dst[2 + at] = sum;
+            dst[4 + at] = sum;
         }
     }
 }
 
-// The splits of a line merged, by WAVES wavefronts, which take them in turn, eight loads under way at a time, and add up through LDS.  Block:
-// 4 / WAVES lines of a unit.
-template <typename T, int D, int LINES, int KIND, int WAVES>
+// The splits of a line merged, one block a line: its wavefronts take them in turn, eight loads under way at a time, and add up through LDS.
+template <typename T, int D, int LINES>
 __global__ void __launch_bounds__(64 * kWaves) paged_merge_kernel(const RowsArgs<T> a) {
     constexpr int V = D / 64;
     __shared__ float sums[kWaves][D], tops[kWaves], totals[kWaves];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), first = wave / WAVES * WAVES;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     PagedItem item;
-    if (!paged_item<LINES, KIND, true>(a.batch, lane, blockIdx.x, item)) return;
-    const int rep = a.batch.rep, ln = blockIdx.y * (kWaves / WAVES) + wave / WAVES;
-    const int part = KIND == 0 ? item.part : item.s.parts - 1 - item.part, line = part * LINES + ln;  // (the kernel of many lines counts from the last)
-    const bool real = ln < LINES && line < item.s.rows * rep;
+    if (!paged_item<LINES, 0, true>(a.batch, lane, blockIdx.x, item)) return;
+    const int rep = a.batch.rep, ln = blockIdx.y, line = item.part * LINES + ln;
+    if (line >= item.s.rows * rep) return;
+    const int64_t stride = (int64_t)a.batch.key_heads * LINES * kState<D>;  // of a split's states
+    const float *src = a.states + ((int64_t)item.slot * LINES + ln) * kState<D>;
     float top = -1.0e30f, total = 0.0f, sum[V] = {};
-    if (real) {
-        const int64_t stride = (int64_t)a.batch.key_heads * LINES * (D + 2);  // of a split's states
-        const float *src = a.states + ((int64_t)item.slot * LINES + ln) * (D + 2);
-        for (int z0 = wave - first; z0 < item.splits; z0 += 8 * WAVES) {
-            float m[8], d[8], v[8][V];
+    for (int z0 = wave; z0 < item.splits; z0 += 8 * kWaves) {
+        float m[8], d[8], v[8][V];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int z = z0 + WAVES * i < item.splits ? z0 + WAVES * i : z0;
-                const float *state = src + z * stride;
-                m[i] = state[0], d[i] = state[1];
+        for (int i = 0; i < 8; i++) {
+            const int z = z0 + kWaves * i < item.splits ? z0 + kWaves * i : z0;
+            const float *state = src + z * stride;
+            m[i] = state[0], d[i] = state[1];
 #pragma unroll
-                for (int e = 0; e < V; e++) v[i][e] = state[2 + V * lane + e];
-            }
-            float most = top;
-#pragma unroll
-            for (int i = 0; i < 8; i++) most = fmaxf(most, m[i]);
-            const float f = exp2f(top - most);
-            top = most, total *= f;
-#pragma unroll
-            for (int e = 0; e < V; e++) sum[e] *= f;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float w = z0 + WAVES * i < item.splits ? exp2f(m[i] - top) : 0.0f;
-                total = __builtin_fmaf(d[i], w, total);
-#pragma unroll
-                for (int e = 0; e < V; e++) sum[e] = __builtin_fmaf(v[i][e], w, sum[e]);
-            }
+            for (int e = 0; e < V; e++) v[i][e] = state[4 + V * lane + e];
         }
-    }
-    if constexpr (WAVES > 1) {
-        tops[wave] = top, totals[wave] = total;
-#pragma unroll
-        for (int e = 0; e < V; e++) sums[wave][V * lane + e] = sum[e];
-        __syncthreads();
-        if (wave != first) return;
         float most = top;
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) most = fmaxf(most, tops[first + w]);
+        for (int i = 0; i < 8; i++) most = fmaxf(most, m[i]);
         const float f = exp2f(top - most);
         top = most, total *= f;
 #pragma unroll
         for (int e = 0; e < V; e++) sum[e] *= f;
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) {
-            const float g = exp2f(tops[first + w] - top);
-            total = __builtin_fmaf(totals[first + w], g, total);
+        for (int i = 0; i < 8; i++) {
+            const float w = z0 + kWaves * i < item.splits ? exp2f(m[i] - top) : 0.0f;
+            total = __builtin_fmaf(d[i], w, total);
 #pragma unroll
-            for (int e = 0; e < V; e++) sum[e] = __builtin_fmaf(sums[first + w][V * lane + e], g, sum[e]);
+            for (int e = 0; e < V; e++) sum[e] = __builtin_fmaf(v[i][e], w, sum[e]);
         }
     }
-    if (!real) return;
+    tops[wave] = top, totals[wave] = total;
+#pragma unroll
+    for (int e = 0; e < V; e++) sums[wave][V * lane + e] = sum[e];
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) top = fmaxf(top, tops[w]);
+    total = 0.0f;
+#pragma unroll
+    for (int e = 0; e < V; e++) sum[e] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+        const float f = exp2f(tops[w] - top);
+        total = __builtin_fmaf(totals[w], f, total);
+#pragma unroll
+        for (int e = 0; e < V; e++) sum[e] = __builtin_fmaf(sums[w][V * lane + e], f, sum[e]);
+    }
     const int head = item.head * rep + line % rep;
     if (a.sinks != nullptr) {
         const float sink = Elem<T>::load(a.sinks, head) * kLog2e, most = fmaxf(top, sink), f = exp2f(top - most);
@@ -432,18 +438,15 @@ __global__ void __launch_bounds__(64 * kWaves) paged_merge_kernel(const RowsArgs
     for (int e = 0; e < V; e++) Elem<T>::store(out, V * lane + e, total == 0.0f ? 0.0f : sum[e] / total);
 }
 
-template <typename T, int D, int LINES, int KIND, int WAVES>
-int32_t launch_merge(const RowsArgs<T> &a, const PagedLaunch &r, hipStream_t s) {
-    hipLaunchKernelGGL((paged_merge_kernel<T, D, LINES, KIND, WAVES>), dim3(r.merge_units, (r.merge_lines * WAVES + kWaves - 1) / kWaves), dim3(64 * kWaves), 0, s, a);
-    NVQ_LAUNCH_CHECK("paged_attention merge");
-    return NVQ_OK;
-}
-
 template <typename T, int BITS, int D, int G>
 int32_t launch_rows_sized(const RowsArgs<T> &a, const PagedLaunch &r, hipStream_t s) {
     hipLaunchKernelGGL((paged_rows_kernel<T, BITS, D, G>), dim3(r.grid), dim3(64 * kWaves), 0, s, a, a.batch.place.table);
     NVQ_LAUNCH_CHECK("paged_attention");
-    return r.merge_units == 0 ? NVQ_OK : launch_merge<T, D, 16 / G, 0, kWaves>(a, r, s);
+    if (r.merge_units > 0) {
+        hipLaunchKernelGGL((paged_merge_kernel<T, D, 16 / G>), dim3(r.merge_units, r.merge_lines), dim3(64 * kWaves), 0, s, a);
+        NVQ_LAUNCH_CHECK("paged_attention merge");
+    }
+    return NVQ_OK;
 }
 
 template <typename T, int BITS>

@@ -48,18 +48,35 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedBatch &a, int
     return s;
 }
 
-template <typename V> __device__ __forceinline__ V wave_total(V v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-    return v;
+// Scans on the vector unit alone (data-parallel moves; the same through LDS took 1 us of a call): shifts by 1, 2, 4, 8 in each row of 16
+// lanes, then the rows' totals carried into the next rows.
+template <int CTRL, int ROWS> __device__ __forceinline__ int32_t scan_step(int32_t v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true); }
+__device__ __forceinline__ int32_t wave_prefix(int32_t v) {  // inclusive
+    v = scan_step<0x111, 0xF>(v);
+    v = scan_step<0x112, 0xF>(v);
+    v = scan_step<0x114, 0xF>(v);
+    v = scan_step<0x118, 0xF>(v);
+    v = scan_step<0x142, 0xA>(v);
+    return scan_step<0x143, 0xC>(v);
 }
-__device__ __forceinline__ int32_t wave_prefix(int32_t v, int lane) {  // inclusive
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int32_t u = __shfl_up(v, o);
-        if (lane >= o) v += u;
-    }
-    return v;
+__device__ __forceinline__ int32_t wave_total(int32_t v) { return __builtin_amdgcn_readlane(wave_prefix(v), 63); }
+// Of whole numbers below 2^53.
+template <int CTRL, int ROWS> __device__ __forceinline__ double scan_step(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xF, true);
+    return v + __builtin_bit_cast(double, (uint64_t)lo | (uint64_t)hi << 32);
+}
+__device__ __forceinline__ double wave_total(double v) {
+    v = scan_step<0x111, 0xF>(v);
+    v = scan_step<0x112, 0xF>(v);
+    v = scan_step<0x114, 0xF>(v);
+    v = scan_step<0x118, 0xF>(v);
+    v = scan_step<0x142, 0xA>(v);
+    v = scan_step<0x143, 0xC>(v);
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), 63);
+    return __builtin_bit_cast(double, (uint64_t)lo | (uint64_t)hi << 32);
 }
 
 struct PagedPlan {
@@ -69,11 +86,12 @@ struct PagedPlan {
 
 template <int LINES, int KIND>
 __device__ __forceinline__ PagedPlan paged_plan(const PagedBatch &a, int lane, const PagedSequence &first) {
-    int64_t total = 0, units = 0;
+    double total = 0.0;
+    int32_t units = 0;
     for (int b0 = 0; b0 < a.sequences; b0 += 64) {
         const PagedSequence s = b0 == 0 ? first : paged_sequence<LINES, KIND>(a, b0 + lane);
-        const int64_t u = (int64_t)s.parts * a.key_heads;
-        units += u, total += u * s.tiles;
+        const int32_t u = s.parts * a.key_heads;
+        units += u, total += (double)u * (double)s.tiles;
     }
     units = wave_total(units), total = wave_total(total);
     // Every unit's last item may be short.  The shortest items of three whose number is within the target: none, half an item, or one of
@@ -81,8 +99,9 @@ __device__ __forceinline__ PagedPlan paged_plan(const PagedBatch &a, int lane, c
     PagedPlan p[3];
 #pragma unroll
     for (int i = 0; i < 3; i++) {
-        const int64_t left = a.target - units * i / 2 > a.target / 2 ? a.target - units * i / 2 : a.target / 2, per = (total + left - 1) / left;
-        p[i].per = (int32_t)(per < kScheduleTiles ? kScheduleTiles : per < (1 << 26) ? per : 1 << 26), p[i].items = 0;
+        const int32_t spare = units > a.target ? a.target : units, left = a.target - spare * i / 2 > a.target / 2 ? a.target - spare * i / 2 : a.target / 2;
+        const double per = ceil(total / (double)left);
+        p[i].per = per < kScheduleTiles ? kScheduleTiles : per < (double)(1 << 26) ? (int32_t)per : 1 << 26, p[i].items = 0;
     }
     for (int b0 = 0; b0 < a.sequences; b0 += 64) {
         const PagedSequence s = b0 == 0 ? first : paged_sequence<LINES, KIND>(a, b0 + lane);
@@ -90,7 +109,7 @@ __device__ __forceinline__ PagedPlan paged_plan(const PagedBatch &a, int lane, c
         for (int i = 0; i < 3; i++) p[i].items += s.parts * p[i].splits(s) * a.key_heads;
     }
 #pragma unroll
-    for (int i = 0; i < 3; i++) p[i].items = wave_total(p[i].items);
+    for (int i = 0; i < 3; i++) p[i].items = wave_total(p[i].items), p[i].per = __builtin_amdgcn_readfirstlane(p[i].per);
     return p[0].items <= a.target ? p[0] : p[1].items <= a.target ? p[1] : p[2];
 }
 
@@ -108,7 +127,7 @@ __device__ __forceinline__ bool paged_find(const PagedBatch &a, const PagedPlan 
         const PagedSequence s = b0 == 0 ? first : paged_sequence<LINES, KIND>(a, b0 + lane);
         const int32_t splits = p.splits(s), own = s.parts * a.key_heads, count = UNITS ? (splits > 1 ? own : 0) : own * splits;
         const int32_t state = splits > 1 ? own * splits : 0;
-        const int32_t end = wave_prefix(count, lane), state_end = wave_prefix(state, lane);
+        const int32_t end = wave_prefix(count), state_end = wave_prefix(state);
         const uint64_t behind = __ballot(end > at);
         if (behind != 0) {
             const int l = __builtin_ctzll(behind);
@@ -129,12 +148,25 @@ __device__ __forceinline__ bool paged_find(const PagedBatch &a, const PagedPlan 
     return false;
 }
 
+// What all lanes hold, as the compiler can see: in a scalar register, and branches on it without masks of lanes.  (Of a value that has come
+// through the search for an item the move alone is folded away, and the value taken for one that differs by lane.)
+__device__ __forceinline__ int32_t uniform(int32_t v) {
+    v = __builtin_amdgcn_readfirstlane(v);
+    asm("" : "+s"(v));
+    return v;
+}
+
 // Item (or unit) `at` of the whole plan; false behind the last.
 template <int LINES, int KIND, bool UNITS>
 __device__ __forceinline__ bool paged_item(const PagedBatch &a, int lane, int32_t at, PagedItem &item) {
     const PagedSequence first = paged_sequence<LINES, KIND>(a, lane);
     const PagedPlan plan = paged_plan<LINES, KIND>(a, lane, first);
-    return at < plan.items && paged_find<LINES, KIND, UNITS>(a, plan, lane, first, at, item);
+    const bool found = at < plan.items && paged_find<LINES, KIND, UNITS>(a, plan, lane, first, at, item);
+    if (uniform(found) == 0) return false;
+    const PagedSequence &s = item.s;
+    item = PagedItem{{uniform(s.start), uniform(s.rows), uniform(s.length), uniform(s.base), uniform(s.tiles), uniform(s.parts)},
+                     uniform(item.b), uniform(item.splits), uniform(item.per), uniform(item.part), uniform(item.split), uniform(item.head), uniform(item.slot)};
+    return true;
 }
 
 }  // namespace
