@@ -22,8 +22,10 @@ PagedBatch batch_of(const nvq_paged_attention_desc &d, const PagedAttentionOpera
 
 namespace {
 
-// Lines of a sequence that the kernel of few lines takes, where the other kernel has the type.
-constexpr int32_t kFewLines = 32;
+// Lines of a sequence that the kernel of few lines takes, where the other kernel has the type.  (8 sequences of 4096 positions, 4 heads of 128 on
+// each of 8 key heads, 4 bits: 32 lines a sequence 42 us against the other's 50, 64 lines 59 against 52; one sequence: 17 against 26, 23 against 27;
+// 8 of them, 2 heads of 64 a key head: 32 lines 29 against 35, 64 lines 40 against 36.)
+constexpr int32_t kFewLines = 48;
 constexpr int64_t kPromptLines = 128;
 
 struct Kernel {
@@ -59,12 +61,12 @@ size_t paged_attention_workspace_bytes(const nvq_paged_attention_desc &d) {
 
 int32_t launch_paged_attention(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, hipStream_t s) {
     const nvq_paged_desc &c = d.cache;
-    const bool starts = o.starts != nullptr, many = takes_many(d, starts);
+    const bool starts = o.starts != nullptr, many = takes_many(d, starts), alone = many && c.sequences == 1;  // (alone: one launch, whatever its lines)
     auto launch_of = [&](bool of_many) {
         const Kernel k = kernel_of(d, of_many);
         paged::PagedLaunch r{};
         r.batch = paged::batch_of(d, o);
-        r.batch.few = many ? kFewLines : INT32_MAX, r.batch.target = k.target;
+        r.batch.few = alone ? -1 : many ? kFewLines : INT32_MAX, r.batch.target = k.target;
         const int64_t rep = r.batch.rep;
         // At most so many units and items, whatever the lengths and starts on the device say (paged_schedule.h).
         const int64_t each = many && !of_many ? (kFewLines + k.lines - 1) / k.lines : (rep + k.lines - 1) / k.lines;
@@ -80,9 +82,11 @@ int32_t launch_paged_attention(const nvq_paged_attention_desc &d, const PagedAtt
         r.states = of_many ? kernel_of(d, false).bytes : 0;
         return r;
     };
-    const paged::PagedLaunch few = launch_of(false);
-    const int32_t rc = c.dtype == NVQ_F32 ? paged::launch_rows_f32(d, o, few, s) : c.dtype == NVQ_BF16 ? paged::launch_rows_bf16(d, o, few, s) : paged::launch_rows_f16(d, o, few, s);
-    if (rc != NVQ_OK || !many) return rc;
+    if (!alone) {
+        const paged::PagedLaunch few = launch_of(false);
+        const int32_t rc = c.dtype == NVQ_F32 ? paged::launch_rows_f32(d, o, few, s) : c.dtype == NVQ_BF16 ? paged::launch_rows_bf16(d, o, few, s) : paged::launch_rows_f16(d, o, few, s);
+        if (rc != NVQ_OK || !many) return rc;
+    }
     return c.dtype == NVQ_BF16 ? paged::launch_prompt_bf16(d, o, launch_of(true), s) : paged::launch_prompt_f16(d, o, launch_of(true), s);
 }
 

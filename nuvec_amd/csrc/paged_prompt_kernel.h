@@ -12,6 +12,12 @@
 // mantissa; 8 bits through float32); the 16, and for V the middle of the codes' range, are taken off the sums: the scores' by the
 // bias, the outputs' by the sum of the rounded weights.
 //
+// Measured: 1024 rows of 32 heads of 128 over 4096 positions, 8 key heads, 4 bits in groups of 64, bfloat16: 135 us, 444 TFLOP/s (vector
+// unit busy 49%, matrix cores 19%, LDS 41%; staging 32 us of it, scores and softmax 44, values 44, queries and states 19); 117 us in groups of
+// 128, 186 in groups of 32: each group of a head has its own scaling of scores and weights.  Eight wavefronts with 256 lines were 134 us there
+// but 128 against 118 with 2048 rows over as many positions, where the longest of fewer blocks is what the others wait for; 64 keys' scores before
+// their softmax (256 registers), the keys' biases or scales through the matrix cores: no faster.
+//
 // Terms: queries are exact in their own type.  Weights x scale are rounded to bfloat16, to two terms of it where the element type is float16.
 #pragma once
 
@@ -42,6 +48,27 @@ __device__ __forceinline__ uint4 key_codes(const CodeConstants<BITS == 8 ? 4 : B
     }
 }
 
+// What a unit's lines see: keys from `begin` (rounded down to a tile) to `end`, and the splits that hold some of them.  The others' states are
+// neither written nor read, and a split that holds them all writes the result.
+struct PromptSpan {
+    int32_t begin, end, first_split, end_split;
+};
+__device__ __forceinline__ PromptSpan prompt_span(const PagedBatch &a, const PagedItem &item, int part) {
+    const int32_t from = part * kPromptLines, lines = item.s.rows * a.rep, to = lines - from < kPromptLines ? lines : from + kPromptLines;
+    int32_t begin = 0, end = item.s.length;
+    if (a.causal) {
+        const int32_t before = item.s.length - item.s.rows, seen = before + (to - 1) / a.rep + 1;
+        const int64_t first = a.window > 0 ? before + from / a.rep + 1 - a.window : 0;
+        end = seen < end ? seen : end, begin = first > 0 ? (int32_t)first / kTile * kTile : 0;
+    }
+    PromptSpan s{uniform(begin), uniform(end), 0, 1};
+    if (item.splits > 1) {
+        const int32_t keys = item.per * kTile, splits = end > item.s.base ? (end - item.s.base + keys - 1) / keys : 0;
+        s.first_split = uniform(begin > item.s.base ? (begin - item.s.base) / keys : 0), s.end_split = uniform(splits < item.splits ? splits : item.splits);
+    }
+    return s;
+}
+
 template <typename T, int BITS, int D, int G>
 __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const RowsArgs<T> a, const int32_t *__restrict__ table) {
     constexpr int TP = Elem<T>::code == NVQ_BF16 ? 1 : 2;
@@ -68,12 +95,10 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
     auto last_of = [&](int i) { return a.batch.causal ? S - n + i : S - 1; };
     auto first_of = [&](int i) { return window > 0 && a.batch.causal ? last_of(i) - window + 1 : 0; };
     // the block's keys
-    const int b_first = part * kPromptLines / rep, b_end = (part + 1) * kPromptLines < lines ? (part + 1) * kPromptLines : lines, b_last = (b_end - 1) / rep;
-    const int split_begin = item.s.base + item.split * item.per * kTile;
-    int s_begin = split_begin, s_end = item.splits == 1 ? S : split_begin + item.per * kTile < S ? split_begin + item.per * kTile : S;
-    if (last_of(b_last) + 1 < s_end) s_end = last_of(b_last) + 1;
-    if (first_of(b_first) / kTile * kTile > s_begin) s_begin = first_of(b_first) / kTile * kTile;
-    s_begin = uniform(s_begin), s_end = uniform(s_end);
+    const PromptSpan span = prompt_span(a.batch, item, part);
+    if (item.split < span.first_split || item.split >= span.end_split) return;
+    const int split_begin = item.s.base + item.split * item.per * kTile, split_end = item.splits == 1 ? S : split_begin + item.per * kTile;
+    const int s_begin = uniform(span.begin > split_begin ? span.begin : split_begin), s_end = uniform(span.end < split_end ? span.end : split_end);
     // the wavefront's lines
     const int r0 = part * kPromptLines + wave * 32, r = r0 + col;
     const bool live = r < lines;
@@ -320,7 +345,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
         accb[g] = __builtin_fmaf(-(kValueOff + kMiddle), ones[g], accb[g]);  // (the operands and kValueOff + kMiddle went through the same weights)
     }
     if (!live) return;
-    const bool whole = item.splits == 1;
+    const bool whole = span.end_split - span.first_split == 1;
     float inv = 1.0f;
     float *state = nullptr;  // of this line and split: maximum, denominator, weighted sums
     if (whole) {
@@ -358,18 +383,19 @@ __global__ void __launch_bounds__(64 * kWaves) paged_merge_many_kernel(const Row
     PagedItem item;
     if (!paged_item<kPromptLines, 1, true>(a.batch, threadIdx.x & 63, blockIdx.x, item)) return;
     const int rep = a.batch.rep, ln = blockIdx.y * kLines + (int)threadIdx.x / kThreads, at = (int)threadIdx.x % kThreads * 4;
-    const int line = (item.s.parts - 1 - item.part) * kPromptLines + ln;  // (items count the parts from the last)
-    if (line >= item.s.rows * rep) return;
+    const int part = item.s.parts - 1 - item.part, line = part * kPromptLines + ln;  // (items count the parts from the last)
+    const PromptSpan span = prompt_span(a.batch, item, part);
+    if (line >= item.s.rows * rep || span.end_split - span.first_split == 1) return;
     const int64_t stride = (int64_t)a.batch.key_heads * kPromptLines * kState<D>;  // of a split's states
     const float *src = a.states + ((int64_t)item.slot * kPromptLines + ln) * kState<D>;
     float top = -1.0e30f, total = 0.0f;
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int z0 = 0; z0 < item.splits; z0 += 4) {
+    for (int z0 = span.first_split; z0 < span.end_split; z0 += 4) {
         float2 m[4];
         float4 v[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float *state = src + (z0 + i < item.splits ? z0 + i : z0) * stride;
+            const float *state = src + (z0 + i < span.end_split ? z0 + i : z0) * stride;
             m[i] = *reinterpret_cast<const float2 *>(state), v[i] = *reinterpret_cast<const float4 *>(state + 4 + at);
         }
         float most = top;
@@ -379,7 +405,7 @@ __global__ void __launch_bounds__(64 * kWaves) paged_merge_many_kernel(const Row
         top = most, total *= f, sum.x *= f, sum.y *= f, sum.z *= f, sum.w *= f;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float w = z0 + i < item.splits ? exp2f(m[i].x - top) : 0.0f;
+            const float w = z0 + i < span.end_split ? exp2f(m[i].x - top) : 0.0f;
             total = __builtin_fmaf(m[i].y, w, total);
             sum.x = __builtin_fmaf(v[i].x, w, sum.x), sum.y = __builtin_fmaf(v[i].y, w, sum.y);
             sum.z = __builtin_fmaf(v[i].z, w, sum.z), sum.w = __builtin_fmaf(v[i].w, w, sum.w);
