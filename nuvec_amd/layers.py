@@ -10,7 +10,7 @@ from typing import Optional
 
 import torch
 
-from . import _lib, ops
+from . import _lib, ops, paged
 from .ops import Quant, QuantMode, Quantized
 
 
@@ -342,6 +342,48 @@ class MoeMlp:
         top, scores = self.route(x)
         experts = self.switch_mlp.forward(x, top)  # [B, L, k, D]
         return ops.weighted_sum(experts, scores)
+
+    __call__ = forward
+
+
+@dataclass
+class PagedAttention:
+    """A model's attention for serving many sequences at once: the projections of every token, `append_paged` (norms of the heads, rotary positions,
+    quantization, one launch), `paged_attention`, the output projection.  Weights of the norms are `[head_dim]`, `sinks` `[query_heads]`."""
+    q_proj: QuantizedLinear
+    k_proj: QuantizedLinear
+    v_proj: QuantizedLinear
+    o_proj: QuantizedLinear
+    query_heads: int
+    key_heads: int
+    rotation: Optional[paged.Rotation] = None
+    q_norm: Optional[torch.Tensor] = None
+    k_norm: Optional[torch.Tensor] = None
+    sinks: Optional[torch.Tensor] = None
+    scale: Optional[float] = None  # None: head_dim^-1/2
+    window: int = 0
+    eps: float = 1e-6
+
+    def forward(self, x: torch.Tensor, cache: paged.PagedCache, page_table: torch.Tensor, positions: torch.Tensor, lengths: torch.Tensor,
+                sequences: Optional[torch.Tensor] = None, query_starts: Optional[torch.Tensor] = None, max_queries: Optional[int] = None) -> torch.Tensor:
+        """`x` `[tokens, dims]`: the rows of sequence b are `query_starts[b]` to `query_starts[b + 1] - 1`, row t is position `positions[t]` of
+        sequence `sequences[t]`, and `lengths[b]` counts the positions of sequence b with these rows (all int32).  `sequences` and `query_starts`
+        None: one token per sequence.  Padding rows (a negative position, behind the last start) write nothing; their results are undefined."""
+        if (sequences is None) != (query_starts is None):
+            raise ops.InvalidArgument("paged_attention: sequences and query starts go together")
+        if x.ndim != 2:
+            raise ops.InvalidArgument(f"paged_attention: tokens must be [tokens, dims], got {list(x.shape)}")
+        q, k, v = self._heads(self.q_proj(x), self.query_heads), self._heads(self.k_proj(x), self.key_heads), self._heads(self.v_proj(x), self.key_heads)
+        q = paged.append_paged(cache, k, v, page_table, positions, sequences, self.rotation, self.k_norm, q, self.q_norm, self.eps)
+        scale = q.shape[2] ** -0.5 if self.scale is None else self.scale
+        y = paged.paged_attention(q, cache, page_table, lengths, scale, query_starts, max_queries, self.sinks, True, self.window)
+        return self.o_proj(y.flatten(1))
+
+    @staticmethod
+    def _heads(y: torch.Tensor, n: int) -> torch.Tensor:
+        if n < 1 or y.shape[1] % n:
+            raise ops.InvalidArgument(f"paged_attention: {y.shape[1]} projected values of {n} heads")
+        return y.view(y.shape[0], n, y.shape[1] // n)
 
     __call__ = forward
 
