@@ -126,29 +126,38 @@ __device__ __forceinline__ Turn read_turn(const float2 *__restrict__ angles, int
     return t;
 }
 
-// The lane's values of a head and those that the rotation mixes into them.
+// The lane's values of a head and those that the rotation mixes into them, as they lie in memory: a head's are requested before the one in front of it is
+// worked on.
 template <typename T, bool WIDE>
-struct HeadRun {
-    float v[8], p[8];
+struct HeadRaw {
+    T v[8], p[8];
     __device__ __forceinline__ void load(const T *row, int j0, int dim, int half, bool interleaved) {
         if (WIDE) {
+            struct alignas(16) Run { T t[8]; };
             if (j0 < dim) {
-                load_run(row + j0, v);
-                if (!interleaved && j0 < 2 * half) load_run(row + (j0 < half ? j0 + half : j0 - half), p);
+                __builtin_memcpy(v, reinterpret_cast<const Run *>(row + j0), sizeof(Run));
+                if (!interleaved && j0 < 2 * half) __builtin_memcpy(p, reinterpret_cast<const Run *>(row + (j0 < half ? j0 + half : j0 - half)), sizeof(Run));
             }
             return;
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int j = j0 + i;
-            v[i] = j < dim ? Elem<T>::load(row, j) : 0.0f;
-            p[i] = j < 2 * half ? Elem<T>::load(row, interleaved ? j ^ 1 : j < half ? j + half : j - half) : 0.0f;
+            if (j < dim) v[i] = row[j];
+            if (j < 2 * half) p[i] = row[interleaved ? j ^ 1 : j < half ? j + half : j - half];
         }
     }
+};
+template <typename T, bool WIDE>
+struct HeadRun {
+    float v[8], p[8];
+    HeadRun() = default;
+    __device__ __forceinline__ explicit HeadRun(const HeadRaw<T, WIDE> &raw) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = Elem<T>::load(raw.v, i), p[i] = Elem<T>::load(raw.p, i);
+    }
     // times the factor and the weight: two roundings in float32, those of the partners likewise
-    __device__ __forceinline__ void scale(float r, const T *__restrict__ weight, int j0, int dim, int half, bool interleaved) {
-        HeadRun<T, WIDE> w;
-        w.load(weight, j0, dim, half, interleaved);
+    __device__ __forceinline__ void scale(float r, const HeadRun &w) {
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = v[i] * r * w.v[i], p[i] = p[i] * r * w.p[i];
     }

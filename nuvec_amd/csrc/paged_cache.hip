@@ -12,7 +12,9 @@
 //
 // Bound by memory when there are many tokens, by one round trip for the table, one for the inputs and one for the page's id when there
 // are few.  A block takes 256 / P tokens of a head at a time (P lanes a head), so that the codes, scales and biases of consecutive
-// positions, which lie together, are written by one block.
+// positions, which lie together, are written by one block; a head is requested before the one in front of it is quantized.  Measured,
+bfloat16 to 4 bits in groups of 64: 6000 tokens of 32 query heads and 8 key heads of 128 in 32 us, 4.1 TB/s; 64 tokens with norms in 5 us, a
+launch; the 6000 tokens read back in 11 us, 2.9 TB/s.
 #include "heads.h"
 #include "nvq_internal.h"
 #include "paged.h"
@@ -102,24 +104,38 @@ __global__ void __launch_bounds__(kHeadBlock) append_paged_kernel(const AppendAr
         position = position < 0 ? 0 : position < a.table_rows ? position : a.table_rows - 1;
         turn = read_turn<WIDE>(a.table + position * a.half, j0, a.half, interleaved);
     }
-    const int keys = a.query_heads, values = keys + a.key_heads, all = values + a.key_heads;
-    const int h1 = min((int)(blockIdx.y + 1) * a.per_block, all);
-    for (int h = blockIdx.y * a.per_block; h < h1; h++) {
-        const bool is_q = h < keys, is_v = h >= values;
-        const int64_t head = is_q ? h : is_v ? h - values : h - keys;
-        if (!is_q && row < 0) continue;
-        const T *x = is_q ? a.q + token * a.qs[0] + head * a.qs[1] : is_v ? a.v + token * a.vst[0] + head * a.vst[1] : a.k + token * a.kst[0] + head * a.kst[1];
-        const T *weight = is_q ? a.q_weight : is_v ? nullptr : a.k_weight;
-        const int half = is_v ? 0 : a.half;
-        HeadRun<T, WIDE> run{};
-        run.load(x, j0, a.dim, half, interleaved);
-        if (weight != nullptr) run.scale(norm_factor<P>(run.v, a.dim, a.eps), weight, j0, a.dim, half, interleaved);
-        run.turn(turn, j0, half, interleaved);
-        if (is_q) {
-            T *y = a.q_out + (token * a.query_heads + head) * a.dim + j0;
-            store_run(y, run.v);
-            continue;
+    const int h0 = blockIdx.y * a.per_block, h1 = min(h0 + a.per_block, a.query_heads + 2 * a.key_heads);
+    auto normed = [&](HeadRun<T, WIDE> &run, const T *w, const HeadRun<T, WIDE> &weight) __attribute__((always_inline)) {
+        if (w != nullptr) run.scale(norm_factor<P>(run.v, a.dim, a.eps), weight);
+        run.turn(turn, j0, a.half, interleaved);
+    };
+    HeadRaw<T, WIDE> raw{};
+    if (h0 < a.query_heads) {
+        if (a.q_weight != nullptr) raw.load(a.q_weight, j0, a.dim, a.half, interleaved);
+        const HeadRun<T, WIDE> weight(raw);
+        const T *x = a.q + token * a.qs[0];
+        T *y = a.q_out + token * a.query_heads * a.dim + j0;
+        const int to = min(h1, a.query_heads);
+        raw.load(x + h0 * a.qs[1], j0, a.dim, a.half, interleaved);
+        for (int64_t head = h0; head < to; head++) {
+            HeadRun<T, WIDE> run(raw);
+            raw.load(x + (head + 1 < to ? head + 1 : head) * a.qs[1], j0, a.dim, a.half, interleaved);
+            normed(run, a.q_weight, weight);
+            store_run(y + head * a.dim, run.v);
         }
+    }
+    const int from = max(h0 - a.query_heads, 0), to = h1 - a.query_heads;
+    if (row < 0 || from >= to) return;
+    if (a.k_weight != nullptr) raw.load(a.k_weight, j0, a.dim, a.half, interleaved);
+    const HeadRun<T, WIDE> weight(raw);
+    auto row_at = [&](int h) { return h < a.key_heads ? a.k + token * a.kst[0] + h * a.kst[1] : a.v + token * a.vst[0] + (h - a.key_heads) * a.vst[1]; };
+    raw.load(row_at(from), j0, a.dim, a.half, interleaved);
+    for (int h = from; h < to; h++) {
+        const bool is_v = h >= a.key_heads;
+        const int64_t head = is_v ? h - a.key_heads : h;
+        HeadRun<T, WIDE> run(raw);
+        raw.load(row_at(h + 1 < to ? h + 1 : h), j0, a.dim, a.half, interleaved);
+        if (!is_v) normed(run, a.k_weight, weight);
         uint32_t words[kWords];
         float scale, bias;
         if (a.group == 32) quantize_run<T, BITS, 4>(run.v, words, scale, bias);
@@ -186,7 +202,8 @@ PagedPlace place_of(const nvq_paged_desc &d, const int32_t *page_table) {
     return p;
 }
 
-// Heads of a block: all that leave four blocks a compute unit, one where even that does not fill them.
+// Heads of a block: all that leave four blocks a compute unit, one where even that does not fill them.  (The 6000 tokens: two blocks a
+// compute unit 46 us, four 32, eight 36.)
 int32_t heads_of_block(int64_t blocks, int64_t heads) {
     const int64_t per = blocks * heads / (4 * (int64_t)compute_units());
     return (int32_t)(per < 1 ? 1 : per < heads ? per : heads);
