@@ -7,9 +7,11 @@
 namespace nvq {
 namespace paged {
 
+constexpr size_t kPlanBytes = 64;  // in front of a kernel's states
+
 struct PagedLaunch {
     PagedBatch batch;
-    size_t states;                            // where in the workspace the kernel's states lie
+    size_t states;                            // where in the workspace the kernel's plan and states lie
     uint32_t grid, merge_units, merge_lines;  // merge_units 0: no sequence can be split
 };
 // few lines: query rows x query heads of a key head

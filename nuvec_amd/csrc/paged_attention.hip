@@ -23,9 +23,9 @@ PagedBatch batch_of(const nvq_paged_attention_desc &d, const PagedAttentionOpera
 namespace {
 
 // Lines of a sequence that the kernel of few lines takes, where the other kernel has the type.  (8 sequences of 4096 positions, 4 heads of 128 on
-// each of 8 key heads, 4 bits: 32 lines a sequence 42 us against the other's 50, 64 lines 59 against 52; one sequence: 17 against 26, 23 against 27;
-// 8 of them, 2 heads of 64 a key head: 32 lines 29 against 35, 64 lines 40 against 36.)
-constexpr int32_t kFewLines = 48;
+// each of 8 key heads, 4 bits: 16 lines a sequence 29 us against the other's 41, 32 lines 41 against 42, 40 lines 50 against 42, 64 lines 56
+// against 45; one sequence: 32 lines 17 against 21, 64 lines 22 against 21; 2 heads of 64 a key head: 32 lines 25 against 30, 64 lines 35 against 32.)
+constexpr int32_t kFewLines = 32;
 constexpr int64_t kPromptLines = 128;
 
 struct Kernel {
@@ -40,7 +40,7 @@ Kernel kernel_of(const nvq_paged_attention_desc &d, bool many) {
     Kernel k;
     k.lines = many ? kPromptLines : 16 / groups;
     k.target = (many || d.cache.dtype == NVQ_F32 || groups == 4 ? 2 : 3) * compute_units();
-    k.bytes = (size_t)(2 * (int64_t)k.target * k.lines * (d.cache.head_dim + 4)) * sizeof(float);
+    k.bytes = paged::kPlanBytes + (size_t)(2 * (int64_t)k.target * k.lines * (d.cache.head_dim + 4)) * sizeof(float);
     return k;
 }
 

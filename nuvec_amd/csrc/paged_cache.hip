@@ -202,8 +202,8 @@ PagedPlace place_of(const nvq_paged_desc &d, const int32_t *page_table) {
     return p;
 }
 
-// Heads of a block: all that leave four blocks a compute unit, one where even that does not fill them.  (The 6000 tokens: two blocks a
-// compute unit 46 us, four 32, eight 36.)
+// Heads of a block: all that leave four blocks a compute unit, one where even that does not fill them.  (The 6000 tokens, two blocks a
+// compute unit 58 us appended and read back, four 43, eight 48.)
 int32_t heads_of_block(int64_t blocks, int64_t heads) {
     const int64_t per = blocks * heads / (4 * (int64_t)compute_units());
     return (int32_t)(per < 1 ? 1 : per < heads ? per : heads);

@@ -2,23 +2,24 @@
 //
 // The products run on the matrix cores over the codes, as for few lines (paged_rows_kernel.h): scale and bias of a key's groups
 // are applied to the float32 scores, those of a value's to the softmax's weights, so that no key or value is rounded.
-// A block has 128 lines, a wavefront 32 of them: S^T = K . Q^T with v_mfma_f32_32x32x16, a group of the head at a time, leaves a lane
-// with 16 of 32 keys of ONE line; its maximum and sum are in-lane but for one exchange, and its weights are already the operand of
+// A block has 128 lines, a wavefront 16 of them: S^T = K . Q^T with v_mfma_f32_16x16x32, a group of the head at a time, leaves a lane
+// with 4 of 16 keys of ONE line; its maximum and sum are in-lane but for two exchanges, and the weights of 32 keys are already the operand of
 // O^T = V^T . P^T, whose keys are stored in the order in which the lanes hold them.
 //
-// 64 keys at a time become operands in LDS, once for the block: expanded by each wavefront for itself they would cost it three times
-// the instructions, which are what bounds the kernel.  The next 64 keys' codes are requested before, and expanded after, this
-// tile's products; two buffers, one barrier a tile.  A code becomes an element in two instructions for two of them (16 + code in the
-// mantissa; 8 bits through float32); the 16, and for V the middle of the codes' range, are taken off the sums: the scores' by the
-// bias, the outputs' by the sum of the rounded weights.
-//
-// Measured: 1024 rows of 32 heads of 128 over 4096 positions, 8 key heads, 4 bits in groups of 64, bfloat16: 135 us, 444 TFLOP/s (vector
-// unit busy 49%, matrix cores 19%, LDS 41%; staging 32 us of it, scores and softmax 44, values 44, queries and states 19); 117 us in groups of
-// 128, 186 in groups of 32: each group of a head has its own scaling of scores and weights.  Eight wavefronts with 256 lines were 134 us there
-// but 128 against 118 with 2048 rows over as many positions, where the longest of fewer blocks is what the others wait for; 64 keys' scores before
-// their softmax (256 registers), the keys' biases or scales through the matrix cores: no faster.
+// 64 keys at a time become operands in LDS, once for the block: expanded by each wavefront for itself they would cost it six times
+// the instructions.  The next 64 keys' codes are requested before, and expanded after, this tile's products; two buffers, one barrier a tile.  A
+// code becomes an element in two instructions for two of them (16 + code in the mantissa; 8 bits through float32); the 16, and for V the
+// middle of the codes' range, are taken off the sums: the scores' by the bias, the outputs' by the sum of the rounded weights.  The
+// keys' biases are one more product (qb below).
 //
 // Terms: queries are exact in their own type.  Weights x scale are rounded to bfloat16, to two terms of it where the element type is float16.
+//
+// Measured: 1024 rows of 32 heads of 128 over 4096 positions, 8 key heads, 4 bits in groups of 64, bfloat16: 123 us, 489 TFLOP/s (groups of 128:
+// 110, of 32: 156: each group of a head has its own scaling of scores and weights); 2048 rows over as many positions 105 us, 1024 43 us, 512
+// 26 us.  While a compute unit is busy its vector units are at 60%, LDS at 67%, the matrix cores at 26%; a block alone takes nearly as long for a tile as
+// two that share a compute unit.  The same with 32 lines a wavefront (v_mfma_f32_32x32x16, four wavefronts of 256 registers) is as fast over a
+// long prefix and 2 to 15% slower on the diagonal; eight of those wavefronts with 256 lines to a block 5% faster at 1024 rows over 4096 and 15%
+// slower at 2048 over 2048; scales laid out by products instead of read from LDS: no faster.
 #pragma once
 
 #include "paged_rows_kernel.h"
@@ -27,8 +28,7 @@ namespace nvq {
 namespace paged {
 namespace {
 
-using qmf::floatx16_t;
-constexpr int kPromptLines = 128, kStageKeys = 64;
+constexpr int kPromptWaves = 8, kPromptLines = 16 * kPromptWaves, kStageKeys = 64;
 
 // Eight codes of a row as an operand of the element type, value code_at<BITS>(j) of them in place j, each plus key_offset.
 template <typename T, int BITS> constexpr float key_offset = BITS == 4 ? 16.0f : Elem<T>::code == NVQ_BF16 ? 0.0f : 1024.0f;
@@ -48,10 +48,11 @@ __device__ __forceinline__ uint4 key_codes(const CodeConstants<BITS == 8 ? 4 : B
     }
 }
 
-// What a unit's lines see: keys from `begin` (rounded down to a tile) to `end`, and the splits that hold some of them.  The others' states are
-// neither written nor read, and a split that holds them all writes the result.
+// What a unit's lines see, keys from `begin` (rounded down to a tile) to `end`, and how its items share them: evenly, `keys` each, so that the first lines of
+// a prompt, which see less than the last, are shorter items rather than some whole and some empty ones (the 1024 rows above 137 us so).  An item
+// that has them all writes the result.
 struct PromptSpan {
-    int32_t begin, end, first_split, end_split;
+    int32_t begin, end, keys, items;
 };
 __device__ __forceinline__ PromptSpan prompt_span(const PagedBatch &a, const PagedItem &item, int part) {
     const int32_t from = part * kPromptLines, lines = item.s.rows * a.rep, to = lines - from < kPromptLines ? lines : from + kPromptLines;
@@ -62,32 +63,44 @@ __device__ __forceinline__ PromptSpan prompt_span(const PagedBatch &a, const Pag
         end = seen < end ? seen : end, begin = first > 0 ? (int32_t)first / kTile * kTile : 0;
     }
     PromptSpan s{uniform(begin), uniform(end), 0, 1};
-    if (item.splits > 1) {
-        const int32_t keys = item.per * kTile, splits = end > item.s.base ? (end - item.s.base + keys - 1) / keys : 0;
-        s.first_split = uniform(begin > item.s.base ? (begin - item.s.base) / keys : 0), s.end_split = uniform(splits < item.splits ? splits : item.splits);
-    }
+    const int32_t tiles = end > begin ? (end - begin + kTile - 1) / kTile : 0;
+    int32_t per = (tiles + item.splits - 1) / item.splits;
+    per = per > kScheduleTiles ? per : kScheduleTiles;
+    s.keys = uniform(item.splits == 1 ? tiles * kTile : per * kTile), s.items = uniform(item.splits == 1 || tiles <= per ? 1 : (tiles + per - 1) / per);
     return s;
 }
 
+// Keys x queries, in the element type.
+template <typename T>
+__device__ __forceinline__ floatx4_t key_product(uint4 k, uint4 q, floatx4_t c) {
+    if constexpr (Elem<T>::code == NVQ_BF16) {
+        return mfma16(k, q, c);
+    } else {
+        typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, k), __builtin_bit_cast(f16x8_t, q), c, 0, 0, 0);
+    }
+}
+
 template <typename T, int BITS, int D, int G>
-__global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const RowsArgs<T> a, const int32_t *__restrict__ table) {
+__global__ void __launch_bounds__(64 * kPromptWaves, 4) paged_prompt_kernel(const RowsArgs<T> a, const int32_t *__restrict__ table) {
     constexpr int TP = Elem<T>::code == NVQ_BF16 ? 1 : 2;
-    constexpr int KS = D / 16, DB = D / 32, GS = KS / G, GB = DB / G > 0 ? DB / G : 1;  // steps of K, blocks of D; of a group
-    constexpr int kRowBytes = D * BITS / 8, kPart = kRowBytes / 4;     // a row; a quarter of one, a thread's share of the keys' codes
-    constexpr int kChunks = D / 32, kVals = D / 16, kSlot = BITS * kVals;  // eight-code chunks of a quarter; values of a sixteenth and its bits
+    constexpr int KS = D / 32, ND = D / 16, GS = KS / G, GB = ND / G;                  // steps of K, blocks of D; of a group
+    constexpr int kRowBytes = D * BITS / 8, kQuarter = kRowBytes / 4, kShare = kQuarter / 2;  // a row; a quarter; a thread's share of the keys' codes
+    constexpr int kChunks = D / 64, kVals = D / 32, kSlot = BITS * kVals;              // of a thread: eight-code chunks; values of a row and their bits
     constexpr float kOff = key_offset<T, BITS>, kValueOff = BITS == 4 ? 16.0f : 0.0f, kMiddle = 1 << (BITS - 1);
-    // Operands, 16 bytes a lane, with gaps: those that a quarter-wavefront writes at once, 2 keys of four pairs of steps, 16 sixteenths of a row's
-    // values, fall on different banks, and every address is one register and a constant.
+    // Operands, 16 bytes a lane, with gaps, so that what 16 lanes write at once falls on different banks.
     struct Stage {
-        uint4 keys[2][KS][64 + 1];      // [half of the tile][step][half of the step x key]
-        uint4 values[4][DB][2 * 36 + 1];  // [16 keys][block][half of the keys: value, four places after the sixteenth]
-        float scale[4][G][kStageKeys];  // of keys and what goes with it, of values and what goes with it (expand)
-        uint16_t wild[2][G][2];         // a bit for every key whose value's scale or bias is not finite
+        uint4 keys[4][KS][64 + 2];         // [16 keys][step][quarter of the step x key]
+        uint4 values[2][ND][64 + 1];       // [32 keys][block][run of four keys of each half x value]
+        uint4 key_bias[4][64];             // [16 keys][group x key]: terms of their products with the queries' sums
+        float scale[3][G][kStageKeys];     // of keys, of values, the values' biases
+        uint16_t wild[2][G][2];            // a bit for every key whose value's scale or bias is not finite
     };
+    static_assert(4 * sizeof(Stage) <= 160 * 1024);
     __shared__ Stage stages[2];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quarter = lane >> 4;
     PagedItem item;
-    if (!paged_item<kPromptLines, 1, false>(a.batch, lane, blockIdx.x, item)) return;
+    if (!paged_item<kPromptLines, 1, false>(a.batch, lane, blockIdx.x, a.length, item)) return;
     const int rep = a.batch.rep, hk = item.head, S = item.s.length, n = item.s.rows;
     const int part = item.s.parts - 1 - item.part;  // (the lines that see most first)
     const int lines = n * rep;
@@ -96,15 +109,14 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
     auto first_of = [&](int i) { return window > 0 && a.batch.causal ? last_of(i) - window + 1 : 0; };
     // the block's keys
     const PromptSpan span = prompt_span(a.batch, item, part);
-    if (item.split < span.first_split || item.split >= span.end_split) return;
-    const int split_begin = item.s.base + item.split * item.per * kTile, split_end = item.splits == 1 ? S : split_begin + item.per * kTile;
-    const int s_begin = uniform(span.begin > split_begin ? span.begin : split_begin), s_end = uniform(span.end < split_end ? span.end : split_end);
+    if (item.split >= span.items) return;
+    const int s_begin = uniform(span.begin + item.split * span.keys), s_end = uniform(span.end < s_begin + span.keys ? span.end : s_begin + span.keys);
     // the wavefront's lines
-    const int r0 = part * kPromptLines + wave * 32, r = r0 + col;
+    const int r0 = part * kPromptLines + wave * 16, r = r0 + col;
     const bool live = r < lines;
     const int my_row = (live ? r : lines - 1) / rep, my_head = hk * rep + (live ? r % rep : 0);
     const int my_last = last_of(my_row), my_first = first_of(my_row);
-    const int w_first = (r0 < lines ? r0 : lines - 1) / rep, w_last = (r0 + 31 < lines ? r0 + 31 : lines - 1) / rep;
+    const int w_first = (r0 < lines ? r0 : lines - 1) / rep, w_last = (r0 + 15 < lines ? r0 + 15 : lines - 1) / rep;
     const int all_last = uniform(last_of(w_first)), all_first = uniform(first_of(w_last));                       // keys up to / from which all of them see
     const int any_last = uniform(r0 < lines ? last_of(w_last) : -1), any_first = uniform(first_of(w_first));  // and any does
 
@@ -115,7 +127,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
     const T *query = a.q + (int64_t)(item.s.start + my_row) * a.q_strides[0] + (int64_t)my_head * a.q_strides[1];
 #pragma unroll
     for (int s = 0; s < KS; s++) {
-        const uint4 w = load_any<uint4>(query + 16 * s + 8 * half);
+        const uint4 w = load_any<uint4>(query + 32 * s + 8 * quarter);
         T t[8], to[8];
         __builtin_memcpy(t, &w, 16);
         float sum = 0.0f;
@@ -124,62 +136,78 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
         __builtin_memcpy(&qf[s], to, 16);
         qsum[s / GS] += sum;
     }
+    // The biases' share of a score, sum over the groups of bias x (sum of the group's queries), is one more product: both as three bfloat16 terms
+    // h, m, l, whose six largest products are the contraction (h h, h m, m h, h l, l h, m m), a group in each quarter of it.
+    uint4 qb = make_uint4(0u, 0u, 0u, 0u);
+    {
+        float sum = 0.0f;
 #pragma unroll
-    for (int g = 0; g < G; g++) qsum[g] += __shfl_xor(qsum[g], 32);
+        for (int g = 0; g < G; g++) {
+            float all = qsum[g] + __shfl_xor(qsum[g], 16);
+            all += __shfl_xor(all, 32);
+            if (quarter == g) sum = all;
+        }
+        uint32_t t[3];
+        split_pair<3>(sum, sum, t);
+        const uint32_t hm = (t[0] & 0xFFFFu) | (t[1] & 0xFFFF0000u), hl = (t[0] & 0xFFFFu) | (t[2] & 0xFFFF0000u);
+        qb = make_uint4(hm, hl, hm, 0u);
+    }
 
     // ── staging ──
     const CodeConstants<4> constants;
     const float scale = a.scale * kLog2e;
-    // A wavefront's 16 of the tile's 64 keys lie in one page: its place is a scalar, whose page is looked up a tile ahead.
+    // The 16 keys that two wavefronts expand lie in one page: their place is a scalar, whose page is looked up a tile ahead.
+    const int my_keys = wave >> 1, share = wave & 1;
     const int shift = a.batch.place.page_shift, last_column = S > 0 ? (S - 1) >> shift : 0, pages = (int)a.batch.place.pages;
     typedef const int32_t __attribute__((address_space(4))) *Columns;  // (constant memory: scalar loads)
     const Columns columns = (Columns)(uintptr_t)table + item.b * a.batch.place.stride;
     auto look_up = [&](int s0) __attribute__((always_inline)) {
-        const int column = (s0 + 16 * wave) >> shift;
+        const int column = (s0 + 16 * my_keys) >> shift;
         return columns[uniform(column < last_column ? column : last_column)];  // (a tile behind the end reads the last page)
     };
-    // This lane's: a quarter of a key's codes; a sixteenth of four values' codes (keys 8 high + 4 half + 0 .. 3 of the sixteen); half of the lanes: the
-    // scales and biases of a key or of a value.
-    const int k_key = lane >> 2, k_part = lane & 3;
-    const int v_slot = lane & 15, v_run = lane >> 4, v_high = v_run >> 1, v_half = v_run & 1;
-    const int s_key = lane & 15, s_values = lane >> 4 & 1;
-    uint32_t kc[kPart / 4], vc[4][(kSlot + 31) / 32];
-    struct __attribute__((packed)) Groups { T v[G]; } sc, bc;
+    // This lane's: a share of a quarter of a key's codes; of four values (keys 4 v_run .. + 3 of the sixteen) a share of a sixteenth of the
+    // codes; a scale and a bias of one group, of a key in the one wavefront and of a value in the other.
+    const int k_key = lane >> 2, k_quarter = lane & 3;
+    const int v_slot = lane & 15, v_run = lane >> 4;
+    const int s_key = lane & 15, s_group = lane >> 4 < G ? lane >> 4 : 0;
+    uint32_t kc[(kShare + 3) / 4], vc[4][(kSlot + 31) / 32];
+    T sc, bc;
     bool s_real;
     auto request = [&](int32_t id, int s0) __attribute__((always_inline)) {
         const int32_t page = id < 0 ? 0 : id < pages ? id : pages - 1;
-        const int64_t row = (((int64_t)page * a.batch.key_heads + hk) << shift) + ((s0 + 16 * wave) & ((1 << shift) - 1));
-        struct Words { uint32_t w[kPart / 4]; };
-        const Words w = *reinterpret_cast<const Words *>(reinterpret_cast<const uint8_t *>(a.kw) + row * kRowBytes + (uint32_t)(lane * kPart));
+        const int64_t row = (((int64_t)page * a.batch.key_heads + hk) << shift) + ((s0 + 16 * my_keys) & ((1 << shift) - 1));
+        struct Words { uint32_t w[kShare / 4]; };
+        const Words w = *reinterpret_cast<const Words *>(reinterpret_cast<const uint8_t *>(a.kw) + row * kRowBytes + (uint32_t)(lane * kQuarter + share * kShare));
 #pragma unroll
-        for (int i = 0; i < kPart / 4; i++) kc[i] = w.w[i];
+        for (int i = 0; i < kShare / 4; i++) kc[i] = w.w[i];
         const uint8_t *rows = reinterpret_cast<const uint8_t *>(a.vw) + row * kRowBytes;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const uint8_t *at = rows + (uint32_t)(4 * v_run * kRowBytes + kSlot / 8 * v_slot) + j * kRowBytes;
+            const uint8_t *at = rows + (uint32_t)(4 * v_run * kRowBytes + (kRowBytes / 16) * v_slot + share * (kSlot / 8)) + j * kRowBytes;
             if constexpr (kSlot == 64) {
                 const uint2 v = *reinterpret_cast<const uint2 *>(at);
                 vc[j][0] = v.x, vc[j][1] = v.y;
             } else if constexpr (kSlot == 32) {
                 vc[j][0] = *reinterpret_cast<const uint32_t *>(at);
-            } else {
+            } else if constexpr (kSlot == 16) {
                 vc[j][0] = *reinterpret_cast<const uint16_t *>(at);
+            } else {
+                vc[j][0] = *at;
             }
         }
-        const T *ss = s_values != 0 ? a.vs : a.ks, *bb = s_values != 0 ? a.vb : a.kb;
-        sc = *reinterpret_cast<const Groups *>(ss + row * G + s_key * G), bc = *reinterpret_cast<const Groups *>(bb + row * G + s_key * G);
-        s_real = s0 + 16 * wave + s_key < S;
+        const int64_t from = (row + s_key) * G + s_group;
+        sc = (share != 0 ? a.vs : a.ks)[from], bc = (share != 0 ? a.vb : a.kb)[from];
+        s_real = s0 + 16 * my_keys + s_key < S;
     };
     auto expand = [&](Stage &to) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < kChunks; j++) {
-            const int c = kChunks * k_part + j;  // (step c / 2, half c % 2)
-            const uint4 v = key_codes<T, BITS>(constants, kc[BITS == 8 ? 2 * j : j], BITS == 8 ? kc[2 * j + 1] : 0u);
-            to.keys[wave >> 1][c >> 1][(c & 1) * 32 + 16 * (wave & 1) + k_key] = v;
+            const int c = (D / 32) * k_quarter + kChunks * share + j;  // (step c / 4, quarter c % 4)
+            to.keys[my_keys][c >> 2][16 * (c & 3) + k_key] = key_codes<T, BITS>(constants, kc[BITS == 8 ? 2 * j : j], BITS == 8 ? kc[2 * j + 1] : 0u);
         }
 #pragma unroll
         for (int i = 0; i < kVals; i++) {
-            const int d = kVals * v_slot + i, row = (d & 31) + (d >> 2 & 4);
+            const int d = (D / 16) * v_slot + kVals * share + i;
             uint32_t p[2];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
@@ -191,127 +219,135 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
                     p[j] = two_codes(constants, both, 4 * (i & 3));
                 }
             }
-            reinterpret_cast<uint2 *>(&to.values[wave][d >> 5][v_half * 36 + row])[v_high] = make_uint2(p[0], p[1]);
+            reinterpret_cast<uint2 *>(&to.values[my_keys >> 1][d >> 4][16 * v_run + (d & 15)])[my_keys & 1] = make_uint2(p[0], p[1]);
         }
         // Keys: both with the softmax's scale, the bias without the codes' offset; values: the bias from the middle of the codes' range.  What lies
         // behind the sequence's end may hold anything: zeros.
-        if (lane < 32) {
-#pragma unroll
-            for (int g = 0; g < G; g++) {
-                const float v = Elem<T>::load(sc.v, g), b = Elem<T>::load(bc.v, g);
-                const float own = s_values != 0 ? v : v * scale, with = s_values != 0 ? __builtin_fmaf(kMiddle, v, b) : __builtin_fmaf(-kOff, v, b) * scale;
-                const bool wild = s_values != 0 && !(fabsf(with) < INFINITY && fabsf(own) < INFINITY), used = s_real && !wild;
-                to.scale[2 * s_values][g][16 * wave + s_key] = used ? own : 0.0f;
-                to.scale[2 * s_values + 1][g][16 * wave + s_key] = used ? with : 0.0f;
-                const uint64_t all = __ballot(wild && s_real);
-                if (lane == 0) to.wild[wave >> 1][g][wave & 1] = (uint16_t)(all >> 16);
+        const float v = Elem<T>::load(&sc, 0), b = Elem<T>::load(&bc, 0);
+        float own = share != 0 ? v : v * scale, with = share != 0 ? __builtin_fmaf(kMiddle, v, b) : __builtin_fmaf(-kOff, v, b) * scale;
+        const bool wild = share != 0 && !(fabsf(with) < INFINITY && fabsf(own) < INFINITY), used = s_real && !wild;
+        own = used ? own : 0.0f, with = used ? with : 0.0f;
+        const uint64_t all = __ballot(wild && s_real);
+        if (lane >> 4 < G) {
+            to.scale[share][s_group][16 * my_keys + s_key] = own;
+            if (share != 0) {
+                to.scale[2][s_group][16 * my_keys + s_key] = with;
+                if (s_key == 0) to.wild[my_keys >> 1][s_group][my_keys & 1] = (uint16_t)(all >> (lane & 48));
             }
+        }
+        if (share == 0) {
+            with = lane >> 4 < G ? with : 0.0f;  // (no more groups: zeros)
+            uint32_t t[3];
+            split_pair<3>(with, with, t);
+            to.key_bias[my_keys][lane] = make_uint4(t[0], (t[1] & 0xFFFFu) | (t[0] & 0xFFFF0000u), (t[2] & 0xFFFFu) | (t[1] & 0xFFFF0000u), 0u);
         }
     };
 
-    floatx16_t o[DB];
+    const floatx4_t zeros = {0.0f, 0.0f, 0.0f, 0.0f};
+    floatx4_t o[ND];
 #pragma unroll
-    for (int d = 0; d < DB; d++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
+    for (int d = 0; d < ND; d++) o[d] = zeros;
     float m = -1.0e30f, l = 0.0f, ones[G], accb[G];
 #pragma unroll
     for (int g = 0; g < G; g++) ones[g] = accb[g] = 0.0f;
 
-    // 32 keys from s0 on, half `sub` of the stage.  (One piece of code: a second for masked tiles cost forty registers, which there are not.)
-    auto tile = [&](const Stage &from, int s0, int sub, bool masked) __attribute__((always_inline)) {
-        const int base = 32 * sub + 4 * half;  // register e: key 8 (e / 4) + e % 4 from there
-        float x[16];
+    // The weights of 32 keys, half `sub` of the stage, times their values.
+    auto values = [&](const Stage &from, int sub, const float (&x)[8]) __attribute__((always_inline)) {
 #pragma unroll
         for (int g = 0; g < G; g++) {
-            floatx16_t s;
+            uint32_t p[TP][4];
 #pragma unroll
-            for (int e = 0; e < 16; e++) s[e] = 0.0f;
+            for (int t = 0; t < 2; t++) {
+                const int at = 32 * sub + 16 * t + 4 * quarter;
+                const float4 sv = *reinterpret_cast<const float4 *>(&from.scale[1][g][at]), bv = *reinterpret_cast<const float4 *>(&from.scale[2][g][at]);
+                const float *e = x + 4 * t;
+                accb[g] = __builtin_fmaf(e[0], bv.x, accb[g]), accb[g] = __builtin_fmaf(e[1], bv.y, accb[g]);
+                accb[g] = __builtin_fmaf(e[2], bv.z, accb[g]), accb[g] = __builtin_fmaf(e[3], bv.w, accb[g]);
+                uint32_t w[TP];
+                split_pair<TP>(sv.x * e[0], sv.y * e[1], w);
 #pragma unroll
-            for (int k = g * GS; k < (g + 1) * GS; k++) s = qmf::Ops<T>::mfma(from.keys[sub][k][lane], qf[k], s);
-            const float sum = qsum[g];
+                for (int i = 0; i < TP; i++) p[i][2 * t] = w[i];
+                split_pair<TP>(sv.z * e[2], sv.w * e[3], w);
 #pragma unroll
-            for (int q4 = 0; q4 < 4; q4++) {
-                const float4 sk = *reinterpret_cast<const float4 *>(&from.scale[0][g][base + 8 * q4]), bk = *reinterpret_cast<const float4 *>(&from.scale[1][g][base + 8 * q4]);
-                auto one = [&](int i, float ss, float bb) __attribute__((always_inline)) {
-                    const int e = 4 * q4 + i;
-                    const float v = g == 0 ? bb * sum : __builtin_fmaf(bb, sum, x[e]);
-                    x[e] = __builtin_fmaf(ss, s[e], v);
-                };
-                one(0, sk.x, bk.x), one(1, sk.y, bk.y), one(2, sk.z, bk.z), one(3, sk.w, bk.w);
-            }
-        }
-        if (masked) {
-            asm volatile("");  // (a branch: as selects it would cost every tile)
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int key = s0 + 4 * half + 8 * (e >> 2) + (e & 3);
-                if (key > my_last || key < my_first || key >= S) x[e] = -INFINITY;
-            }
-        }
-        float top = x[0];
-#pragma unroll
-        for (int e = 1; e < 16; e++) top = fmaxf(top, x[e]);
-        // Rescaled only when a maximum has grown by more than 2^8: until then the weights are at most 2^8.
-        if (__any(top > m + 8.0f)) {
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float m_new = fmaxf(m, top), f = exp2f(m - m_new);
-            m = m_new, l *= f;
-#pragma unroll
-            for (int g = 0; g < G; g++) ones[g] *= f, accb[g] *= f;
-#pragma unroll
-            for (int d = 0; d < DB; d++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) o[d][e] *= f;
-        }
-#pragma unroll
-        for (int e = 0; e < 16; e++) x[e] = __builtin_amdgcn_exp2f(x[e] - m), l += x[e];
-        // Values whose scales are not finite were made zeros, so that lines that do not see them stay clean: those that do get a NaN.
-        uint32_t wild[G], any = 0;
-#pragma unroll
-        for (int g = 0; g < G; g++) wild[g] = *reinterpret_cast<const uint32_t *>(from.wild[sub][g]), any |= wild[g];
-        if (uniform((int32_t)any) != 0) {
-            asm volatile("");
-#pragma unroll
-            for (int g = 0; g < G; g++)
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    if (x[e] != 0.0f && (wild[g] >> (4 * half + 8 * (e >> 2) + (e & 3)) & 1) != 0) accb[g] = NAN;
-        }
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-            uint32_t p[TP][8];
-#pragma unroll
-            for (int q4 = 0; q4 < 4; q4++) {
-                float4 sv = *reinterpret_cast<const float4 *>(&from.scale[2][g][base + 8 * q4]), bv = *reinterpret_cast<const float4 *>(&from.scale[3][g][base + 8 * q4]);
-                auto one = [&](int i, float &ss, float bb) __attribute__((always_inline)) {
-                    const int e = 4 * q4 + i;
-                    accb[g] = __builtin_fmaf(x[e], bb, accb[g]);
-                    ss *= x[e];
-                };
-                one(0, sv.x, bv.x), one(1, sv.y, bv.y), one(2, sv.z, bv.z), one(3, sv.w, bv.w);
-                uint32_t t[TP];
-                split_pair<TP>(sv.x, sv.y, t);
-#pragma unroll
-                for (int i = 0; i < TP; i++) p[i][2 * q4] = t[i];
-                split_pair<TP>(sv.z, sv.w, t);
-#pragma unroll
-                for (int i = 0; i < TP; i++) p[i][2 * q4 + 1] = t[i];
+                for (int i = 0; i < TP; i++) p[i][2 * t + 1] = w[i];
             }
             typedef __bf16 pair_t __attribute__((ext_vector_type(2)));
             const pair_t one2 = {(__bf16)1.0f, (__bf16)1.0f};
 #pragma unroll
             for (int i = 0; i < TP; i++)
 #pragma unroll
-                for (int w = 0; w < 8; w++) ones[g] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair_t, p[i][w]), one2, ones[g], false);
+                for (int w = 0; w < 4; w++) ones[g] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair_t, p[i][w]), one2, ones[g], false);
 #pragma unroll
-            for (int t = 0; t < 2; t++)
+            for (int d = g * GB; d < (g + 1) * GB; d++) {
+                const uint4 v = from.values[sub][d][lane];
 #pragma unroll
-                for (int d = g * DB / G; d < g * DB / G + GB; d++) {
-                    const uint4 v = from.values[2 * sub + t][d][half * 36 + col + (col >> 2 & 4)];
+                for (int i = 0; i < TP; i++) o[d] = mfma16(v, make_uint4(p[i][0], p[i][1], p[i][2], p[i][3]), o[d]);
+            }
+        }
+    };
+    // A tile of 64 keys from s0 on: the scores, one look at their maximum, the weights and their products.  x[u][4 t + e]: key 32 u + 16 t + 4 quarter + e.
+    auto tile = [&](const Stage &from, int s0) __attribute__((always_inline)) {
+        float x[2][8];
 #pragma unroll
-                    for (int i = 0; i < TP; i++) o[d] = qmf::Ops<bf16_t>::mfma(v, make_uint4(p[i][4 * t], p[i][4 * t + 1], p[i][4 * t + 2], p[i][4 * t + 3]), o[d]);
+        for (int t = 0; t < 4; t++) {
+            floatx4_t sum = mfma16(from.key_bias[t][lane], qb, zeros);
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                floatx4_t s = zeros;
+#pragma unroll
+                for (int k = g * GS; k < (g + 1) * GS; k++) s = key_product<T>(from.keys[t][k][lane], qf[k], s);
+                const float4 sk = *reinterpret_cast<const float4 *>(&from.scale[0][g][16 * t + 4 * quarter]);
+                sum[0] = __builtin_fmaf(sk.x, s[0], sum[0]), sum[1] = __builtin_fmaf(sk.y, s[1], sum[1]);
+                sum[2] = __builtin_fmaf(sk.z, s[2], sum[2]), sum[3] = __builtin_fmaf(sk.w, s[3], sum[3]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[t >> 1][4 * (t & 1) + e] = sum[e];
+        }
+        if (s0 + kStageKeys - 1 > all_last || s0 < all_first || s0 + kStageKeys > s_end) {
+            asm volatile("");  // (a branch: as selects it would cost every tile)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int key = s0 + 32 * u + 16 * (e >> 2) + 4 * quarter + (e & 3);
+                    if (key > my_last || key < my_first || key >= s_end) x[u][e] = -INFINITY;
                 }
+        }
+        float top = x[0][0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) top = fmaxf(top, x[e >> 3][e & 7]);
+        // Rescaled only when a maximum has grown by more than 2^8: until then the weights are at most 2^8.
+        if (__any(top > m + 8.0f)) {
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float m_new = fmaxf(m, top), f = exp2f(m - m_new);
+            m = m_new, l *= f;
+#pragma unroll
+            for (int g = 0; g < G; g++) ones[g] *= f, accb[g] *= f;
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[d][e] *= f;
+        }
+        // Values whose scales are not finite were made zeros, so that lines that do not see them stay clean: those that do get a NaN.
+        uint32_t any = 0;
+#pragma unroll
+        for (int g = 0; g < G; g++) any |= *reinterpret_cast<const uint32_t *>(from.wild[0][g]) | *reinterpret_cast<const uint32_t *>(from.wild[1][g]);
+        if (uniform((int32_t)any) != 0) {
+            asm volatile("");
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int bit = 16 * (e >> 2 & 1) + 4 * quarter + (e & 3);
+                    if (x[e >> 3][e & 7] > -INFINITY && (*reinterpret_cast<const uint32_t *>(from.wild[e >> 3][g]) >> bit & 1) != 0) accb[g] = NAN;
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[u][e] = __builtin_amdgcn_exp2f(x[u][e] - m), l += x[u][e];
+            values(from, u, x[u]);
         }
     };
 
@@ -328,24 +364,21 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
         const bool more = s0 + kStageKeys < s_end;
         if (more) request(next, s0 + kStageKeys);
         next = look_up(s0 + 2 * kStageKeys);
-#pragma unroll 1
-        for (int sub = 0; sub < 2; sub++) {
-            const int k0 = s0 + 32 * sub;
-            if (k0 > any_last || k0 >= s_end || k0 + 31 < any_first) continue;  // (uniform in the wavefront)
-            tile(stages[at], k0, sub, k0 + 31 > all_last || k0 < all_first || k0 + 31 >= S);
-        }
+        if (s0 <= any_last && s0 + kStageKeys > any_first) tile(stages[at], s0);  // (uniform in the wavefront)
         if (more) expand(stages[at ^ 1]);
         __syncthreads();
         at ^= 1;
     }
+    l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
 #pragma unroll
     for (int g = 0; g < G; g++) {
+        ones[g] += __shfl_xor(ones[g], 16), accb[g] += __shfl_xor(accb[g], 16);
         ones[g] += __shfl_xor(ones[g], 32), accb[g] += __shfl_xor(accb[g], 32);
         accb[g] = __builtin_fmaf(-(kValueOff + kMiddle), ones[g], accb[g]);  // (the operands and kValueOff + kMiddle went through the same weights)
     }
     if (!live) return;
-    const bool whole = span.end_split - span.first_split == 1;
+    const bool whole = span.items == 1;
     float inv = 1.0f;
     float *state = nullptr;  // of this line and split: maximum, denominator, weighted sums
     if (whole) {
@@ -356,24 +389,22 @@ __global__ void __launch_bounds__(64 * kWaves, 2) paged_prompt_kernel(const Rows
         }
         inv = denom == 0.0f ? 0.0f : f / denom;  // (a row that sees nothing: zeros)
     } else {
-        state = a.states + ((int64_t)item.slot * kPromptLines + wave * 32 + col) * kState<D>;
-        if (half == 0) *reinterpret_cast<float2 *>(state) = make_float2(m, l);
+        state = a.states + ((int64_t)item.slot * kPromptLines + wave * 16 + col) * kState<D>;
+        if (quarter == 0) *reinterpret_cast<float2 *>(state) = make_float2(m, l);
     }
     T *out = a.out + (int64_t)(item.s.start + my_row) * a.out_strides[0] + (int64_t)my_head * a.out_strides[1];
 #pragma unroll
-    for (int d = 0; d < DB; d++)
-#pragma unroll
-        for (int q4 = 0; q4 < 4; q4++) {
-            const int c = 32 * d + 8 * q4 + 4 * half;
-            const float b = accb[d * G / DB];
-            const float v0 = o[d][4 * q4] + b, v1 = o[d][4 * q4 + 1] + b, v2 = o[d][4 * q4 + 2] + b, v3 = o[d][4 * q4 + 3] + b;
-            if (whole) {
-                struct __attribute__((packed)) Four { uint32_t w[2]; };
-                *reinterpret_cast<Four *>(out + c) = Four{{qmf::Ops<T>::pack(v0 * inv, v1 * inv), qmf::Ops<T>::pack(v2 * inv, v3 * inv)}};
-            } else {
-                *reinterpret_cast<float4 *>(state + 4 + c) = make_float4(v0, v1, v2, v3);
-            }
+    for (int d = 0; d < ND; d++) {
+        const int c = 16 * d + 4 * quarter;
+        const float b = accb[d / GB];
+        const float v0 = o[d][0] + b, v1 = o[d][1] + b, v2 = o[d][2] + b, v3 = o[d][3] + b;
+        if (whole) {
+            struct __attribute__((packed)) Four { uint32_t w[2]; };
+            *reinterpret_cast<Four *>(out + c) = Four{{qmf::Ops<T>::pack(v0 * inv, v1 * inv), qmf::Ops<T>::pack(v2 * inv, v3 * inv)}};
+        } else {
+            *reinterpret_cast<float4 *>(state + 4 + c) = make_float4(v0, v1, v2, v3);
         }
+    }
 }
 
 // The splits of many lines merged: D / 4 threads a line, four splits' loads under way at a time.
@@ -381,21 +412,21 @@ template <typename T, int D>
 __global__ void __launch_bounds__(64 * kWaves) paged_merge_many_kernel(const RowsArgs<T> a) {
     constexpr int kThreads = D / 4, kLines = 64 * kWaves / kThreads;
     PagedItem item;
-    if (!paged_item<kPromptLines, 1, true>(a.batch, threadIdx.x & 63, blockIdx.x, item)) return;
+    if (!paged_item<kPromptLines, 1, true>(a.batch, threadIdx.x & 63, blockIdx.x, a.length, item)) return;
     const int rep = a.batch.rep, ln = blockIdx.y * kLines + (int)threadIdx.x / kThreads, at = (int)threadIdx.x % kThreads * 4;
     const int part = item.s.parts - 1 - item.part, line = part * kPromptLines + ln;  // (items count the parts from the last)
     const PromptSpan span = prompt_span(a.batch, item, part);
-    if (line >= item.s.rows * rep || span.end_split - span.first_split == 1) return;
+    if (line >= item.s.rows * rep || span.items == 1) return;
     const int64_t stride = (int64_t)a.batch.key_heads * kPromptLines * kState<D>;  // of a split's states
     const float *src = a.states + ((int64_t)item.slot * kPromptLines + ln) * kState<D>;
     float top = -1.0e30f, total = 0.0f;
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int z0 = span.first_split; z0 < span.end_split; z0 += 4) {
+    for (int z0 = 0; z0 < span.items; z0 += 4) {
         float2 m[4];
         float4 v[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float *state = src + (z0 + i < span.end_split ? z0 + i : z0) * stride;
+            const float *state = src + (z0 + i < span.items ? z0 + i : z0) * stride;
             m[i] = *reinterpret_cast<const float2 *>(state), v[i] = *reinterpret_cast<const float4 *>(state + 4 + at);
         }
         float most = top;
@@ -405,7 +436,7 @@ __global__ void __launch_bounds__(64 * kWaves) paged_merge_many_kernel(const Row
         top = most, total *= f, sum.x *= f, sum.y *= f, sum.z *= f, sum.w *= f;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float w = z0 + i < span.end_split ? exp2f(m[i].x - top) : 0.0f;
+            const float w = z0 + i < span.items ? exp2f(m[i].x - top) : 0.0f;
             total = __builtin_fmaf(m[i].y, w, total);
             sum.x = __builtin_fmaf(v[i].x, w, sum.x), sum.y = __builtin_fmaf(v[i].y, w, sum.y);
             sum.z = __builtin_fmaf(v[i].z, w, sum.z), sum.w = __builtin_fmaf(v[i].w, w, sum.w);
@@ -433,7 +464,7 @@ int32_t launch_merge_many(const RowsArgs<T> &a, const PagedLaunch &r, hipStream_
 
 template <typename T, int BITS>
 int32_t launch_prompt_bits(const RowsArgs<T> &a, const nvq_paged_desc &c, uint32_t grid, hipStream_t s) {
-#define NVQ_PROMPT(D, G) hipLaunchKernelGGL((paged_prompt_kernel<T, BITS, D, G>), dim3(grid), dim3(64 * kWaves), 0, s, a, a.batch.place.table)
+#define NVQ_PROMPT(D, G) hipLaunchKernelGGL((paged_prompt_kernel<T, BITS, D, G>), dim3(grid), dim3(64 * kPromptWaves), 0, s, a, a.batch.place.table)
     if (c.head_dim == 64 && c.group_size == 32) NVQ_PROMPT(64, 2);
     else if (c.head_dim == 64) NVQ_PROMPT(64, 1);
     else if (c.group_size == 32) NVQ_PROMPT(128, 4);

@@ -35,7 +35,8 @@ struct RowsArgs {
     const T *q, *ks, *kb, *vs, *vb, *sinks;
     const uint32_t *kw, *vw;
     T *out;
-    float *states;  // [slots][LINES][kState<D>]: maximum of the base-2 scores, denominator, two unused, D weighted sums
+    int32_t *length;  // of the plan, for the merge; NULL: no merge
+    float *states;    // [slots][LINES][kState<D>]: maximum of the base-2 scores, denominator, two unused, D weighted sums
     int64_t q_strides[2], out_strides[2];
     float scale;
 };
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(64 * kWaves, (rows_blocks<T, G>())) paged_rows
     const float scale = a.scale * kLog2e;
     const CodeConstants<BITS> constants;
     PagedItem item;
-    if (!paged_item<R, 0, false>(a.batch, lane, blockIdx.x, item)) return;
+    if (!paged_item<R, 0, false>(a.batch, lane, blockIdx.x, a.length, item)) return;
     const int rep = a.batch.rep, hk = item.head, S = item.s.length, n = item.s.rows;
     const int lines = n * rep - item.part * R < R ? n * rep - item.part * R : R;  // of this unit
     // the keys that row i of n sees
@@ -378,7 +379,7 @@ __global__ void __launch_bounds__(64 * kWaves) paged_merge_kernel(const RowsArgs
     __shared__ float sums[kWaves][D], tops[kWaves], totals[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     PagedItem item;
-    if (!paged_item<LINES, 0, true>(a.batch, lane, blockIdx.x, item)) return;
+    if (!paged_item<LINES, 0, true>(a.batch, lane, blockIdx.x, a.length, item)) return;
     const int rep = a.batch.rep, ln = blockIdx.y, line = item.part * LINES + ln;
     if (line >= item.s.rows * rep) return;
     const int64_t stride = (int64_t)a.batch.key_heads * LINES * kState<D>;  // of a split's states
@@ -461,7 +462,8 @@ RowsArgs<T> rows_args(const nvq_paged_attention_desc &d, const PagedAttentionOpe
     RowsArgs<T> a{};
     a.batch = r.batch;
     a.q = (const T *)o.q, a.ks = (const T *)o.ks, a.kb = (const T *)o.kb, a.vs = (const T *)o.vs, a.vb = (const T *)o.vb, a.sinks = (const T *)o.sinks;
-    a.kw = (const uint32_t *)o.kw, a.vw = (const uint32_t *)o.vw, a.out = (T *)o.out, a.states = (float *)((char *)o.workspace + r.states);
+    a.kw = (const uint32_t *)o.kw, a.vw = (const uint32_t *)o.vw, a.out = (T *)o.out, a.states = (float *)((char *)o.workspace + r.states + kPlanBytes);
+    a.length = r.merge_units > 0 ? (int32_t *)((char *)o.workspace + r.states) : nullptr;
     for (int i = 0; i < 2; i++) a.q_strides[i] = d.q_strides[i], a.out_strides[i] = d.out_strides[i];
     a.scale = d.scale;
     return a;

@@ -79,6 +79,14 @@ __device__ __forceinline__ double wave_total(double v) {
     return __builtin_bit_cast(double, (uint64_t)lo | (uint64_t)hi << 32);
 }
 
+// What all lanes hold, as the compiler can see: in a scalar register, and branches on it without masks of lanes.  (Of a value that has come
+// through the search for an item the move alone is folded away, and the value taken for one that differs by lane.)
+__device__ __forceinline__ int32_t uniform(int32_t v) {
+    v = __builtin_amdgcn_readfirstlane(v);
+    asm("" : "+s"(v));
+    return v;
+}
+
 struct PagedPlan {
     int32_t per, items;  // tiles of an item; items of all sequences
     __device__ __forceinline__ int32_t splits(const PagedSequence &s) const { return s.tiles <= per ? 1 : (s.tiles + per - 1) / per; }
@@ -148,19 +156,18 @@ __device__ __forceinline__ bool paged_find(const PagedBatch &a, const PagedPlan 
     return false;
 }
 
-// What all lanes hold, as the compiler can see: in a scalar register, and branches on it without masks of lanes.  (Of a value that has come
-// through the search for an item the move alone is folded away, and the value taken for one that differs by lane.)
-__device__ __forceinline__ int32_t uniform(int32_t v) {
-    v = __builtin_amdgcn_readfirstlane(v);
-    asm("" : "+s"(v));
-    return v;
-}
-
-// Item (or unit) `at` of the whole plan; false behind the last.
+// Item (or unit, which comes after the items) `at` of the whole plan; false behind the last.  `length`: where the first block of the items leaves the
+// plan's length for the units'; NULL: nothing is split.
 template <int LINES, int KIND, bool UNITS>
-__device__ __forceinline__ bool paged_item(const PagedBatch &a, int lane, int32_t at, PagedItem &item) {
+__device__ __forceinline__ bool paged_item(const PagedBatch &a, int lane, int32_t at, int32_t *length, PagedItem &item) {
     const PagedSequence first = paged_sequence<LINES, KIND>(a, lane);
-    const PagedPlan plan = paged_plan<LINES, KIND>(a, lane, first);
+    PagedPlan plan;
+    if constexpr (UNITS) {
+        plan.per = *length, plan.items = INT32_MAX;
+    } else {
+        plan = paged_plan<LINES, KIND>(a, lane, first);
+        if (at == 0 && threadIdx.x == 0 && length != nullptr) *length = plan.per;
+    }
     const bool found = at < plan.items && paged_find<LINES, KIND, UNITS>(a, plan, lane, first, at, item);
     if (uniform(found) == 0) return false;
     const PagedSequence &s = item.s;
