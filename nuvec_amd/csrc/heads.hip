@@ -7,8 +7,8 @@
 // Bound by memory: each value is read and written once, but for the partner's run of eight, which the lane that turns it reads
 // too, from lines that are in the L1 by then.  A block takes 256 / P tokens and walks heads of them, so that a token's angles (eight bytes a
 // pair, more than a 16-bit head itself) are read once for all of a block's heads, and the norm's weight too; a head is requested before the one
-in front of it is worked on.  Measured, bfloat16, 2 x 2049 tokens, 40 heads of 128 with norms: 20.2 us, 4.3 TB/s (a large copy: 4.9; the weight
-read for each head: 23.5 us); a call of few tokens is one launch, 4.6 to 5 us.
+// in front of it is worked on.  Measured, bfloat16, 2 x 2049 tokens, 40 heads of 128 with norms: 20.2 us, 4.3 TB/s (a large copy: 4.9; the weight
+// read for each head: 23.5 us); a call of few tokens is one launch, 4.6 to 5 us.
 #include "heads.h"
 #include "nvq_internal.h"
 

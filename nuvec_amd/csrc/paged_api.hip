@@ -99,7 +99,8 @@ int32_t nvq_append_paged(const nvq_paged_append_desc *d, const int32_t *page_tab
     NVQ_TRY(check_rotation(op, c.head_dim, d->rotary_dims, d->table_rows, table));
     NVQ_TRY(check_eps(op, d->eps));
     if (d->tokens < 0 || d->query_heads < 0) return fail(NVQ_INVALID_ARGUMENT, "%s: negative size", op);
-    if (d->tokens >= 1LL << 32 || d->query_heads >= 1 << 15) return fail(NVQ_UNSUPPORTED, "%s: more than 2^32 tokens or 2^15 query heads", op);
+    if (d->tokens >= 1LL << 32 || d->query_heads + 2 * c.key_heads >= 1 << 16)  // (a row of blocks a head where there are few tokens)
+        return fail(NVQ_UNSUPPORTED, "%s: more than 2^32 tokens or 2^16 heads of them", op);
     const bool queries = q != nullptr && d->query_heads > 0;
     if (d->tokens == 0 || (c.key_heads == 0 && !queries)) return NVQ_OK;
     if (positions == nullptr || (c.key_heads > 0 && (k == nullptr || v == nullptr)) || (queries && q_out == nullptr))

@@ -13,8 +13,8 @@
 // Bound by memory when there are many tokens, by one round trip for the table, one for the inputs and one for the page's id when there
 // are few.  A block takes 256 / P tokens of a head at a time (P lanes a head), so that the codes, scales and biases of consecutive
 // positions, which lie together, are written by one block; a head is requested before the one in front of it is quantized.  Measured,
-bfloat16 to 4 bits in groups of 64: 6000 tokens of 32 query heads and 8 key heads of 128 in 32 us, 4.1 TB/s; 64 tokens with norms in 5 us, a
-launch; the 6000 tokens read back in 11 us, 2.9 TB/s.
+// bfloat16 to 4 bits in groups of 64: 6000 tokens of 32 query heads and 8 key heads of 128 in 32 us, 4.1 TB/s; 64 tokens with norms in 5 us, a
+// launch; the 6000 tokens read back in 11 us, 2.9 TB/s.
 #include "heads.h"
 #include "nvq_internal.h"
 #include "paged.h"

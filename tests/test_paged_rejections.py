@@ -122,6 +122,8 @@ def test_null_operands():
     assert lib.nvq_append_paged(C.byref(p), *none * 17) == _lib.INVALID_ARGUMENT and "130 rotary values of heads of 128" in _lib.last_error()
     p.rotary_dims = 64
     assert lib.nvq_append_paged(C.byref(p), *none * 17) == _lib.INVALID_ARGUMENT and "no table" in _lib.last_error()
+    p.rotary_dims, p.query_heads = 0, (1 << 16) - 4  # (with the two key heads' keys and values 2^16)
+    assert lib.nvq_append_paged(C.byref(p), *none * 17) == _lib.UNSUPPORTED
     assert lib.nvq_read_paged(C.byref(paged()), 1, *none * 12) == _lib.INVALID_ARGUMENT
     r = _lib.HeadRopeDescC(_lib.BF16, 64, 0, 0, 0, 0, 1, 1)
     r.heads[0] = 1
