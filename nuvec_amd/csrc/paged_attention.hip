@@ -44,8 +44,11 @@ Kernel kernel_of(const nvq_paged_attention_desc &d, bool many) {
     return k;
 }
 
-// (the device decides by the lengths, which are at most the table's columns)
-bool may_split(const nvq_paged_attention_desc &d) { return d.cache.columns * d.cache.page_size > kScheduleKeys * kScheduleTiles; }
+// Tiles of an item at least, of few and of many lines.  (4 in place of 8 for many: one prompt of 20 rows over 300 positions 21 -> 16 us, three of 45 over
+// 500 27 -> 24, one of 512 over as many 27.5 -> 29.4.)
+constexpr int32_t kLeastFew = 8, kLeastMany = 4;
+// (the device decides by the lengths, which are at most the table's columns; up to 8 tiles a second launch costs more than it saves)
+bool may_split(const nvq_paged_attention_desc &d) { return d.cache.columns * d.cache.page_size > kScheduleKeys * kLeastFew; }
 // Whether a sequence may have more lines than the kernel of few takes.
 bool takes_many(const nvq_paged_attention_desc &d, bool starts) {
     const int64_t most = d.max_queries < d.rows ? d.max_queries : d.rows;
@@ -74,7 +77,8 @@ int32_t launch_paged_attention(const nvq_paged_attention_desc &d, const PagedAtt
         if (starts) units = of_many ? d.rows * rep / k.lines + c.sequences : (d.rows * rep + k.lines - 1) / k.lines + c.sequences;
         if (many && !of_many && units > c.sequences * each) units = c.sequences * each;
         units *= c.key_heads;
-        const int64_t splits = (c.columns * c.page_size + kScheduleKeys * kScheduleTiles - 1) / (kScheduleKeys * kScheduleTiles), full = k.target, spare = full / 2 + units;
+        r.batch.least = !may_split(d) ? 1 << 26 : of_many ? kLeastMany : kLeastFew;
+        const int64_t least = (int64_t)kScheduleKeys * r.batch.least, splits = (c.columns * c.page_size + least - 1) / least, full = k.target, spare = full / 2 + units;
         const int64_t items = full > spare ? full : spare;
         r.grid = (uint32_t)(units * splits < items ? units * splits : items);
         r.merge_units = may_split(d) ? (uint32_t)(units < full ? units : full) : 0;
@@ -82,12 +86,13 @@ int32_t launch_paged_attention(const nvq_paged_attention_desc &d, const PagedAtt
         r.states = of_many ? kernel_of(d, false).bytes : 0;
         return r;
     };
+    paged::PagedLaunch few{};
     if (!alone) {
-        const paged::PagedLaunch few = launch_of(false);
+        few = launch_of(false), few.merged_later = many;
         const int32_t rc = c.dtype == NVQ_F32 ? paged::launch_rows_f32(d, o, few, s) : c.dtype == NVQ_BF16 ? paged::launch_rows_bf16(d, o, few, s) : paged::launch_rows_f16(d, o, few, s);
         if (rc != NVQ_OK || !many) return rc;
     }
-    return c.dtype == NVQ_BF16 ? paged::launch_prompt_bf16(d, o, launch_of(true), s) : paged::launch_prompt_f16(d, o, launch_of(true), s);
+    return c.dtype == NVQ_BF16 ? paged::launch_prompt_bf16(d, o, few, launch_of(true), s) : paged::launch_prompt_f16(d, o, few, launch_of(true), s);
 }
 
 }  // namespace nvq

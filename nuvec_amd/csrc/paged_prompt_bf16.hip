@@ -4,8 +4,8 @@
 namespace nvq {
 namespace paged {
 
-int32_t launch_prompt_bf16(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const PagedLaunch &r, hipStream_t s) {
-    return launch_prompt<bf16_t>(d, o, r, s);
+int32_t launch_prompt_bf16(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const PagedLaunch &few, const PagedLaunch &r, hipStream_t s) {
+    return launch_prompt<bf16_t>(d, o, few, r, s);
 }
 
 }  // namespace paged

@@ -65,7 +65,7 @@ __device__ __forceinline__ PromptSpan prompt_span(const PagedBatch &a, const Pag
     PromptSpan s{uniform(begin), uniform(end), 0, 1};
     const int32_t tiles = end > begin ? (end - begin + kTile - 1) / kTile : 0;
     int32_t per = (tiles + item.splits - 1) / item.splits;
-    per = per > kScheduleTiles ? per : kScheduleTiles;
+    per = per > a.least ? per : a.least;
     s.keys = uniform(item.splits == 1 ? tiles * kTile : per * kTile), s.items = uniform(item.splits == 1 || tiles <= per ? 1 : (tiles + per - 1) / per);
     return s;
 }
@@ -408,12 +408,13 @@ __global__ void __launch_bounds__(64 * kPromptWaves, 4) paged_prompt_kernel(cons
 }
 
 // The splits of many lines merged: D / 4 threads a line, four splits' loads under way at a time.
+template <int D> constexpr int kMergeLines = 64 * kWaves / (D / 4);  // of a block
 template <typename T, int D>
-__global__ void __launch_bounds__(64 * kWaves) paged_merge_many_kernel(const RowsArgs<T> a) {
-    constexpr int kThreads = D / 4, kLines = 64 * kWaves / kThreads;
+__device__ __forceinline__ void merge_many(const RowsArgs<T> &a, int32_t unit, int block) {
+    constexpr int kThreads = D / 4;
     PagedItem item;
-    if (!paged_item<kPromptLines, 1, true>(a.batch, threadIdx.x & 63, blockIdx.x, a.length, item)) return;
-    const int rep = a.batch.rep, ln = blockIdx.y * kLines + (int)threadIdx.x / kThreads, at = (int)threadIdx.x % kThreads * 4;
+    if (!paged_item<kPromptLines, 1, true>(a.batch, threadIdx.x & 63, unit, a.length, item)) return;
+    const int rep = a.batch.rep, ln = block * kMergeLines<D> + (int)threadIdx.x / kThreads, at = (int)threadIdx.x % kThreads * 4;
     const int part = item.s.parts - 1 - item.part, line = part * kPromptLines + ln;  // (items count the parts from the last)
     const PromptSpan span = prompt_span(a.batch, item, part);
     if (line >= item.s.rows * rep || span.items == 1) return;
@@ -454,33 +455,36 @@ __global__ void __launch_bounds__(64 * kWaves) paged_merge_many_kernel(const Row
         Four{{qmf::Ops<T>::pack(sum.x * inv, sum.y * inv), qmf::Ops<T>::pack(sum.z * inv, sum.w * inv)}};
 }
 
-template <typename T, int D>
-int32_t launch_merge_many(const RowsArgs<T> &a, const PagedLaunch &r, hipStream_t s) {
-    constexpr int kLines = 64 * kWaves / (D / 4);
-    hipLaunchKernelGGL((paged_merge_many_kernel<T, D>), dim3(r.merge_units, (r.merge_lines + kLines - 1) / kLines), dim3(64 * kWaves), 0, s, a);
+// Both kernels' splits in one launch (nine sequences of one to 200 rows 49 -> 46 us): the blocks of few lines, a line each, behind those of many.
+template <typename T, int D, int LINES>
+__global__ void __launch_bounds__(64 * kWaves) paged_merge_both_kernel(const RowsArgs<T> few, const RowsArgs<T> many, uint32_t many_units, uint32_t few_units) {
+    const uint32_t many_blocks = many_units * (kPromptLines / kMergeLines<D>), at = blockIdx.x - many_blocks;
+    if (blockIdx.x < many_blocks) merge_many<T, D>(many, blockIdx.x % many_units, blockIdx.x / many_units);
+    else merge_few<T, D, LINES>(few, at % few_units, at / few_units);
+}
+
+template <typename T, int BITS, int D, int G>
+int32_t launch_prompt_sized(const RowsArgs<T> &few, const RowsArgs<T> &a, const PagedLaunch &f, const PagedLaunch &r, hipStream_t s) {
+    hipLaunchKernelGGL((paged_prompt_kernel<T, BITS, D, G>), dim3(r.grid), dim3(64 * kPromptWaves), 0, s, a, a.batch.place.table);
+    NVQ_LAUNCH_CHECK("paged_attention");
+    if (r.merge_units == 0) return NVQ_OK;
+    const uint32_t blocks = r.merge_units * (kPromptLines / kMergeLines<D>) + f.merge_units * f.merge_lines;
+    hipLaunchKernelGGL((paged_merge_both_kernel<T, D, 16 / G>), dim3(blocks), dim3(64 * kWaves), 0, s, few, a, r.merge_units, f.merge_units);
     NVQ_LAUNCH_CHECK("paged_attention merge");
     return NVQ_OK;
 }
 
 template <typename T, int BITS>
-int32_t launch_prompt_bits(const RowsArgs<T> &a, const nvq_paged_desc &c, uint32_t grid, hipStream_t s) {
-#define NVQ_PROMPT(D, G) hipLaunchKernelGGL((paged_prompt_kernel<T, BITS, D, G>), dim3(grid), dim3(64 * kPromptWaves), 0, s, a, a.batch.place.table)
-    if (c.head_dim == 64 && c.group_size == 32) NVQ_PROMPT(64, 2);
-    else if (c.head_dim == 64) NVQ_PROMPT(64, 1);
-    else if (c.group_size == 32) NVQ_PROMPT(128, 4);
-    else if (c.group_size == 64) NVQ_PROMPT(128, 2);
-    else NVQ_PROMPT(128, 1);
-#undef NVQ_PROMPT
-    NVQ_LAUNCH_CHECK("paged_attention");
-    return NVQ_OK;
+int32_t launch_prompt_bits(const nvq_paged_desc &c, const RowsArgs<T> &few, const RowsArgs<T> &a, const PagedLaunch &f, const PagedLaunch &r, hipStream_t s) {
+    if (c.head_dim == 64) return c.group_size == 32 ? launch_prompt_sized<T, BITS, 64, 2>(few, a, f, r, s) : launch_prompt_sized<T, BITS, 64, 1>(few, a, f, r, s);
+    if (c.group_size == 32) return launch_prompt_sized<T, BITS, 128, 4>(few, a, f, r, s);
+    return c.group_size == 64 ? launch_prompt_sized<T, BITS, 128, 2>(few, a, f, r, s) : launch_prompt_sized<T, BITS, 128, 1>(few, a, f, r, s);
 }
 
 template <typename T>
-int32_t launch_prompt(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const PagedLaunch &r, hipStream_t s) {
-    const RowsArgs<T> a = rows_args<T>(d, o, r);
-    const int32_t rc = d.cache.bits == 4 ? launch_prompt_bits<T, 4>(a, d.cache, r.grid, s) : launch_prompt_bits<T, 8>(a, d.cache, r.grid, s);
-    if (rc != NVQ_OK || r.merge_units == 0) return rc;
-    return d.cache.head_dim == 64 ? launch_merge_many<T, 64>(a, r, s) : launch_merge_many<T, 128>(a, r, s);
+int32_t launch_prompt(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, const PagedLaunch &f, const PagedLaunch &r, hipStream_t s) {
+    const RowsArgs<T> few = rows_args<T>(d, o, f), a = rows_args<T>(d, o, r);
+    return d.cache.bits == 4 ? launch_prompt_bits<T, 4>(d.cache, few, a, f, r, s) : launch_prompt_bits<T, 8>(d.cache, few, a, f, r, s);
 }
 
 }  // namespace

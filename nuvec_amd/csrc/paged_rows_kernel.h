@@ -374,13 +374,13 @@ __global__ void __launch_bounds__(64 * kWaves, (rows_blocks<T, G>())) paged_rows
 
 // The splits of a line merged, one block a line: its wavefronts take them in turn, eight loads under way at a time, and add up through LDS.
 template <typename T, int D, int LINES>
-__global__ void __launch_bounds__(64 * kWaves) paged_merge_kernel(const RowsArgs<T> a) {
+__device__ __forceinline__ void merge_few(const RowsArgs<T> &a, int32_t unit, int ln) {
     constexpr int V = D / 64;
     __shared__ float sums[kWaves][D], tops[kWaves], totals[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     PagedItem item;
-    if (!paged_item<LINES, 0, true>(a.batch, lane, blockIdx.x, a.length, item)) return;
-    const int rep = a.batch.rep, ln = blockIdx.y, line = item.part * LINES + ln;
+    if (!paged_item<LINES, 0, true>(a.batch, lane, unit, a.length, item)) return;
+    const int rep = a.batch.rep, line = item.part * LINES + ln;
     if (line >= item.s.rows * rep) return;
     const int64_t stride = (int64_t)a.batch.key_heads * LINES * kState<D>;  // of a split's states
     const float *src = a.states + ((int64_t)item.slot * LINES + ln) * kState<D>;
@@ -439,11 +439,14 @@ __global__ void __launch_bounds__(64 * kWaves) paged_merge_kernel(const RowsArgs
     for (int e = 0; e < V; e++) Elem<T>::store(out, V * lane + e, total == 0.0f ? 0.0f : sum[e] / total);
 }
 
+template <typename T, int D, int LINES>
+__global__ void __launch_bounds__(64 * kWaves) paged_merge_kernel(const RowsArgs<T> a) { merge_few<T, D, LINES>(a, blockIdx.x, blockIdx.y); }
+
 template <typename T, int BITS, int D, int G>
 int32_t launch_rows_sized(const RowsArgs<T> &a, const PagedLaunch &r, hipStream_t s) {
     hipLaunchKernelGGL((paged_rows_kernel<T, BITS, D, G>), dim3(r.grid), dim3(64 * kWaves), 0, s, a, a.batch.place.table);
     NVQ_LAUNCH_CHECK("paged_attention");
-    if (r.merge_units > 0) {
+    if (r.merge_units > 0 && !r.merged_later) {
         hipLaunchKernelGGL((paged_merge_kernel<T, D, 16 / G>), dim3(r.merge_units, r.merge_lines), dim3(64 * kWaves), 0, s, a);
         NVQ_LAUNCH_CHECK("paged_attention merge");
     }

@@ -19,12 +19,12 @@ struct PagedBatch {
     int32_t sequences, key_heads, rep, causal;
     int32_t few;     // lines of a sequence that the kernel of few rows takes; more are the other kernel's
     int32_t target;  // items that fill the chip
+    int32_t least;   // tiles of an item, where a unit is more than one
 };
 
 namespace {
 
 constexpr int kScheduleKeys = 32;   // keys of a tile
-constexpr int kScheduleTiles = 8;   // of an item at least, where a unit is more than one item
 
 struct PagedSequence {
     int32_t start, rows, length, base, tiles, parts;  // base: the first key that a row sees, rounded down to a tile
@@ -109,7 +109,7 @@ __device__ __forceinline__ PagedPlan paged_plan(const PagedBatch &a, int lane, c
     for (int i = 0; i < 3; i++) {
         const int32_t spare = units > a.target ? a.target : units, left = a.target - spare * i / 2 > a.target / 2 ? a.target - spare * i / 2 : a.target / 2;
         const double per = ceil(total / (double)left);
-        p[i].per = per < kScheduleTiles ? kScheduleTiles : per < (double)(1 << 26) ? (int32_t)per : 1 << 26, p[i].items = 0;
+        p[i].per = per < a.least ? a.least : per < (double)(1 << 26) ? (int32_t)per : 1 << 26, p[i].items = 0;
     }
     for (int b0 = 0; b0 < a.sequences; b0 += 64) {
         const PagedSequence s = b0 == 0 ? first : paged_sequence<LINES, KIND>(a, b0 + lane);
