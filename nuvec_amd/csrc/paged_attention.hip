@@ -22,10 +22,11 @@ PagedBatch batch_of(const nvq_paged_attention_desc &d, const PagedAttentionOpera
 
 namespace {
 
-// Lines of a sequence that the kernel of few lines takes, where the other kernel has the type.  (8 sequences of 4096 positions, 4 heads of 128 on
-// each of 8 key heads, 4 bits: 16 lines a sequence 29 us against the other's 41, 32 lines 41 against 42, 40 lines 50 against 42, 64 lines 56
-// against 45; one sequence: 32 lines 17 against 21, 64 lines 22 against 21; 2 heads of 64 a key head: 32 lines 25 against 30, 64 lines 35 against 32.)
-constexpr int32_t kFewLines = 32;
+// Lines of a sequence that the kernel of few lines takes, where the other kernel has the type: four units of it, two where they are of 16 lines.  (8
+// sequences of 4096 positions, 4 heads of 128 on each of 8 key heads, 4 bits.  Groups of 64: 16 lines a sequence 29 us against the other's 41, 32 lines
+// 41 against 42, 40 lines 50 against 42, 64 lines 56 against 45; of 32: 16 lines 40 against 45, 20 lines 58 against 47; of 128: 32 lines 33 against
+// 36, 48 lines 39 against 37, 64 lines 45 against 40.  One sequence, groups of 64: 32 lines 17 against 21, 64 lines 22 against 21.)
+int32_t few_lines(const nvq_paged_attention_desc &d) { return d.cache.head_dim / d.cache.group_size == 4 ? 16 : 32; }
 constexpr int64_t kPromptLines = 128;
 
 struct Kernel {
@@ -52,7 +53,7 @@ bool may_split(const nvq_paged_attention_desc &d) { return d.cache.columns * d.c
 // Whether a sequence may have more lines than the kernel of few takes.
 bool takes_many(const nvq_paged_attention_desc &d, bool starts) {
     const int64_t most = d.max_queries < d.rows ? d.max_queries : d.rows;
-    return starts && d.cache.dtype != NVQ_F32 && most * (d.query_heads / d.cache.key_heads) > kFewLines;
+    return starts && d.cache.dtype != NVQ_F32 && most * (d.query_heads / d.cache.key_heads) > few_lines(d);
 }
 
 }  // namespace
@@ -69,10 +70,10 @@ int32_t launch_paged_attention(const nvq_paged_attention_desc &d, const PagedAtt
         const Kernel k = kernel_of(d, of_many);
         paged::PagedLaunch r{};
         r.batch = paged::batch_of(d, o);
-        r.batch.few = alone ? -1 : many ? kFewLines : INT32_MAX, r.batch.target = k.target;
+        r.batch.few = alone ? -1 : many ? few_lines(d) : INT32_MAX, r.batch.target = k.target;
         const int64_t rep = r.batch.rep;
         // At most so many units and items, whatever the lengths and starts on the device say (paged_schedule.h).
-        const int64_t each = many && !of_many ? (kFewLines + k.lines - 1) / k.lines : (rep + k.lines - 1) / k.lines;
+        const int64_t each = many && !of_many ? (few_lines(d) + k.lines - 1) / k.lines : (rep + k.lines - 1) / k.lines;
         int64_t units = c.sequences * each;
         if (starts) units = of_many ? d.rows * rep / k.lines + c.sequences : (d.rows * rep + k.lines - 1) / k.lines + c.sequences;
         if (many && !of_many && units > c.sequences * each) units = c.sequences * each;

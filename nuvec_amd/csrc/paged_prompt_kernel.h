@@ -19,7 +19,8 @@
 // 26 us.  While a compute unit is busy its vector units are at 60%, LDS at 67%, the matrix cores at 26%; a block alone takes nearly as long for a tile as
 // two that share a compute unit.  The same with 32 lines a wavefront (v_mfma_f32_32x32x16, four wavefronts of 256 registers) is as fast over a
 // long prefix and 2 to 15% slower on the diagonal; eight of those wavefronts with 256 lines to a block 5% faster at 1024 rows over 4096 and 15%
-// slower at 2048 over 2048; scales laid out by products instead of read from LDS: no faster.
+// slower at 2048 over 2048; sixteen wavefronts of 16 lines and tiles of 128 keys 15 to 30% slower; scales laid out by products instead of read
+// from LDS: no faster.
 #pragma once
 
 #include "paged_rows_kernel.h"
