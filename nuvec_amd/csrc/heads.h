@@ -84,11 +84,15 @@ __device__ __forceinline__ float norm_factor(const float (&v)[8], int dim, doubl
 struct Turn {
     float c[8], n[8];  // cosine, and sine with the sign of the partner's share; 1 and 0 where nothing turns
 };
-// WIDE: whole runs of eight turn or stay, and their partners are one run (half layout) or in the same run (interleaved).
-template <bool WIDE>
+// How a lane's run of eight is read.  kWhole: whole runs turn or stay, and their partners are one run (half layout) or in the same run
+// (interleaved).  kRuns: runs as such, their partners, which lie across two runs, through LDS.  kSingle: value by value.  (4096 positions of 32 heads of
+// 128, bfloat16, 64 values rotated as kWhole 13.0 us; 50 rotated as kRuns 15.0, value by value 41.8.)
+enum { kSingle, kRuns, kWhole };
+
+template <int READ>
 __device__ __forceinline__ Turn read_turn(const float2 *__restrict__ angles, int j0, int half, bool interleaved) {
     Turn t;
-    if (WIDE) {
+    if (READ == kWhole) {
         const bool turns = j0 < 2 * half, second = !interleaved && j0 >= half;
         if (turns) {
             if (interleaved) {
@@ -128,15 +132,15 @@ __device__ __forceinline__ Turn read_turn(const float2 *__restrict__ angles, int
 
 // The lane's values of a head and those that the rotation mixes into them, as they lie in memory: a head's are requested before the one in front of it is
 // worked on.
-template <typename T, bool WIDE>
+template <typename T, int READ>
 struct HeadRaw {
     T v[8], p[8];
     __device__ __forceinline__ void load(const T *row, int j0, int dim, int half, bool interleaved) {
-        if (WIDE) {
+        if (READ != kSingle) {
             struct alignas(16) Run { T t[8]; };
             if (j0 < dim) {
                 __builtin_memcpy(v, reinterpret_cast<const Run *>(row + j0), sizeof(Run));
-                if (!interleaved && j0 < 2 * half) __builtin_memcpy(p, reinterpret_cast<const Run *>(row + (j0 < half ? j0 + half : j0 - half)), sizeof(Run));
+                if (READ == kWhole && !interleaved && j0 < 2 * half) __builtin_memcpy(p, reinterpret_cast<const Run *>(row + (j0 < half ? j0 + half : j0 - half)), sizeof(Run));
             }
             return;
         }
@@ -148,13 +152,36 @@ struct HeadRaw {
         }
     }
 };
-template <typename T, bool WIDE>
+// kRuns: the heads that a block's lanes hold, eight values' room around each; a head's lanes are of one wavefront, whose LDS operations are in order.
+template <typename T, int P, int READ> constexpr int kHeldHeads = READ == kRuns ? kHeadBlock / P : 1;
+template <typename T, int P, int READ>
+struct HeldHeads {
+    struct alignas(16) Run { T t[8]; };
+    Run runs[kHeldHeads<T, P, READ>][P + 2];
+};
+template <typename T, int READ>
 struct HeadRun {
     float v[8], p[8];
     HeadRun() = default;
-    __device__ __forceinline__ explicit HeadRun(const HeadRaw<T, WIDE> &raw) {
+    template <int FROM>
+    __device__ __forceinline__ explicit HeadRun(const HeadRaw<T, FROM> &raw) {
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = Elem<T>::load(raw.v, i), p[i] = Elem<T>::load(raw.p, i);
+    }
+    // kRuns, half layout: the partners, `half` values further or before, from the other lanes of the head.
+    template <int P>
+    __device__ __forceinline__ void meet(const HeadRaw<T, READ> &raw, HeldHeads<T, P, READ> &held, int half) {
+        struct __attribute__((packed)) Any { T t[8]; };
+        auto &head = held.runs[threadIdx.x / P];
+        const int lane = threadIdx.x % P, j0 = 8 * lane;
+        __builtin_memcpy(&head[1 + lane], raw.v, sizeof(head[0]));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const T *at = head[1].t;
+        const int further = j0 + half < 8 * P ? j0 + half : 8 * P, before = j0 - half > -8 ? j0 - half : -8;  // (in the room around: of no use)
+        const Any a = *reinterpret_cast<const Any *>(at + further), b = *reinterpret_cast<const Any *>(at + before);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < 8; i++) p[i] = j0 + i < half ? Elem<T>::load(a.t, i) : Elem<T>::load(b.t, i);
     }
     // times the factor and the weight: two roundings in float32, those of the partners likewise
     __device__ __forceinline__ void scale(float r, const HeadRun &w) {
@@ -166,17 +193,20 @@ struct HeadRun {
         float y[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const float other = WIDE && interleaved ? v[i ^ 1] : p[i];
+            const float other = READ != kSingle && interleaved ? v[i ^ 1] : p[i];
             const float turned = v[i] * t.c[i] + other * t.n[i];
-            y[i] = WIDE || j0 + i < 2 * half ? turned : v[i];
+            y[i] = READ == kWhole || j0 + i < 2 * half ? turned : v[i];
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = y[i];
     }
 };
 
-// Whether a head's runs of eight can be read as such (the pointers' and strides' alignment aside).
-inline bool whole_runs(int dim, int half, bool interleaved) { return dim % 8 == 0 && (interleaved ? half % 4 == 0 : half % 8 == 0); }
+// How heads are read whose rows are 16-byte aligned where `aligned`, and their weights and the table of angles where `all_aligned`.
+inline int read_of(int dim, int half, bool interleaved, bool aligned, bool all_aligned) {
+    if (dim % 8 != 0 || !aligned) return kSingle;
+    return all_aligned && (interleaved ? half % 4 == 0 : half % 8 == 0) ? kWhole : kRuns;
+}
 
 }  // namespace
 }  // namespace nvq

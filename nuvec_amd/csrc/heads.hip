@@ -33,9 +33,10 @@ struct HeadArgs {
     double eps;
 };
 
-template <typename T, int P, bool WIDE>
+template <typename T, int P, int READ>
 __global__ void __launch_bounds__(kHeadBlock) head_norm_rope_kernel(const HeadArgs<T> a) {
     constexpr int kSlots = kHeadBlock / P;
+    __shared__ HeldHeads<T, P, READ> held;
     const int j0 = 8 * (threadIdx.x % P);
     const int64_t token = (int64_t)blockIdx.x * kSlots + threadIdx.x / P;
     if (token >= a.tokens) return;  // (whole heads: the lanes that are left meet all of theirs)
@@ -45,7 +46,7 @@ __global__ void __launch_bounds__(kHeadBlock) head_norm_rope_kernel(const HeadAr
     if (a.half > 0) {
         int64_t position = a.offsets == nullptr ? a.offset + l : a.per_position ? (int64_t)a.offsets[token] : (int64_t)a.offsets[b] + l;
         position = position < 0 ? 0 : position < a.table_rows ? position : a.table_rows - 1;  // (outside the table is the caller's error: clamped)
-        turn = read_turn<WIDE>(a.table + position * a.half, j0, a.half, interleaved);
+        turn = read_turn<READ>(a.table + position * a.half, j0, a.half, interleaved);
     }
     const int h0 = blockIdx.y * a.per_block, h1 = min(h0 + a.per_block, a.all_heads);
 #pragma unroll
@@ -53,19 +54,21 @@ __global__ void __launch_bounds__(kHeadBlock) head_norm_rope_kernel(const HeadAr
         const Operand<T> &o = a.of[i];
         const int from = i == 0 ? h0 : max(h0 - a.first_heads, 0), to = i == 0 ? min(h1, a.first_heads) : h1 - a.first_heads;
         if (from >= to) continue;
-        HeadRaw<T, WIDE> raw{};
-        if (o.weight != nullptr) raw.load(o.weight, j0, a.dim, a.half, interleaved);
-        const HeadRun<T, WIDE> weight(raw);
+        HeadRaw<T, READ == kWhole ? kWhole : kSingle> weights{};
+        if (o.weight != nullptr) weights.load(o.weight, j0, a.dim, a.half, interleaved);
+        const HeadRun<T, READ> weight(weights);
+        HeadRaw<T, READ> raw{};
         const T *x = o.x + b * o.xs[0] + l * o.xs[2];
         T *y = o.y + b * o.ys[0] + l * o.ys[2];
         raw.load(x + from * o.xs[1], j0, a.dim, a.half, interleaved);
         for (int64_t head = from; head < to; head++) {
-            HeadRun<T, WIDE> run(raw);
+            HeadRun<T, READ> run(raw);
+            if (READ == kRuns && !interleaved) run.template meet<P>(raw, held, a.half);
             raw.load(x + (head + 1 < to ? head + 1 : head) * o.xs[1], j0, a.dim, a.half, interleaved);
             if (o.weight != nullptr) run.scale(norm_factor<P>(run.v, a.dim, a.eps), weight);
             run.turn(turn, j0, a.half, interleaved);
             T *to_y = y + head * o.ys[1];
-            if (WIDE) {
+            if (READ != kSingle) {
                 if (j0 < a.dim) store_run(to_y + j0, run.v);
             } else {
 #pragma unroll
@@ -77,10 +80,11 @@ __global__ void __launch_bounds__(kHeadBlock) head_norm_rope_kernel(const HeadAr
 }
 
 template <typename T, int P>
-int32_t run_heads(const HeadArgs<T> &a, bool wide, hipStream_t s) {
+int32_t run_heads(const HeadArgs<T> &a, int read, hipStream_t s) {
     const dim3 grid((unsigned)((a.tokens + kHeadBlock / P - 1) / (kHeadBlock / P)), (unsigned)((a.all_heads + a.per_block - 1) / a.per_block));
-    if (wide) hipLaunchKernelGGL((head_norm_rope_kernel<T, P, true>), grid, dim3(kHeadBlock), 0, s, a);
-    else hipLaunchKernelGGL((head_norm_rope_kernel<T, P, false>), grid, dim3(kHeadBlock), 0, s, a);
+    if (read == kWhole) hipLaunchKernelGGL((head_norm_rope_kernel<T, P, kWhole>), grid, dim3(kHeadBlock), 0, s, a);
+    else if (read == kRuns) hipLaunchKernelGGL((head_norm_rope_kernel<T, P, kRuns>), grid, dim3(kHeadBlock), 0, s, a);
+    else hipLaunchKernelGGL((head_norm_rope_kernel<T, P, kSingle>), grid, dim3(kHeadBlock), 0, s, a);
     NVQ_LAUNCH_CHECK("head_norm_rope");
     return NVQ_OK;
 }
@@ -89,21 +93,22 @@ template <typename T>
 int32_t run_type(const nvq_head_rope_desc &d, const float *table, const int32_t *offsets, const void *const (&x)[2], const void *const (&w)[2],
                  void *const (&y)[2], hipStream_t s) {
     HeadArgs<T> a{};
-    bool wide = whole_runs(d.head_dim, d.rotary_dims / 2, d.interleaved != 0) && (uintptr_t)table % 16 == 0;
+    uintptr_t rows = 0, others = (uintptr_t)table;  // addresses and strides in bytes: their lowest bits
     for (int i = 0; i < 2; i++) {
         if (d.heads[i] == 0) continue;
         Operand<T> &o = a.of[i];
         o.x = (const T *)x[i], o.weight = (const T *)w[i], o.y = (T *)y[i];
-        wide = wide && ((uintptr_t)x[i] | (uintptr_t)w[i] | (uintptr_t)y[i]) % 16 == 0;
+        rows |= (uintptr_t)x[i] | (uintptr_t)y[i], others |= (uintptr_t)w[i];
         for (int k = 0; k < 3; k++) {
             o.xs[k] = d.x_strides[i][k], o.ys[k] = d.y_strides[i][k];
-            wide = wide && o.xs[k] * sizeof(T) % 16 == 0 && o.ys[k] * sizeof(T) % 16 == 0;
+            rows |= (uintptr_t)o.xs[k] * sizeof(T) | (uintptr_t)o.ys[k] * sizeof(T);
         }
     }
     a.first_heads = (int32_t)d.heads[0], a.all_heads = (int32_t)(d.heads[0] + d.heads[1]);
     a.table = (const float2 *)table, a.offsets = offsets, a.offset = d.offset, a.table_rows = d.table_rows;
     a.tokens = d.batch * d.length, a.length = d.length, a.per_position = d.per_position;
     a.dim = d.head_dim, a.half = d.rotary_dims / 2, a.interleaved = d.interleaved, a.eps = d.eps;
+    const int read = read_of(a.dim, a.half, a.interleaved != 0, rows % 16 == 0, others % 16 == 0);
     const int p = d.head_dim <= 64 ? 8 : d.head_dim <= 128 ? 16 : d.head_dim <= 256 ? 32 : 64;
     // Heads of a block: all that leave four blocks a compute unit, one where even that does not fill them.  (The 2 x 2049 tokens above: two blocks
     // a compute unit 23.5 us, four 20.2, eight 21.6.)
@@ -111,10 +116,10 @@ int32_t run_type(const nvq_head_rope_desc &d, const float *table, const int32_t 
     const int64_t per = blocks * a.all_heads / want;
     a.per_block = (int32_t)(per < 1 ? 1 : per < a.all_heads ? per : a.all_heads);
     switch (p) {
-    case 8: return run_heads<T, 8>(a, wide, s);
-    case 16: return run_heads<T, 16>(a, wide, s);
-    case 32: return run_heads<T, 32>(a, wide, s);
-    default: return run_heads<T, 64>(a, wide, s);
+    case 8: return run_heads<T, 8>(a, read, s);
+    case 16: return run_heads<T, 16>(a, read, s);
+    case 32: return run_heads<T, 32>(a, read, s);
+    default: return run_heads<T, 64>(a, read, s);
     }
 }
 

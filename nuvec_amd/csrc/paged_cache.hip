@@ -90,9 +90,10 @@ __device__ __forceinline__ int64_t row_of(const PagedPlace &p, const int32_t *se
     return (id * key_heads << p.page_shift) + (position & ((1 << p.page_shift) - 1));
 }
 
-template <typename T, int P, int BITS, bool WIDE>
+template <typename T, int P, int BITS, int READ>
 __global__ void __launch_bounds__(kHeadBlock) append_paged_kernel(const AppendArgs<T> a) {
     constexpr int kSlots = kHeadBlock / P, kWords = BITS / 4;
+    __shared__ HeldHeads<T, P, READ> held;
     const int lane = threadIdx.x % P, j0 = 8 * lane;
     const int64_t token = (int64_t)blockIdx.x * kSlots + threadIdx.x / P;
     if (token >= a.tokens) return;
@@ -102,23 +103,28 @@ __global__ void __launch_bounds__(kHeadBlock) append_paged_kernel(const AppendAr
     if (a.half > 0) {
         int64_t position = a.positions[token];
         position = position < 0 ? 0 : position < a.table_rows ? position : a.table_rows - 1;
-        turn = read_turn<WIDE>(a.table + position * a.half, j0, a.half, interleaved);
+        turn = read_turn<READ>(a.table + position * a.half, j0, a.half, interleaved);
     }
     const int h0 = blockIdx.y * a.per_block, h1 = min(h0 + a.per_block, a.query_heads + 2 * a.key_heads);
-    auto normed = [&](HeadRun<T, WIDE> &run, const T *w, const HeadRun<T, WIDE> &weight) __attribute__((always_inline)) {
+    auto normed = [&](HeadRun<T, READ> &run, const T *w, const HeadRun<T, READ> &weight) __attribute__((always_inline)) {
         if (w != nullptr) run.scale(norm_factor<P>(run.v, a.dim, a.eps), weight);
         run.turn(turn, j0, a.half, interleaved);
     };
-    HeadRaw<T, WIDE> raw{};
+    auto weight_of = [&](const T *w) __attribute__((always_inline)) {
+        HeadRaw<T, READ == kWhole ? kWhole : kSingle> raw{};
+        if (w != nullptr) raw.load(w, j0, a.dim, a.half, interleaved);
+        return HeadRun<T, READ>(raw);
+    };
+    HeadRaw<T, READ> raw{};
     if (h0 < a.query_heads) {
-        if (a.q_weight != nullptr) raw.load(a.q_weight, j0, a.dim, a.half, interleaved);
-        const HeadRun<T, WIDE> weight(raw);
+        const HeadRun<T, READ> weight = weight_of(a.q_weight);
         const T *x = a.q + token * a.qs[0];
         T *y = a.q_out + token * a.query_heads * a.dim + j0;
         const int to = min(h1, a.query_heads);
         raw.load(x + h0 * a.qs[1], j0, a.dim, a.half, interleaved);
         for (int64_t head = h0; head < to; head++) {
-            HeadRun<T, WIDE> run(raw);
+            HeadRun<T, READ> run(raw);
+            if (READ == kRuns && !interleaved) run.template meet<P>(raw, held, a.half);
             raw.load(x + (head + 1 < to ? head + 1 : head) * a.qs[1], j0, a.dim, a.half, interleaved);
             normed(run, a.q_weight, weight);
             store_run(y + head * a.dim, run.v);
@@ -126,14 +132,14 @@ __global__ void __launch_bounds__(kHeadBlock) append_paged_kernel(const AppendAr
     }
     const int from = max(h0 - a.query_heads, 0), to = h1 - a.query_heads;
     if (row < 0 || from >= to) return;
-    if (a.k_weight != nullptr) raw.load(a.k_weight, j0, a.dim, a.half, interleaved);
-    const HeadRun<T, WIDE> weight(raw);
+    const HeadRun<T, READ> weight = weight_of(a.k_weight);
     auto row_at = [&](int h) { return h < a.key_heads ? a.k + token * a.kst[0] + h * a.kst[1] : a.v + token * a.vst[0] + (h - a.key_heads) * a.vst[1]; };
     raw.load(row_at(from), j0, a.dim, a.half, interleaved);
     for (int h = from; h < to; h++) {
         const bool is_v = h >= a.key_heads;
         const int64_t head = is_v ? h - a.key_heads : h;
-        HeadRun<T, WIDE> run(raw);
+        HeadRun<T, READ> run(raw);
+        if (READ == kRuns && !interleaved && !is_v) run.template meet<P>(raw, held, a.half);
         raw.load(row_at(h + 1 < to ? h + 1 : h), j0, a.dim, a.half, interleaved);
         if (!is_v) normed(run, a.k_weight, weight);
         uint32_t words[kWords];
@@ -210,13 +216,14 @@ int32_t heads_of_block(int64_t blocks, int64_t heads) {
 }
 
 template <typename T, int P, int BITS>
-int32_t run_append(AppendArgs<T> &a, bool wide, hipStream_t s) {
+int32_t run_append(AppendArgs<T> &a, int read, hipStream_t s) {
     const int64_t blocks = (a.tokens + kHeadBlock / P - 1) / (kHeadBlock / P);
     const int32_t all = a.query_heads + 2 * a.key_heads;
     a.per_block = heads_of_block(blocks, all);
     const dim3 grid((unsigned)blocks, (unsigned)((all + a.per_block - 1) / a.per_block));
-    if (wide) hipLaunchKernelGGL((append_paged_kernel<T, P, BITS, true>), grid, dim3(kHeadBlock), 0, s, a);
-    else hipLaunchKernelGGL((append_paged_kernel<T, P, BITS, false>), grid, dim3(kHeadBlock), 0, s, a);
+    if (read == kWhole) hipLaunchKernelGGL((append_paged_kernel<T, P, BITS, kWhole>), grid, dim3(kHeadBlock), 0, s, a);
+    else if (read == kRuns) hipLaunchKernelGGL((append_paged_kernel<T, P, BITS, kRuns>), grid, dim3(kHeadBlock), 0, s, a);
+    else hipLaunchKernelGGL((append_paged_kernel<T, P, BITS, kSingle>), grid, dim3(kHeadBlock), 0, s, a);
     NVQ_LAUNCH_CHECK("append_paged");
     return NVQ_OK;
 }
@@ -232,16 +239,16 @@ int32_t run_append_type(const nvq_paged_append_desc &d, const PagedAppendOperand
     a.kw = (uint32_t *)o.kw, a.ks = (T *)o.ks, a.kb = (T *)o.kb, a.vw = (uint32_t *)o.vw, a.vs = (T *)o.vs, a.vb = (T *)o.vb;
     a.query_heads = o.q == nullptr ? 0 : (int32_t)d.query_heads, a.key_heads = (int32_t)c.key_heads;
     a.dim = c.head_dim, a.half = d.rotary_dims / 2, a.interleaved = d.interleaved, a.group = c.group_size, a.eps = d.eps;
-    bool wide = whole_runs(a.dim, a.half, a.interleaved != 0);
-    uintptr_t at = (uintptr_t)o.q | (uintptr_t)o.k | (uintptr_t)o.v | (uintptr_t)o.q_weight | (uintptr_t)o.k_weight | (uintptr_t)o.table;
+    uintptr_t rows = (uintptr_t)o.q | (uintptr_t)o.k | (uintptr_t)o.v;  // addresses and strides in bytes: their lowest bits
     for (int i = 0; i < 2; i++) {
         a.qs[i] = d.q_strides[i], a.kst[i] = d.k_strides[i], a.vst[i] = d.v_strides[i];
-        at |= (uintptr_t)(a.kst[i] * (int64_t)sizeof(T)) | (uintptr_t)(a.vst[i] * (int64_t)sizeof(T));
-        if (a.query_heads > 0) at |= (uintptr_t)(a.qs[i] * (int64_t)sizeof(T));
+        rows |= (uintptr_t)a.kst[i] * sizeof(T) | (uintptr_t)a.vst[i] * sizeof(T);
+        if (a.query_heads > 0) rows |= (uintptr_t)a.qs[i] * sizeof(T);
     }
-    wide = wide && at % 16 == 0;
-    if (c.head_dim == 64) return c.bits == 4 ? run_append<T, 8, 4>(a, wide, s) : run_append<T, 8, 8>(a, wide, s);
-    return c.bits == 4 ? run_append<T, 16, 4>(a, wide, s) : run_append<T, 16, 8>(a, wide, s);
+    const uintptr_t others = (uintptr_t)o.q_weight | (uintptr_t)o.k_weight | (uintptr_t)o.table;
+    const int read = read_of(a.dim, a.half, a.interleaved != 0, rows % 16 == 0, others % 16 == 0);
+    if (c.head_dim == 64) return c.bits == 4 ? run_append<T, 8, 4>(a, read, s) : run_append<T, 8, 8>(a, read, s);
+    return c.bits == 4 ? run_append<T, 16, 4>(a, read, s) : run_append<T, 16, 8>(a, read, s);
 }
 
 template <typename T, int P, int BITS>

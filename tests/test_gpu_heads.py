@@ -42,6 +42,27 @@ def test_rope(dim, dims, interleaved, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,dims", [(128, 2), (128, 14), (128, 16), (128, 18), (128, 50), (128, 126), (64, 24), (64, 62), (80, 40), (256, 102), (512, 510), (8, 6)])
+def test_partners_across_runs(dim, dims, dtype):
+    """Heads of whole runs of eight whose halves are not: every place of a half's end in a run; what stays is infinite and NaN; the norm before it."""
+    torch.manual_seed(dim + dims)
+    for interleaved in (False, True):
+        rotation = nv.Rotation(table(300, dims), interleaved)
+        x = torch.randn(2, 61, 5, dim, device="cuda").to(dtype).transpose(1, 2)
+        want, size = turned(x.double(), angles(rotation, 2, 61, 3), interleaved)
+        close(nv.rope(x, rotation, 3), want, size, 3)
+        w = (1 + 0.3 * torch.randn(dim, device="cuda")).to(dtype)
+        for got, weight in zip(nv.head_norm_rope(x, x, w, None, rotation, 3), (w, None)):
+            want, size = turned(normed(x, weight, 1e-6), angles(rotation, 2, 61, 3), interleaved)
+            close(got, want, size, 8)
+        x = x.clone()
+        x[..., dims:] = torch.tensor([float("inf"), float("nan")], device="cuda").repeat(256)[:dim - dims].to(dtype)
+        y = nv.rope(x, rotation, 3)
+        bits = torch.int32 if dtype == torch.float32 else torch.int16
+        assert torch.equal(y[..., dims:].contiguous().view(bits), x[..., dims:].contiguous().view(bits)) and y[..., :dims].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("dim", [128, 80, 50])
 def test_rope_layouts(dtype, dim):
     """Tokens outermost, a slice of a wider projection, rows at odd addresses, every second head; the results' own strides; in place."""
