@@ -17,8 +17,8 @@ __device__ __forceinline__ floatx4_t mfma16(uint4 a, uint4 b, floatx4_t c) {
 // A value from any address, in as few loads as it has dwords.
 template <typename V>
 __device__ __forceinline__ V load_any(const void *p) {
-    struct __attribute__((packed)) Raw { V v; };
-    return reinterpret_cast<const Raw *>(p)->v;
+    struct __attribute__((packed)) Raw { uint8_t b[sizeof(V)]; };
+    return __builtin_bit_cast(V, *reinterpret_cast<const Raw *>(p));
 }
 
 // An operand is kOffset + code.  WIDE: float32.
@@ -28,7 +28,7 @@ template <int BITS> constexpr uint32_t kMagic = BITS == 4 ? 0x41804180u : 0x4100
 // mask and the exponent are one instruction (v_and_or_b32, which takes no literal; from constants they were two).
 template <int BITS>
 struct CodeConstants {
-    uint32_t mask = ((1u << BITS) - 1u) * 0x00010001u << (7 - BITS), magic = kMagic<BITS>;
+    uint32_t mask = ((1u << BITS) - 1u) * 0x00010001u << (BITS < 7 ? 7 - BITS : 0), magic = kMagic<BITS>;
     __device__ __forceinline__ CodeConstants() {
         asm("" : "+s"(mask));
         asm("" : "+v"(magic));

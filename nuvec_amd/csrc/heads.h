@@ -10,20 +10,6 @@ namespace {
 constexpr int kHeadBlock = 256;
 
 template <typename T>
-__device__ __forceinline__ void load_run(const T *p, float (&v)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-        const uint4 w = *reinterpret_cast<const uint4 *>(p);
-        T t[8];
-        __builtin_memcpy(t, &w, 16);
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = Elem<T>::load(t, i);
-    }
-}
-
-template <typename T>
 __device__ __forceinline__ void store_run(T *p, const float (&v)[8]) {
     if constexpr (sizeof(T) == 4) {
         reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -162,7 +148,6 @@ struct HeldHeads {
 template <typename T, int READ>
 struct HeadRun {
     float v[8], p[8];
-    HeadRun() = default;
     template <int FROM>
     __device__ __forceinline__ explicit HeadRun(const HeadRaw<T, FROM> &raw) {
 #pragma unroll
