@@ -80,3 +80,42 @@ def test_captured_steps_follow_their_inputs():
         assert torch.equal(y, a(x, caches[1], table, positions, lengths)), step
     for one, other in zip((caches[0].keys, caches[0].values), (caches[1].keys, caches[1].values)):
         assert torch.equal(one.weight.view(torch.int32), other.weight.view(torch.int32)) and torch.equal(one.scales, other.scales)
+
+
+def test_captured_batches_follow_their_inputs():
+    """One graph of 64 rows for prompts, steps and padding, whose starts, positions and lengths change between the replays; padding rows' keys are
+    not written, and the others' results are those of a call without them."""
+    torch.manual_seed(4)
+    a = layer(128, 4, 2, 64, True, torch.bfloat16)
+    caches = [nv.PagedCache.new(24, 2, 16, 64) for _ in range(2)]
+    table = torch.randperm(24, device="cuda").to(torch.int32).reshape(2, 12)
+    x = torch.randn(64, 128, device="cuda", dtype=torch.bfloat16)
+    positions, sequences, starts, lengths = ints([-1] * 64), ints([0] * 64), ints([0, 0, 0]), ints([0, 0])
+    a(x, caches[0], table, positions, lengths, sequences, starts)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = a(x, caches[0], table, positions, lengths, sequences, starts)
+    held = [0, 0]
+    for rows in ([60, 4], [1, 1], [1, 50], [0, 3], [20, 20]):
+        n = sum(rows)
+        x.normal_()
+        now = [h + r for h, r in zip(held, rows)]
+        positions.copy_(ints([*range(held[0], now[0]), *range(held[1], now[1])] + [-1] * (64 - n)))
+        sequences.copy_(ints([0] * rows[0] + [1] * rows[1] + [0] * (64 - n)))
+        starts.copy_(ints([0, rows[0], n]))
+        lengths.copy_(ints(now))
+        held = now
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = a(x, caches[1], table, positions, lengths, sequences, starts)
+        assert torch.equal(y[:n], eager[:n]), rows
+        for one, other in zip((caches[0].keys, caches[0].values), (caches[1].keys, caches[1].values)):
+            assert torch.equal(one.weight.view(torch.int32), other.weight.view(torch.int32)) and torch.equal(one.scales, other.scales) and torch.equal(one.biases, other.biases)
+    assert held == [82, 78]
+
+
+def test_no_tokens():
+    a = layer(128, 2, 1, 64, False, torch.bfloat16)
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    y = a(torch.zeros(0, 128, device="cuda", dtype=torch.bfloat16), nv.PagedCache.new(2, 1, 16, 64), ints([[0, 1]]), none, ints([0]), none, ints([0, 0]))
+    assert y.shape == (0, 128)

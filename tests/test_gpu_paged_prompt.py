@@ -96,3 +96,33 @@ def test_prompts_on_two_streams_at_once():
                 got[i].append(nv.paged_attention(qs[i], cache, page_table, lengths, 0.1, starts))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_pages_beyond_32_bits(bits):
+    """Pages at the end of a pool whose codes are more than 2^32 bytes, beside its first."""
+    pages = (1 << 32) // (8 * 1024 * 128 * bits // 8) + 2
+    empty = lambda last, t: torch.empty((pages, 8, 1024, last), dtype=t, device="cuda")
+    of = lambda: nv.Quantized.affine(empty(4 * bits, torch.int32).view(torch.uint32), empty(2, torch.float16), empty(2, torch.float16), 64, bits)
+    cache = nv.PagedCache(of(), of())
+    page_table = ints([[pages - 1, 0, pages - 2]])
+    torch.manual_seed(0)
+    k, v = (torch.randn(2100, 8, 128, device="cuda", dtype=torch.float16) for _ in range(2))
+    nv.append_paged(cache, k, v, page_table, ints(range(2100)), torch.zeros(2100, dtype=torch.int32, device="cuda"))
+    q = torch.randn(40, 16, 128, device="cuda", dtype=torch.float16)
+    got = nv.paged_attention(q, cache, page_table, ints([2100]), 0.1, ints([0, 40]))
+    want, bound = attention(q, cache, page_table, [2100], 0.1, [0, 40])
+    assert ((got.double() - want).abs() <= bound).all()
+
+
+def test_calls_of_nothing():
+    """No rows, no lengths, sequences without rows around one that has some."""
+    page_table, pages = tables([300, 300, 300], 64)
+    cache = random_cache(pages, 2, 64, 128, nv.Quant.affine(64, 4), torch.bfloat16)
+    q = torch.randn(40, 8, 128, device="cuda", dtype=torch.bfloat16)
+    assert nv.paged_attention(q[:0], cache, page_table, ints([300, 300, 300]), 0.1, ints([0, 0, 0, 0])).shape == (0, 8, 128)
+    out = torch.full_like(q, 7.0)
+    nv.paged_attention(q, cache, page_table, ints([300, 300, 300]), 0.1, ints([0, 0, 0, 0]), out=out)
+    assert (out == 7).all()
+    nv.paged_attention(q, cache, page_table, ints([0, 0, 0]), 0.1, ints([0, 0, 40, 40]), out=out)
+    assert (out == 0).all()
