@@ -23,9 +23,9 @@ PagedBatch batch_of(const nvq_paged_attention_desc &d, const PagedAttentionOpera
 namespace {
 
 // Lines of a sequence that the kernel of few lines takes, where the other kernel has the type: four units of it, two where they are of 16 lines.  (8
-// sequences of 4096 positions, 4 heads of 128 on each of 8 key heads, 4 bits.  Groups of 64: 16 lines a sequence 29 us against the other's 41, 32 lines
-// 41 against 42, 40 lines 50 against 42, 64 lines 56 against 45; of 32: 16 lines 40 against 45, 20 lines 58 against 47; of 128: 32 lines 33 against
-// 36, 48 lines 39 against 37, 64 lines 45 against 40.  One sequence, groups of 64: 32 lines 17 against 21, 64 lines 22 against 21.)
+// sequences of 4096 positions, 4 heads of 128 on each of 8 key heads, 4 bits.  Groups of 64: 16 lines a sequence 31 us against the other's 40, 32 lines
+// 43 against 42, 40 lines 53 against 43, 64 lines 60 against 44; of 32: 16 lines 39 against 46, 20 lines 61 against 49; of 128: 32 lines 34 against
+// 36, 48 lines 40 against 37, 64 lines 47 against 39.  One sequence, groups of 64: 32 lines 17 against 19, 64 lines 22 against 20.)
 int32_t few_lines(const nvq_paged_attention_desc &d) { return d.cache.head_dim / d.cache.group_size == 4 ? 16 : 32; }
 constexpr int64_t kPromptLines = 128;
 

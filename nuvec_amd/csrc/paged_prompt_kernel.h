@@ -8,19 +8,20 @@
 //
 // 64 keys at a time become operands in LDS, once for the block: expanded by each wavefront for itself they would cost it six times
 // the instructions.  The next 64 keys' codes are requested before, and expanded after, this tile's products; two buffers, one barrier a tile.  A
-// code becomes an element in two instructions for two of them (16 + code in the mantissa; 8 bits through float32); the 16, and for V the
-// middle of the codes' range, are taken off the sums: the scores' by the bias, the outputs' by the sum of the rounded weights.  The
-// keys' biases are one more product (qb below).
+// code becomes an element in two instructions for two of them (16 + code in the mantissa; 8 bits through float32); the 16 is taken off the sums
+// again, by the biases (in float16 the outputs', and the middle of V's codes with it, by the sum of the rounded weights).  The keys'
+// biases are one more product (qb below).
 //
-// Terms: queries are exact in their own type.  Weights x scale are rounded to bfloat16, to two terms of it where the element type is float16.
+// Terms: queries are exact in their own type.  Weights x scale are two terms of bfloat16, 16 bits (one where the element type is bfloat16: 123 us
+// instead of 139 below, and the results' error 1.4 times that of their rounding; with two it is that of the rounding).
 //
-// Measured: 1024 rows of 32 heads of 128 over 4096 positions, 8 key heads, 4 bits in groups of 64, bfloat16: 123 us, 489 TFLOP/s (groups of 128:
-// 110, of 32: 156: each group of a head has its own scaling of scores and weights); 2048 rows over as many positions 105 us, 1024 43 us, 512
-// 26 us.  While a compute unit is busy its vector units are at 60%, LDS at 67%, the matrix cores at 26%; a block alone takes nearly as long for a tile as
-// two that share a compute unit.  The same with 32 lines a wavefront (v_mfma_f32_32x32x16, four wavefronts of 256 registers) is as fast over a
-// long prefix and 2 to 15% slower on the diagonal; eight of those wavefronts with 256 lines to a block 5% faster at 1024 rows over 4096 and 15%
-// slower at 2048 over 2048; sixteen wavefronts of 16 lines and tiles of 128 keys 15 to 30% slower; scales laid out by products instead of read
-// from LDS: no faster.
+// Measured: 1024 rows of 32 heads of 128 over 4096 positions, 8 key heads, 4 bits in groups of 64, bfloat16: 139 us, 432 TFLOP/s (groups of 128:
+// 121, of 32: 180: each group of a head has its own scaling of scores and weights); 2048 rows over as many positions 114 us, 1024 47 us, 512
+// 28 us.  While a compute unit is busy its vector units are at 61%, LDS at 50%, the matrix cores at 34%.  With one term a block alone took nearly
+// as long for a tile as two that share a compute unit, and the same with 32 lines a wavefront (v_mfma_f32_32x32x16, four wavefronts of 256
+// registers) is as fast over a long prefix and 2 to 15% slower on the diagonal; eight of those wavefronts with 256 lines to a block 5% faster at
+// 1024 rows over 4096 and 15% slower at 2048 over 2048; sixteen wavefronts of 16 lines and tiles of 128 keys 15 to 30% slower; scales laid out
+// by products instead of read from LDS: no faster.
 #pragma once
 
 #include "paged_rows_kernel.h"
@@ -84,11 +85,14 @@ __device__ __forceinline__ floatx4_t key_product(uint4 k, uint4 q, floatx4_t c) 
 
 template <typename T, int BITS, int D, int G>
 __global__ void __launch_bounds__(64 * kPromptWaves, 4) paged_prompt_kernel(const RowsArgs<T> a, const int32_t *__restrict__ table) {
-    constexpr int TP = Elem<T>::code == NVQ_BF16 ? 1 : 2;
+    constexpr int TP = weight_terms<T>();
     constexpr int KS = D / 32, ND = D / 16, GS = KS / G, GB = ND / G;                  // steps of K, blocks of D; of a group
     constexpr int kRowBytes = D * BITS / 8, kQuarter = kRowBytes / 4, kShare = kQuarter / 2;  // a row; a quarter; a thread's share of the keys' codes
     constexpr int kChunks = D / 64, kVals = D / 32, kSlot = BITS * kVals;              // of a thread: eight-code chunks; values of a row and their bits
-    constexpr float kOff = key_offset<T, BITS>, kValueOff = BITS == 4 ? 16.0f : 0.0f, kMiddle = 1 << (BITS - 1);
+    // Where the values' codes count from: float16, the middle of their range, taken off by the sum of the same, rounded weights; bfloat16, whose two terms
+    // hold 16 bits where the result has 8, the operands' own zero, taken off the bias.
+    constexpr bool kOnes = Elem<T>::code != NVQ_BF16;
+    constexpr float kOff = key_offset<T, BITS>, kValueOff = BITS == 4 ? 16.0f : 0.0f, kMiddle = kOnes ? 1 << (BITS - 1) : -kValueOff;
     // Operands, 16 bytes a lane, with gaps, so that what 16 lanes write at once falls on different banks.
     struct Stage {
         uint4 keys[4][KS][64 + 2];         // [16 keys][step][quarter of the step x key]
@@ -272,17 +276,22 @@ __global__ void __launch_bounds__(64 * kPromptWaves, 4) paged_prompt_kernel(cons
 #pragma unroll
                 for (int i = 0; i < TP; i++) p[i][2 * t + 1] = w[i];
             }
-            typedef __bf16 pair_t __attribute__((ext_vector_type(2)));
-            const pair_t one2 = {(__bf16)1.0f, (__bf16)1.0f};
+            if constexpr (kOnes) {
+                typedef __bf16 pair_t __attribute__((ext_vector_type(2)));
+                const pair_t one2 = {(__bf16)1.0f, (__bf16)1.0f};
 #pragma unroll
-            for (int i = 0; i < TP; i++)
+                for (int i = 0; i < TP; i++)
 #pragma unroll
-                for (int w = 0; w < 4; w++) ones[g] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair_t, p[i][w]), one2, ones[g], false);
+                    for (int w = 0; w < 4; w++) ones[g] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair_t, p[i][w]), one2, ones[g], false);
+            }
 #pragma unroll
-            for (int d = g * GB; d < (g + 1) * GB; d++) {
-                const uint4 v = from.values[sub][d][lane];
+            for (int d = g * GB; d < (g + 1) * GB; d += 2) {  // (two at a time: no product waits for the one in front of it; 142 -> 139 us)
+                const uint4 v0 = from.values[sub][d][lane], v1 = from.values[sub][d + 1][lane];
 #pragma unroll
-                for (int i = 0; i < TP; i++) o[d] = mfma16(v, make_uint4(p[i][0], p[i][1], p[i][2], p[i][3]), o[d]);
+                for (int i = 0; i < TP; i++) {
+                    const uint4 w = make_uint4(p[i][0], p[i][1], p[i][2], p[i][3]);
+                    o[d] = mfma16(v0, w, o[d]), o[d + 1] = mfma16(v1, w, o[d + 1]);
+                }
             }
         }
     };
@@ -376,7 +385,7 @@ __global__ void __launch_bounds__(64 * kPromptWaves, 4) paged_prompt_kernel(cons
     for (int g = 0; g < G; g++) {
         ones[g] += __shfl_xor(ones[g], 16), accb[g] += __shfl_xor(accb[g], 16);
         ones[g] += __shfl_xor(ones[g], 32), accb[g] += __shfl_xor(accb[g], 32);
-        accb[g] = __builtin_fmaf(-(kValueOff + kMiddle), ones[g], accb[g]);  // (the operands and kValueOff + kMiddle went through the same weights)
+        if constexpr (kOnes) accb[g] = __builtin_fmaf(-(kValueOff + kMiddle), ones[g], accb[g]);  // (the operands and kValueOff + kMiddle went through the same weights)
     }
     if (!live) return;
     const bool whole = span.items == 1;

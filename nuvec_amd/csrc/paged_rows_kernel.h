@@ -3,15 +3,15 @@
 // K and V of the row's sequence, read through its page table, lengths and all from device memory.
 //
 // The bound is the stream of the cache.  Both products run on the matrix cores over the codes, which bfloat16 holds exactly, as in
-// qattn.hip: the 16 columns of v_mfma_f32_16x16x32 are (group of D, line), S^T = K . Q^T with zeros of Q outside a column's group, scale
-// and bias of the group applied to the partial score, O^T = V^T . P^T with the weights times the column's group's scale.  A lane holds in
-// S^T the keys 4 quarter .. + 3 of two halves of 16 keys, which are the eight keys of its operand P^T.  Half a tile lies within one page
-// (pages have 16 positions at least), so a tile's addresses are two scalars, looked up a tile ahead.
+// qattn.hip (its weights are three terms in every type, though): the 16 columns of v_mfma_f32_16x16x32 are (group of D, line), S^T = K . Q^T
+// with zeros of Q outside a column's group, scale and bias of the group applied to the partial score, O^T = V^T . P^T with the weights times the
+// column's group's scale.  A lane holds in S^T the keys 4 quarter .. + 3 of two halves of 16 keys, which are the eight keys of its operand P^T.
+// Half a tile lies within one page (pages have 16 positions at least), so a tile's addresses are two scalars, looked up a tile ahead.
 //
-// Terms.  Queries are exact: one bfloat16 term, two in float16, three in float32.  The weights p x scale are one term in bfloat16 (its
-// rounding, 2^-8, is the output's own, and averages over the keys), two in float16, three in float32.  The codes of V count from the
-// middle of their range: the operands themselves in float32, else by an operand of ones whose products with the same, rounded weights
-// are taken off.  Scores, maxima, sums and accumulators are float32.
+// Terms.  Queries are exact: one bfloat16 term, two in float16, three in float32.  The weights p x scale are two terms in bfloat16 and float16
+// (16 bits: the result's own rounding is all that is left of the error; one term in bfloat16 was 1 to 3% faster and a result's error 1.4 times
+// its rounding's), three in float32.  The codes of V count from the middle of their range: the operands themselves in float32, else by an
+// operand of ones whose products with the same, rounded weights are taken off.  Scores, maxima, sums and accumulators are float32.
 //
 // Masked keys (behind the sequence's end, in front of a row or outside its window) are given no weight whatever their pages hold: their
 // scores are replaced and their values' scales and biases too, which may be infinite or NaN.
@@ -48,7 +48,7 @@ template <int D> constexpr int kState = D + 4;  // (rows of 16 bytes)
 // Blocks on a compute unit.  Three need 168 registers at most: heads of 128 read their queries from LDS in every tile there.
 template <typename T, int G> constexpr int rows_blocks() { return sizeof(T) == 4 || G == 4 ? 2 : 3; }
 template <typename T, int D, int G> constexpr bool rows_queries_in_lds() { return rows_blocks<T, G>() == 3 && D == 128; }
-template <typename T> constexpr int weight_terms() { return sizeof(T) == 4 ? 3 : Elem<T>::code == NVQ_BF16 ? 1 : 2; }
+template <typename T> constexpr int weight_terms() { return sizeof(T) == 4 ? 3 : 2; }
 
 template <typename T, int BITS, int D, int G>
 __global__ void __launch_bounds__(64 * kWaves, (rows_blocks<T, G>())) paged_rows_kernel(const RowsArgs<T> a, const int32_t *__restrict__ table) {

@@ -343,8 +343,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
     zeros; rows of no sequence are left as they were in `out` (and undefined in a new result).  `max_queries` is the most rows of a sequence, as
     far as the caller knows: it sizes the launch, more rows are right all the same.
 
-    The keys' and values' codes are exact operands; the softmax's weights, times the values' scales, are rounded to the precision of the element type,
-    everything else is float32."""
+    The keys' and values' codes are exact operands; the softmax's weights, times the values' scales, hold 16 bits (24 in float32), everything else is
+    float32."""
     y = (_lib._native or _lib.native()).paged_attention(q, cache, page_table, lengths, scale, query_starts, max_queries, sinks, causal, window, out)
     if y is not None:
         return y if out is None else out
