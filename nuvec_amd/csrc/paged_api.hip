@@ -33,6 +33,11 @@ int32_t check_paged(const char *op, const nvq_paged_desc &c) {
     return NVQ_OK;
 }
 
+// The page of every token is looked up before anything else of the pool, which may be empty.
+int32_t check_page_table(const char *op, const nvq_paged_desc &c, const int32_t *page_table) {
+    return c.sequences > 0 && c.columns > 0 && page_table == nullptr ? fail(NVQ_INVALID_ARGUMENT, "%s: null page table", op) : NVQ_OK;
+}
+
 int32_t check_pool(const char *op, const nvq_paged_desc &c, const void *kw, const void *ks, const void *kb, const void *vw, const void *vs,
                    const void *vb) {
     if (kw == nullptr || ks == nullptr || kb == nullptr || vw == nullptr || vs == nullptr || vb == nullptr)
@@ -105,10 +110,8 @@ int32_t nvq_append_paged(const nvq_paged_append_desc *d, const int32_t *page_tab
     if (d->tokens == 0 || (c.key_heads == 0 && !queries)) return NVQ_OK;
     if (positions == nullptr || (c.key_heads > 0 && (k == nullptr || v == nullptr)) || (queries && q_out == nullptr))
         return fail(NVQ_INVALID_ARGUMENT, "%s: null operand", op);
-    if (c.key_heads > 0 && c.pages > 0 && c.sequences > 0 && c.columns > 0) {
-        NVQ_TRY(check_pool(op, c, k_w, k_s, k_b, v_w, v_s, v_b));
-        if (page_table == nullptr) return fail(NVQ_INVALID_ARGUMENT, "%s: null operand", op);
-    }
+    NVQ_TRY(check_page_table(op, c, page_table));
+    if (c.key_heads > 0 && c.pages > 0 && c.sequences > 0 && c.columns > 0) NVQ_TRY(check_pool(op, c, k_w, k_s, k_b, v_w, v_s, v_b));
     for (const void *p : {q, q_weight, k, k_weight, v}) NVQ_TRY(check_elements(op, "an operand", p, c.dtype));
     NVQ_TRY(check_aligned(op, "the queries' output", q_out));
     NVQ_TRY(require_device());
@@ -126,10 +129,8 @@ int32_t nvq_read_paged(const nvq_paged_desc *d, int64_t tokens, const int32_t *p
     if (tokens >= 1LL << 32) return fail(NVQ_UNSUPPORTED, "%s: more than 2^32 tokens", op);
     if (tokens == 0 || d->key_heads == 0) return NVQ_OK;
     if (positions == nullptr || keys == nullptr || values == nullptr) return fail(NVQ_INVALID_ARGUMENT, "%s: null operand", op);
-    if (d->pages > 0 && d->sequences > 0 && d->columns > 0) {
-        NVQ_TRY(check_pool(op, *d, k_w, k_s, k_b, v_w, v_s, v_b));
-        if (page_table == nullptr) return fail(NVQ_INVALID_ARGUMENT, "%s: null operand", op);
-    }
+    NVQ_TRY(check_page_table(op, *d, page_table));
+    if (d->pages > 0 && d->sequences > 0 && d->columns > 0) NVQ_TRY(check_pool(op, *d, k_w, k_s, k_b, v_w, v_s, v_b));
     NVQ_TRY(check_aligned(op, "the keys' output", keys));
     NVQ_TRY(check_aligned(op, "the values' output", values));
     NVQ_TRY(require_device());
