@@ -12,7 +12,8 @@ PagedBatch batch_of(const nvq_paged_attention_desc &d, const PagedAttentionOpera
     b.place.table = o.page_table, b.place.stride = c.table_stride, b.place.pages = c.pages;
     b.place.sequences = (int32_t)c.sequences, b.place.columns = (int32_t)c.columns;
     while ((1LL << b.place.page_shift) < c.page_size) b.place.page_shift++;
-    b.lengths = o.lengths, b.starts = o.starts, b.rows = d.rows, b.window = d.window;
+    b.lengths = o.lengths, b.starts = o.starts, b.rows = d.rows;
+    b.window = d.window < 1LL << 30 ? d.window : 1LL << 30;  // (as good as any larger one, and sums with it stay far from 64 bits)
     b.sequences = (int32_t)c.sequences, b.key_heads = (int32_t)c.key_heads, b.rep = (int32_t)(d.query_heads / c.key_heads), b.causal = d.causal;
     b.few = INT32_MAX;
     return b;

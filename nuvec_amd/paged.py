@@ -376,7 +376,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
     desc = _lib.PagedAttentionDescC(cd, n, heads, 1 if query_starts is None else n if max_queries is None else max(1, min(n, int(max_queries))))
     for i in range(2):
         desc.q_strides[i], desc.out_strides[i] = q.stride(i), out.stride(i)
-    desc.window, desc.causal, desc.scale = window, int(causal), float(scale)
+    desc.window, desc.causal, desc.scale = min(window, 1 << 62), int(causal), float(scale)  # (ctypes would take a larger one modulo 2^64)
     _init(q)
     lib = _lib.load()
     need = lib.nvq_paged_attention_workspace_bytes(C.byref(desc))
