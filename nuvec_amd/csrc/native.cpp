@@ -750,7 +750,7 @@ bool is_heads(const Tensor &x, const Place &at, at::ScalarType type) {
     return x.defined() && x.dim() == 4 && x.numel() > 0 && x.device() == at.device && x.scalar_type() == type && x.stride(3) == 1 && x.size(3) <= 512;
 }
 
-// Operands of one call (queries and keys, or one alone) rotated into dense outputs of their strides' order, or `out` of the first.
+// Operands of one call (queries and keys, or one alone) rotated into dense outputs with consecutive values, or `out` of the first.
 bool rotate(const Place &at, const Tensor *xs, const Tensor *weights, int count, const Angles &angles, const Tensor &offsets, int64_t offset, double eps,
             Tensor *ys) {
     const Tensor &x = xs[0];
@@ -768,8 +768,10 @@ bool rotate(const Place &at, const Tensor *xs, const Tensor *weights, int count,
     }
     for (int i = 0; i < count; i++) {
         if (!ys[i].defined()) {
+            // (the strides' order is x's; one of overlapping rows may put another dimension innermost)
             const auto strides = at::infer_dense_strides(xs[i].sizes(), xs[i].strides());
-            ys[i] = at::detail::empty_strided_cuda(xs[i].sizes(), strides, xs[i].scalar_type(), at.device);
+            ys[i] = strides[3] == 1 || xs[i].size(3) == 1 ? at::detail::empty_strided_cuda(xs[i].sizes(), strides, xs[i].scalar_type(), at.device)
+                                                          : at.empty(xs[i].sizes(), xs[i].scalar_type());
         } else if (!is_heads(ys[i], at, x.scalar_type()) || ys[i].sizes() != xs[i].sizes()) {
             return false;
         }

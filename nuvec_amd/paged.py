@@ -129,7 +129,8 @@ def _heads(op: str, x: torch.Tensor) -> torch.Tensor:
 
 def _out_like(op: str, x: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
     if out is None:
-        return torch.empty_like(x)  # (the strides' order is x's)
+        y = torch.empty_like(x)  # (the strides' order is x's; one of overlapping rows may put another dimension innermost)
+        return y if y.stride(3) == 1 or x.shape[3] == 1 else torch.empty_like(x, memory_format=torch.contiguous_format)
     if out.dtype != x.dtype or out.shape != x.shape or (out.numel() > 0 and out.stride(-1) != 1 and out.shape[-1] != 1):
         raise InvalidArgument(f"{op}: the output must be {_name(x.dtype)} {list(x.shape)} with consecutive values")
     _same_device(op, x, out)
