@@ -750,6 +750,13 @@ bool is_heads(const Tensor &x, const Place &at, at::ScalarType type) {
     return x.defined() && x.dim() == 4 && x.numel() > 0 && x.device() == at.device && x.scalar_type() == type && x.stride(3) == 1 && x.size(3) <= 512;
 }
 
+// Rows that share their memory: never written.
+bool is_expanded(const Tensor &y) {
+    for (int64_t i = 0; i < y.dim(); i++)
+        if (y.size(i) > 1 && y.stride(i) == 0) return true;
+    return false;
+}
+
 // Operands of one call (queries and keys, or one alone) rotated into dense outputs with consecutive values, or `out` of the first.
 bool rotate(const Place &at, const Tensor *xs, const Tensor *weights, int count, const Angles &angles, const Tensor &offsets, int64_t offset, double eps,
             Tensor *ys) {
@@ -772,7 +779,7 @@ bool rotate(const Place &at, const Tensor *xs, const Tensor *weights, int count,
             const auto strides = at::infer_dense_strides(xs[i].sizes(), xs[i].strides());
             ys[i] = strides[3] == 1 || xs[i].size(3) == 1 ? at::detail::empty_strided_cuda(xs[i].sizes(), strides, xs[i].scalar_type(), at.device)
                                                           : at.empty(xs[i].sizes(), xs[i].scalar_type());
-        } else if (!is_heads(ys[i], at, x.scalar_type()) || ys[i].sizes() != xs[i].sizes()) {
+        } else if (!is_heads(ys[i], at, x.scalar_type()) || ys[i].sizes() != xs[i].sizes() || is_expanded(ys[i])) {
             return false;
         }
         d.heads[i] = xs[i].size(1);
@@ -947,7 +954,7 @@ PyObject *py_paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
         const int64_t rows = q.size(0), heads = q.size(1), dim = q.size(2);
         if (!p.fits(at, type) || p.d.head_dim != dim || !is_rows(q, at, type, rows, dim) || !is_index(lengths, at, p.d.sequences) ||
             (starts.defined() ? !is_index(starts, at, p.d.sequences + 1) : p.d.sequences != rows) || !bias_fits(sinks, at, type, heads) ||
-            (y.defined() && (!is_rows(y, at, type, rows, dim) || y.size(1) != heads)))
+            (y.defined() && (!is_rows(y, at, type, rows, dim) || y.size(1) != heads || is_expanded(y))))
             return none();
         nvq_paged_attention_desc d{};
         d.cache = p.d, d.rows = rows, d.query_heads = heads, d.max_queries = !starts.defined() ? 1 : most < 1 ? 1 : most < rows ? most : rows;

@@ -127,12 +127,19 @@ def _heads(op: str, x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous()
 
 
+def _own_rows(op: str, out: torch.Tensor) -> None:
+    """An expanded output would be written by several rows at once."""
+    if any(n > 1 and step == 0 for n, step in zip(out.shape, out.stride())):
+        raise InvalidArgument(f"{op}: rows of the output {list(out.shape)} share their memory")
+
+
 def _out_like(op: str, x: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
     if out is None:
         y = torch.empty_like(x)  # (the strides' order is x's; one of overlapping rows may put another dimension innermost)
         return y if y.stride(3) == 1 or x.shape[3] == 1 else torch.empty_like(x, memory_format=torch.contiguous_format)
     if out.dtype != x.dtype or out.shape != x.shape or (out.numel() > 0 and out.stride(-1) != 1 and out.shape[-1] != 1):
         raise InvalidArgument(f"{op}: the output must be {_name(x.dtype)} {list(x.shape)} with consecutive values")
+    _own_rows(op, out)
     _same_device(op, x, out)
     return out
 
@@ -169,7 +176,7 @@ def _rotate(op: str, xs, weights, outs, rotation, offset, eps):
 def rope(x: torch.Tensor, rotation: Rotation, offset: Union[int, torch.Tensor] = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rotary positions of `x` `[batch, heads, length, dim]` (any strides with consecutive values of a head; MLX's `fast.rope`): the first
     `rotation.dims` values of a head turn, the others stay.  Element l is at position `offset + l`; `offset` is an int, int32 `[batch]`, or int32
-    `[batch, length]` for positions one by one.  Positions on the device outside the table are clamped to it.  `out` may be `x` itself."""
+    `[batch, length]` for positions one by one.  Positions on the device outside the table are clamped to it.  `out` may be `x` itself, unless rows of it share their memory."""
     y = (_lib._native or _lib.native()).rope(x, rotation, offset, out)
     if y is not None:
         return y if out is None else out
@@ -373,6 +380,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     elif out.dtype != q.dtype or out.shape != q.shape or out.stride(2) != 1:
         raise InvalidArgument(f"{op}: the output must be {_name(q.dtype)} {list(q.shape)} with consecutive values")
+    _own_rows(op, out)
     _same_device(op, q, out)
     desc = _lib.PagedAttentionDescC(cd, n, heads, 1 if query_starts is None else n if max_queries is None else max(1, min(n, int(max_queries))))
     for i in range(2):
