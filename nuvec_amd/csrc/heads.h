@@ -63,7 +63,7 @@ __device__ __forceinline__ float norm_factor(const float (&v)[8], int dim, doubl
     double y = __builtin_amdgcn_rsq(x);  // (half its digits; each step doubles them)
 #pragma unroll
     for (int i = 0; i < 2; i++) y = y * __builtin_fma(-0.5 * x * y, y, 1.5);
-    return (float)y;
+    return x == (double)INFINITY ? 0.0f : (float)y;  // (the steps make infinity x 0 of it)
 }
 
 // Which values of a head the rotation turns and with which others, for the lane's run of eight.
