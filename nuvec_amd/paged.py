@@ -25,7 +25,7 @@ from .ops import _CODE, _FLOATS, InvalidArgument, Quant, QuantMode, Quantized, U
 def rotation_freqs(dims: int, base: float = 10000.0, scaling: Optional[dict] = None) -> Tuple[Optional[torch.Tensor], float, float]:
     """`(freqs, scale, magnitude)` for `Rotation.new` from a checkpoint's `rope_scaling` entry: none, "linear" (positions divided by
     `factor`), "llama3" (long waves slowed by `factor`, short ones kept, a blend between) or "yarn" (the same by the number of turns, with a
-    magnitude).  `freqs` is None or float32 `[dims / 2]`: the values that positions are divided by."""
+    magnitude; the blend begins and ends at whole pairs unless `truncate` is false).  `freqs` is None or float32 `[dims / 2]`: the values that positions are divided by."""
     kind = "default" if scaling is None else scaling.get("rope_type", scaling.get("type", "default"))
     if kind == "default":
         return None, 1.0, 1.0
@@ -43,8 +43,10 @@ def rotation_freqs(dims: int, base: float = 10000.0, scaling: Optional[dict] = N
     if kind == "yarn":
         most = float(scaling["original_max_position_embeddings"])
         at = lambda turns: dims * math.log(most / (turns * 2 * math.pi)) / (2 * math.log(base))
-        low = max(math.floor(at(float(scaling.get("beta_fast", 32.0)))), 0)
-        high = min(math.ceil(at(float(scaling.get("beta_slow", 1.0)))), dims - 1)
+        low, high = at(float(scaling.get("beta_fast", 32.0))), at(float(scaling.get("beta_slow", 1.0)))
+        if scaling.get("truncate", True):  # (the blend begins and ends at whole pairs)
+            low, high = math.floor(low), math.ceil(high)
+        low, high = max(low, 0), min(high, dims - 1)
         slowed = ((torch.arange(dims // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
         magnitude = lambda m: 1.0 if factor <= 1.0 else 0.1 * m * math.log(factor) + 1.0
         given = scaling.get("attention_factor")
