@@ -368,9 +368,11 @@ NVQ_API int32_t nvq_quantized_attention_prompt_f32(const nvq_attention_prompt_de
                                 void *out, void *workspace, void *stream);
 
 /* Angles of positions 0 .. rows - 1: table f32 [rows, dims / 2, 2] = magnitude * (cos, sin)(scale * position / f_i), with f_i = freqs[i]
- * (f32 [dims / 2]) or, with freqs NULL, base^(2 i / dims); the angles in 64 bits. */
+ * (f32 [dims / 2]; _f64: f64, as scaled frequencies of long contexts need) or, with freqs NULL, base^(2 i / dims); the angles in 64 bits. */
 NVQ_API int32_t nvq_rotation_table(const float *freqs, int32_t dims, int64_t rows, double base, double scale, double magnitude, float *table,
                            void *stream);
+NVQ_API int32_t nvq_rotation_table_f64(const double *freqs, int32_t dims, int64_t rows, double base, double scale, double magnitude, float *table,
+                               void *stream);
 
 /* y = rotate(norm(x)): float32 throughout, rounded once.  x1 NULL: one operand; a weight ([head_dim] dtype) NULL: that operand is not
  * normed; table NULL (rotary_dims 0): not rotated.  y may be x itself.  Positions outside the table are clamped to it. */

@@ -131,6 +131,7 @@ SIGNATURES = {
     "nvq_quantized_attention_prompt_f32_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionPromptDescC)]),
     "nvq_quantized_attention_prompt_f32": (C.c_int32, [C.POINTER(AttentionPromptDescC)] + [C.c_void_p] * 11),
     "nvq_rotation_table": (C.c_int32, [C.c_void_p, C.c_int32, C.c_int64, C.c_double, C.c_double, C.c_double, C.c_void_p, C.c_void_p]),
+    "nvq_rotation_table_f64": (C.c_int32, [C.c_void_p, C.c_int32, C.c_int64, C.c_double, C.c_double, C.c_double, C.c_void_p, C.c_void_p]),
     "nvq_head_norm_rope": (C.c_int32, [C.POINTER(HeadRopeDescC)] + [C.c_void_p] * 9),
     "nvq_append_paged": (C.c_int32, [C.POINTER(PagedAppendDescC)] + [C.c_void_p] * 17),
     "nvq_read_paged": (C.c_int32, [C.POINTER(PagedDescC), C.c_int64] + [C.c_void_p] * 12),

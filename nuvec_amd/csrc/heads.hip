@@ -123,8 +123,10 @@ int32_t run_type(const nvq_head_rope_desc &d, const float *table, const int32_t 
     }
 }
 
-// angle = scale x position / wavelength's base i, in 64 bits: at position 100000 a float32 angle is off by 0.004.
-__global__ void __launch_bounds__(256) rotation_table_kernel(const float *__restrict__ freqs, int half, int64_t rows, double base, double scale,
+// angle = scale x position / wavelength's base i, in 64 bits: at position 100000 a float32 angle is off by 0.004, and one of frequencies that were
+// rounded to float32 by 0.0016.
+template <typename F>
+__global__ void __launch_bounds__(256) rotation_table_kernel(const F *__restrict__ freqs, int half, int64_t rows, double base, double scale,
                                                              double magnitude, float2 *__restrict__ table) {
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (at >= rows * half) return;
@@ -147,11 +149,14 @@ int32_t launch_head_rope(const nvq_head_rope_desc &d, const float *table, const 
     }
 }
 
-int32_t launch_rotation_table(const float *freqs, int half, int64_t rows, double base, double scale, double magnitude, float *table, hipStream_t s) {
-    hipLaunchKernelGGL(rotation_table_kernel, dim3((unsigned)((rows * half + 255) / 256)), dim3(256), 0, s, freqs, half, rows, base, scale, magnitude,
+template <typename F>
+int32_t launch_rotation_table(const F *freqs, int half, int64_t rows, double base, double scale, double magnitude, float *table, hipStream_t s) {
+    hipLaunchKernelGGL((rotation_table_kernel<F>), dim3((unsigned)((rows * half + 255) / 256)), dim3(256), 0, s, freqs, half, rows, base, scale, magnitude,
                        (float2 *)table);
     NVQ_LAUNCH_CHECK("rotation_table");
     return NVQ_OK;
 }
+template int32_t launch_rotation_table<float>(const float *, int, int64_t, double, double, double, float *, hipStream_t);
+template int32_t launch_rotation_table<double>(const double *, int, int64_t, double, double, double, float *, hipStream_t);
 
 }  // namespace nvq

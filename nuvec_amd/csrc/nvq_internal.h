@@ -217,7 +217,8 @@ struct PagedAttentionOperands {
     const int32_t *page_table, *lengths, *starts;
     void *out, *workspace;
 };
-int32_t launch_rotation_table(const float *freqs, int half, int64_t rows, double base, double scale, double magnitude, float *table, hipStream_t s);
+template <typename F>  // float or double
+int32_t launch_rotation_table(const F *freqs, int half, int64_t rows, double base, double scale, double magnitude, float *table, hipStream_t s);
 int32_t launch_head_rope(const nvq_head_rope_desc &d, const float *table, const int32_t *offsets, const void *const (&x)[2],
                          const void *const (&w)[2], void *const (&y)[2], hipStream_t s);
 int32_t launch_append_paged(const nvq_paged_append_desc &d, const PagedAppendOperands &o, hipStream_t s);

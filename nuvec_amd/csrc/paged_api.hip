@@ -53,9 +53,8 @@ int32_t check_pool(const char *op, const nvq_paged_desc &c, const void *kw, cons
 
 using namespace nvq;
 
-extern "C" {
-
-int32_t nvq_rotation_table(const float *freqs, int32_t dims, int64_t rows, double base, double scale, double magnitude, float *table, void *stream) {
+template <typename F>
+static int32_t rotation_table(const F *freqs, int32_t dims, int64_t rows, double base, double scale, double magnitude, float *table, void *stream) {
     const char *op = "rotation_table";
     if (dims < 0 || dims % 2 != 0 || rows < 0) return fail(NVQ_INVALID_ARGUMENT, "%s: %d values, %lld positions", op, dims, (long long)rows);
     if (dims == 0 || rows == 0) return NVQ_OK;
@@ -64,7 +63,18 @@ int32_t nvq_rotation_table(const float *freqs, int32_t dims, int64_t rows, doubl
     if (table == nullptr) return fail(NVQ_INVALID_ARGUMENT, "%s: null operand", op);
     NVQ_TRY(require_device());
     NVQ_TRY(check_aligned(op, "the table of angles", table, 8));
+    NVQ_TRY(check_aligned(op, "the frequencies", freqs, sizeof(F)));
     return launch_rotation_table(freqs, dims / 2, rows, base, scale, magnitude, table, (hipStream_t)stream);
+}
+
+extern "C" {
+
+int32_t nvq_rotation_table(const float *freqs, int32_t dims, int64_t rows, double base, double scale, double magnitude, float *table, void *stream) {
+    return rotation_table(freqs, dims, rows, base, scale, magnitude, table, stream);
+}
+
+int32_t nvq_rotation_table_f64(const double *freqs, int32_t dims, int64_t rows, double base, double scale, double magnitude, float *table, void *stream) {
+    return rotation_table(freqs, dims, rows, base, scale, magnitude, table, stream);
 }
 
 int32_t nvq_head_norm_rope(const nvq_head_rope_desc *d, const float *table, const int32_t *offsets, const void *x0, const void *weight0, void *y0,

@@ -25,7 +25,7 @@ from .ops import _CODE, _FLOATS, InvalidArgument, Quant, QuantMode, Quantized, U
 def rotation_freqs(dims: int, base: float = 10000.0, scaling: Optional[dict] = None) -> Tuple[Optional[torch.Tensor], float, float]:
     """`(freqs, scale, magnitude)` for `Rotation.new` from a checkpoint's `rope_scaling` entry: none, "linear" (positions divided by
     `factor`), "llama3" (long waves slowed by `factor`, short ones kept, a blend between) or "yarn" (the same by the number of turns, with a
-    magnitude; the blend begins and ends at whole pairs unless `truncate` is false).  `freqs` is None or float32 `[dims / 2]`: the values that positions are divided by."""
+    magnitude; the blend begins and ends at whole pairs unless `truncate` is false).  `freqs` is None or float64 `[dims / 2]`: the values that positions are divided by."""
     kind = "default" if scaling is None else scaling.get("rope_type", scaling.get("type", "default"))
     if kind == "default":
         return None, 1.0, 1.0
@@ -39,7 +39,7 @@ def rotation_freqs(dims: int, base: float = 10000.0, scaling: Optional[dict] = N
         low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
         turns = float(scaling["original_max_position_embeddings"]) / (2 * math.pi * freqs)
         keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
-        return (1.0 / ((1.0 - keep) / (factor * freqs) + keep / freqs)).float(), 1.0, 1.0
+        return (1.0 / ((1.0 - keep) / (factor * freqs) + keep / freqs)), 1.0, 1.0
     if kind == "yarn":
         most = float(scaling["original_max_position_embeddings"])
         at = lambda turns: dims * math.log(most / (turns * 2 * math.pi)) / (2 * math.log(base))
@@ -52,7 +52,7 @@ def rotation_freqs(dims: int, base: float = 10000.0, scaling: Optional[dict] = N
         given = scaling.get("attention_factor")
         if given is None:
             given = magnitude(float(scaling.get("mscale", 1.0))) / (magnitude(float(scaling["mscale_all_dim"])) if "mscale_all_dim" in scaling else 1.0)
-        return (1.0 / (slowed / (factor * freqs) + (1.0 - slowed) / freqs)).float(), 1.0, float(given)
+        return (1.0 / (slowed / (factor * freqs) + (1.0 - slowed) / freqs)), 1.0, float(given)
     raise Unsupported(f"rotation_freqs: scaling '{kind}'")
 
 
@@ -70,7 +70,8 @@ class Rotation:
     @staticmethod
     def new(dims: int, positions: int, base: float = 10000.0, scale: float = 1.0, interleaved: bool = False,
             freqs: Optional[torch.Tensor] = None, magnitude: float = 1.0, device="cuda") -> "Rotation":
-        """Angles `scale * position / freqs[i]`, freqs `base^(2 i / dims)` unless given; cosines and sines times `magnitude`."""
+        """Angles `scale * position / freqs[i]` in 64 bits, freqs `base^(2 i / dims)` unless given (float64, or float32 values); cosines and sines
+        times `magnitude`, rounded once."""
         if dims <= 0 or dims % 2 or positions < 1:
             raise InvalidArgument(f"rotation: {dims} values, {positions} positions")
         table = torch.empty((positions, dims // 2, 2), dtype=torch.float32, device=device)
@@ -78,8 +79,10 @@ class Rotation:
         if freqs is not None:
             if tuple(freqs.shape) != (dims // 2,):
                 raise InvalidArgument(f"rotation: freqs {list(freqs.shape)} for {dims} values")
-            freqs = freqs.to(device=table.device, dtype=torch.float32).contiguous()
-        _lib.check(_lib.load().nvq_rotation_table(_ptr(freqs), dims, positions, float(base), float(scale), float(magnitude), _ptr(table), _stream()))
+            freqs = freqs.to(device=table.device, dtype=torch.float64 if freqs.dtype == torch.float64 else torch.float32).contiguous()
+        lib = _lib.load()
+        make = lib.nvq_rotation_table_f64 if freqs is not None and freqs.dtype == torch.float64 else lib.nvq_rotation_table
+        _lib.check(make(_ptr(freqs), dims, positions, float(base), float(scale), float(magnitude), _ptr(table), _stream()))
         return Rotation(table, interleaved)
 
 
