@@ -109,7 +109,7 @@ int32_t run_type(const nvq_head_rope_desc &d, const float *table, const int32_t 
     a.tokens = d.batch * d.length, a.length = d.length, a.per_position = d.per_position;
     a.dim = d.head_dim, a.half = d.rotary_dims / 2, a.interleaved = d.interleaved, a.eps = d.eps;
     const int read = read_of(a.dim, a.half, a.interleaved != 0, rows % 16 == 0, others % 16 == 0);
-    const int p = d.head_dim <= 64 ? 8 : d.head_dim <= 128 ? 16 : d.head_dim <= 256 ? 32 : 64;
+    const int p = head_lanes(d.head_dim);
     // Heads of a block: all that leave four blocks a compute unit, one where even that does not fill them.  (The 2 x 2049 tokens above: two blocks
     // a compute unit 23.5 us, four 20.2, eight 21.6.)
     const int64_t blocks = (a.tokens + kHeadBlock / p - 1) / (kHeadBlock / p), want = 4 * (int64_t)compute_units();

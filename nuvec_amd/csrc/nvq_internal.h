@@ -38,6 +38,9 @@ int32_t fail(int32_t status, const char *fmt, ...) __attribute__((format(printf,
         if (nvq_rc_ != NVQ_OK) return nvq_rc_; \
     } while (0)
 
+// A launch has fewer than 2^32 threads along x.
+constexpr bool launchable(int64_t blocks, int64_t threads) { return blocks < (1LL << 32) / threads; }
+
 int32_t require_device();          // NVQ_OK once nvq_init succeeded
 int32_t compute_units();           // of the bound device
 int32_t check_quant(const nvq_quant *q, const char *op);
@@ -205,7 +208,9 @@ size_t attention_prompt_f32_workspace_bytes(const nvq_attention_prompt_desc &d);
 int32_t launch_attention_prompt_f32(const nvq_attention_prompt_desc &d, const void *q, const void *kw, const void *ks, const void *kb,
                                     const void *vw, const void *vs, const void *vb, const void *sinks, void *out, void *workspace,
                                     hipStream_t s);
-// Heads and the paged cache.
+// Heads and the paged cache.  Lanes of a head, eight values each, in blocks of 256; the most positions that one launch takes.
+constexpr int head_lanes(int head_dim) { return head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : head_dim <= 256 ? 32 : 64; }
+constexpr int64_t most_positions(int head_dim) { return ((1LL << 32) / 256 - 1) * (256 / head_lanes(head_dim)); }
 struct PagedAppendOperands {
     const int32_t *page_table, *sequences, *positions;
     const float *table;
@@ -223,6 +228,7 @@ int32_t launch_head_rope(const nvq_head_rope_desc &d, const float *table, const 
                          const void *const (&w)[2], void *const (&y)[2], hipStream_t s);
 int32_t launch_append_paged(const nvq_paged_append_desc &d, const PagedAppendOperands &o, hipStream_t s);
 int32_t launch_read_paged(const nvq_paged_desc &c, int64_t tokens, const PagedAppendOperands &o, void *keys, void *values, hipStream_t s);
+bool paged_attention_launchable(const nvq_paged_attention_desc &d, bool starts);
 size_t paged_attention_workspace_bytes(const nvq_paged_attention_desc &d);
 int32_t launch_paged_attention(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, hipStream_t s);
 int32_t launch_calibrate(int32_t kind, const void *buffer, int64_t bytes, int32_t iters, void *sink, int64_t *work, hipStream_t s);

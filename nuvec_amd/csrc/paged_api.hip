@@ -28,7 +28,7 @@ int32_t check_paged(const char *op, const nvq_paged_desc &c) {
     if (c.page_size < 16 || c.page_size > 1024 || (c.page_size & (c.page_size - 1)) != 0)
         return fail(NVQ_UNSUPPORTED, "%s: pages of %lld positions (a power of two from 16 to 1024)", op, (long long)c.page_size);
     if (c.sequences > 1 && c.table_stride < c.columns) return fail(NVQ_INVALID_ARGUMENT, "%s: the page table's rows overlap", op);
-    if (c.pages >= 1LL << 31 || c.key_heads >= 1 << 15 || c.sequences >= 1 << 20 || c.columns * c.page_size >= 1LL << 30)
+    if (c.pages >= 1LL << 31 || c.key_heads >= 1 << 15 || c.sequences >= 1 << 20 || c.columns > ((1LL << 30) - 1) / c.page_size)
         return fail(NVQ_UNSUPPORTED, "%s: more than 2^31 pages, 2^15 key heads, 2^20 sequences or 2^30 positions of one", op);
     return NVQ_OK;
 }
@@ -58,7 +58,7 @@ static int32_t rotation_table(const F *freqs, int32_t dims, int64_t rows, double
     const char *op = "rotation_table";
     if (dims < 0 || dims % 2 != 0 || rows < 0) return fail(NVQ_INVALID_ARGUMENT, "%s: %d values, %lld positions", op, dims, (long long)rows);
     if (dims == 0 || rows == 0) return NVQ_OK;
-    if (rows * (dims / 2) >= 1LL << 36) return fail(NVQ_UNSUPPORTED, "%s: more than 2^36 angles", op);
+    if (rows >= (1LL << 32) || !launchable((rows * (dims / 2) + 255) / 256, 256)) return fail(NVQ_UNSUPPORTED, "%s: 2^32 angles or more", op);
     if (freqs == nullptr && !(base > 0.0)) return fail(NVQ_INVALID_ARGUMENT, "%s: base %g", op, base);
     if (table == nullptr) return fail(NVQ_INVALID_ARGUMENT, "%s: null operand", op);
     NVQ_TRY(require_device());
@@ -87,9 +87,10 @@ int32_t nvq_head_norm_rope(const nvq_head_rope_desc *d, const float *table, cons
     if (d->head_dim > 512) return fail(NVQ_UNSUPPORTED, "%s: heads of %d values (512 at most)", op, d->head_dim);
     NVQ_TRY(check_rotation(op, d->head_dim, d->rotary_dims, d->table_rows, table));
     NVQ_TRY(check_eps(op, d->eps));
-    // 32-bit head numbers; blocks of four tokens at least
-    if (d->heads[0] + d->heads[1] >= 1 << 16 || (d->length > 0 && d->batch >= (1LL << 32) / d->length))
-        return fail(NVQ_UNSUPPORTED, "%s: more than 2^16 heads or 2^32 positions", op);
+    // (a row of blocks a head where there are few positions)
+    const int64_t most = most_positions(d->head_dim);
+    if (d->heads[0] >= 1 << 16 || d->heads[1] >= 1 << 16 || d->heads[0] + d->heads[1] >= 1 << 16 || (d->length > 0 && d->batch > most / d->length))
+        return fail(NVQ_UNSUPPORTED, "%s: more than 2^16 heads or %lld positions of %d values", op, (long long)most, d->head_dim);
     if (d->batch == 0 || d->length == 0 || d->heads[0] + d->heads[1] == 0) return NVQ_OK;
     const void *const x[2] = {x0, x1}, *const w[2] = {weight0, weight1};
     void *const y[2] = {y0, y1};
@@ -114,8 +115,9 @@ int32_t nvq_append_paged(const nvq_paged_append_desc *d, const int32_t *page_tab
     NVQ_TRY(check_rotation(op, c.head_dim, d->rotary_dims, d->table_rows, table));
     NVQ_TRY(check_eps(op, d->eps));
     if (d->tokens < 0 || d->query_heads < 0) return fail(NVQ_INVALID_ARGUMENT, "%s: negative size", op);
-    if (d->tokens >= 1LL << 32 || d->query_heads + 2 * c.key_heads >= 1 << 16)  // (a row of blocks a head where there are few tokens)
-        return fail(NVQ_UNSUPPORTED, "%s: more than 2^32 tokens or 2^16 heads of them", op);
+    const int64_t most = most_positions(c.head_dim);
+    if (d->tokens > most || d->query_heads >= 1 << 16 || d->query_heads + 2 * c.key_heads >= 1 << 16)  // (a row of blocks a head where there are few tokens)
+        return fail(NVQ_UNSUPPORTED, "%s: more than %lld tokens or 2^16 heads of them", op, (long long)most);
     const bool queries = q != nullptr && d->query_heads > 0;
     if (d->tokens == 0 || (c.key_heads == 0 && !queries)) return NVQ_OK;
     if (positions == nullptr || (c.key_heads > 0 && (k == nullptr || v == nullptr)) || (queries && q_out == nullptr))
@@ -136,7 +138,8 @@ int32_t nvq_read_paged(const nvq_paged_desc *d, int64_t tokens, const int32_t *p
     if (d == nullptr) return fail(NVQ_INVALID_ARGUMENT, "%s: null descriptor", op);
     NVQ_TRY(check_paged(op, *d));
     if (tokens < 0) return fail(NVQ_INVALID_ARGUMENT, "%s: negative size", op);
-    if (tokens >= 1LL << 32) return fail(NVQ_UNSUPPORTED, "%s: more than 2^32 tokens", op);
+    const int64_t most = most_positions(d->head_dim);
+    if (tokens > most) return fail(NVQ_UNSUPPORTED, "%s: more than %lld tokens", op, (long long)most);
     if (tokens == 0 || d->key_heads == 0) return NVQ_OK;
     if (positions == nullptr || keys == nullptr || values == nullptr) return fail(NVQ_INVALID_ARGUMENT, "%s: null operand", op);
     NVQ_TRY(check_page_table(op, *d, page_table));
@@ -159,7 +162,7 @@ static int32_t check_paged_attention(const nvq_paged_attention_desc *d) {
     if (c.key_heads == 0 || d->query_heads % c.key_heads != 0)
         return fail(NVQ_INVALID_ARGUMENT, "%s: %lld query heads over %lld key heads", op, (long long)d->query_heads, (long long)c.key_heads);
     if (d->window > 0 && !d->causal) return fail(NVQ_INVALID_ARGUMENT, "%s: a window without the causal mask", op);
-    if (d->query_heads >= 1 << 15 || d->rows * d->query_heads >= 1LL << 30) return fail(NVQ_UNSUPPORTED, "%s: more than 2^30 rows and heads", op);
+    if (d->query_heads >= 1 << 15 || d->rows >= 1LL << 30 || d->rows * d->query_heads >= 1LL << 30) return fail(NVQ_UNSUPPORTED, "%s: more than 2^30 rows and heads", op);
     for (int i = 0; i < 2; i++)
         if (d->q_strides[i] < 0 || d->out_strides[i] < 0) return fail(NVQ_INVALID_ARGUMENT, "%s: negative stride", op);
     return NVQ_OK;
@@ -180,6 +183,8 @@ int32_t nvq_paged_attention(const nvq_paged_attention_desc *d, const void *q, co
     if (query_starts == nullptr && c.sequences != d->rows)
         return fail(NVQ_INVALID_ARGUMENT, "%s: %lld rows of %lld sequences without query starts", op, (long long)d->rows, (long long)c.sequences);
     if (c.pages == 0 || c.columns == 0) return fail(NVQ_INVALID_ARGUMENT, "%s: a cache of no pages", op);
+    if (!paged_attention_launchable(*d, query_starts != nullptr))
+        return fail(NVQ_UNSUPPORTED, "%s: %lld rows of %lld sequences, %lld heads each, in one launch", op, (long long)d->rows, (long long)c.sequences, (long long)d->query_heads);
     if (q == nullptr || page_table == nullptr || lengths == nullptr || out == nullptr) return fail(NVQ_INVALID_ARGUMENT, "%s: null operand", op);
     NVQ_TRY(check_pool(op, c, k_w, k_s, k_b, v_w, v_s, v_b));
     for (const void *p : {q, sinks, (const void *)out}) NVQ_TRY(check_elements(op, "an operand", p, c.dtype));

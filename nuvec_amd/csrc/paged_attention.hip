@@ -35,12 +35,13 @@ struct Kernel {
     int32_t target;  // blocks that the chip holds at once
     size_t bytes;    // of its states
 };
+int64_t lines_of(const nvq_paged_attention_desc &d, bool many) { return many ? kPromptLines : 16 / (d.cache.head_dim / d.cache.group_size); }
 // States of every item of the sequences that are split: at most twice the target (paged_schedule.h: each of their splits but the last is a
 // whole item).
 Kernel kernel_of(const nvq_paged_attention_desc &d, bool many) {
     const int groups = d.cache.head_dim / d.cache.group_size;
     Kernel k;
-    k.lines = many ? kPromptLines : 16 / groups;
+    k.lines = lines_of(d, many);
     k.target = (many || d.cache.dtype == NVQ_F32 || groups == 4 ? 2 : 3) * compute_units();
     k.bytes = paged::kPlanBytes + (size_t)(2 * (int64_t)k.target * k.lines * (d.cache.head_dim + 4)) * sizeof(float);
     return k;
@@ -57,7 +58,25 @@ bool takes_many(const nvq_paged_attention_desc &d, bool starts) {
     return starts && d.cache.dtype != NVQ_F32 && most * (d.query_heads / d.cache.key_heads) > few_lines(d);
 }
 
+// Units of one of the kernels at most, whatever the lengths and starts on the device say.  `many`: whether both kernels are launched, or that of many
+// lines alone.
+int64_t most_units(const nvq_paged_attention_desc &d, bool starts, bool many, bool of_many) {
+    const nvq_paged_desc &c = d.cache;
+    const int64_t rep = d.query_heads / c.key_heads, lines = lines_of(d, of_many);
+    const int64_t each = many && !of_many ? (few_lines(d) + lines - 1) / lines : (rep + lines - 1) / lines;
+    int64_t units = c.sequences * each;
+    if (starts) units = of_many ? d.rows * rep / lines + c.sequences : (d.rows * rep + lines - 1) / lines + c.sequences;
+    if (many && !of_many && units > c.sequences * each) units = c.sequences * each;
+    return units * c.key_heads;
+}
+
 }  // namespace
+
+// (2^12 blocks: more than the items that splits add, half of what the chip holds)
+bool paged_attention_launchable(const nvq_paged_attention_desc &d, bool starts) {
+    const bool many = takes_many(d, starts);
+    return launchable(most_units(d, starts, many, false) + (1 << 12), 256) && (!many || launchable(most_units(d, starts, many, true) + (1 << 12), 512));
+}
 
 size_t paged_attention_workspace_bytes(const nvq_paged_attention_desc &d) {
     if (!may_split(d) || d.rows == 0) return 0;
@@ -72,13 +91,7 @@ int32_t launch_paged_attention(const nvq_paged_attention_desc &d, const PagedAtt
         paged::PagedLaunch r{};
         r.batch = paged::batch_of(d, o);
         r.batch.few = alone ? -1 : many ? few_lines(d) : INT32_MAX, r.batch.target = k.target;
-        const int64_t rep = r.batch.rep;
-        // At most so many units and items, whatever the lengths and starts on the device say (paged_schedule.h).
-        const int64_t each = many && !of_many ? (few_lines(d) + k.lines - 1) / k.lines : (rep + k.lines - 1) / k.lines;
-        int64_t units = c.sequences * each;
-        if (starts) units = of_many ? d.rows * rep / k.lines + c.sequences : (d.rows * rep + k.lines - 1) / k.lines + c.sequences;
-        if (many && !of_many && units > c.sequences * each) units = c.sequences * each;
-        units *= c.key_heads;
+        const int64_t rep = r.batch.rep, units = most_units(d, starts, many, of_many);  // (and so many items at most: paged_schedule.h)
         r.batch.least = !may_split(d) ? 1 << 26 : of_many ? kLeastMany : kLeastFew;
         const int64_t least = (int64_t)kScheduleKeys * r.batch.least, splits = (c.columns * c.page_size + least - 1) / least, full = k.target, spare = full / 2 + units;
         const int64_t items = full > spare ? full : spare;
