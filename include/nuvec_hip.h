@@ -382,6 +382,7 @@ NVQ_API int32_t nvq_head_norm_rope(const nvq_head_rope_desc *desc, const float *
 /* New keys (normed where k_weight, rotated where rotary_dims) and values quantized into the cache, and q_out = rotate(norm(q)) beside
  * them.  Codes are made from float32 results, each the nearest to the scale and bias as they are stored.  A token whose position is
  * negative (padding) or outside the table, the cache or the sequences writes no row of the cache; its queries are computed all the same.
+ * The page table is read for every token, of an empty pool too: NULL only without sequences or columns.
  * Two tokens of one position: either's codes and scales may stay. */
 NVQ_API int32_t nvq_append_paged(const nvq_paged_append_desc *desc, const int32_t *page_table, const int32_t *sequences, const int32_t *positions,
                          const float *table, const void *q, const void *q_weight, void *q_out, const void *k, const void *k_weight, const void *v,
