@@ -31,29 +31,34 @@ def rotation_freqs(dims: int, base: float = 10000.0, scaling: Optional[dict] = N
         return None, 1.0, 1.0
     if dims <= 0 or dims % 2:
         raise InvalidArgument(f"rotation_freqs: {dims} rotary values")
+    if kind not in ("linear", "llama3", "yarn"):
+        raise Unsupported(f"rotation_freqs: scaling '{kind}'")
+
+    def number(key: str, otherwise: Optional[float] = None) -> float:
+        value = scaling.get(key)
+        if value is None and otherwise is None:
+            raise InvalidArgument(f"rotation_freqs: scaling '{kind}' without {key}")
+        return float(otherwise if value is None else value)
+
+    factor = number("factor")
     if kind == "linear":
-        return None, 1.0 / float(scaling["factor"]), 1.0
+        return None, 1.0 / factor, 1.0
     freqs = base ** (torch.arange(0, dims, 2, dtype=torch.float64) / dims)
-    factor = float(scaling["factor"])
     if kind == "llama3":
-        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
-        turns = float(scaling["original_max_position_embeddings"]) / (2 * math.pi * freqs)
+        low, high = number("low_freq_factor"), number("high_freq_factor")
+        turns = number("original_max_position_embeddings") / (2 * math.pi * freqs)
         keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
-        return (1.0 / ((1.0 - keep) / (factor * freqs) + keep / freqs)), 1.0, 1.0
-    if kind == "yarn":
-        most = float(scaling["original_max_position_embeddings"])
-        at = lambda turns: dims * math.log(most / (turns * 2 * math.pi)) / (2 * math.log(base))
-        low, high = at(float(scaling.get("beta_fast", 32.0))), at(float(scaling.get("beta_slow", 1.0)))
-        if scaling.get("truncate", True):  # (the blend begins and ends at whole pairs)
-            low, high = math.floor(low), math.ceil(high)
-        low, high = max(low, 0), min(high, dims - 1)
-        slowed = ((torch.arange(dims // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
-        magnitude = lambda m: 1.0 if factor <= 1.0 else 0.1 * m * math.log(factor) + 1.0
-        given = scaling.get("attention_factor")
-        if given is None:
-            given = magnitude(float(scaling.get("mscale", 1.0))) / (magnitude(float(scaling["mscale_all_dim"])) if "mscale_all_dim" in scaling else 1.0)
-        return (1.0 / (slowed / (factor * freqs) + (1.0 - slowed) / freqs)), 1.0, float(given)
-    raise Unsupported(f"rotation_freqs: scaling '{kind}'")
+        return 1.0 / ((1.0 - keep) / (factor * freqs) + keep / freqs), 1.0, 1.0
+    most = number("original_max_position_embeddings")
+    at = lambda turns: dims * math.log(most / (turns * 2 * math.pi)) / (2 * math.log(base))
+    low, high = at(number("beta_fast", 32.0)), at(number("beta_slow", 1.0))
+    if scaling.get("truncate") in (None, True):  # (the blend begins and ends at whole pairs)
+        low, high = math.floor(low), math.ceil(high)
+    low, high = max(low, 0), min(high, dims - 1)
+    slowed = ((torch.arange(dims // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
+    magnitude = lambda m: 1.0 if factor <= 1.0 else 0.1 * m * math.log(factor) + 1.0
+    magnitudes = magnitude(number("mscale", 1.0)) / magnitude(number("mscale_all_dim", 0.0))
+    return 1.0 / (slowed / (factor * freqs) + (1.0 - slowed) / freqs), 1.0, number("attention_factor", magnitudes)
 
 
 @dataclass

@@ -60,3 +60,20 @@ def test_yarn_magnitudes():
     assert of(attention_factor=0.5) == 0.5
     assert abs(of(mscale=0.7, mscale_all_dim=0.9) - by(0.7) / by(0.9)) < 1e-12
     assert abs(of(mscale=0.7) - by(0.7)) < 1e-12 and of(factor=1.0) == 1.0
+
+
+@pytest.mark.parametrize("scaling,missing", [
+    ({"rope_type": "linear"}, "factor"), ({"rope_type": "yarn", "factor": 4.0}, "original_max_position_embeddings"),
+    ({"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "original_max_position_embeddings": 8192}, "high_freq_factor")])
+def test_entries_that_lack_a_value(scaling, missing):
+    for entry in (scaling, {**scaling, missing: None}):
+        with pytest.raises(nv.InvalidArgument, match=f"without {missing}"):
+            nv.rotation_freqs(64, 10000.0, entry)
+
+
+def test_nulls_count_as_absent():
+    """As checkpoints' JSON has them."""
+    scaling = {"rope_type": "yarn", "factor": 40.0, "original_max_position_embeddings": 4096}
+    plain = nv.rotation_freqs(64, 10000.0, scaling)
+    nulls = nv.rotation_freqs(64, 10000.0, {**scaling, **dict.fromkeys(("beta_fast", "beta_slow", "mscale", "mscale_all_dim", "attention_factor", "truncate"))})
+    assert nulls[0].equal(plain[0]) and nulls[1:] == plain[1:]
