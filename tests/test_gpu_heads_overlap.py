@@ -30,3 +30,14 @@ def test_overlapping_rows(dtype):
             assert y.stride(3) == 1 and torch.equal(y, want), x.stride()
             for one, other in zip(nv.head_norm_rope(x, x, w, None, rotation, offset), nv.head_norm_rope(x.contiguous(), x.contiguous(), w, None, rotation, offset)):
                 assert one.stride(3) == 1 and torch.equal(one, other), x.stride()
+
+
+def test_expanded_outputs_are_refused():
+    """On the device too, where a call takes the native path first; a single row may have any stride."""
+    rotation = nv.Rotation(table(300, 64))
+    x = torch.randn(1, 1, 5, 64, device="cuda")
+    wide = x.expand(2, 3, 5, 64)
+    with pytest.raises(nv.InvalidArgument, match="share their memory"):
+        nv.rope(wide, rotation, 3, out=wide)
+    y = torch.zeros(330, device="cuda").as_strided((1, 1, 5, 64), (0, 0, 64, 1))
+    assert nv.rope(x, rotation, 3, out=y) is y and torch.equal(y, nv.rope(x, rotation, 3))
