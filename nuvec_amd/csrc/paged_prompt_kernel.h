@@ -13,9 +13,9 @@
 // biases are one more product (qb below).
 //
 // Terms: queries are exact in their own type.  Weights x scale are two terms of bfloat16, 16 bits (one where the element type is bfloat16: 123 us
-// instead of 139 below, and the results' error 1.4 times that of their rounding; with two it is that of the rounding).
+// instead of 140 below, and the results' error 1.4 times that of their rounding; with two it is that of the rounding).
 //
-// Measured: 1024 rows of 32 heads of 128 over 4096 positions, 8 key heads, 4 bits in groups of 64, bfloat16: 139 us, 432 TFLOP/s (groups of 128:
+// Measured: 1024 rows of 32 heads of 128 over 4096 positions, 8 key heads, 4 bits in groups of 64, bfloat16: 140 us, 430 TFLOP/s (groups of 128:
 // 121, of 32: 180: each group of a head has its own scaling of scores and weights); 2048 rows over as many positions 114 us, 1024 47 us, 512
 // 28 us.  While a compute unit is busy its vector units are at 61%, LDS at 50%, the matrix cores at 34%.  With one term a block alone took nearly
 // as long for a tile as two that share a compute unit, and the same with 32 lines a wavefront (v_mfma_f32_32x32x16, four wavefronts of 256
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(64 * kPromptWaves, 4) paged_prompt_kernel(cons
                     for (int w = 0; w < 4; w++) ones[g] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair_t, p[i][w]), one2, ones[g], false);
             }
 #pragma unroll
-            for (int d = g * GB; d < (g + 1) * GB; d += 2) {  // (two at a time: no product waits for the one in front of it; 142 -> 139 us)
+            for (int d = g * GB; d < (g + 1) * GB; d += 2) {  // (two at a time: no product waits for the one in front of it; 142 -> 140 us)
                 const uint4 v0 = from.values[sub][d][lane], v1 = from.values[sub][d + 1][lane];
 #pragma unroll
                 for (int i = 0; i < TP; i++) {
