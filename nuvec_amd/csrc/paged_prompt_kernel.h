@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(64 * kPromptWaves, 4) paged_prompt_kernel(cons
     floatx4_t o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = zeros;
-    float m = -1.0e30f, l = 0.0f, ones[G], accb[G];
+    float m = kLowest, l = 0.0f, ones[G], accb[G];
 #pragma unroll
     for (int g = 0; g < G; g++) ones[g] = accb[g] = 0.0f;
 
@@ -430,7 +430,7 @@ __device__ __forceinline__ void merge_many(const RowsArgs<T> &a, int32_t unit, i
     if (line >= item.s.rows * rep || span.items == 1) return;
     const int64_t stride = (int64_t)a.batch.key_heads * kPromptLines * kState<D>;  // of a split's states
     const float *src = a.states + ((int64_t)item.slot * kPromptLines + ln) * kState<D>;
-    float top = -1.0e30f, total = 0.0f;
+    float top = kLowest, total = 0.0f;
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int z0 = 0; z0 < span.items; z0 += 4) {
         float2 m[4];

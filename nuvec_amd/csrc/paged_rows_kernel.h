@@ -28,6 +28,9 @@ namespace paged {
 
 constexpr int kWaves = 4;
 constexpr int kTile = kScheduleKeys;
+// Where maxima start: under every score but the last thousandth of float32's range, and finite, so that a masked score's weight is
+// exp2(-inf - m) = 0 from the first tile on.
+constexpr float kLowest = -3.4e38f;
 
 template <typename T>
 struct RowsArgs {
@@ -190,7 +193,7 @@ __global__ void __launch_bounds__(64 * kWaves, (rows_blocks<T, G>())) paged_rows
     };
 
     floatx4_t acc[ND], ones = {0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -1.0e30f, denom = 0.0f, accb = 0.0f;  // (finite: a masked score's weight is exp2(-inf - m) = 0 from the first tile on)
+    float m = kLowest, denom = 0.0f, accb = 0.0f;
 #pragma unroll
     for (int i = 0; i < ND; i++) acc[i] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
     const int step = kWaves * kTile;
@@ -346,7 +349,7 @@ __global__ void __launch_bounds__(64 * kWaves, (rows_blocks<T, G>())) paged_rows
     __syncthreads();
     for (int e = tid; e < lines * D; e += 64 * kWaves) {
         const int ln = e / D, at = e % D;
-        float top = -1.0e30f;
+        float top = kLowest;
 #pragma unroll
         for (int w = 0; w < kWaves; w++) top = fmaxf(top, wave_m[w][ln]);
         float sum = 0.0f, total = 0.0f;
@@ -384,7 +387,7 @@ __device__ __forceinline__ void merge_few(const RowsArgs<T> &a, int32_t unit, in
     if (line >= item.s.rows * rep) return;
     const int64_t stride = (int64_t)a.batch.key_heads * LINES * kState<D>;  // of a split's states
     const float *src = a.states + ((int64_t)item.slot * LINES + ln) * kState<D>;
-    float top = -1.0e30f, total = 0.0f, sum[V] = {};
+    float top = kLowest, total = 0.0f, sum[V] = {};
     for (int z0 = wave; z0 < item.splits; z0 += 8 * kWaves) {
         float m[8], d[8], v[8][V];
 #pragma unroll
