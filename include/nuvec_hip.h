@@ -171,6 +171,13 @@ typedef struct nvq_head_rope_desc {
     double eps;              /* of the norm of operands with a weight */
 } nvq_head_rope_desc;
 
+/* The axes (time, height, width, ...) that the pairs of a rotation belong to: pair i (of up to 256) to axis
+ * of_pairs[i / 16] >> 2 (i % 16) & 3, below count (1 .. 4). */
+typedef struct nvq_rotary_axes {
+    int32_t count;
+    uint32_t of_pairs[16];
+} nvq_rotary_axes;
+
 /* A paged, affine-quantized key / value cache: a pool of pages [pages, key_heads, page_size, ...] for each of
  *   k_w, v_w u32 [.., head_dim*bits/32];  k_s, k_b, v_s, v_b dtype [.., head_dim/group_size], all contiguous,
  * and page_table i32 [sequences, columns] (rows table_stride apart): position p of a sequence lies in page
@@ -209,6 +216,30 @@ typedef struct nvq_paged_attention_desc {
     int32_t causal;                     /* 0: every row of a sequence sees all its positions (window must be 0) */
     float scale;
 } nvq_paged_attention_desc;
+
+/* Low-rank adapters of one projection: down dtype [adapters, rank, inputs], up dtype [adapters, outputs, rank], contiguous; rows of x,
+ * y and out as far apart as the strides say, values of a row consecutive. */
+typedef struct nvq_adapters_desc {
+    int32_t dtype;
+    int32_t rank; /* 1 .. 256 */
+    int64_t rows, inputs, outputs, adapters;
+    int64_t x_stride, y_stride, out_stride;
+} nvq_adapters_desc;
+
+/* The choice of experts from a router's logits dtype [rows, experts]. */
+#define NVQ_SCORES_SOFTMAX 0
+#define NVQ_SCORES_SIGMOID 1
+typedef struct nvq_moe_select_desc {
+    int32_t dtype;   /* of the logits and the weights */
+    int32_t scores;  /* NVQ_SCORES_* */
+    int32_t experts; /* 1 .. 1024 */
+    int32_t k;       /* 1 .. 64, at most the experts of the groups that stay */
+    int32_t groups, top_groups; /* 1 .. 64 groups of consecutive experts, of which the best top_groups stay */
+    int32_t group_best;         /* 1 or 2: how many of a group's largest values are its score */
+    int32_t normalize;
+    int64_t rows;
+    double scale;
+} nvq_moe_select_desc;
 
 /* ── runtime ─────────────────────────────────────────────────────────────────────── */
 
@@ -379,6 +410,11 @@ NVQ_API int32_t nvq_rotation_table_f64(const double *freqs, int32_t dims, int64_
 NVQ_API int32_t nvq_head_norm_rope(const nvq_head_rope_desc *desc, const float *table, const int32_t *offsets, const void *x0, const void *weight0,
                            void *y0, const void *x1, const void *weight1, void *y1, void *stream);
 
+/* The same for positions of several axes: positions i32 [axes->count, batch, length], pair i turns by the angle of its axis's position.
+ * `offset` and `per_position` of the descriptor are not read. */
+NVQ_API int32_t nvq_head_norm_rope_axes(const nvq_head_rope_desc *desc, const nvq_rotary_axes *axes, const float *table, const int32_t *positions,
+                                const void *x0, const void *weight0, void *y0, const void *x1, const void *weight1, void *y1, void *stream);
+
 /* New keys (normed where k_weight, rotated where rotary_dims) and values quantized into the cache, and q_out = rotate(norm(q)) beside
  * them.  Codes are made from float32 results, each the nearest to the scale and bias as they are stored.  A token whose position is
  * negative (padding) or outside the table, the cache or the sequences writes no row of the cache; its queries are computed all the same.
@@ -387,6 +423,13 @@ NVQ_API int32_t nvq_head_norm_rope(const nvq_head_rope_desc *desc, const float *
 NVQ_API int32_t nvq_append_paged(const nvq_paged_append_desc *desc, const int32_t *page_table, const int32_t *sequences, const int32_t *positions,
                          const float *table, const void *q, const void *q_weight, void *q_out, const void *k, const void *k_weight, const void *v,
                          uint32_t *k_w, void *k_s, void *k_b, uint32_t *v_w, void *v_s, void *v_b, void *stream);
+
+/* The same where the angles are not those of the places in the cache (images take fewer positions than tokens): rotary_positions i32
+ * [axes->count, tokens].  A token with one of them outside the table writes no row of the cache. */
+NVQ_API int32_t nvq_append_paged_axes(const nvq_paged_append_desc *desc, const nvq_rotary_axes *axes, const int32_t *page_table,
+                              const int32_t *sequences, const int32_t *positions, const int32_t *rotary_positions, const float *table,
+                              const void *q, const void *q_weight, void *q_out, const void *k, const void *k_weight, const void *v,
+                              uint32_t *k_w, void *k_s, void *k_b, uint32_t *v_w, void *v_s, void *v_b, void *stream);
 
 /* Rows of the cache as values, code * scale + bias rounded once: keys, values dtype [tokens, key_heads, head_dim], contiguous; zeros for
  * a token that lies outside the cache. */
@@ -401,6 +444,19 @@ NVQ_API size_t nvq_paged_attention_workspace_bytes(const nvq_paged_attention_des
 NVQ_API int32_t nvq_paged_attention(const nvq_paged_attention_desc *desc, const void *q, const uint32_t *k_w, const void *k_s, const void *k_b,
                             const uint32_t *v_w, const void *v_s, const void *v_b, const int32_t *page_table, const int32_t *lengths,
                             const int32_t *query_starts, const void *sinks, void *out, void *workspace, void *stream);
+
+/* out[r] = y[r] + scales[a] (x[r] . down[a]^T) . up[a]^T with a = ids[r] (i32 [rows]), rounded once; out[r] = y[r] where a is no adapter
+ * (negative, or `adapters` and more).  scales f32 [adapters], NULL: ones.  out may be y itself.  `workspace`: the size query's bytes (float32
+ * x . down^T), one call's at a time. */
+NVQ_API size_t nvq_apply_adapters_workspace_bytes(const nvq_adapters_desc *desc);
+NVQ_API int32_t nvq_apply_adapters(const nvq_adapters_desc *desc, const void *x, const void *down, const void *up, const float *scales,
+                           const int32_t *ids, const void *y, void *out, void *workspace, void *stream);
+
+/* Per row p = softmax or sigmoid of the logits, c = p + bias (f32 [experts], or NULL); a group's score is the sum of its group_best largest
+ * c, the top_groups best groups stay, and of their experts the k with the largest c are chosen, largest first (ties, of groups too: the
+ * lowest index; a NaN below everything).  Without a bias c's order is the logits' own.  indices i32 [rows, k]; weights dtype [rows, k]: p of
+ * the chosen, with `normalize` divided by (their sum + 1e-20), times scale, rounded once.  A softmax of nothing but -inf is zeros. */
+NVQ_API int32_t nvq_moe_select(const nvq_moe_select_desc *desc, const void *logits, const float *bias, int32_t *indices, void *weights, void *stream);
 
 /* GpuEval::sorted_offsets (gpu.rs:6732-6756); kernels::sorted_offsets (kernels.rs:873-892):
  * per row of `indices` u32[rows, m], offsets[row, g] = first position whose value is >= g. */

@@ -7,7 +7,7 @@ nuvec-lm's mixture-of-experts blocks around the gathered products; `formats` and
 into `Quantized` operands in device memory.  `paged` holds what stands between a model's projections and its
 attention: rotary positions, norms of heads, a paged, quantized key / value cache and the attention over it.
 """
-from .ops import (GatherQmm, InvalidArgument, Quant, QuantMode, Quantized, Unsupported, dequantize, embedding,  # noqa: F401
-                  gather_qmm, gather_qmm_glu, gather_qmm_grouped, gather_qqmm, glu, moe_order, pair_rows, moe_route, qqmm, quantize, quantize_dequantize,
+from .ops import (Adapters, GatherQmm, InvalidArgument, Quant, QuantMode, Quantized, Unsupported, apply_adapters, dequantize, embedding,  # noqa: F401
+                  gather_qmm, gather_qmm_glu, gather_qmm_grouped, gather_qqmm, glu, moe_order, pair_rows, moe_route, moe_select, qqmm, quantize, quantize_dequantize,
                   quantized_matmul, quantized_matmul_glu, quantized_matmul_kernel, quantized_matmul_route, quantized_matmul_tile, sorted_offsets, weighted_sum)
-from .paged import (PagedCache, Rotation, append_paged, head_norm_rope, paged_attention, read_paged, rope, rotation_freqs)  # noqa: F401
+from .paged import (PagedCache, Rotation, append_paged, head_norm_rope, paged_attention, read_paged, rope, rotary_axes, rotation_freqs)  # noqa: F401

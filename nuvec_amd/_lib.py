@@ -66,6 +66,20 @@ class HeadRopeDescC(C.Structure):
                 ("x_strides", C.c_int64 * 3 * 2), ("y_strides", C.c_int64 * 3 * 2), ("eps", C.c_double)]
 
 
+class RotaryAxesC(C.Structure):
+    _fields_ = [("count", C.c_int32), ("of_pairs", C.c_uint32 * 16)]
+
+
+class AdaptersDescC(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("rank", C.c_int32), ("rows", C.c_int64), ("inputs", C.c_int64), ("outputs", C.c_int64), ("adapters", C.c_int64),
+                ("x_stride", C.c_int64), ("y_stride", C.c_int64), ("out_stride", C.c_int64)]
+
+
+class MoeSelectDescC(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("scores", C.c_int32), ("experts", C.c_int32), ("k", C.c_int32), ("groups", C.c_int32), ("top_groups", C.c_int32),
+                ("group_best", C.c_int32), ("normalize", C.c_int32), ("rows", C.c_int64), ("scale", C.c_double)]
+
+
 class PagedDescC(C.Structure):
     _fields_ = [("dtype", C.c_int32), ("bits", C.c_int32), ("group_size", C.c_int32), ("head_dim", C.c_int32), ("pages", C.c_int64),
                 ("page_size", C.c_int64), ("key_heads", C.c_int64), ("sequences", C.c_int64), ("columns", C.c_int64), ("table_stride", C.c_int64)]
@@ -133,6 +147,11 @@ SIGNATURES = {
     "nvq_rotation_table": (C.c_int32, [C.c_void_p, C.c_int32, C.c_int64, C.c_double, C.c_double, C.c_double, C.c_void_p, C.c_void_p]),
     "nvq_rotation_table_f64": (C.c_int32, [C.c_void_p, C.c_int32, C.c_int64, C.c_double, C.c_double, C.c_double, C.c_void_p, C.c_void_p]),
     "nvq_head_norm_rope": (C.c_int32, [C.POINTER(HeadRopeDescC)] + [C.c_void_p] * 9),
+    "nvq_head_norm_rope_axes": (C.c_int32, [C.POINTER(HeadRopeDescC), C.POINTER(RotaryAxesC)] + [C.c_void_p] * 9),
+    "nvq_append_paged_axes": (C.c_int32, [C.POINTER(PagedAppendDescC), C.POINTER(RotaryAxesC)] + [C.c_void_p] * 18),
+    "nvq_apply_adapters_workspace_bytes": (C.c_size_t, [C.POINTER(AdaptersDescC)]),
+    "nvq_apply_adapters": (C.c_int32, [C.POINTER(AdaptersDescC)] + [C.c_void_p] * 9),
+    "nvq_moe_select": (C.c_int32, [C.POINTER(MoeSelectDescC)] + [C.c_void_p] * 5),
     "nvq_append_paged": (C.c_int32, [C.POINTER(PagedAppendDescC)] + [C.c_void_p] * 17),
     "nvq_read_paged": (C.c_int32, [C.POINTER(PagedDescC), C.c_int64] + [C.c_void_p] * 12),
     "nvq_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedAttentionDescC)]),

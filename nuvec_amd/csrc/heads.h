@@ -116,6 +116,47 @@ __device__ __forceinline__ Turn read_turn(const float2 *__restrict__ angles, int
     return t;
 }
 
+// Rotations whose pairs belong to axes (time, height, width, ...): each axis has a position a token, pair i turns by the angle of its axis's.
+// A token's positions are a handful of words, the angles are gathered pair by pair, once for all heads that a block walks.
+struct NoAxes {
+    static constexpr bool kAny = false;
+};
+struct PairAxes {
+    static constexpr bool kAny = true;
+    const int32_t *positions;  // [axes, tokens]
+    nvq_rotary_axes axes;
+    __device__ __forceinline__ int64_t at(int axis, int64_t token, int64_t tokens) const { return positions[axis * tokens + token]; }
+    // Whether every axis's position of the token has angles.
+    __device__ __forceinline__ bool inside(int64_t token, int64_t tokens, int64_t table_rows) const {
+        bool all = true;
+        for (int i = 0; i < axes.count; i++) all = all && at(i, token, tokens) >= 0 && at(i, token, tokens) < table_rows;
+        return all;
+    }
+    // Positions outside the table are the caller's error: clamped to it.
+    __device__ __forceinline__ Turn turn(const float2 *__restrict__ table, int64_t table_rows, int64_t token, int64_t tokens, int j0, int half, bool interleaved) const {
+        const float2 *rows[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int64_t p = at(i < axes.count ? i : 0, token, tokens);
+            rows[i] = table + (p < 0 ? 0 : p < table_rows ? p : table_rows - 1) * half;
+        }
+        Turn t;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int j = j0 + i;
+            t.c[i] = 1.0f, t.n[i] = 0.0f;
+            if (j < 2 * half) {
+                const bool second = interleaved ? (j & 1) != 0 : j >= half;
+                const int pair = interleaved ? j >> 1 : second ? j - half : j;
+                const uint32_t axis = axes.of_pairs[pair >> 4] >> (2 * (pair & 15)) & 3u;
+                const float2 a = (axis & 2u ? (axis & 1u ? rows[3] : rows[2]) : axis & 1u ? rows[1] : rows[0])[pair];
+                t.c[i] = a.x, t.n[i] = second ? a.y : -a.y;
+            }
+        }
+        return t;
+    }
+};
+
 // The lane's values of a head and those that the rotation mixes into them, as they lie in memory: a head's are requested before the one in front of it is
 // worked on.
 template <typename T, int READ>

@@ -33,8 +33,8 @@ struct HeadArgs {
     double eps;
 };
 
-template <typename T, int P, int READ>
-__global__ void __launch_bounds__(kHeadBlock) head_norm_rope_kernel(const HeadArgs<T> a) {
+template <typename T, int P, int READ, typename Axes>
+__global__ void __launch_bounds__(kHeadBlock) head_norm_rope_kernel(const HeadArgs<T> a, const Axes axes) {
     constexpr int kSlots = kHeadBlock / P;
     __shared__ HeldHeads<T, P, READ> held;
     const int j0 = 8 * (threadIdx.x % P);
@@ -43,7 +43,9 @@ __global__ void __launch_bounds__(kHeadBlock) head_norm_rope_kernel(const HeadAr
     const int64_t b = token / a.length, l = token - b * a.length;
     const bool interleaved = a.interleaved != 0;
     Turn turn{};
-    if (a.half > 0) {
+    if constexpr (Axes::kAny) {
+        if (a.half > 0) turn = axes.turn(a.table, a.table_rows, token, a.tokens, j0, a.half, interleaved);
+    } else if (a.half > 0) {
         int64_t position = a.offsets == nullptr ? a.offset + l : a.per_position ? (int64_t)a.offsets[token] : (int64_t)a.offsets[b] + l;
         position = position < 0 ? 0 : position < a.table_rows ? position : a.table_rows - 1;  // (outside the table is the caller's error: clamped)
         turn = read_turn<READ>(a.table + position * a.half, j0, a.half, interleaved);
@@ -79,19 +81,19 @@ __global__ void __launch_bounds__(kHeadBlock) head_norm_rope_kernel(const HeadAr
     }
 }
 
-template <typename T, int P>
-int32_t run_heads(const HeadArgs<T> &a, int read, hipStream_t s) {
+template <typename T, int P, typename Axes>
+int32_t run_heads(const HeadArgs<T> &a, const Axes &axes, int read, hipStream_t s) {
     const dim3 grid((unsigned)((a.tokens + kHeadBlock / P - 1) / (kHeadBlock / P)), (unsigned)((a.all_heads + a.per_block - 1) / a.per_block));
-    if (read == kWhole) hipLaunchKernelGGL((head_norm_rope_kernel<T, P, kWhole>), grid, dim3(kHeadBlock), 0, s, a);
-    else if (read == kRuns) hipLaunchKernelGGL((head_norm_rope_kernel<T, P, kRuns>), grid, dim3(kHeadBlock), 0, s, a);
-    else hipLaunchKernelGGL((head_norm_rope_kernel<T, P, kSingle>), grid, dim3(kHeadBlock), 0, s, a);
+    if (read == kWhole) hipLaunchKernelGGL((head_norm_rope_kernel<T, P, kWhole, Axes>), grid, dim3(kHeadBlock), 0, s, a, axes);
+    else if (read == kRuns) hipLaunchKernelGGL((head_norm_rope_kernel<T, P, kRuns, Axes>), grid, dim3(kHeadBlock), 0, s, a, axes);
+    else hipLaunchKernelGGL((head_norm_rope_kernel<T, P, kSingle, Axes>), grid, dim3(kHeadBlock), 0, s, a, axes);
     NVQ_LAUNCH_CHECK("head_norm_rope");
     return NVQ_OK;
 }
 
-template <typename T>
-int32_t run_type(const nvq_head_rope_desc &d, const float *table, const int32_t *offsets, const void *const (&x)[2], const void *const (&w)[2],
-                 void *const (&y)[2], hipStream_t s) {
+template <typename T, typename Axes>
+int32_t run_type(const nvq_head_rope_desc &d, const Axes &axes, const float *table, const int32_t *offsets, const void *const (&x)[2],
+                 const void *const (&w)[2], void *const (&y)[2], hipStream_t s) {
     HeadArgs<T> a{};
     uintptr_t rows = 0, others = (uintptr_t)table;  // addresses and strides in bytes: their lowest bits
     for (int i = 0; i < 2; i++) {
@@ -116,10 +118,10 @@ int32_t run_type(const nvq_head_rope_desc &d, const float *table, const int32_t 
     const int64_t per = blocks * a.all_heads / want;
     a.per_block = (int32_t)(per < 1 ? 1 : per < a.all_heads ? per : a.all_heads);
     switch (p) {
-    case 8: return run_heads<T, 8>(a, read, s);
-    case 16: return run_heads<T, 16>(a, read, s);
-    case 32: return run_heads<T, 32>(a, read, s);
-    default: return run_heads<T, 64>(a, read, s);
+    case 8: return run_heads<T, 8>(a, axes, read, s);
+    case 16: return run_heads<T, 16>(a, axes, read, s);
+    case 32: return run_heads<T, 32>(a, axes, read, s);
+    default: return run_heads<T, 64>(a, axes, read, s);
     }
 }
 
@@ -140,13 +142,19 @@ __global__ void __launch_bounds__(256) rotation_table_kernel(const F *__restrict
 
 }  // namespace
 
-int32_t launch_head_rope(const nvq_head_rope_desc &d, const float *table, const int32_t *offsets, const void *const (&x)[2],
-                         const void *const (&w)[2], void *const (&y)[2], hipStream_t s) {
+template <typename Axes>
+static int32_t run_any(const nvq_head_rope_desc &d, const Axes &axes, const float *table, const int32_t *offsets, const void *const (&x)[2],
+                       const void *const (&w)[2], void *const (&y)[2], hipStream_t s) {
     switch (d.dtype) {
-    case NVQ_F32: return run_type<float>(d, table, offsets, x, w, y, s);
-    case NVQ_BF16: return run_type<bf16_t>(d, table, offsets, x, w, y, s);
-    default: return run_type<f16_t>(d, table, offsets, x, w, y, s);
+    case NVQ_F32: return run_type<float>(d, axes, table, offsets, x, w, y, s);
+    case NVQ_BF16: return run_type<bf16_t>(d, axes, table, offsets, x, w, y, s);
+    default: return run_type<f16_t>(d, axes, table, offsets, x, w, y, s);
     }
+}
+
+int32_t launch_head_rope(const nvq_head_rope_desc &d, const nvq_rotary_axes *axes, const float *table, const int32_t *offsets, const void *const (&x)[2],
+                         const void *const (&w)[2], void *const (&y)[2], hipStream_t s) {
+    return axes == nullptr ? run_any(d, NoAxes{}, table, offsets, x, w, y, s) : run_any(d, PairAxes{offsets, *axes}, table, offsets, x, w, y, s);
 }
 
 template <typename F>

@@ -34,7 +34,7 @@ using at::Tensor;
 struct Names {
     PyObject *mode, *group_size, *bits, *weight, *scales, *biases, *bias, *quant, *global_scale;
     PyObject *gate_proj, *up_proj, *down_proj, *gate_up_proj, *geglu;
-    PyObject *keys, *values, *table, *interleaved;
+    PyObject *keys, *values, *table, *interleaved, *axes, *down, *up;
     PyObject *gate, *switch_mlp, *experts_per_token, *norm_topk_prob, *gate_up_paired, *activation, *alpha, *limit;
 } names;
 
@@ -728,6 +728,8 @@ PyObject *py_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
 struct Angles {
     Tensor table;
     bool interleaved = false;
+    nvq_rotary_axes axes{};  // count 0: none; else one more than the largest of the pairs'
+    int64_t pairs = 0;       // that have an axis
     int32_t dims() const { return table.defined() ? (int32_t)(2 * table.size(1)) : 0; }
     int64_t rows() const { return table.defined() ? table.size(0) : 0; }
     bool fits(const Place &at, int64_t dim) const {
@@ -735,8 +737,29 @@ struct Angles {
                                     2 * table.size(1) <= dim && at.holds(table));
     }
 };
+bool read_axes(PyObject *o, Angles &a) {
+    Ref axes(PyObject_GetAttr(o, names.axes));
+    if (axes.p == nullptr) PyErr_Clear();  // (an object without them)
+    if (axes.p == nullptr || axes.p == Py_None) return true;
+    if (!PyTuple_CheckExact(axes.p) || PyTuple_GET_SIZE(axes.p) > 256) return false;
+    a.pairs = PyTuple_GET_SIZE(axes.p);
+    for (int64_t i = 0; i < a.pairs; i++) {
+        PyObject *v = PyTuple_GET_ITEM(axes.p, i);
+        const long axis = PyLong_Check(v) ? PyLong_AsLong(v) : -1;
+        if (PyErr_Occurred()) return declined();
+        if (axis < 0 || axis > 3) return false;
+        a.axes.of_pairs[i / 16] |= (uint32_t)axis << 2 * (i % 16);
+        if (axis >= a.axes.count) a.axes.count = (int32_t)axis + 1;
+    }
+    return true;
+}
 bool read_angles(PyObject *o, Angles &a) {
-    return o == Py_None || (read_tensor(o, names.table, a.table) && a.table.defined() && read_truth(o, names.interleaved, a.interleaved));
+    return o == Py_None || (read_tensor(o, names.table, a.table) && a.table.defined() && read_truth(o, names.interleaved, a.interleaved) && read_axes(o, a));
+}
+// The axes for positions of `count` of them.
+bool axes_fit(const Angles &a, int64_t count, nvq_rotary_axes &axes) {
+    axes = a.axes, axes.count = (int32_t)count;
+    return a.table.defined() && a.pairs > 0 && a.pairs == a.table.size(1) && count >= a.axes.count && count <= 4;
 }
 
 bool weight_fits(const Tensor &w, const Place &at, at::ScalarType type, int64_t dim) {
@@ -764,7 +787,13 @@ bool rotate(const Place &at, const Tensor *xs, const Tensor *weights, int count,
     nvq_head_rope_desc d{};
     d.dtype = code_of(x.scalar_type()), d.head_dim = (int32_t)x.size(3), d.rotary_dims = angles.dims(), d.interleaved = angles.interleaved;
     d.table_rows = angles.rows(), d.batch = x.size(0), d.length = x.size(2), d.eps = eps;
-    if (offsets.defined()) {
+    nvq_rotary_axes axes;
+    const bool several = offsets.defined() && offsets.dim() == 3;
+    if (several) {
+        if (!axes_fit(angles, offsets.size(0), axes) || offsets.scalar_type() != at::kInt || !at.holds(offsets) || offsets.size(1) != d.batch ||
+            offsets.size(2) != d.length)
+            return false;
+    } else if (offsets.defined()) {
         d.per_position = offsets.dim() == 2;
         if (offsets.scalar_type() != at::kInt || !at.holds(offsets) || offsets.dim() < 1 || offsets.dim() > 2 || offsets.size(0) != d.batch ||
             (d.per_position && offsets.size(1) != d.length))
@@ -786,6 +815,10 @@ bool rotate(const Place &at, const Tensor *xs, const Tensor *weights, int count,
         for (int k = 0; k < 3; k++) d.x_strides[i][k] = xs[i].stride(k), d.y_strides[i][k] = ys[i].stride(k);
     }
     const bool two = count == 2;
+    if (several)
+        return nvq_head_norm_rope_axes(&d, &axes, (const float *)ptr(angles.table), (const int32_t *)ptr(offsets), ptr(xs[0]), ptr(weights[0]),
+                                       ys[0].mutable_data_ptr(), two ? ptr(xs[1]) : nullptr, two ? ptr(weights[1]) : nullptr,
+                                       two ? ys[1].mutable_data_ptr() : nullptr, at.stream()) == NVQ_OK;
     return nvq_head_norm_rope(&d, (const float *)ptr(angles.table), (const int32_t *)ptr(offsets), ptr(xs[0]), ptr(weights[0]), ys[0].mutable_data_ptr(),
                               two ? ptr(xs[1]) : nullptr, two ? ptr(weights[1]) : nullptr, two ? ys[1].mutable_data_ptr() : nullptr,
                               at.stream()) == NVQ_OK;
@@ -869,13 +902,13 @@ bool is_rows(const Tensor &x, const Place &at, at::ScalarType type, int64_t toke
            x.stride(2) == 1;
 }
 
-// append_paged(cache, k, v, page table, positions, sequences, rotation, k weight, q, q weight, eps): the queries, or True without any
+// append_paged(cache, k, v, page table, positions, sequences, rotation, k weight, q, q weight, eps, rotary positions): the queries, or True without any
 PyObject *py_append_paged(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
         Paged p;
         Angles angles;
-        Tensor k, v, positions, sequences, k_weight, q, q_weight, y;
-        if (n != 11 || !as_tensor(args[1], k) || !as_tensor(args[2], v) || !read_paged(args[0], args[3], p) || !as_tensor(args[4], positions) ||
+        Tensor k, v, positions, sequences, k_weight, q, q_weight, rotary, y;
+        if (n != 12 || !as_tensor(args[11], rotary) || !as_tensor(args[1], k) || !as_tensor(args[2], v) || !read_paged(args[0], args[3], p) || !as_tensor(args[4], positions) ||
             !as_tensor(args[5], sequences) || !read_angles(args[6], angles) || !as_tensor(args[7], k_weight) || !as_tensor(args[8], q) ||
             !as_tensor(args[9], q_weight))
             return none();
@@ -897,8 +930,21 @@ PyObject *py_append_paged(PyObject *, PyObject *const *args, Py_ssize_t n) {
             d.k_strides[i] = k.stride(i), d.v_strides[i] = v.stride(i);
             if (q.defined()) d.q_strides[i] = q.stride(i);
         }
+        nvq_rotary_axes axes{1, {}};
+        if (rotary.defined()) {
+            const bool one = rotary.dim() == 1;
+            if (!angles.table.defined() || (one ? !is_index(rotary, at, tokens) : rotary.dim() != 2 || !axes_fit(angles, rotary.size(0), axes) ||
+                                                                                      rotary.scalar_type() != at::kInt || rotary.size(1) != tokens || !at.holds(rotary)))
+                return none();
+        }
         const bool done = unlocked([&] {
             if (q.defined()) y = at.empty(q.sizes(), type);
+            if (rotary.defined())
+                return nvq_append_paged_axes(&d, &axes, (const int32_t *)ptr(p.table), (const int32_t *)ptr(sequences), (const int32_t *)ptr(positions),
+                                             (const int32_t *)ptr(rotary), (const float *)ptr(angles.table), ptr(q), q.defined() ? ptr(q_weight) : nullptr,
+                                             q.defined() ? y.mutable_data_ptr() : nullptr, ptr(k), ptr(k_weight), ptr(v), (uint32_t *)p.k.w.mutable_data_ptr(),
+                                             p.k.s.mutable_data_ptr(), p.k.b.mutable_data_ptr(), (uint32_t *)p.v.w.mutable_data_ptr(),
+                                             p.v.s.mutable_data_ptr(), p.v.b.mutable_data_ptr(), at.stream()) == NVQ_OK;
             return nvq_append_paged(&d, (const int32_t *)ptr(p.table), (const int32_t *)ptr(sequences), (const int32_t *)ptr(positions),
                                     (const float *)ptr(angles.table), ptr(q), q.defined() ? ptr(q_weight) : nullptr,
                                     q.defined() ? y.mutable_data_ptr() : nullptr, ptr(k), ptr(k_weight), ptr(v), (uint32_t *)p.k.w.mutable_data_ptr(),
@@ -973,6 +1019,82 @@ PyObject *py_paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
+// ── adapters and the choice of experts ──────────────────────────────────────────────────────────────────────────────
+// apply_adapters(y, x, adapters, ids, out or None)
+PyObject *py_apply_adapters(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        Tensor x, y, ids, down, up, scales, out;
+        if (n != 5 || !as_tensor(args[0], y) || !as_tensor(args[1], x) || !read_tensor(args[2], names.down, down) || !read_tensor(args[2], names.up, up) ||
+            !read_tensor(args[2], names.scales, scales) || !as_tensor(args[3], ids) || !as_tensor(args[4], out))
+            return none();
+        const Place at(x);
+        if (!at.usable() || !y.defined() || !ids.defined() || !down.defined() || !up.defined()) return none();
+        const at::ScalarType type = x.scalar_type();
+        const int64_t dims = x.dim();
+        if (code_of(type) < 0 || dims < 1 || x.numel() == 0 || y.numel() == 0 || !at.holds(x) || !at.holds(y) || y.scalar_type() != type || y.dim() != dims ||
+            down.dim() != 3 || up.dim() != 3 || down.scalar_type() != type || up.scalar_type() != type || !at.holds(down) || !at.holds(up) ||
+            down.numel() == 0 || up.numel() == 0)
+            return none();
+        const int64_t inputs = x.size(dims - 1), outputs = y.size(dims - 1), rows = x.numel() / inputs, count = down.size(0), rank = down.size(1);
+        if (down.size(2) != inputs || up.size(0) != count || up.size(1) != outputs || up.size(2) != rank || rank > INT32_MAX ||
+            ids.scalar_type() != at::kInt || !at.holds(ids) || ids.sizes() != x.sizes().slice(0, dims - 1) || ids.sizes() != y.sizes().slice(0, dims - 1) ||
+            (scales.defined() && (scales.scalar_type() != at::kFloat || scales.dim() != 1 || scales.size(0) != count || !at.holds(scales))) ||
+            (out.defined() && (out.scalar_type() != type || !at.holds(out) || out.sizes() != y.sizes())))
+            return none();
+        const nvq_adapters_desc d{code_of(type), (int32_t)rank, rows, inputs, outputs, count, inputs, outputs, outputs};
+        const bool done = unlocked([&] {
+            if (!out.defined()) out = at.empty(y.sizes(), type);
+            const size_t need = nvq_apply_adapters_workspace_bytes(&d);
+            Tensor workspace;
+            if (need > 0) workspace = at.empty({(int64_t)need}, at::kByte);
+            return nvq_apply_adapters(&d, ptr(x), ptr(down), ptr(up), (const float *)ptr(scales), (const int32_t *)ptr(ids), ptr(y), out.mutable_data_ptr(),
+                                      need > 0 ? workspace.mutable_data_ptr() : nullptr, at.stream()) == NVQ_OK;
+        });
+        return wrap(done, out);
+    });
+}
+
+bool read_count(PyObject *o, int32_t otherwise, int32_t &v) {
+    if (o == Py_None) return v = otherwise, true;
+    if (!PyLong_Check(o)) return false;
+    const long n = PyLong_AsLong(o);
+    if (n == -1 && PyErr_Occurred()) return declined();
+    return n >= 0 && n <= 1024 ? (v = (int32_t)n, true) : false;
+}
+
+// moe_select(logits, k, sigmoid or None, bias, groups, top groups, group best, normalize, scale)
+PyObject *py_moe_select(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        Tensor logits, bias, experts, weights;
+        nvq_moe_select_desc d{};
+        if (n != 9 || !as_tensor(args[0], logits) || !read_count(args[1], 0, d.k) || !PyBool_Check(args[2]) || !as_tensor(args[3], bias) ||
+            !read_count(args[4], 0, d.groups) || !read_count(args[5], d.groups, d.top_groups) || !read_count(args[6], bias.defined() ? 2 : 1, d.group_best))
+            return none();
+        const int normalize = PyObject_IsTrue(args[7]);
+        if (normalize < 0) return nullptr;
+        d.scale = PyFloat_AsDouble(args[8]);
+        if (d.scale == -1.0 && PyErr_Occurred()) return declined(), none();
+        const Place at(logits);
+        if (!at.usable() || code_of(logits.scalar_type()) < 0 || logits.dim() < 1 || logits.numel() == 0 || !at.holds(logits) || d.k < 1) return none();
+        const int64_t e = logits.size(logits.dim() - 1);
+        if (e > 1024 || (bias.defined() && (bias.scalar_type() != at::kFloat || bias.dim() != 1 || bias.size(0) != e || !at.holds(bias)))) return none();
+        d.dtype = code_of(logits.scalar_type()), d.scores = args[2] == Py_True ? NVQ_SCORES_SIGMOID : NVQ_SCORES_SOFTMAX, d.experts = (int32_t)e;
+        d.normalize = normalize;
+        if (nvq_moe_select(&d, nullptr, nullptr, nullptr, nullptr, nullptr) != NVQ_OK) return none();  // (the sizes)
+        d.rows = logits.numel() / e;
+        const bool done = unlocked([&] {
+            std::vector<int64_t> sizes = logits.sizes().vec();
+            sizes.back() = d.k;
+            experts = at.empty(sizes, at::kInt), weights = at.empty(sizes, logits.scalar_type());
+            return nvq_moe_select(&d, ptr(logits), (const float *)ptr(bias), (int32_t *)experts.mutable_data_ptr(), weights.mutable_data_ptr(), at.stream()) ==
+                   NVQ_OK;
+        });
+        if (!done) return none();
+        Ref i(THPVariable_Wrap(std::move(experts))), w(THPVariable_Wrap(std::move(weights)));
+        return i.p && w.p ? PyTuple_Pack(2, i.p, w.p) : nullptr;
+    });
+}
+
 // register((type, {name: function}), ...): QuantizedLinear, SwitchProjection, SwitchGlu and MoeMlp with their own methods
 PyObject *py_register(PyObject *, PyObject *const *args, Py_ssize_t n) {
     Kind *const kinds[] = {&linear_kind, &projection_kind, &switch_glu_kind, &moe_kind};
@@ -1018,6 +1140,8 @@ PyMethodDef methods[] = {
     {"append_paged", NVQ_FAST(py_append_paged), nullptr},
     {"read_paged", NVQ_FAST(py_read_paged), nullptr},
     {"paged_attention", NVQ_FAST(py_paged_attention), nullptr},
+    {"apply_adapters", NVQ_FAST(py_apply_adapters), nullptr},
+    {"moe_select", NVQ_FAST(py_moe_select), nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
@@ -1033,7 +1157,7 @@ extern "C" __attribute__((visibility("default"))) PyObject *PyInit__native(void)
         {&names.gate, "gate"}, {&names.switch_mlp, "switch_mlp"}, {&names.experts_per_token, "experts_per_token"},
         {&names.norm_topk_prob, "norm_topk_prob"}, {&names.gate_up_paired, "gate_up_paired"}, {&names.activation, "activation"},
         {&names.alpha, "alpha"}, {&names.limit, "limit"}, {&names.keys, "keys"}, {&names.values, "values"},
-        {&names.table, "table"}, {&names.interleaved, "interleaved"},
+        {&names.table, "table"}, {&names.interleaved, "interleaved"}, {&names.axes, "axes"}, {&names.down, "down"}, {&names.up, "up"},
     };
     for (auto &n : all) {
         *n.at = PyUnicode_InternFromString(n.text);

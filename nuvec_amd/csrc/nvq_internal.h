@@ -212,7 +212,7 @@ int32_t launch_attention_prompt_f32(const nvq_attention_prompt_desc &d, const vo
 constexpr int head_lanes(int head_dim) { return head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : head_dim <= 256 ? 32 : 64; }
 constexpr int64_t most_positions(int head_dim) { return ((1LL << 32) / 256 - 1) * (256 / head_lanes(head_dim)); }
 struct PagedAppendOperands {
-    const int32_t *page_table, *sequences, *positions;
+    const int32_t *page_table, *sequences, *positions, *rotary_positions;
     const float *table;
     const void *q, *q_weight, *k, *k_weight, *v;
     void *q_out, *kw, *ks, *kb, *vw, *vs, *vb;
@@ -224,10 +224,16 @@ struct PagedAttentionOperands {
 };
 template <typename F>  // float or double
 int32_t launch_rotation_table(const F *freqs, int half, int64_t rows, double base, double scale, double magnitude, float *table, hipStream_t s);
-int32_t launch_head_rope(const nvq_head_rope_desc &d, const float *table, const int32_t *offsets, const void *const (&x)[2],
+// `axes`: NULL, or the axes of the rotation's pairs; `offsets` are then each axis's positions
+int32_t launch_head_rope(const nvq_head_rope_desc &d, const nvq_rotary_axes *axes, const float *table, const int32_t *offsets, const void *const (&x)[2],
                          const void *const (&w)[2], void *const (&y)[2], hipStream_t s);
-int32_t launch_append_paged(const nvq_paged_append_desc &d, const PagedAppendOperands &o, hipStream_t s);
+int32_t launch_append_paged(const nvq_paged_append_desc &d, const nvq_rotary_axes *axes, const PagedAppendOperands &o, hipStream_t s);
 int32_t launch_read_paged(const nvq_paged_desc &c, int64_t tokens, const PagedAppendOperands &o, void *keys, void *values, hipStream_t s);
+// Low-rank adapters (float32 shares of the first product in the workspace) and the choice of experts.
+size_t adapters_workspace_bytes(const nvq_adapters_desc &d);
+int32_t launch_adapters(const nvq_adapters_desc &d, const void *x, const void *down, const void *up, const float *scales, const int32_t *ids, const void *y,
+                        void *out, void *workspace, hipStream_t s);
+int32_t launch_moe_select(const nvq_moe_select_desc &d, const void *logits, const float *bias, int32_t *indices, void *weights, hipStream_t s);
 bool paged_attention_launchable(const nvq_paged_attention_desc &d, bool starts);
 size_t paged_attention_workspace_bytes(const nvq_paged_attention_desc &d);
 int32_t launch_paged_attention(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, hipStream_t s);

@@ -17,6 +17,15 @@ int32_t check_eps(const char *op, double eps) {
     return eps >= 0.0 && eps < 1e30 ? NVQ_OK : fail(NVQ_INVALID_ARGUMENT, "%s: eps %g", op, eps);
 }
 
+int32_t check_axes(const char *op, const nvq_rotary_axes *axes, int32_t pairs) {
+    if (axes == nullptr || axes->count < 1 || axes->count > 4) return fail(NVQ_INVALID_ARGUMENT, "%s: one to four axes", op);
+    if (pairs > 256) return fail(NVQ_UNSUPPORTED, "%s: axes of %d pairs (256 at most)", op, pairs);
+    for (int32_t i = 0; i < pairs; i++)
+        if ((int32_t)(axes->of_pairs[i / 16] >> (2 * (i % 16)) & 3u) >= axes->count)
+            return fail(NVQ_INVALID_ARGUMENT, "%s: pair %d belongs to none of %d axes", op, i, axes->count);
+    return NVQ_OK;
+}
+
 int32_t check_paged(const char *op, const nvq_paged_desc &c) {
     NVQ_TRY(check_float(op, c.dtype));
     const nvq_quant quant{NVQ_AFFINE, c.group_size, c.bits};
@@ -67,18 +76,8 @@ static int32_t rotation_table(const F *freqs, int32_t dims, int64_t rows, double
     return launch_rotation_table(freqs, dims / 2, rows, base, scale, magnitude, table, (hipStream_t)stream);
 }
 
-extern "C" {
-
-int32_t nvq_rotation_table(const float *freqs, int32_t dims, int64_t rows, double base, double scale, double magnitude, float *table, void *stream) {
-    return rotation_table(freqs, dims, rows, base, scale, magnitude, table, stream);
-}
-
-int32_t nvq_rotation_table_f64(const double *freqs, int32_t dims, int64_t rows, double base, double scale, double magnitude, float *table, void *stream) {
-    return rotation_table(freqs, dims, rows, base, scale, magnitude, table, stream);
-}
-
-int32_t nvq_head_norm_rope(const nvq_head_rope_desc *d, const float *table, const int32_t *offsets, const void *x0, const void *weight0, void *y0,
-                           const void *x1, const void *weight1, void *y1, void *stream) {
+static int32_t head_norm_rope(const nvq_head_rope_desc *d, const nvq_rotary_axes *axes, const float *table, const int32_t *offsets, const void *x0,
+                              const void *weight0, void *y0, const void *x1, const void *weight1, void *y1, void *stream) {
     const char *op = "head_norm_rope";
     if (d == nullptr) return fail(NVQ_INVALID_ARGUMENT, "%s: null descriptor", op);
     NVQ_TRY(check_float(op, d->dtype));
@@ -102,12 +101,13 @@ int32_t nvq_head_norm_rope(const nvq_head_rope_desc *d, const float *table, cons
         NVQ_TRY(check_elements(op, "an output", y[i], d->dtype));
     }
     NVQ_TRY(require_device());
-    return launch_head_rope(*d, table, offsets, x, w, y, (hipStream_t)stream);
+    return launch_head_rope(*d, axes, table, offsets, x, w, y, (hipStream_t)stream);
 }
 
-int32_t nvq_append_paged(const nvq_paged_append_desc *d, const int32_t *page_table, const int32_t *sequences, const int32_t *positions,
-                         const float *table, const void *q, const void *q_weight, void *q_out, const void *k, const void *k_weight, const void *v,
-                         uint32_t *k_w, void *k_s, void *k_b, uint32_t *v_w, void *v_s, void *v_b, void *stream) {
+static int32_t append_paged(const nvq_paged_append_desc *d, const nvq_rotary_axes *axes, const int32_t *page_table, const int32_t *sequences,
+                            const int32_t *positions, const int32_t *rotary_positions, const float *table, const void *q, const void *q_weight,
+                            void *q_out, const void *k, const void *k_weight, const void *v, uint32_t *k_w, void *k_s, void *k_b, uint32_t *v_w,
+                            void *v_s, void *v_b, void *stream) {
     const char *op = "append_paged";
     if (d == nullptr) return fail(NVQ_INVALID_ARGUMENT, "%s: null descriptor", op);
     const nvq_paged_desc &c = d->cache;
@@ -127,8 +127,50 @@ int32_t nvq_append_paged(const nvq_paged_append_desc *d, const int32_t *page_tab
     for (const void *p : {q, q_weight, k, k_weight, v}) NVQ_TRY(check_elements(op, "an operand", p, c.dtype));
     NVQ_TRY(check_aligned(op, "the queries' output", q_out));
     NVQ_TRY(require_device());
-    const PagedAppendOperands o{page_table, sequences, positions, table, queries ? q : nullptr, q_weight, k, k_weight, v, q_out, k_w, k_s, k_b, v_w, v_s, v_b};
-    return launch_append_paged(*d, o, (hipStream_t)stream);
+    const PagedAppendOperands o{page_table, sequences, positions, rotary_positions, table, queries ? q : nullptr, q_weight, k, k_weight, v, q_out, k_w, k_s, k_b, v_w, v_s, v_b};
+    return launch_append_paged(*d, axes, o, (hipStream_t)stream);
+}
+
+extern "C" {
+
+int32_t nvq_rotation_table(const float *freqs, int32_t dims, int64_t rows, double base, double scale, double magnitude, float *table, void *stream) {
+    return rotation_table(freqs, dims, rows, base, scale, magnitude, table, stream);
+}
+
+int32_t nvq_rotation_table_f64(const double *freqs, int32_t dims, int64_t rows, double base, double scale, double magnitude, float *table, void *stream) {
+    return rotation_table(freqs, dims, rows, base, scale, magnitude, table, stream);
+}
+
+int32_t nvq_head_norm_rope(const nvq_head_rope_desc *d, const float *table, const int32_t *offsets, const void *x0, const void *weight0, void *y0,
+                           const void *x1, const void *weight1, void *y1, void *stream) {
+    return head_norm_rope(d, nullptr, table, offsets, x0, weight0, y0, x1, weight1, y1, stream);
+}
+
+int32_t nvq_head_norm_rope_axes(const nvq_head_rope_desc *d, const nvq_rotary_axes *axes, const float *table, const int32_t *positions, const void *x0,
+                                const void *weight0, void *y0, const void *x1, const void *weight1, void *y1, void *stream) {
+    const char *op = "head_norm_rope";
+    if (d == nullptr) return fail(NVQ_INVALID_ARGUMENT, "%s: null descriptor", op);
+    NVQ_TRY(check_axes(op, axes, d->rotary_dims / 2));
+    if (positions == nullptr && d->batch > 0 && d->length > 0) return fail(NVQ_INVALID_ARGUMENT, "%s: null positions", op);
+    return head_norm_rope(d, axes, table, positions, x0, weight0, y0, x1, weight1, y1, stream);
+}
+
+int32_t nvq_append_paged(const nvq_paged_append_desc *d, const int32_t *page_table, const int32_t *sequences, const int32_t *positions,
+                         const float *table, const void *q, const void *q_weight, void *q_out, const void *k, const void *k_weight, const void *v,
+                         uint32_t *k_w, void *k_s, void *k_b, uint32_t *v_w, void *v_s, void *v_b, void *stream) {
+    return append_paged(d, nullptr, page_table, sequences, positions, nullptr, table, q, q_weight, q_out, k, k_weight, v, k_w, k_s, k_b, v_w, v_s, v_b, stream);
+}
+
+int32_t nvq_append_paged_axes(const nvq_paged_append_desc *d, const nvq_rotary_axes *axes, const int32_t *page_table, const int32_t *sequences,
+                              const int32_t *positions, const int32_t *rotary_positions, const float *table, const void *q, const void *q_weight,
+                              void *q_out, const void *k, const void *k_weight, const void *v, uint32_t *k_w, void *k_s, void *k_b, uint32_t *v_w,
+                              void *v_s, void *v_b, void *stream) {
+    const char *op = "append_paged";
+    if (d == nullptr) return fail(NVQ_INVALID_ARGUMENT, "%s: null descriptor", op);
+    NVQ_TRY(check_axes(op, axes, d->rotary_dims / 2));
+    if (rotary_positions == nullptr && d->tokens > 0) return fail(NVQ_INVALID_ARGUMENT, "%s: null positions", op);
+    return append_paged(d, axes, page_table, sequences, positions, rotary_positions, table, q, q_weight, q_out, k, k_weight, v, k_w, k_s, k_b, v_w, v_s, v_b,
+                        stream);
 }
 
 int32_t nvq_read_paged(const nvq_paged_desc *d, int64_t tokens, const int32_t *page_table, const int32_t *sequences, const int32_t *positions,

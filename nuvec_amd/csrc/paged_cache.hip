@@ -90,17 +90,22 @@ __device__ __forceinline__ int64_t row_of(const PagedPlace &p, const int32_t *se
     return (id * key_heads << p.page_shift) + (position & ((1 << p.page_shift) - 1));
 }
 
-template <typename T, int P, int BITS, int READ>
-__global__ void __launch_bounds__(kHeadBlock) append_paged_kernel(const AppendArgs<T> a) {
+template <typename T, int P, int BITS, int READ, typename Axes>
+__global__ void __launch_bounds__(kHeadBlock) append_paged_kernel(const AppendArgs<T> a, const Axes axes) {
     constexpr int kSlots = kHeadBlock / P, kWords = BITS / 4;
     __shared__ HeldHeads<T, P, READ> held;
     const int lane = threadIdx.x % P, j0 = 8 * lane;
     const int64_t token = (int64_t)blockIdx.x * kSlots + threadIdx.x / P;
     if (token >= a.tokens) return;
     const bool interleaved = a.interleaved != 0;
-    const int64_t row = row_of<T>(a.place, a.sequences, a.positions, token, a.key_heads, a.half > 0 ? a.table_rows : INT64_MAX);
+    int64_t row = row_of<T>(a.place, a.sequences, a.positions, token, a.key_heads, a.half > 0 && !Axes::kAny ? a.table_rows : INT64_MAX);
     Turn turn{};
-    if (a.half > 0) {
+    if constexpr (Axes::kAny) {
+        if (a.half > 0) {
+            if (!axes.inside(token, a.tokens, a.table_rows)) row = -1;
+            turn = axes.turn(a.table, a.table_rows, token, a.tokens, j0, a.half, interleaved);
+        }
+    } else if (a.half > 0) {
         int64_t position = a.positions[token];
         position = position < 0 ? 0 : position < a.table_rows ? position : a.table_rows - 1;
         turn = read_turn<READ>(a.table + position * a.half, j0, a.half, interleaved);
@@ -215,21 +220,21 @@ int32_t heads_of_block(int64_t blocks, int64_t heads) {
     return (int32_t)(per < 1 ? 1 : per < heads ? per : heads);
 }
 
-template <typename T, int P, int BITS>
-int32_t run_append(AppendArgs<T> &a, int read, hipStream_t s) {
+template <typename T, int P, int BITS, typename Axes>
+int32_t run_append(AppendArgs<T> &a, const Axes &axes, int read, hipStream_t s) {
     const int64_t blocks = (a.tokens + kHeadBlock / P - 1) / (kHeadBlock / P);
     const int32_t all = a.query_heads + 2 * a.key_heads;
     a.per_block = heads_of_block(blocks, all);
     const dim3 grid((unsigned)blocks, (unsigned)((all + a.per_block - 1) / a.per_block));
-    if (read == kWhole) hipLaunchKernelGGL((append_paged_kernel<T, P, BITS, kWhole>), grid, dim3(kHeadBlock), 0, s, a);
-    else if (read == kRuns) hipLaunchKernelGGL((append_paged_kernel<T, P, BITS, kRuns>), grid, dim3(kHeadBlock), 0, s, a);
-    else hipLaunchKernelGGL((append_paged_kernel<T, P, BITS, kSingle>), grid, dim3(kHeadBlock), 0, s, a);
+    if (read == kWhole) hipLaunchKernelGGL((append_paged_kernel<T, P, BITS, kWhole, Axes>), grid, dim3(kHeadBlock), 0, s, a, axes);
+    else if (read == kRuns) hipLaunchKernelGGL((append_paged_kernel<T, P, BITS, kRuns, Axes>), grid, dim3(kHeadBlock), 0, s, a, axes);
+    else hipLaunchKernelGGL((append_paged_kernel<T, P, BITS, kSingle, Axes>), grid, dim3(kHeadBlock), 0, s, a, axes);
     NVQ_LAUNCH_CHECK("append_paged");
     return NVQ_OK;
 }
 
-template <typename T>
-int32_t run_append_type(const nvq_paged_append_desc &d, const PagedAppendOperands &o, hipStream_t s) {
+template <typename T, typename Axes>
+int32_t run_append_type(const nvq_paged_append_desc &d, const Axes &axes, const PagedAppendOperands &o, hipStream_t s) {
     AppendArgs<T> a{};
     const nvq_paged_desc &c = d.cache;
     a.place = place_of(c, o.page_table);
@@ -247,8 +252,8 @@ int32_t run_append_type(const nvq_paged_append_desc &d, const PagedAppendOperand
     }
     const uintptr_t others = (uintptr_t)o.q_weight | (uintptr_t)o.k_weight | (uintptr_t)o.table;
     const int read = read_of(a.dim, a.half, a.interleaved != 0, rows % 16 == 0, others % 16 == 0);
-    if (c.head_dim == 64) return c.bits == 4 ? run_append<T, 8, 4>(a, read, s) : run_append<T, 8, 8>(a, read, s);
-    return c.bits == 4 ? run_append<T, 16, 4>(a, read, s) : run_append<T, 16, 8>(a, read, s);
+    if (c.head_dim == 64) return c.bits == 4 ? run_append<T, 8, 4>(a, axes, read, s) : run_append<T, 8, 8>(a, axes, read, s);
+    return c.bits == 4 ? run_append<T, 16, 4>(a, axes, read, s) : run_append<T, 16, 8>(a, axes, read, s);
 }
 
 template <typename T, int P, int BITS>
@@ -274,12 +279,17 @@ int32_t run_read_type(const nvq_paged_desc &c, A... args) {
 
 }  // namespace
 
-int32_t launch_append_paged(const nvq_paged_append_desc &d, const PagedAppendOperands &o, hipStream_t s) {
+template <typename Axes>
+static int32_t run_append_any(const nvq_paged_append_desc &d, const Axes &axes, const PagedAppendOperands &o, hipStream_t s) {
     switch (d.cache.dtype) {
-    case NVQ_F32: return run_append_type<float>(d, o, s);
-    case NVQ_BF16: return run_append_type<bf16_t>(d, o, s);
-    default: return run_append_type<f16_t>(d, o, s);
+    case NVQ_F32: return run_append_type<float>(d, axes, o, s);
+    case NVQ_BF16: return run_append_type<bf16_t>(d, axes, o, s);
+    default: return run_append_type<f16_t>(d, axes, o, s);
     }
+}
+
+int32_t launch_append_paged(const nvq_paged_append_desc &d, const nvq_rotary_axes *axes, const PagedAppendOperands &o, hipStream_t s) {
+    return axes == nullptr ? run_append_any(d, NoAxes{}, o, s) : run_append_any(d, PairAxes{o.rotary_positions, *axes}, o, s);
 }
 
 int32_t launch_read_paged(const nvq_paged_desc &c, int64_t tokens, const PagedAppendOperands &o, void *keys, void *values, hipStream_t s) {

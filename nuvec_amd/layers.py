@@ -72,6 +72,25 @@ class QuantizedLinear:
 
 
 @dataclass
+class AdaptedLinear:
+    """A `QuantizedLinear` that many requests share, with low-rank adapters of their own (`ops.apply_adapters`)."""
+    linear: QuantizedLinear
+    adapters: ops.Adapters
+
+    def forward(self, x: torch.Tensor, ids: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """`x` `[..., input_dims]`; `ids` int32 `[...]`: each row's adapter, none where it is negative (None: no row has one)."""
+        y = self.linear(x)
+        return y if ids is None else ops.apply_adapters(y, x, self.adapters, ids, out=y)
+
+    __call__ = forward
+
+
+def _adapted(p, x: torch.Tensor, ids: Optional[torch.Tensor]) -> torch.Tensor:
+    """Rows through a projection, with its adapters if it has some."""
+    return p(x, ids) if isinstance(p, AdaptedLinear) else p(x)
+
+
+@dataclass
 class Mlp:
     """model.rs:2044-2075 (`Mlp`): `down(act(gate(x), up(x)))` with SwiGLU, or Gemma's GeGLU (`geglu`)."""
     gate_proj: QuantizedLinear
@@ -86,6 +105,8 @@ class Mlp:
         (`ops.quantized_matmul_glu`).  Left apart: projections that differ in shape or quantization, hidden sizes off
         whole runs, affine projections of fewer than 1024 rows (they take the kernels with the CPU's weights at every row count)."""
         g, u = self.gate_proj, self.up_proj
+        if isinstance(g, AdaptedLinear) or isinstance(u, AdaptedLinear):
+            return self
         hidden = g.weight.shape[0]
         if g.quant != u.quant or g.weight.shape != u.weight.shape or (g.bias is None) != (u.bias is None) or hidden % 64 != 0:
             return self
@@ -95,8 +116,11 @@ class Mlp:
         self.gate_up_proj = QuantizedLinear(cat(g.weight, u.weight), cat(g.scales, u.scales), cat(g.biases, u.biases), cat(g.bias, u.bias), g.quant)
         return self
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        """model.rs:2066-2074."""
+    def forward(self, x: torch.Tensor, adapter_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """model.rs:2066-2074.  `adapter_ids`: of the projections that are `AdaptedLinear` (all three are run one by one then)."""
+        if adapter_ids is not None or any(isinstance(p, AdaptedLinear) for p in (self.gate_proj, self.up_proj, self.down_proj)):
+            gate, up = _adapted(self.gate_proj, x, adapter_ids), _adapted(self.up_proj, x, adapter_ids)
+            return _adapted(self.down_proj, ops.glu(gate, up, "geglu" if self.geglu else "swiglu"), adapter_ids)
         y = (_native or _calls()).mlp(self, x)
         if y is not None:
             return y
@@ -322,21 +346,39 @@ class MoeMlp:
     """model.rs:2218-2272 (`MoeMlp`, mlx-lm's sparse MoE blocks): the router's probabilities (a softmax in the
     activations' type), each token's best `k` experts (`moe_route`), the experts' gated MLPs (`SwitchGlu`) and their
     outputs weighted by the (renormalised) scores and summed (`weighted_sum`).  `gate` is the router's dense weight
-    `[experts, D]`; the shared expert of some models is a dense MLP outside this path and is left to the caller."""
+    `[experts, D]`; the shared expert of some models is a dense MLP outside this path and is left to the caller.
+
+    Routers with sigmoid scores, a `bias` float32 `[experts]` for balance, groups of experts or a `scale` of the weights choose by
+    `ops.moe_select`, over logits of the wider of the gate's and x's types."""
     gate: torch.Tensor
     switch_mlp: SwitchGlu
     experts_per_token: int
     norm_topk_prob: bool = True
+    scores: str = "softmax"
+    bias: Optional[torch.Tensor] = None
+    groups: int = 1
+    top_groups: Optional[int] = None
+    group_best: Optional[int] = None
+    scale: float = 1.0
+
+    def _selects(self) -> bool:
+        return self.scores != "softmax" or self.bias is not None or self.groups != 1 or self.scale != 1.0
 
     def route(self, x: torch.Tensor):
-        """The router: `(top, scores)` of `moe_route` over `softmax(x gate^T)`."""
+        """The router: `(top, scores)` of `moe_route` over `softmax(x gate^T)`, or of `moe_select`."""
+        if self._selects():
+            dtype = torch.promote_types(x.dtype, self.gate.dtype)
+            logits = torch.nn.functional.linear(x.to(dtype), self.gate.to(dtype))
+            top, scores = ops.moe_select(logits, self.experts_per_token, self.scores, self.bias, self.groups, self.top_groups, self.group_best,
+                                         self.norm_topk_prob, self.scale)
+            return top, scores.to(x.dtype)
         logits = torch.nn.functional.linear(x, self.gate.to(x.dtype))
         probs = torch.softmax(logits.float(), dim=-1).to(x.dtype)  # softmax_precise: float32 inside, one rounding
         return ops.moe_route(probs, self.experts_per_token, self.norm_topk_prob)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         """`x` `[B, L, D]` -> `[B, L, D]`."""
-        y = (_native or _calls()).moe(self, x)
+        y = None if self._selects() else (_native or _calls()).moe(self, x)
         if y is not None:
             return y
         top, scores = self.route(x)
@@ -365,19 +407,22 @@ class PagedAttention:
     eps: float = 1e-6
 
     def forward(self, x: torch.Tensor, cache: paged.PagedCache, page_table: torch.Tensor, positions: torch.Tensor, lengths: torch.Tensor,
-                sequences: Optional[torch.Tensor] = None, query_starts: Optional[torch.Tensor] = None, max_queries: Optional[int] = None) -> torch.Tensor:
+                sequences: Optional[torch.Tensor] = None, query_starts: Optional[torch.Tensor] = None, max_queries: Optional[int] = None,
+                rotary_positions: Optional[torch.Tensor] = None, adapter_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
         """`x` `[tokens, dims]`: the rows of sequence b are `query_starts[b]` to `query_starts[b + 1] - 1`, row t is position `positions[t]` of
         sequence `sequences[t]`, and `lengths[b]` counts the positions of sequence b with these rows (all int32).  `sequences` and `query_starts`
-        None: one token per sequence.  Padding rows (a negative position, behind the last start) write nothing; their results are undefined."""
+        None: one token per sequence.  Padding rows (a negative position, behind the last start) write nothing; their results are undefined.
+        `rotary_positions` as in `append_paged`; `adapter_ids` int32 `[tokens]`: of the projections that are `AdaptedLinear`."""
         if (sequences is None) != (query_starts is None):
             raise ops.InvalidArgument("paged_attention: sequences and query starts go together")
         if x.ndim != 2:
             raise ops.InvalidArgument(f"paged_attention: tokens must be [tokens, dims], got {list(x.shape)}")
-        q, k, v = self._heads(self.q_proj(x), self.query_heads), self._heads(self.k_proj(x), self.key_heads), self._heads(self.v_proj(x), self.key_heads)
-        q = paged.append_paged(cache, k, v, page_table, positions, sequences, self.rotation, self.k_norm, q, self.q_norm, self.eps)
+        q, k, v = (self._heads(_adapted(p, x, adapter_ids), n)
+                   for p, n in ((self.q_proj, self.query_heads), (self.k_proj, self.key_heads), (self.v_proj, self.key_heads)))
+        q = paged.append_paged(cache, k, v, page_table, positions, sequences, self.rotation, self.k_norm, q, self.q_norm, self.eps, rotary_positions)
         scale = q.shape[2] ** -0.5 if self.scale is None else self.scale
         y = paged.paged_attention(q, cache, page_table, lengths, scale, query_starts, max_queries, self.sinks, True, self.window)
-        return self.o_proj(y.flatten(1))
+        return _adapted(self.o_proj, y.flatten(1), adapter_ids)
 
     @staticmethod
     def _heads(y: torch.Tensor, n: int) -> torch.Tensor:

@@ -137,6 +137,12 @@ def _stream() -> C.c_void_p:
     return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
+def _here(op: str, x: torch.Tensor) -> None:
+    """Calls go to the current device's stream: operands of another device are refused."""
+    if x.is_cuda and x.device.index != torch.cuda.current_device():
+        raise InvalidArgument(f"{op}: operands on {x.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
 def _ptr(t: Optional[torch.Tensor]) -> C.c_void_p:
     """The tensor's device address; NULL means "operand absent" in the C ABI, so an empty
     tensor (torch gives it address 0) is passed as a never-dereferenced aligned non-null value."""
@@ -653,6 +659,113 @@ def moe_route(probs: torch.Tensor, k: int, normalize: bool):
     scores = torch.empty(p.shape[:-1] + (k,), dtype=p.dtype, device=p.device)
     _lib.check(_lib.load().nvq_moe_route(_CODE[p.dtype], _ptr(p), rows, e, k, int(bool(normalize)), _ptr(top), _ptr(scores), _stream()))
     return top, scores
+
+
+MOE_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def moe_select(logits: torch.Tensor, k: int, scores: str = "softmax", bias: Optional[torch.Tensor] = None, groups: int = 1,
+               top_groups: Optional[int] = None, group_best: Optional[int] = None, normalize: bool = True, scale: float = 1.0):
+    """The choice of experts of routers that `moe_route` does not describe: `(experts, weights)` of router logits `[..., E]`, int32 and the logits'
+    type `[..., k]`.  p = softmax or sigmoid of the logits, c = p + `bias` (float32 `[E]`: it moves the choice, not the weights).  Of `groups` groups of
+    consecutive experts the `top_groups` best stay (None: all), by the sum of their `group_best` largest c (1 or 2; None: 2 with a bias, else 1), and of their
+    experts the k with the largest c are chosen, largest first; ties, of groups too, go to the lowest index, a NaN is below everything.  The weights are the p of the chosen, with
+    `normalize` divided by (their sum + 1e-20), times `scale`, rounded once.  Without a bias c has the logits' order; with one it is compared in 64 bits.  A softmax of
+    nothing but -inf is zeros."""
+    if bias is None or isinstance(bias, torch.Tensor):
+        done = (_lib._native or _lib.native()).moe_select(logits, k, scores == "sigmoid" if scores in MOE_SCORES else None, bias, groups, top_groups, group_best, normalize, scale)
+        if done is not None:
+            return done
+    op = "moe_select"
+    if scores not in MOE_SCORES:
+        raise InvalidArgument(f"{op}: unknown scores {scores!r}")
+    if logits.dtype not in _CODE:
+        raise InvalidArgument(f"{op}: logits must be floating point, got {logits.dtype}")
+    e = logits.shape[-1] if logits.ndim else 0
+    if e < 1:
+        raise InvalidArgument(f"{op}: logits of shape {list(logits.shape)}")
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (e,)):
+        raise InvalidArgument(f"{op}: the bias must be float32 [{e}], got {_name(bias.dtype)} {list(bias.shape)}")
+    if bias is not None and bias.device != logits.device:
+        raise InvalidArgument(f"{op}: operands on {logits.device} and {bias.device}")
+    top_groups = groups if top_groups is None else top_groups
+    group_best = (1 if bias is None else 2) if group_best is None else group_best
+    if not 1 <= groups <= e or not 1 <= top_groups <= groups or e % groups:
+        raise InvalidArgument(f"{op}: the best {top_groups} of {groups} groups of {e} experts")
+    if not 1 <= k <= e // groups * top_groups:
+        raise InvalidArgument(f"{op}: k must be in 1..={e // groups * top_groups}, got {k}")
+    if group_best not in (1, 2):
+        raise InvalidArgument(f"{op}: a group's best {group_best} (1 or 2)")
+    rows = logits.numel() // e
+    d = _lib.MoeSelectDescC(_CODE[logits.dtype], MOE_SCORES[scores], e, k, groups, top_groups, group_best, int(bool(normalize)), 0, float(scale))
+    _lib.check(_lib.load().nvq_moe_select(C.byref(d), *[None] * 5))  # (the sizes alone, before anything is allocated)
+    _init(logits)
+    _here(op, logits)
+    x = logits.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    d.rows = rows
+    experts = torch.empty(x.shape[:-1] + (k,), dtype=torch.int32, device=x.device)
+    weights = torch.empty(x.shape[:-1] + (k,), dtype=x.dtype, device=x.device)
+    _lib.check(_lib.load().nvq_moe_select(C.byref(d), _ptr(x), _ptr(bias), _ptr(experts), _ptr(weights), _stream()))
+    return experts, weights
+
+
+@dataclass
+class Adapters:
+    """Low-rank adapters of one projection, stacked: `down` `[adapters, rank, K]`, `up` `[adapters, N, rank]`, `scales` float32 `[adapters]` (None: ones).
+    Adapters of smaller ranks end in zeros."""
+    down: torch.Tensor
+    up: torch.Tensor
+    scales: Optional[torch.Tensor] = None
+
+
+def apply_adapters(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, ids: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """What the adapters of many requests add to a shared projection's result: `y[r] + scales[a] * (x[r] . down[a]^T) . up[a]^T` for the rows `x`
+    `[..., K]` and `y` `[..., N]`, a = `ids[r]` (int32, one a row: `[...]`); rows whose id is no adapter (negative, say) stay y's.  Rows of one adapter
+    are fastest next to each other, no other order is needed.  `out` may be `y` itself.
+
+    Products are float32 sums; between them a value holds 16 bits (float16: 22, float32: 24), the result is rounded once."""
+    done = (_lib._native or _lib.native()).apply_adapters(y, x, adapters, ids, out)
+    if done is not None:
+        return done if out is None else out
+    op = "apply_adapters"
+    down, up, scales = adapters.down, adapters.up, adapters.scales
+    if x.dtype not in _CODE or y.dtype != x.dtype or down.dtype != x.dtype or up.dtype != x.dtype:
+        raise InvalidArgument(f"{op}: x, y and the adapters must share a floating-point type, got {_name(x.dtype)}, {_name(y.dtype)}, {_name(down.dtype)}, {_name(up.dtype)}")
+    if x.ndim < 1 or y.ndim != x.ndim or y.shape[:-1] != x.shape[:-1]:
+        raise InvalidArgument(f"{op}: x must be [..., K] and y [..., N], got {list(x.shape)} and {list(y.shape)}")
+    if down.ndim != 3 or up.ndim != 3 or down.shape[0] != up.shape[0] or down.shape[1] != up.shape[2] or down.shape[2] != x.shape[-1] or up.shape[1] != y.shape[-1]:
+        raise InvalidArgument(f"{op}: down must be [adapters, rank, {x.shape[-1]}] and up [adapters, {y.shape[-1]}, rank], got {list(down.shape)} and {list(up.shape)}")
+    if scales is not None and (scales.dtype != torch.float32 or tuple(scales.shape) != (down.shape[0],)):
+        raise InvalidArgument(f"{op}: scales must be float32 [{down.shape[0]}], got {_name(scales.dtype)} {list(scales.shape)}")
+    if ids.dtype != torch.int32 or ids.shape != x.shape[:-1]:
+        raise InvalidArgument(f"{op}: ids must be int32 {list(x.shape[:-1])}, got {_name(ids.dtype)} {list(ids.shape)}")
+    for t in (y, down, up, scales, ids, out):
+        if t is not None and t.device != x.device:
+            raise InvalidArgument(f"{op}: operands on {x.device} and {t.device}")
+    if out is not None and (out.dtype != y.dtype or out.shape != y.shape):
+        raise InvalidArgument(f"{op}: the output must be {_name(y.dtype)} {list(y.shape)}, got {_name(out.dtype)} {list(out.shape)}")
+    rows, n = ids.numel(), y.shape[-1]
+    if out is None:
+        out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    try:
+        to = out.view(rows, n)
+    except RuntimeError:
+        to = None
+    if to is None or (n > 1 and to.stride(1) != 1) or (rows > 1 and to.stride(0) < n):
+        raise InvalidArgument(f"{op}: the output's rows must be consecutive values of their own, evenly apart")
+    _init(x)
+    _here(op, x)
+    flat = lambda t: t.reshape(rows, t.shape[-1])
+    as_rows = lambda t: t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+    x2, y2, ids, down, up = as_rows(flat(x)), as_rows(flat(y)), ids.contiguous(), down.contiguous(), up.contiguous()
+    scales = None if scales is None else scales.contiguous()
+    d = _lib.AdaptersDescC(_CODE[x.dtype], down.shape[1], rows, x.shape[-1], n, down.shape[0], x2.stride(0), y2.stride(0), to.stride(0))
+    lib = _lib.load()
+    need = lib.nvq_apply_adapters_workspace_bytes(C.byref(d))
+    workspace = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _lib.check(lib.nvq_apply_adapters(C.byref(d), _ptr(x2), _ptr(down), _ptr(up), _ptr(scales), _ptr(ids), _ptr(y2), _ptr(out), _ptr(workspace), _stream()))
+    return out
 
 
 def weighted_sum(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:

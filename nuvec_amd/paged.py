@@ -13,12 +13,13 @@ from __future__ import annotations
 import ctypes as C
 import math
 from dataclasses import dataclass
-from typing import Optional, Tuple, Union
+from functools import lru_cache
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _lib
-from .ops import _CODE, _FLOATS, InvalidArgument, Quant, QuantMode, Quantized, Unsupported, _init, _name, _ptr, _stream, _u32
+from .ops import _CODE, _FLOATS, InvalidArgument, Quant, QuantMode, Quantized, Unsupported, _here, _init, _name, _ptr, _stream, _u32
 
 
 # ── rotary positions ────────────────────────────────────────────────────────────────────────────────────────────────
@@ -61,12 +62,25 @@ def rotation_freqs(dims: int, base: float = 10000.0, scaling: Optional[dict] = N
     return 1.0 / (slowed / (factor * freqs) + (1.0 - slowed) / freqs), 1.0, number("attention_factor", magnitudes)
 
 
+def rotary_axes(sections: Sequence[int], dealt: bool = False) -> Tuple[int, ...]:
+    """The axis of each pair for `Rotation.axes`, of `sections[a]` pairs of axis a (up to four axes: time, height, width, ...): each axis's pairs behind
+    the last one's or, `dealt`, one pair each in turn as long as an axis has pairs left."""
+    left = [int(n) for n in sections]
+    if not 1 <= len(left) <= 4 or min(left) < 0:
+        raise InvalidArgument(f"rotary_axes: sections {list(sections)} of one to four axes")
+    if not dealt:
+        return tuple(a for a, n in enumerate(left) for _ in range(n))
+    return tuple(a for turn in range(max(left)) for a, n in enumerate(left) if turn < n)
+
+
 @dataclass
 class Rotation:
     """The angles of positions 0 .. positions - 1, float32 `[positions, dims / 2, 2]` (cosine, sine), and which values of a head pair up:
-    `(i, i + dims / 2)` or, `interleaved`, `(2 i, 2 i + 1)`, of its first `dims` values."""
+    `(i, i + dims / 2)` or, `interleaved`, `(2 i, 2 i + 1)`, of its first `dims` values.  `axes`: the axis, 0 to 3, of each pair, where tokens have a
+    position on each of several axes (`rotary_axes`); None: one position turns all pairs."""
     table: torch.Tensor
     interleaved: bool = False
+    axes: Optional[Tuple[int, ...]] = None
 
     @property
     def dims(self) -> int:
@@ -74,7 +88,7 @@ class Rotation:
 
     @staticmethod
     def new(dims: int, positions: int, base: float = 10000.0, scale: float = 1.0, interleaved: bool = False,
-            freqs: Optional[torch.Tensor] = None, magnitude: float = 1.0, device="cuda") -> "Rotation":
+            freqs: Optional[torch.Tensor] = None, magnitude: float = 1.0, device="cuda", axes: Optional[Sequence[int]] = None) -> "Rotation":
         """Angles `scale * position / freqs[i]` in 64 bits, freqs `base^(2 i / dims)` unless given (float64, or float32 values); cosines and sines
         times `magnitude`, rounded once."""
         if dims <= 0 or dims % 2 or positions < 1:
@@ -88,7 +102,20 @@ class Rotation:
         lib = _lib.load()
         make = lib.nvq_rotation_table_f64 if freqs is not None and freqs.dtype == torch.float64 else lib.nvq_rotation_table
         _lib.check(make(_ptr(freqs), dims, positions, float(base), float(scale), float(magnitude), _ptr(table), _stream()))
-        return Rotation(table, interleaved)
+        return Rotation(table, interleaved, None if axes is None else tuple(axes))
+
+
+@lru_cache(maxsize=64)
+def _axes(op: str, axes: Tuple[int, ...], count: int, pairs: int) -> _lib.RotaryAxesC:
+    """The axes of a rotation's pairs, for positions of `count` axes (read-only)."""
+    if len(axes) != pairs or not 1 <= count <= 4 or any(not 0 <= a < count for a in axes):
+        raise InvalidArgument(f"{op}: {len(axes)} pairs of axes {sorted(set(axes))} for {pairs} pairs and positions of {count} axes")
+    if pairs > 256:
+        raise Unsupported(f"{op}: axes of {pairs} pairs (256 at most)")
+    c = _lib.RotaryAxesC(count)
+    for i, a in enumerate(axes):
+        c.of_pairs[i // 16] |= a << 2 * (i % 16)
+    return c
 
 
 def _same_device(op: str, x: torch.Tensor, *others) -> None:
@@ -159,8 +186,11 @@ def _rotate(op: str, xs, weights, outs, rotation, offset, eps):
     b, _, l, d = x.shape
     table, dims, interleaved, rows = _angles(op, rotation, d, x)
     desc = _lib.HeadRopeDescC(_CODE[x.dtype], d, dims, interleaved, 0, rows, b, l)
-    offsets = None
-    if isinstance(offset, torch.Tensor):
+    offsets = axes = None
+    if isinstance(offset, torch.Tensor) and offset.ndim == 3 and getattr(rotation, "axes", None) is not None:
+        axes = _axes(op, tuple(rotation.axes), offset.shape[0], dims // 2)
+        offsets = _indices(op, "positions", offset, (axes.count, b, l), x)
+    elif isinstance(offset, torch.Tensor):
         if offset.ndim not in (1, 2):
             raise InvalidArgument(f"{op}: offsets must be [batch] or [batch, length], got {list(offset.shape)}")
         offsets = _indices(op, "offsets", offset, (b,) if offset.ndim == 1 else (b, l), x)
@@ -179,6 +209,10 @@ def _rotate(op: str, xs, weights, outs, rotation, offset, eps):
         ys.append(y)
     _init(x)
     p = [_ptr(v) for t, w, y in zip(xs, weights, ys) for v in (t, w, y)] + [C.c_void_p(None)] * (6 - 3 * len(xs))
+    if axes is not None:
+        _here(op, x)
+        _lib.check(_lib.load().nvq_head_norm_rope_axes(C.byref(desc), C.byref(axes), _ptr(table), _ptr(offsets), *p, _stream()))
+        return ys
     _lib.check(_lib.load().nvq_head_norm_rope(C.byref(desc), _ptr(table), _ptr(offsets), *p, _stream()))
     return ys
 
@@ -186,7 +220,8 @@ def _rotate(op: str, xs, weights, outs, rotation, offset, eps):
 def rope(x: torch.Tensor, rotation: Rotation, offset: Union[int, torch.Tensor] = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rotary positions of `x` `[batch, heads, length, dim]` (any strides with consecutive values of a head; MLX's `fast.rope`): the first
     `rotation.dims` values of a head turn, the others stay.  Element l is at position `offset + l`; `offset` is an int, int32 `[batch]`, or int32
-    `[batch, length]` for positions one by one.  Positions on the device outside the table are clamped to it.  `out` may be `x` itself, unless rows of it share their memory."""
+    `[batch, length]` for positions one by one; a rotation with `axes` takes int32 `[axes, batch, length]` too, a position on each axis (any other offset is
+    every axis's position).  Positions on the device outside the table are clamped to it.  `out` may be `x` itself, unless rows of it share their memory."""
     y = (_lib._native or _lib.native()).rope(x, rotation, offset, out)
     if y is not None:
         return y if out is None else out
@@ -283,15 +318,19 @@ def _rows(op: str, what: str, x: torch.Tensor, heads: Optional[int], like: torch
 
 def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, positions: torch.Tensor,
                  sequences: Optional[torch.Tensor] = None, rotation: Optional[Rotation] = None, k_weight: Optional[torch.Tensor] = None,
-                 q: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> Optional[torch.Tensor]:
+                 q: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 rotary_positions: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Writes token t's keys and values (`[tokens, key_heads, dim]`) to position `positions[t]` of sequence `sequences[t]` (int32; None: t) of the
     cache: the keys normed (`k_weight`), rotated to their position and quantized from the float32 result, the values quantized.  `q` `[tokens,
     query_heads, dim]`: the same tokens' queries, normed (`q_weight`) and rotated in the same launch; they are the result (None without them).
 
     A token with a negative position is padding: nothing is written.  Neither is one whose position lies outside the rotation's table or the page
     table, or whose page is not in the pool.  Two tokens of one position are the caller's error.  (Codes are the nearest to the scale and bias as
-    stored, those of `quantize` to the unrounded ones.)"""
-    done = (_lib._native or _lib.native()).append_paged(cache, k, v, page_table, positions, sequences, rotation, k_weight, q, q_weight, eps)
+    stored, those of `quantize` to the unrounded ones.)
+
+    `rotary_positions` int32 `[tokens]`, or `[axes, tokens]` with a rotation of several `axes`: the positions whose angles the heads are turned by, where they
+    are not the places in the cache (an image's tokens); outside the rotation's table they are like positions outside it."""
+    done = (_lib._native or _lib.native()).append_paged(cache, k, v, page_table, positions, sequences, rotation, k_weight, q, q_weight, eps, rotary_positions)
     if done is not None:
         return None if done is True else done
     op = "append_paged"
@@ -308,6 +347,13 @@ def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table
         raise InvalidArgument(f"{op}: {tokens} tokens of {page_table.shape[0]} sequences without `sequences`")
     table, dims, interleaved, rows = _angles(op, rotation, k.shape[2], k)
     k_weight = _weight(op, k_weight, k)
+    axes = None
+    if rotary_positions is not None:
+        if rotation is None:
+            raise InvalidArgument(f"{op}: rotary positions without a rotation")
+        one = rotary_positions.ndim == 1 or getattr(rotation, "axes", None) is None
+        axes = _axes(op, (0,) * (dims // 2) if one else tuple(rotation.axes), 1 if one else rotary_positions.shape[0], dims // 2)
+        rotary_positions = _indices(op, "rotary positions", rotary_positions, (tokens,) if one else (axes.count, tokens), k)
     desc = _lib.PagedAppendDescC(cd, tokens, 0, dims, interleaved, rows)
     desc.eps = eps
     out = None
@@ -323,8 +369,12 @@ def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table
         if q is not None:
             desc.q_strides[i] = q.stride(i)
     _init(k)
-    _lib.check(_lib.load().nvq_append_paged(C.byref(desc), _ptr(page_table), _ptr(sequences), _ptr(positions), _ptr(table), _ptr(q), _ptr(q_weight),
-                                            _ptr(out), _ptr(k), _ptr(k_weight), _ptr(v), *(_ptr(t) for t in pool), _stream()))
+    rest = (_ptr(table), _ptr(q), _ptr(q_weight), _ptr(out), _ptr(k), _ptr(k_weight), _ptr(v), *(_ptr(t) for t in pool), _stream())
+    if axes is not None:
+        _here(op, k)
+        _lib.check(_lib.load().nvq_append_paged_axes(C.byref(desc), C.byref(axes), _ptr(page_table), _ptr(sequences), _ptr(positions), _ptr(rotary_positions), *rest))
+    else:
+        _lib.check(_lib.load().nvq_append_paged(C.byref(desc), _ptr(page_table), _ptr(sequences), _ptr(positions), *rest))
     return out
 
 
