@@ -217,6 +217,19 @@ typedef struct nvq_paged_attention_desc {
     float scale;
 } nvq_paged_attention_desc;
 
+/* Attention of whole prompts over keys and values as the projections leave them: rows q dtype [rows, query_heads, head_dim] and keys, values
+ * dtype [keys, key_heads, head_dim] of `sequences` sequences behind one another.  Of a sequence with n rows and S keys row i sees the keys up
+ * to S - n + i, with `window` > 0 the last `window` of those alone. */
+typedef struct nvq_prompt_attention_desc {
+    int32_t dtype;    /* NVQ_F16 / NVQ_BF16 / NVQ_F32 */
+    int32_t head_dim; /* a multiple of 8, up to 256 */
+    int64_t rows, keys, query_heads, key_heads, sequences;
+    int64_t q_strides[2], k_strides[2], v_strides[2], out_strides[2]; /* elements between rows, heads */
+    int64_t window;
+    int32_t causal;   /* 0: every row of a sequence sees all its keys (window must be 0) */
+    float scale;
+} nvq_prompt_attention_desc;
+
 /* Low-rank adapters of one projection: down dtype [adapters, rank, inputs], up dtype [adapters, outputs, rank], contiguous; rows of x,
  * y and out as far apart as the strides say, values of a row consecutive. */
 typedef struct nvq_adapters_desc {
@@ -444,6 +457,15 @@ NVQ_API size_t nvq_paged_attention_workspace_bytes(const nvq_paged_attention_des
 NVQ_API int32_t nvq_paged_attention(const nvq_paged_attention_desc *desc, const void *q, const uint32_t *k_w, const void *k_s, const void *k_b,
                             const uint32_t *v_w, const void *v_s, const void *v_b, const int32_t *page_table, const int32_t *lengths,
                             const int32_t *query_starts, const void *sinks, void *out, void *workspace, void *stream);
+
+/* softmax(scale * q . k^T [masked] [, sinks]) . v of every row over its sequence's keys; a row that sees no key is zeros.  Sequence b has rows
+ * query_starts[b] .. query_starts[b + 1] - 1 and keys key_starts[b] .. key_starts[b + 1] - 1 (i32 [sequences + 1], ascending); query_starts
+ * NULL: one sequence of all rows; key_starts NULL: those of the rows, or one sequence's all keys.  Rows outside every sequence are left as
+ * they were; starts outside the operands are clamped to them.  `workspace`: the size query's bytes (float32 states of splits of the
+ * keys), NULL where it says 0. */
+NVQ_API size_t nvq_prompt_attention_workspace_bytes(const nvq_prompt_attention_desc *desc);
+NVQ_API int32_t nvq_prompt_attention(const nvq_prompt_attention_desc *desc, const void *q, const void *k, const void *v, const int32_t *query_starts,
+                             const int32_t *key_starts, const void *sinks, void *out, void *workspace, void *stream);
 
 /* out[r] = y[r] + scales[a] (x[r] . down[a]^T) . up[a]^T with a = ids[r] (i32 [rows]), rounded once; out[r] = y[r] where a is no adapter
  * (negative, or `adapters` and more).  scales f32 [adapters], NULL: ones.  out may be y itself.  `workspace`: the size query's bytes (float32

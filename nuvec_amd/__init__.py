@@ -10,4 +10,4 @@ attention: rotary positions, norms of heads, a paged, quantized key / value cach
 from .ops import (Adapters, GatherQmm, InvalidArgument, Quant, QuantMode, Quantized, Unsupported, apply_adapters, dequantize, embedding,  # noqa: F401
                   gather_qmm, gather_qmm_glu, gather_qmm_grouped, gather_qqmm, glu, moe_order, pair_rows, moe_route, moe_select, qqmm, quantize, quantize_dequantize,
                   quantized_matmul, quantized_matmul_glu, quantized_matmul_kernel, quantized_matmul_route, quantized_matmul_tile, sorted_offsets, weighted_sum)
-from .paged import (PagedCache, Rotation, append_paged, head_norm_rope, paged_attention, read_paged, rope, rotary_axes, rotation_freqs)  # noqa: F401
+from .paged import (PagedCache, Rotation, append_paged, head_norm_rope, paged_attention, prompt_attention, read_paged, rope, rotary_axes, rotation_freqs)  # noqa: F401

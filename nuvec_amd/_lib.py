@@ -70,6 +70,12 @@ class RotaryAxesC(C.Structure):
     _fields_ = [("count", C.c_int32), ("of_pairs", C.c_uint32 * 16)]
 
 
+class PromptAttentionDescC(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("head_dim", C.c_int32), ("rows", C.c_int64), ("keys", C.c_int64), ("query_heads", C.c_int64),
+                ("key_heads", C.c_int64), ("sequences", C.c_int64), ("q_strides", C.c_int64 * 2), ("k_strides", C.c_int64 * 2),
+                ("v_strides", C.c_int64 * 2), ("out_strides", C.c_int64 * 2), ("window", C.c_int64), ("causal", C.c_int32), ("scale", C.c_float)]
+
+
 class AdaptersDescC(C.Structure):
     _fields_ = [("dtype", C.c_int32), ("rank", C.c_int32), ("rows", C.c_int64), ("inputs", C.c_int64), ("outputs", C.c_int64), ("adapters", C.c_int64),
                 ("x_stride", C.c_int64), ("y_stride", C.c_int64), ("out_stride", C.c_int64)]
@@ -149,6 +155,8 @@ SIGNATURES = {
     "nvq_head_norm_rope": (C.c_int32, [C.POINTER(HeadRopeDescC)] + [C.c_void_p] * 9),
     "nvq_head_norm_rope_axes": (C.c_int32, [C.POINTER(HeadRopeDescC), C.POINTER(RotaryAxesC)] + [C.c_void_p] * 9),
     "nvq_append_paged_axes": (C.c_int32, [C.POINTER(PagedAppendDescC), C.POINTER(RotaryAxesC)] + [C.c_void_p] * 18),
+    "nvq_prompt_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PromptAttentionDescC)]),
+    "nvq_prompt_attention": (C.c_int32, [C.POINTER(PromptAttentionDescC)] + [C.c_void_p] * 9),
     "nvq_apply_adapters_workspace_bytes": (C.c_size_t, [C.POINTER(AdaptersDescC)]),
     "nvq_apply_adapters": (C.c_int32, [C.POINTER(AdaptersDescC)] + [C.c_void_p] * 9),
     "nvq_moe_select": (C.c_int32, [C.POINTER(MoeSelectDescC)] + [C.c_void_p] * 5),

@@ -20,7 +20,7 @@ SOURCES = ["qmg_b8.hip", "qmg_b6.hip", "qmg_b5.hip", "qmg_b4.hip", "qmg_b3.hip",
            "qms_b8.hip", "qms_b6.hip", "qms_b5.hip", "qms_b4.hip", "qms_b3.hip", "qms_b2.hip", "qms_fp4.hip", "qms_fp8.hip", "qms_nvfp4.hip", "qms.hip",
            "qmf_b8.hip", "qmf_fp8.hip", "qmf_b6.hip", "qmf_b5.hip", "qmf_b4.hip", "qmf_fp4.hip", "qmf_nvfp4.hip", "qmf_b3.hip", "qmf_b2.hip", "qmf_b1.hip", "qmm.hip", "qmv.hip", "qmv_dot8.hip", "qmm_f32.hip", "qmm_dense.hip", "qmr.hip",
            "qvm.hip", "nvq_api.hip", "affine_quant.hip", "fp_quant.hip", "qmf.hip", "gather.hip", "repack.hip", "calib.hip", "qattn.hip", "qattn_prompt.hip", "qattn_prompt_f32.hip", "qmd.hip", "glu.hip",
-           "paged_prompt_bf16.hip", "paged_prompt_f16.hip", "paged_rows_bf16.hip", "paged_rows_f16.hip", "paged_rows_f32.hip", "paged_attention.hip", "paged_cache.hip", "heads.hip", "adapters.hip", "select.hip",
+           "paged_prompt_bf16.hip", "paged_prompt_f16.hip", "paged_rows_bf16.hip", "paged_rows_f16.hip", "paged_rows_f32.hip", "paged_attention.hip", "paged_cache.hip", "heads.hip", "prompt_bf16.hip", "prompt_f16.hip", "prompt_f32.hip", "prompt_attention.hip", "adapters.hip", "select.hip",
            "paged_api.hip", "serving_api.hip"]  # slowest to compile first
 
 # -ffp-contract=off: the quantizers must round every operation as the CPU does; fused

@@ -1019,6 +1019,49 @@ PyObject *py_paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
+// Starts of sequences.
+bool is_starts(const Tensor &t, const Place &at) { return t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) > 0 && at.holds(t); }
+
+// prompt_attention(q, k, v, scale, query starts, key starts, sinks, causal, window, out or None)
+PyObject *py_prompt_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        Tensor q, k, v, starts, key_starts, sinks, y;
+        if (n != 10 || !as_tensor(args[0], q) || !as_tensor(args[1], k) || !as_tensor(args[2], v) || !as_tensor(args[4], starts) || !as_tensor(args[5], key_starts) ||
+            !as_tensor(args[6], sinks) || !as_tensor(args[9], y) || !PyLong_Check(args[8]))
+            return none();
+        const double scale = PyFloat_AsDouble(args[3]);
+        if (scale == -1.0 && PyErr_Occurred()) return declined(), none();
+        const int64_t window = PyLong_AsLongLong(args[8]);
+        if (PyErr_Occurred()) return declined(), none();
+        const int causal = PyObject_IsTrue(args[7]);
+        if (causal < 0) return nullptr;
+        const Place at(q);
+        if (!at.usable() || q.dim() != 3 || !k.defined() || k.dim() != 3 || !v.defined() || window < 0) return none();
+        const at::ScalarType type = q.scalar_type();
+        const int64_t rows = q.size(0), heads = q.size(1), dim = q.size(2), keys = k.size(0);
+        const int64_t sequences = starts.defined() && starts.dim() == 1 ? starts.size(0) - 1 : 1;
+        if (code_of(type) < 0 || !is_rows(q, at, type, rows, dim) || !is_rows(k, at, type, keys, dim) || !is_rows(v, at, type, keys, dim) || v.size(1) != k.size(1) ||
+            (starts.defined() && !is_starts(starts, at)) ||
+            (key_starts.defined() ? !is_starts(key_starts, at) || key_starts.size(0) != sequences + 1 : sequences != 1 && keys != rows) ||
+            !bias_fits(sinks, at, type, heads) || (y.defined() && (!is_rows(y, at, type, rows, dim) || y.size(1) != heads || is_expanded(y))))
+            return none();
+        nvq_prompt_attention_desc d{};
+        d.dtype = code_of(type), d.head_dim = (int32_t)dim, d.rows = rows, d.keys = keys, d.query_heads = heads, d.key_heads = k.size(1), d.sequences = sequences;
+        d.window = window, d.causal = causal, d.scale = (float)scale;
+        const bool done = unlocked([&] {
+            if (!y.defined()) y = at.empty(q.sizes(), type);
+            for (int i = 0; i < 2; i++)
+                d.q_strides[i] = q.stride(i), d.k_strides[i] = k.stride(i), d.v_strides[i] = v.stride(i), d.out_strides[i] = y.stride(i);
+            const size_t need = nvq_prompt_attention_workspace_bytes(&d);
+            Tensor workspace;
+            if (need > 0) workspace = at.empty({(int64_t)need}, at::kByte);
+            return nvq_prompt_attention(&d, ptr(q), ptr(k), ptr(v), (const int32_t *)ptr(starts), (const int32_t *)ptr(key_starts), ptr(sinks),
+                                        y.mutable_data_ptr(), need > 0 ? workspace.mutable_data_ptr() : nullptr, at.stream()) == NVQ_OK;
+        });
+        return wrap(done, y);
+    });
+}
+
 // ── adapters and the choice of experts ──────────────────────────────────────────────────────────────────────────────
 // apply_adapters(y, x, adapters, ids, out or None)
 PyObject *py_apply_adapters(PyObject *, PyObject *const *args, Py_ssize_t n) {
@@ -1140,6 +1183,7 @@ PyMethodDef methods[] = {
     {"append_paged", NVQ_FAST(py_append_paged), nullptr},
     {"read_paged", NVQ_FAST(py_read_paged), nullptr},
     {"paged_attention", NVQ_FAST(py_paged_attention), nullptr},
+    {"prompt_attention", NVQ_FAST(py_prompt_attention), nullptr},
     {"apply_adapters", NVQ_FAST(py_apply_adapters), nullptr},
     {"moe_select", NVQ_FAST(py_moe_select), nullptr},
     {nullptr, nullptr, 0, nullptr},

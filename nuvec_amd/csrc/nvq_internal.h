@@ -234,6 +234,14 @@ size_t adapters_workspace_bytes(const nvq_adapters_desc &d);
 int32_t launch_adapters(const nvq_adapters_desc &d, const void *x, const void *down, const void *up, const float *scales, const int32_t *ids, const void *y,
                         void *out, void *workspace, hipStream_t s);
 int32_t launch_moe_select(const nvq_moe_select_desc &d, const void *logits, const float *bias, int32_t *indices, void *weights, hipStream_t s);
+struct PromptAttentionOperands {
+    const void *q, *k, *v, *sinks;
+    const int32_t *query_starts, *key_starts;
+    void *out, *workspace;
+};
+bool prompt_attention_launchable(const nvq_prompt_attention_desc &d);
+size_t prompt_attention_workspace_bytes(const nvq_prompt_attention_desc &d);
+int32_t launch_prompt_attention(const nvq_prompt_attention_desc &d, const PromptAttentionOperands &o, hipStream_t s);
 bool paged_attention_launchable(const nvq_paged_attention_desc &d, bool starts);
 size_t paged_attention_workspace_bytes(const nvq_paged_attention_desc &d);
 int32_t launch_paged_attention(const nvq_paged_attention_desc &d, const PagedAttentionOperands &o, hipStream_t s);

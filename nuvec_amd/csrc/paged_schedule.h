@@ -20,6 +20,11 @@ struct PagedBatch {
     int32_t few;     // lines of a sequence that the kernel of few rows takes; more are the other kernel's
     int32_t target;  // items that fill the chip
     int32_t least;   // tiles of an item, where a unit is more than one
+
+    __device__ __forceinline__ int64_t first_row(int b) const { return starts == nullptr ? b : starts[b]; }
+    __device__ __forceinline__ int64_t end_row(int b) const { return starts == nullptr ? b + 1 : starts[b + 1]; }
+    __device__ __forceinline__ int64_t length(int b) const { return lengths[b]; }
+    __device__ __forceinline__ int64_t most() const { return place.capacity(); }
 };
 
 namespace {
@@ -30,14 +35,14 @@ struct PagedSequence {
     int32_t start, rows, length, base, tiles, parts;  // base: the first key that a row sees, rounded down to a tile
 };
 
-// KIND 0: the sequences of few lines, 1: the others (parts 0: not this kernel's).
-template <int LINES, int KIND>
-__device__ __forceinline__ PagedSequence paged_sequence(const PagedBatch &a, int b) {
+// KIND 0: the sequences of few lines, 1: the others (parts 0: not this kernel's).  Batch: PagedBatch, or another that has its names.
+template <int LINES, int KIND, typename Batch>
+__device__ __forceinline__ PagedSequence paged_sequence(const Batch &a, int b) {
     PagedSequence s{};
     if (b >= a.sequences) return s;
-    const int64_t first = a.starts == nullptr ? b : a.starts[b], end = a.starts == nullptr ? b + 1 : a.starts[b + 1];
+    const int64_t first = a.first_row(b), end = a.end_row(b);
     const int64_t from = first < 0 ? 0 : first < a.rows ? first : a.rows, to = end < from ? from : end < a.rows ? end : a.rows;
-    const int64_t length = a.lengths[b], most = a.place.capacity();
+    const int64_t length = a.length(b), most = a.most();
     s.start = (int32_t)from, s.rows = (int32_t)(to - from);
     s.length = (int32_t)(length < 0 ? 0 : length < most ? length : most);
     const int64_t seen = (int64_t)s.length - s.rows - a.window + 1;
@@ -92,8 +97,8 @@ struct PagedPlan {
     __device__ __forceinline__ int32_t splits(const PagedSequence &s) const { return s.tiles <= per ? 1 : (s.tiles + per - 1) / per; }
 };
 
-template <int LINES, int KIND>
-__device__ __forceinline__ PagedPlan paged_plan(const PagedBatch &a, int lane, const PagedSequence &first) {
+template <int LINES, int KIND, typename Batch>
+__device__ __forceinline__ PagedPlan paged_plan(const Batch &a, int lane, const PagedSequence &first) {
     double total = 0.0;
     int32_t units = 0;
     for (int b0 = 0; b0 < a.sequences; b0 += 64) {
@@ -128,8 +133,8 @@ struct PagedItem {
 };
 
 // Item `at`, or (UNITS) unit `at` of the sequences with several splits, its `slot` that of its first split.
-template <int LINES, int KIND, bool UNITS>
-__device__ __forceinline__ bool paged_find(const PagedBatch &a, const PagedPlan &p, int lane, const PagedSequence &first, int32_t at, PagedItem &item) {
+template <int LINES, int KIND, bool UNITS, typename Batch>
+__device__ __forceinline__ bool paged_find(const Batch &a, const PagedPlan &p, int lane, const PagedSequence &first, int32_t at, PagedItem &item) {
     int32_t slots = 0;
     for (int b0 = 0; b0 < a.sequences; b0 += 64) {
         const PagedSequence s = b0 == 0 ? first : paged_sequence<LINES, KIND>(a, b0 + lane);
@@ -158,8 +163,8 @@ __device__ __forceinline__ bool paged_find(const PagedBatch &a, const PagedPlan 
 
 // Item (or unit, which comes after the items) `at` of the whole plan; false behind the last.  `length`: where the first block of the items leaves the
 // plan's length for the units'; NULL: nothing is split.
-template <int LINES, int KIND, bool UNITS>
-__device__ __forceinline__ bool paged_item(const PagedBatch &a, int lane, int32_t at, int32_t *length, PagedItem &item) {
+template <int LINES, int KIND, bool UNITS, typename Batch>
+__device__ __forceinline__ bool paged_item(const Batch &a, int lane, int32_t at, int32_t *length, PagedItem &item) {
     const PagedSequence first = paged_sequence<LINES, KIND>(a, lane);
     PagedPlan plan;
     if constexpr (UNITS) {

@@ -1,0 +1,636 @@
+// Attention of whole prompts over keys and values as the projections leave them:
+//     out[row, h, :] = softmax(scale * q[row, h, :] . K^T [masked] [, sink[h]]) . V
+// over the keys and values of the row's sequence.
+//
+// A block has 128 lines (line r of a sequence: row r / rep, query head r % rep of the key head, so that the heads that share keys share their tile), a
+// wavefront 32 of them, and walks the keys it sees in tiles in LDS: S^T = K . Q^T on v_mfma_f32_32x32x16 leaves a lane with half of a tile's scores of
+// ONE line, its maximum and sum are in-lane but for an exchange of two lanes, and the weights of 16 keys are already the operand of
+// O^T = V^T . P^T, whose V is read from LDS through the transposing read in the order in which the lanes hold the keys.  float32 runs the same way on
+// v_mfma_f32_32x32x2_f32.
+//
+// Terms.  Queries and keys are exact operands.  The weights: in bfloat16 one term of float16 (11 bits beside the result's 8; the values, 8 bits,
+// are exact in float16 within its range, below), in float16 two terms (22 bits), in float32 themselves.  Scores, maxima, sums and accumulators are float32.
+//
+// bfloat16 values as float16: a block's first tile tells their size; where it is far from 1 they are scaled by a power of two.  A later tile
+// that leaves float16's range is laid out again with the scale it needs, and the accumulators follow.
+//
+// Masked keys (behind the sequence's end, in front of a row or outside its window) have no weight whatever their keys hold.  Values that are not finite
+// are zeros in the tile, so that lines that do not see them stay clean; the lines that do are given them afterwards.
+#pragma once
+
+#include "matrix.h"
+#include "nvq_device.h"
+#include "nvq_internal.h"
+#include "prompt_attention.h"
+
+namespace nvq {
+namespace prompt {
+
+constexpr int kWaves = 4;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLowest = -3.4e38f;  // where maxima start (paged_rows_kernel.h says why it is finite)
+
+template <typename T>
+struct PromptArgs {
+    PromptBatch batch;
+    const T *q, *k, *v, *sinks;
+    T *out;
+    int32_t *length;  // of the plan, for the merge; NULL: no merge
+    float *states;    // [slots][kLines][D + 4]: maximum of the base-2 scores, denominator, two unused, D weighted means
+    int64_t q_strides[2], k_strides[2], v_strides[2], out_strides[2];
+    int32_t dim;
+    float scale;
+};
+
+namespace {
+
+typedef float acc16_t __attribute__((ext_vector_type(16)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+
+template <int D> constexpr int kState = D + 4;
+
+// K's rows have a 16-byte run more than their values, an odd number of them: the 16 lanes that read one run of 16 rows meet different banks.  V's
+// rows are an odd number of 64 bytes apart: the 32 lanes that read 64 bytes of four rows.
+template <typename T, int D>
+struct Tile {
+    static constexpr int kKeys = sizeof(T) == 4 || D > 128 ? 32 : 64;  // (of a lane 32 at most: the bits of a word)
+    static constexpr int kRuns = D * (int)sizeof(T) / 16;  // of a row
+    static constexpr int kKeyRow = 16 * (kRuns + 1), kValueRow = 64 * (kRuns / 4 + (kRuns / 4 % 2 == 0 ? 1 : 0));
+    static constexpr int kShare = kKeys * kRuns / (64 * kWaves);  // runs of a thread
+    static_assert(kKeys * kRuns % (64 * kWaves) == 0);
+    struct Stage {
+        uint8_t keys[kKeys * kKeyRow], values[kKeys * kValueRow];
+    };
+};
+
+template <typename T>
+__device__ __forceinline__ acc16_t scores32(uint4 k, uint4 q, acc16_t c) {
+    if constexpr (Elem<T>::code == NVQ_BF16) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, k), __builtin_bit_cast(bf16x8_t, q), c, 0, 0, 0);
+    } else if constexpr (Elem<T>::code == NVQ_F16) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, k), __builtin_bit_cast(half8_t, q), c, 0, 0, 0);
+    } else {
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(u2f(k.x), u2f(q.x), c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(u2f(k.y), u2f(q.y), c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(u2f(k.z), u2f(q.z), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x2f32(u2f(k.w), u2f(q.w), c, 0, 0, 0);
+    }
+}
+
+__device__ __forceinline__ uint32_t half_pair(float a, float b) {
+    typedef float f32x2_t __attribute__((ext_vector_type(2)));
+    typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+    const f32x2_t v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
+}
+__device__ __forceinline__ float half_of(uint32_t w, int i) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> (16 * i)));
+}
+
+// The keys that a block's lines see, from `begin` to `end`, and how its items share them: evenly, `keys` each.  An item that has them all writes the result.
+struct Span {
+    int32_t begin, end, keys, items;
+};
+__device__ __forceinline__ Span span_of(const PromptBatch &a, const PagedItem &item, int part) {
+    const int32_t from = part * kLines, lines = item.s.rows * a.rep, to = lines - from < kLines ? lines : from + kLines;
+    int32_t begin = 0, end = item.s.length;
+    if (a.causal) {
+        const int32_t before = item.s.length - item.s.rows, seen = before + (to - 1) / a.rep + 1;
+        const int64_t first = a.window > 0 ? before + from / a.rep + 1 - a.window : 0;
+        end = seen < end ? seen : end, begin = first > 0 ? (int32_t)first / kScheduleKeys * kScheduleKeys : 0;
+    }
+    Span s{uniform(begin), uniform(end), 0, 1};
+    const int32_t tiles = end > begin ? (end - begin + kScheduleKeys - 1) / kScheduleKeys : 0;
+    int32_t per = (tiles + item.splits - 1) / item.splits;
+    per = ((per > a.least ? per : a.least) + 1) & ~1;
+    s.keys = uniform(item.splits == 1 ? tiles * kScheduleKeys : per * kScheduleKeys);
+    s.items = uniform(item.splits == 1 || tiles <= per ? 1 : (tiles + per - 1) / per);
+    return s;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(const PromptArgs<T> a) {
+    using Of = Tile<T, D>;
+    using Stage = typename Of::Stage;
+    constexpr bool kWide = sizeof(T) == 4, kBf16 = Elem<T>::code == NVQ_BF16;
+    constexpr int KT = Of::kKeys, TB = KT / 32, RUN = kFragRun<T>;      // keys of a tile, blocks of 32; values of a run
+    constexpr int KS = D / (2 * RUN), ND = D / 32;                     // steps of a score (a run of both halves of the wavefront), blocks of D
+    constexpr int SHARE = Of::kShare;
+    __shared__ alignas(16) Stage stages[2];
+    __shared__ uint32_t flags[2];             // of a stage: a value that it does not hold
+    __shared__ uint32_t most[2][kWaves];      // of a tile that is laid out again: the largest finite value's bits; whether one is not finite
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
+    PagedItem item;
+    if (!paged_item<kLines, 1, false>(a.batch, lane, blockIdx.x, a.length, item)) return;
+    const int rep = a.batch.rep, hk = item.head, S = item.s.length, n = item.s.rows;
+    const int part = item.s.parts - 1 - item.part;  // (the lines that see most first)
+    const int lines = n * rep;
+    const int window = (int)(a.batch.window < S + 1 ? a.batch.window : S + 1);
+    auto last_of = [&](int i) { return a.batch.causal ? S - n + i : S - 1; };
+    auto first_of = [&](int i) { return window > 0 && a.batch.causal ? last_of(i) - window + 1 : 0; };
+    const Span span = span_of(a.batch, item, part);
+    if (item.split >= span.items) return;
+    const int s_begin = uniform(span.begin + item.split * span.keys), s_end = uniform(span.end < s_begin + span.keys ? span.end : s_begin + span.keys);
+    // the wavefront's lines
+    const int r0 = part * kLines + wave * 32, r = r0 + col;
+    const bool live = r < lines;
+    const int my_row = (live ? r : lines - 1) / rep, my_head = hk * rep + (live ? r % rep : 0);
+    const int my_last = last_of(my_row), my_first = first_of(my_row);
+    const int w_first = (r0 < lines ? r0 : lines - 1) / rep, w_last = (r0 + 31 < lines ? r0 + 31 : lines - 1) / rep;
+    const int all_last = uniform(last_of(w_first)), all_first = uniform(first_of(w_last));                    // keys up to / from which all of them see
+    const int any_last = uniform(r0 < lines ? last_of(w_last) : -1), any_first = uniform(first_of(w_first));  // and any does
+
+    // Scores are kept positive multiples of the product: a negative scale's sign goes to the queries, and of a scale of 0 they are zeros.
+    const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
+    uint4 qf[KS];
+    {
+        const T *query = a.q + (int64_t)(item.s.start + my_row) * a.q_strides[0] + (int64_t)my_head * a.q_strides[1];
+        const uint32_t sign = a.scale < 0.0f ? (kWide ? 0x80000000u : 0x80008000u) : 0u, keep = a.scale == 0.0f ? 0u : ~0u;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const int d = (2 * s + half) * RUN;
+            const uint4 w = load_run(query + (d < a.dim ? d : 0));
+            const uint32_t k = d < a.dim ? keep : 0u;
+            qf[s] = make_uint4((w.x ^ sign) & k, (w.y ^ sign) & k, (w.z ^ sign) & k, (w.w ^ sign) & k);
+        }
+    }
+
+    // ── staging: run i of a thread is run tid + 256 i of the tile ──
+    const int64_t first_key = a.batch.first_key(item.b);
+    const T *keys = a.k + first_key * a.k_strides[0] + (int64_t)hk * a.k_strides[1], *values = a.v + first_key * a.v_strides[0] + (int64_t)hk * a.v_strides[1];
+    uint4 kr[SHARE], vr[SHARE];
+    auto place = [&](int i, int &row, int &run) __attribute__((always_inline)) {
+        const int at = tid + 64 * kWaves * i;
+        row = at / Of::kRuns, run = at % Of::kRuns;
+    };
+    auto request_values = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < SHARE; i++) {
+            int row, run;
+            place(i, row, run);
+            const int64_t key = s0 + row < S ? s0 + row : S - 1;
+            vr[i] = load_run(values + key * a.v_strides[0] + (run * RUN < a.dim ? run * RUN : 0));
+        }
+    };
+    auto request = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < SHARE; i++) {
+            int row, run;
+            place(i, row, run);
+            const int64_t key = s0 + row < S ? s0 + row : S - 1;
+            kr[i] = load_run(keys + key * a.k_strides[0] + (run * RUN < a.dim ? run * RUN : 0));
+        }
+        request_values(s0);
+    };
+    // What lies behind the head's values and behind the sequence's end: zeros.
+    auto real = [&](int s0, int i) __attribute__((always_inline)) {
+        int row, run;
+        place(i, row, run);
+        return s0 + row < S && run * RUN < a.dim;
+    };
+    float value_scale = 1.0f;  // (bfloat16; a power of two)
+    // A run of values as operands: float16 for both 16-bit types.
+    auto operand = [&](uint4 w, bool scaled) __attribute__((always_inline)) {
+        if constexpr (kBf16) {
+            uint32_t in[4] = {w.x, w.y, w.z, w.w}, out[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float x = u2f(in[j] << 16), y = u2f(in[j] & 0xFFFF0000u);
+                if (scaled) x *= value_scale, y *= value_scale;
+                out[j] = half_pair(x, y);
+            }
+            return make_uint4(out[0], out[1], out[2], out[3]);
+        } else {
+            return w;
+        }
+    };
+    auto value_place = [&](Stage &to, int i) __attribute__((always_inline)) {
+        int row, run;
+        place(i, row, run);
+        return reinterpret_cast<uint4 *>(to.values + row * Of::kValueRow + 16 * run);
+    };
+    // The tile's rows into a stage; its flag where a value is not finite there.
+    auto lay = [&](Stage &to, uint32_t &flag, int s0) __attribute__((always_inline)) {
+        typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+        float wild = 0.0f;
+        f16x2_t wild2 = {(_Float16)0.0f, (_Float16)0.0f};
+#pragma unroll
+        for (int i = 0; i < SHARE; i++) {
+            int row, run;
+            place(i, row, run);
+            const bool used = real(s0, i);
+            const uint32_t k = used ? ~0u : 0u;
+            // (keys behind the head's values meet zeros of the queries, which an infinite value would spoil)
+            const uint32_t in = run * RUN < a.dim ? ~0u : 0u;
+            *reinterpret_cast<uint4 *>(to.keys + row * Of::kKeyRow + 16 * run) = make_uint4(kr[i].x & in, kr[i].y & in, kr[i].z & in, kr[i].w & in);
+            uint4 w = make_uint4(vr[i].x & k, vr[i].y & k, vr[i].z & k, vr[i].w & k);
+            if (kBf16 && value_scale != 1.0f) {
+                asm volatile("");  // (a branch, the same for all)
+                w = operand(w, true);
+            } else {
+                w = operand(w, false);
+            }
+            *value_place(to, i) = w;
+            if constexpr (kWide) {  // x 0 is NaN of what is not finite
+                wild = __builtin_fmaf(u2f(w.x), 0.0f, wild), wild = __builtin_fmaf(u2f(w.y), 0.0f, wild);
+                wild = __builtin_fmaf(u2f(w.z), 0.0f, wild), wild = __builtin_fmaf(u2f(w.w), 0.0f, wild);
+            } else {
+                const f16x2_t zero = {(_Float16)0.0f, (_Float16)0.0f};
+                wild2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, w.x), zero, wild2);
+                wild2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, w.y), zero, wild2);
+                wild2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, w.z), zero, wild2);
+                wild2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, w.w), zero, wild2);
+            }
+        }
+        if constexpr (!kWide) wild = (float)wild2[0] + (float)wild2[1];
+        if (wild != wild) flag = 1u;
+    };
+
+    acc16_t o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+    float m = kLowest, l = 0.0f;
+
+    // V^T . P^T of 16 keys (float32: of two), their weights in `p` as the scores' accumulators hold them.
+    auto value_run = [&](const Stage &from, int c, int d) __attribute__((always_inline)) {
+        const uint8_t *at = from.values + (16 * c + 4 * half + ((lane & 15) >> 2)) * Of::kValueRow + 2 * (32 * d + 16 * (lane >> 4 & 1) + 4 * (lane & 3));
+        typedef __attribute__((address_space(3))) short4_t *Lds;
+        const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(uintptr_t)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(uintptr_t)(at + 8 * Of::kValueRow));
+        struct { short4_t v[2]; } both = {{lo, hi}};
+        return __builtin_bit_cast(half8_t, both);
+    };
+    auto value_at = [&](const Stage &from, int i, int d) __attribute__((always_inline)) {
+        return reinterpret_cast<const float *>(from.values + (8 * (i >> 2) + 4 * half + (i & 3)) * Of::kValueRow)[32 * d + col];
+    };
+    auto weighted = [&](const Stage &from, const float (&x)[TB][16]) __attribute__((always_inline)) {
+        if constexpr (kWide) {
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+#pragma unroll
+                for (int d = 0; d < ND; d++) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(value_at(from, i, d), x[0][i], o[d], 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int c = 0; c < KT / 16; c++) {
+                const float *e = &x[c >> 1][8 * (c & 1)];
+                uint32_t p[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) p[j] = half_pair(e[2 * j], e[2 * j + 1]);
+                const half8_t high = __builtin_bit_cast(half8_t, make_uint4(p[0], p[1], p[2], p[3]));
+                half8_t low;
+                if constexpr (!kBf16) {
+                    uint32_t q[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) q[j] = half_pair(e[2 * j] - half_of(p[j], 0), e[2 * j + 1] - half_of(p[j], 1));
+                    low = __builtin_bit_cast(half8_t, make_uint4(q[0], q[1], q[2], q[3]));
+                }
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    const half8_t v = value_run(from, c, d);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, high, o[d], 0, 0, 0);
+                    if constexpr (!kBf16) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, low, o[d], 0, 0, 0);
+                }
+            }
+        }
+    };
+    // One tile: the scores, one look at their maximum, the weights and their products.  x[t][i]: key 32 t + 8 (i / 4) + 4 half + i % 4.  `seen`, where the
+    // tile is flagged: a bit for each of these keys that has a weight.
+    auto tile = [&](const Stage &from, int s0, bool flagged, uint32_t &seen) __attribute__((always_inline)) {
+        float x[TB][16];
+#pragma unroll
+        for (int t = 0; t < TB; t++) {
+            acc16_t s;
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[i] = 0.0f;
+            const uint8_t *row = from.keys + (32 * t + col) * Of::kKeyRow + 16 * half;
+#pragma unroll
+            for (int k = 0; k < KS; k++) s = scores32<T>(*reinterpret_cast<const uint4 *>(row + 32 * k), qf[k], s);
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[t][i] = s[i];
+        }
+        if (s0 + KT - 1 > all_last || s0 < all_first || s0 + KT > s_end) {
+            asm volatile("");  // (a branch: as selects it would cost every tile)
+#pragma unroll
+            for (int t = 0; t < TB; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int key = s0 + 32 * t + 8 * (i >> 2) + 4 * half + (i & 3);
+                    if (key > my_last || key < my_first || key >= s_end) x[t][i] = -INFINITY;
+                }
+        }
+        float top = x[0][0];
+#pragma unroll
+        for (int i = 1; i < 16 * TB; i++) top = fmaxf(top, x[i >> 4][i & 15]);
+        top *= scale;
+        // Rescaled only when a maximum has grown by more than 2^8: until then the weights are at most 2^8.
+        if (__any(top > m + 8.0f)) {
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float m_new = fmaxf(m, top), f = exp2f(m - m_new);
+            m = m_new, l *= f;
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] *= f;
+        }
+        // The maximum is a rounded product, which the fused one is not: the difference is a factor that all weights of a line share, but one that grows
+        // with the scores' size.  From 2^20 on both are rounded.
+        if (__any(fabsf(m) > 1048576.0f)) {
+            asm volatile("");
+#pragma unroll
+            for (int t = 0; t < TB; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[t][i] = x[t][i] * scale - m;
+        } else {
+#pragma unroll
+            for (int t = 0; t < TB; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[t][i] = __builtin_fmaf(x[t][i], scale, -m);
+        }
+#pragma unroll
+        for (int t = 0; t < TB; t++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[t][i] = __builtin_amdgcn_exp2f(x[t][i]), l += x[t][i];
+        if (flagged) {
+            asm volatile("");
+#pragma unroll
+            for (int t = 0; t < TB; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) seen |= (x[t][i] == 0.0f ? 0u : 1u) << (16 * t + i);
+        }
+        weighted(from, x);
+    };
+
+    // The largest finite value of the tile in vr (its bits as a positive number) and whether one is not finite, for all of the block.
+    auto survey = [&](int s0, uint32_t &top, bool &wild) __attribute__((always_inline)) {
+        uint32_t mine = 0, odd = 0;
+#pragma unroll
+        for (int i = 0; i < SHARE; i++) {
+            const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+            const bool used = real(s0, i);
+#pragma unroll
+            for (int j = 0; j < RUN; j++) {
+                T t[RUN];
+                __builtin_memcpy(t, w, 16);
+                const uint32_t b = f2u(Elem<T>::load(t, j)) & 0x7FFFFFFFu;
+                if (used && b < 0x7F800000u && b > mine) mine = b;
+                odd |= used && b >= 0x7F800000u ? 1u : 0u;
+            }
+        }
+        for (int i = 1; i < 64; i <<= 1) {
+            const uint32_t other = (uint32_t)__shfl_xor((int)mine, i);
+            mine = other > mine ? other : mine, odd |= (uint32_t)__shfl_xor((int)odd, i);
+        }
+        if (lane == 0) most[0][wave] = mine, most[1][wave] = odd;
+        __syncthreads();
+        top = 0, wild = false;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) top = most[0][w] > top ? most[0][w] : top, wild |= most[1][w] != 0;
+        __syncthreads();
+    };
+    // A scale that brings the largest value to 16 .. 32, 2^11 below what float16 holds, where it is outside 2^-3 .. 2^9: the smallest step is then 2^-29 of
+    // it, and at most 2^-21 in between.
+    auto scale_for = [&](uint32_t top) {
+        const int exponent = (int)(top >> 23);  // (of bfloat16's subnormals 0: as 2^-127)
+        if (top == 0 || (exponent >= 127 - 3 && exponent < 127 + 9)) return 1.0f;
+        const int e = 127 + 4 - (exponent - 127);
+        return u2f((uint32_t)(e < 1 ? 1 : e > 254 ? 254 : e) << 23);
+    };
+    // A flagged tile laid out again: the values that are not finite as zeros, the others with the scale they need.
+    auto lay_again = [&](Stage &to, int s0, bool &wild) __attribute__((always_inline)) {
+        request_values(s0);
+        uint32_t top;
+        survey(s0, top, wild);
+        if constexpr (kBf16) {
+            const float before = value_scale;
+            // (down only: what has been added up keeps its precision)
+            const float now = scale_for(top);
+            if (u2f(top) * value_scale >= 32768.0f && now < value_scale) value_scale = now;
+            const float f = value_scale / before;
+            if (f != 1.0f)
+#pragma unroll
+                for (int d = 0; d < ND; d++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[d][i] *= f;
+        }
+#pragma unroll
+        for (int i = 0; i < SHARE; i++) {
+            T t[RUN];
+            __builtin_memcpy(t, &vr[i], 16);
+            const bool used = real(s0, i);
+#pragma unroll
+            for (int j = 0; j < RUN; j++)
+                if (!used || !(fabsf(Elem<T>::load(t, j)) < INFINITY)) Elem<T>::store(t, j, 0.0f);
+            uint4 w;
+            __builtin_memcpy(&w, t, 16);
+            *value_place(to, i) = operand(w, true);
+        }
+        __syncthreads();
+    };
+    // What is not finite, to the lines that see it: by a product of ones at the places of one kind with ones at the keys that are seen.
+    auto add_wild = [&](Stage &to, int s0, uint32_t seen) __attribute__((always_inline)) {
+        request_values(s0);
+        for (int kind = 0; kind < 3; kind++) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < SHARE; i++) {
+                T t[RUN];
+                __builtin_memcpy(t, &vr[i], 16);
+                const bool used = real(s0, i);
+                uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int j = 0; j < RUN; j++) {
+                    const float v = Elem<T>::load(t, j);
+                    const bool is = used && (kind == 0 ? v == INFINITY : kind == 1 ? v == -INFINITY : v != v);
+                    if constexpr (kWide) w[j] = is ? f2u(1.0f) : 0u;
+                    else w[j >> 1] |= (is ? 0x3C00u : 0u) << (16 * (j & 1));
+                }
+                *value_place(to, i) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            __syncthreads();
+            const float special = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                acc16_t count;
+#pragma unroll
+                for (int i = 0; i < 16; i++) count[i] = 0.0f;
+                if constexpr (kWide) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) count = __builtin_amdgcn_mfma_f32_32x32x2f32(value_at(to, i, d), (float)(seen >> i & 1u), count, 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < KT / 16; c++) {
+                        uint32_t p[4];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) p[j] = (seen >> (8 * c + 2 * j) & 1u) * 0x3C00u | (seen >> (8 * c + 2 * j + 1) & 1u) * 0x3C000000u;
+                        count = __builtin_amdgcn_mfma_f32_32x32x16_f16(value_run(to, c, d), __builtin_bit_cast(half8_t, make_uint4(p[0], p[1], p[2], p[3])), count, 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (count[i] > 0.0f) o[d][i] += special;
+            }
+        }
+    };
+
+    if (tid < 2) flags[tid] = 0u;
+    __syncthreads();
+    if (s_begin < s_end) {
+        request(s_begin);
+        if constexpr (kBf16) {
+            uint32_t top;
+            bool wild;
+            survey(s_begin, top, wild);
+            value_scale = scale_for(top);
+        }
+        lay(stages[0], flags[0], s_begin);
+    }
+    __syncthreads();
+    int at = 0;
+    for (int s0 = s_begin; s0 < s_end; s0 += KT) {
+        const bool more = s0 + KT < s_end;
+        const bool flagged = uniform((int32_t)flags[at]) != 0;
+        bool wild = false;
+        if (flagged) {
+            asm volatile("");
+            __syncthreads();
+            if (tid == 0) flags[at] = 0u;
+            lay_again(stages[at], s0, wild);
+        }
+        if (more) request(s0 + KT);
+        uint32_t seen = 0;
+        if (s0 <= any_last && s0 + KT > any_first) tile(stages[at], s0, flagged, seen);  // (uniform in the wavefront)
+        if (wild) {
+            add_wild(stages[at], s0, seen);
+            if (more) request(s0 + KT);
+        }
+        if (more) lay(stages[at ^ 1], flags[at ^ 1], s0 + KT);
+        __syncthreads();
+        at ^= 1;
+    }
+    l += __shfl_xor(l, 32);
+    if (!live) return;
+    const bool whole = span.items == 1;
+    float factor = 1.0f;
+    const float back = 1.0f / value_scale;  // (by itself: times the factor it may leave float32's normal range)
+    float *state = nullptr;  // of this line and split: maximum, denominator, weighted means
+    if (whole) {
+        float denom = l, f = 1.0f;
+        if (a.sinks != nullptr) {
+            const float sink = Elem<T>::load(a.sinks, my_head) * kLog2e, top = fmaxf(m, sink);
+            f = exp2f(m - top), denom = denom * f + exp2f(sink - top);
+        }
+        factor = denom == 0.0f ? 0.0f : f / denom;  // (a row that sees nothing: zeros)
+    } else {
+        factor = l == 0.0f ? 0.0f : 1.0f / l;  // (divided here, so that sums of the largest values do not leave float32)
+        state = a.states + ((int64_t)item.slot * kLines + wave * 32 + col) * kState<D>;
+        if (half == 0) *reinterpret_cast<float2 *>(state) = make_float2(m, l);
+    }
+    T *out = a.out + (int64_t)(item.s.start + my_row) * a.out_strides[0] + (int64_t)my_head * a.out_strides[1];
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const int c = 32 * d + 8 * g + 4 * half;
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = o[d][4 * g + i] * factor * back;
+            if (!whole) {
+                *reinterpret_cast<float4 *>(state + 4 + c) = make_float4(v[0], v[1], v[2], v[3]);
+            } else if (c < a.dim) {
+                struct __attribute__((packed)) Four { T t[4]; };
+                Four four;
+#pragma unroll
+                for (int i = 0; i < 4; i++) Elem<T>::store(four.t, i, v[i]);
+                *reinterpret_cast<Four *>(out + c) = four;
+            }
+        }
+}
+
+// The splits' states merged: D / 4 threads a line, four splits' loads under way at a time.
+template <int D> constexpr int kMergeLines = 256 / (D / 4);  // of a block
+template <typename T, int D>
+__global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptArgs<T> a, uint32_t units) {
+    constexpr int kThreads = D / 4;
+    PagedItem item;
+    if (!paged_item<kLines, 1, true>(a.batch, threadIdx.x & 63, blockIdx.x % units, a.length, item)) return;
+    const int rep = a.batch.rep, ln = (int)(blockIdx.x / units) * kMergeLines<D> + (int)threadIdx.x / kThreads, at = (int)threadIdx.x % kThreads * 4;
+    const int part = item.s.parts - 1 - item.part, line = part * kLines + ln;  // (items count the parts from the last)
+    const Span span = span_of(a.batch, item, part);
+    if ((int)threadIdx.x >= kMergeLines<D> * kThreads || ln >= kLines || line >= item.s.rows * rep || span.items == 1 || at >= a.dim) return;
+    const int64_t stride = (int64_t)a.batch.key_heads * kLines * kState<D>;  // of a split's states
+    const float *src = a.states + ((int64_t)item.slot * kLines + ln) * kState<D>;
+    float top = kLowest, total = 0.0f, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int z0 = 0; z0 < span.items; z0 += 4) {
+        float2 m[4];
+        float4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float *state = src + (z0 + i < span.items ? z0 + i : z0) * stride;
+            m[i] = *reinterpret_cast<const float2 *>(state), v[i] = *reinterpret_cast<const float4 *>(state + 4 + at);
+        }
+        float most = top;
+#pragma unroll
+        for (int i = 0; i < 4; i++) most = fmaxf(most, m[i].x);
+        // (the means' weights add up to 1 as they come, for the same reason)
+        float w[4], all = total * exp2f(top - most);
+        const float before = all;
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = z0 + i < span.items ? m[i].y * exp2f(m[i].x - most) : 0.0f, all += w[i];
+        top = most, total = all;
+        const float share = all == 0.0f ? 0.0f : 1.0f / all, kept = before * share;
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum[i] = kept == 0.0f ? 0.0f : sum[i] * kept;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float part = w[i] * share;
+            if (part == 0.0f) continue;  // (a split that sees nothing, or nothing beside the others)
+            sum[0] = __builtin_fmaf(v[i].x, part, sum[0]), sum[1] = __builtin_fmaf(v[i].y, part, sum[1]);
+            sum[2] = __builtin_fmaf(v[i].z, part, sum[2]), sum[3] = __builtin_fmaf(v[i].w, part, sum[3]);
+        }
+    }
+    const int head = item.head * rep + line % rep;
+    float inv = 1.0f;
+    if (a.sinks != nullptr) {
+        const float sink = Elem<T>::load(a.sinks, head) * kLog2e, most = fmaxf(top, sink);
+        total *= exp2f(top - most);
+        inv = total == 0.0f ? 0.0f : total / (total + exp2f(sink - most));
+    }
+    struct __attribute__((packed)) Four { T t[4]; };
+    Four four;
+#pragma unroll
+    for (int i = 0; i < 4; i++) Elem<T>::store(four.t, i, sum[i] * inv);
+    *reinterpret_cast<Four *>(a.out + (int64_t)(item.s.start + line / rep) * a.out_strides[0] + (int64_t)head * a.out_strides[1] + at) = four;
+}
+
+template <typename T, int D>
+int32_t launch_sized(const PromptArgs<T> &a, const PromptLaunch &r, hipStream_t s) {
+    hipLaunchKernelGGL((prompt_kernel<T, D>), dim3(r.grid), dim3(64 * kWaves), 0, s, a);
+    NVQ_LAUNCH_CHECK("prompt_attention");
+    if (r.merge_units == 0) return NVQ_OK;
+    hipLaunchKernelGGL((prompt_merge_kernel<T, D>), dim3(r.merge_units * ((kLines + kMergeLines<D> - 1) / kMergeLines<D>)), dim3(256), 0, s, a, r.merge_units);
+    NVQ_LAUNCH_CHECK("prompt_attention merge");
+    return NVQ_OK;
+}
+
+template <typename T>
+int32_t launch_type(const nvq_prompt_attention_desc &d, const PromptAttentionOperands &o, const PromptLaunch &r, hipStream_t s) {
+    PromptArgs<T> a{};
+    a.batch = r.batch;
+    a.q = (const T *)o.q, a.k = (const T *)o.k, a.v = (const T *)o.v, a.sinks = (const T *)o.sinks, a.out = (T *)o.out;
+    a.length = r.merge_units > 0 ? (int32_t *)o.workspace : nullptr;
+    a.states = o.workspace == nullptr ? nullptr : (float *)((uint8_t *)o.workspace + kPlanBytes);
+    for (int i = 0; i < 2; i++)
+        a.q_strides[i] = d.q_strides[i], a.k_strides[i] = d.k_strides[i], a.v_strides[i] = d.v_strides[i], a.out_strides[i] = d.out_strides[i];
+    a.dim = d.head_dim, a.scale = d.scale;
+    switch (padded_dim(d.head_dim)) {
+    case 64: return launch_sized<T, 64>(a, r, s);
+    case 96: return launch_sized<T, 96>(a, r, s);
+    case 128: return launch_sized<T, 128>(a, r, s);
+    default: return launch_sized<T, 256>(a, r, s);
+    }
+}
+
+}  // namespace
+}  // namespace prompt
+}  // namespace nvq

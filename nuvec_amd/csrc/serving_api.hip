@@ -1,4 +1,4 @@
-// Host side of the entry points of adapters and of the choice of experts: the argument checks.
+// Host side of the entry points of prompts' attention, of adapters and of the choice of experts: the argument checks.
 #include "nvq_internal.h"
 
 using namespace nvq;
@@ -16,7 +16,47 @@ static int32_t check_adapters(const nvq_adapters_desc *d) {
     return NVQ_OK;
 }
 
+static int32_t check_prompt(const nvq_prompt_attention_desc *d) {
+    const char *op = "prompt_attention";
+    if (d == nullptr) return fail(NVQ_INVALID_ARGUMENT, "%s: null descriptor", op);
+    NVQ_TRY(check_float(op, d->dtype));
+    if (d->rows < 0 || d->keys < 0 || d->query_heads < 0 || d->key_heads < 0 || d->sequences < 0 || d->window < 0 || d->head_dim < 0)
+        return fail(NVQ_INVALID_ARGUMENT, "%s: negative size", op);
+    if (d->key_heads == 0 || d->query_heads % d->key_heads != 0)
+        return fail(NVQ_INVALID_ARGUMENT, "%s: %lld query heads over %lld key heads", op, (long long)d->query_heads, (long long)d->key_heads);
+    if (d->window > 0 && !d->causal) return fail(NVQ_INVALID_ARGUMENT, "%s: a window without the causal mask", op);
+    if (d->head_dim < 8 || d->head_dim > 256 || d->head_dim % 8 != 0) return fail(NVQ_UNSUPPORTED, "%s: heads of %d values (a multiple of 8 up to 256)", op, d->head_dim);
+    if (d->query_heads >= 1 << 15 || d->rows >= 1LL << 30 || d->rows * d->query_heads >= 1LL << 30 || d->keys >= 1LL << 30 || d->sequences >= 1 << 20)
+        return fail(NVQ_UNSUPPORTED, "%s: 2^30 rows and heads, 2^30 keys or 2^20 sequences", op);
+    for (int i = 0; i < 2; i++)
+        if (d->q_strides[i] < 0 || d->k_strides[i] < 0 || d->v_strides[i] < 0 || d->out_strides[i] < 0) return fail(NVQ_INVALID_ARGUMENT, "%s: negative stride", op);
+    if (!prompt_attention_launchable(*d)) return fail(NVQ_UNSUPPORTED, "%s: %lld rows of %lld sequences, %lld heads each, in one launch", op, (long long)d->rows, (long long)d->sequences, (long long)d->query_heads);
+    return NVQ_OK;
+}
+
 extern "C" {
+
+size_t nvq_prompt_attention_workspace_bytes(const nvq_prompt_attention_desc *d) {
+    if (check_prompt(d) != NVQ_OK || require_device() != NVQ_OK) return 0;
+    return prompt_attention_workspace_bytes(*d);
+}
+
+int32_t nvq_prompt_attention(const nvq_prompt_attention_desc *d, const void *q, const void *k, const void *v, const int32_t *query_starts,
+                             const int32_t *key_starts, const void *sinks, void *out, void *workspace, void *stream) {
+    const char *op = "prompt_attention";
+    NVQ_TRY(check_prompt(d));
+    if (d->rows == 0 || d->query_heads == 0 || d->sequences == 0) return NVQ_OK;
+    if (query_starts == nullptr && d->sequences != 1) return fail(NVQ_INVALID_ARGUMENT, "%s: %lld sequences without query starts", op, (long long)d->sequences);
+    if (key_starts == nullptr && d->sequences != 1 && d->keys != d->rows)
+        return fail(NVQ_INVALID_ARGUMENT, "%s: %lld rows and %lld keys of %lld sequences without key starts", op, (long long)d->rows, (long long)d->keys, (long long)d->sequences);
+    if (q == nullptr || out == nullptr || (d->keys > 0 && (k == nullptr || v == nullptr))) return fail(NVQ_INVALID_ARGUMENT, "%s: null operand", op);
+    for (const void *p : {q, k, v, sinks, (const void *)out}) NVQ_TRY(check_aligned(op, "an operand", p, (size_t)dtype_size(d->dtype)));
+    NVQ_TRY(check_aligned(op, "workspace", workspace));
+    NVQ_TRY(require_device());
+    if (workspace == nullptr && prompt_attention_workspace_bytes(*d) != 0) return fail(NVQ_INVALID_ARGUMENT, "%s: null workspace", op);
+    const PromptAttentionOperands o{q, k, v, sinks, query_starts, key_starts == nullptr && d->sequences != 1 ? query_starts : key_starts, out, workspace};
+    return launch_prompt_attention(*d, o, (hipStream_t)stream);
+}
 
 size_t nvq_apply_adapters_workspace_bytes(const nvq_adapters_desc *d) {
     if (check_adapters(d) != NVQ_OK || require_device() != NVQ_OK || d->rows == 0) return 0;

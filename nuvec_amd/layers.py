@@ -408,19 +408,31 @@ class PagedAttention:
 
     def forward(self, x: torch.Tensor, cache: paged.PagedCache, page_table: torch.Tensor, positions: torch.Tensor, lengths: torch.Tensor,
                 sequences: Optional[torch.Tensor] = None, query_starts: Optional[torch.Tensor] = None, max_queries: Optional[int] = None,
-                rotary_positions: Optional[torch.Tensor] = None, adapter_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
+                rotary_positions: Optional[torch.Tensor] = None, adapter_ids: Optional[torch.Tensor] = None, fresh: bool = False) -> torch.Tensor:
         """`x` `[tokens, dims]`: the rows of sequence b are `query_starts[b]` to `query_starts[b + 1] - 1`, row t is position `positions[t]` of
         sequence `sequences[t]`, and `lengths[b]` counts the positions of sequence b with these rows (all int32).  `sequences` and `query_starts`
         None: one token per sequence.  Padding rows (a negative position, behind the last start) write nothing; their results are undefined.
-        `rotary_positions` as in `append_paged`; `adapter_ids` int32 `[tokens]`: of the projections that are `AdaptedLinear`."""
+        `rotary_positions` as in `append_paged`; `adapter_ids` int32 `[tokens]`: of the projections that are `AdaptedLinear`.
+
+        `fresh`: every sequence begins with these rows, so that they attend their own keys and values before these become codes (`prompt_attention`:
+        faster, and without the codes' error); `lengths` are not read.  The cache is written as otherwise, from keys rounded to the element type."""
         if (sequences is None) != (query_starts is None):
             raise ops.InvalidArgument("paged_attention: sequences and query starts go together")
         if x.ndim != 2:
             raise ops.InvalidArgument(f"paged_attention: tokens must be [tokens, dims], got {list(x.shape)}")
         q, k, v = (self._heads(_adapted(p, x, adapter_ids), n)
                    for p, n in ((self.q_proj, self.query_heads), (self.k_proj, self.key_heads), (self.v_proj, self.key_heads)))
-        q = paged.append_paged(cache, k, v, page_table, positions, sequences, self.rotation, self.k_norm, q, self.q_norm, self.eps, rotary_positions)
         scale = q.shape[2] ** -0.5 if self.scale is None else self.scale
+        if fresh:
+            if query_starts is None:
+                raise ops.InvalidArgument("paged_attention: fresh sequences need query starts")
+            if self.rotation is not None or self.q_norm is not None or self.k_norm is not None:
+                at = positions[None] if rotary_positions is None else rotary_positions[None] if rotary_positions.ndim == 1 else rotary_positions[:, None]
+                q, k = (y[0].transpose(0, 1) for y in paged.head_norm_rope(q.transpose(0, 1)[None], k.transpose(0, 1)[None], self.q_norm, self.k_norm, self.rotation, at, self.eps))
+            paged.append_paged(cache, k, v, page_table, positions, sequences)
+            y = paged.prompt_attention(q, k, v, scale, query_starts, query_starts, self.sinks, True, self.window)
+            return _adapted(self.o_proj, y.flatten(1), adapter_ids)
+        q = paged.append_paged(cache, k, v, page_table, positions, sequences, self.rotation, self.k_norm, q, self.q_norm, self.eps, rotary_positions)
         y = paged.paged_attention(q, cache, page_table, lengths, scale, query_starts, max_queries, self.sinks, True, self.window)
         return _adapted(self.o_proj, y.flatten(1), adapter_ids)
 

@@ -453,3 +453,68 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
     _lib.check(lib.nvq_paged_attention(C.byref(desc), _ptr(q), *(_ptr(t) for t in pool), _ptr(page_table), _ptr(lengths), _ptr(query_starts), _ptr(sinks),
                                        _ptr(out), _ptr(workspace), _stream()))
     return out
+
+
+# ── prompts ─────────────────────────────────────────────────────────────────────────────────────────────────────────
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, query_starts: Optional[torch.Tensor] = None,
+                     key_starts: Optional[torch.Tensor] = None, sinks: Optional[torch.Tensor] = None, causal: bool = True, window: int = 0,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """`softmax(scale * q K^T [, sinks]) V` of whole prompts over keys and values as the projections (and `rope`) leave them: `q` `[rows, query_heads, dim]`,
+    `k` and `v` `[keys, key_heads, dim]`, heads of a multiple of 8 values up to 256, any strides with consecutive values of a head.
+
+    Sequence b has the rows `query_starts[b]` to `query_starts[b + 1] - 1` and the keys `key_starts[b]` to `key_starts[b + 1] - 1` (int32 `[sequences + 1]`,
+    ascending, on the device).  `query_starts` None: one sequence; `key_starts` None: the rows' own keys, or all keys of one sequence.  With `causal` row i of n
+    sees the keys up to number keys - n + i of its sequence, with `window` the last `window` of those alone.  `sinks` `[query_heads]` join each head's softmax.
+    Rows that see nothing are zeros; rows of no sequence are left as they were in `out` (and undefined in a new result).  Keys and values that a row does
+    not see may hold anything.
+
+    The softmax's weights hold 11 bits beside the 8 of a bfloat16 result (float16: 22, float32: 24), everything else is float32."""
+    y = (_lib._native or _lib.native()).prompt_attention(q, k, v, scale, query_starts, key_starts, sinks, causal, window, out)
+    if y is not None:
+        return y if out is None else out
+    op = "prompt_attention"
+    if q.ndim != 3 or q.dtype not in _FLOATS:
+        raise InvalidArgument(f"{op}: queries must be [rows, query heads, dim] of a float type, got {_name(q.dtype)} {list(q.shape)}")
+    if k.ndim != 3 or k.dtype != q.dtype or k.shape[2] != q.shape[2] or v.dtype != q.dtype or v.shape != k.shape:
+        raise InvalidArgument(f"{op}: keys {_name(k.dtype)} {list(k.shape)} and values {_name(v.dtype)} {list(v.shape)} beside queries {_name(q.dtype)} {list(q.shape)}")
+    _same_device(op, q, k, v)
+    n, heads, d = q.shape
+    if k.shape[1] == 0 or heads % k.shape[1]:
+        raise InvalidArgument(f"{op}: {heads} query heads over {k.shape[1]} key heads")
+    if d < 8 or d > 256 or d % 8:
+        raise Unsupported(f"{op}: heads of {d} values (a multiple of 8 up to 256)")
+    sequences = 1
+    if query_starts is not None:
+        if query_starts.ndim != 1 or query_starts.shape[0] < 1:
+            raise InvalidArgument(f"{op}: query starts must be int32 [sequences + 1], got {_name(query_starts.dtype)} {list(query_starts.shape)}")
+        sequences = query_starts.shape[0] - 1
+        query_starts = _indices(op, "query starts", query_starts, None, q)
+    if key_starts is not None:
+        key_starts = _indices(op, "key starts", key_starts, (sequences + 1,), q)
+    elif sequences != 1 and k.shape[0] != n:
+        raise InvalidArgument(f"{op}: {n} rows and {k.shape[0]} keys of {sequences} sequences without key starts")
+    if sinks is not None:
+        if sinks.dtype != q.dtype or tuple(sinks.shape) != (heads,):
+            raise InvalidArgument(f"{op}: sinks must be {_name(q.dtype)} [{heads}], got {_name(sinks.dtype)} {list(sinks.shape)}")
+        _same_device(op, q, sinks)
+        sinks = sinks.contiguous()
+    if window < 0 or (window > 0 and not causal):
+        raise InvalidArgument(f"{op}: a window of {window}{'' if causal else ' without the causal mask'}")
+    q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != q.shape or out.stride(2) != 1:
+        raise InvalidArgument(f"{op}: the output must be {_name(q.dtype)} {list(q.shape)} with consecutive values")
+    _own_rows(op, out)
+    _same_device(op, q, out)
+    desc = _lib.PromptAttentionDescC(_CODE[q.dtype], d, n, k.shape[0], heads, k.shape[1], sequences)
+    for i in range(2):
+        desc.q_strides[i], desc.k_strides[i], desc.v_strides[i], desc.out_strides[i] = q.stride(i), k.stride(i), v.stride(i), out.stride(i)
+    desc.window, desc.causal, desc.scale = min(window, 1 << 62), int(causal), float(scale)
+    _init(q)
+    _here(op, q)
+    lib = _lib.load()
+    need = lib.nvq_prompt_attention_workspace_bytes(C.byref(desc))
+    workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _lib.check(lib.nvq_prompt_attention(C.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(query_starts), _ptr(key_starts), _ptr(sinks), _ptr(out), _ptr(workspace), _stream()))
+    return out

@@ -1,4 +1,4 @@
-"""What adapters, the choice of experts and rotations with several axes refuse, before any device is asked: no GPU."""
+"""What prompts' attention, adapters, the choice of experts and rotations with several axes refuse, before any device is asked: no GPU."""
 import ctypes as C
 
 import pytest
@@ -17,6 +17,10 @@ ROT = nv.Rotation(torch.zeros(8, 32, 2), False, nv.rotary_axes((10, 11, 11)))
 
 def adapt(y=Z(4, 32), x=Z(4, 64), adapters=ADAPTERS, ids=ints(4), **more):
     return nv.apply_adapters(y, x, adapters, ids, **more)
+
+
+def prompt(q=Z(4, 2, 64), k=Z(4, 1, 64), v=Z(4, 1, 64), scale=1.0, *args, **more):
+    return nv.prompt_attention(q, k, v, scale, *args, **more)
 
 
 def cache():
@@ -40,6 +44,24 @@ def cache():
     (lambda: adapt(out=F(4, 32)), "the output must be"),
     (lambda: adapt(out=Z(32, 4).T), "consecutive values"),
     (lambda: adapt(out=Z(1, 32).expand(4, 32)), "consecutive values"),
+    (lambda: prompt(q=Z(4, 64)), "queries must be"),
+    (lambda: prompt(q=Z(4, 2, 64, dtype=torch.int32)), "queries must be"),
+    (lambda: prompt(k=F(4, 1, 64)), "beside queries"),
+    (lambda: prompt(v=Z(5, 1, 64)), "beside queries"),
+    (lambda: prompt(k=Z(4, 1, 32), v=Z(4, 1, 32)), "beside queries"),
+    (lambda: prompt(q=Z(4, 3, 64), k=Z(4, 2, 64), v=Z(4, 2, 64)), "3 query heads over 2"),
+    (lambda: prompt(k=Z(4, 0, 64), v=Z(4, 0, 64)), "2 query heads over 0"),
+    (lambda: prompt(query_starts=ints(3).long()), "query starts must be int32"),
+    (lambda: prompt(query_starts=ints(0)), "query starts must be int32"),
+    (lambda: prompt(query_starts=ints(3), key_starts=ints(4)), "key starts must be int32"),
+    (lambda: prompt(key_starts=ints(3)), "key starts must be int32"),
+    (lambda: prompt(k=Z(5, 1, 64), v=Z(5, 1, 64), query_starts=ints(3)), "4 rows and 5 keys of 2 sequences"),
+    (lambda: prompt(sinks=Z(3)), "sinks must be"),
+    (lambda: prompt(sinks=F(2)), "sinks must be"),
+    (lambda: prompt(window=-1), "a window of -1"),
+    (lambda: prompt(window=3, causal=False), "without the causal mask"),
+    (lambda: prompt(out=Z(4, 2, 32)), "the output must be"),
+    (lambda: prompt(out=Z(1, 2, 64).expand(4, 2, 64)), "share their memory"),
     (lambda: nv.moe_select(F(2, 8), 0), "k must be in 1..=8"),
     (lambda: nv.moe_select(F(2, 8), 9), "k must be in 1..=8"),
     (lambda: nv.moe_select(F(2, 8), (1 << 32) + 2), "k must be in 1..=8"),
@@ -75,13 +97,14 @@ def test_arguments(call, message):
 
 
 def test_no_cpu_path():
-    for call in (adapt, lambda: nv.moe_select(F(2, 8), 2), lambda: nv.rope(Z(1, 2, 3, 64), ROT, ints(3, 1, 3))):
+    for call in (prompt, adapt, lambda: nv.moe_select(F(2, 8), 2), lambda: nv.rope(Z(1, 2, 3, 64), ROT, ints(3, 1, 3))):
         with pytest.raises(_lib.NoDevice):
             call()
 
 
 @pytest.mark.parametrize("call", [
-    lambda: nv.moe_select(F(2, 2000), 2), lambda: nv.moe_select(F(2, 256), 65), lambda: nv.moe_select(F(2, 256), 2, groups=128)])
+    lambda: prompt(q=Z(4, 2, 4), k=Z(4, 1, 4), v=Z(4, 1, 4)), lambda: prompt(q=Z(4, 2, 100), k=Z(4, 1, 100), v=Z(4, 1, 100)),
+    lambda: prompt(q=Z(4, 2, 264), k=Z(4, 1, 264), v=Z(4, 1, 264)), lambda: nv.moe_select(F(2, 2000), 2), lambda: nv.moe_select(F(2, 256), 65), lambda: nv.moe_select(F(2, 256), 2, groups=128)])
 def test_unsupported(call):
     with pytest.raises(nv.Unsupported):
         call()
@@ -120,6 +143,24 @@ def test_entry_points():
                          ({"rows": 1}, bad), ({"dtype": _lib.U8}, bad), ({"experts": 1024, "k": 65}, un)):
         assert lib.nvq_moe_select(C.byref(m(**more)), *none * 5) == status, more
     assert lib.nvq_moe_select(None, *none * 5) == bad
+
+    def t(**more):
+        d = _lib.PromptAttentionDescC(_lib.BF16, 128, 0, 10, 8, 2, 1)
+        d.causal, d.scale = 1, 1.0
+        for name, value in more.items():
+            setattr(d, name, value)
+        return d
+    for more, status in (({}, ok), ({"head_dim": 12}, un), ({"head_dim": 264}, un), ({"head_dim": -8}, bad), ({"rows": -1}, bad), ({"keys": -1}, bad),
+                         ({"keys": 1 << 30}, un), ({"rows": 1 << 28}, un), ({"sequences": 1 << 20}, un), ({"sequences": -1}, bad), ({"key_heads": 0}, bad),
+                         ({"query_heads": 7}, bad), ({"window": -1}, bad), ({"window": 4, "causal": 0}, bad), ({"rows": 4}, bad), ({"dtype": _lib.U8}, bad),
+                         ({"rows": 1 << 20, "query_heads": 1 << 15, "key_heads": 1 << 15}, un)):
+        assert lib.nvq_prompt_attention(C.byref(t(**more)), *none * 9) == status, more
+    assert lib.nvq_prompt_attention(None, *none * 9) == bad
+    assert lib.nvq_prompt_attention(C.byref(t(rows=4, sequences=2)), one, one, one, None, None, None, one, one, None) == bad and "query starts" in _lib.last_error()
+    assert lib.nvq_prompt_attention(C.byref(t(rows=4, sequences=2)), one, one, one, one, None, None, one, one, None) == bad and "key starts" in _lib.last_error()
+    d = t(rows=4)
+    d.k_strides[0] = -1
+    assert lib.nvq_prompt_attention(C.byref(d), one, one, one, None, None, None, one, one, None) == bad and "stride" in _lib.last_error()
 
     axes = _lib.RotaryAxesC(3)
     r = _lib.HeadRopeDescC(_lib.BF16, 64, 32, 0, 0, 8, 0, 1)
