@@ -17,7 +17,7 @@
 namespace nvq {
 namespace {
 
-constexpr int kTileRows = 16, kAdapterWaves = 4, kWaveColumns = 64;
+constexpr int kDownWaves = 8, kUpWaves = 4, kBlockColumns = 256;  // (64 a wavefront)
 
 template <typename T>
 struct AdapterArgs {
@@ -27,245 +27,394 @@ struct AdapterArgs {
     T *out;
     float *low;  // [splits][rows][padded]: shares of x . down^T
     int64_t rows, inputs, outputs, x_stride, y_stride, out_stride;
-    int32_t adapters, rank, padded, splits, slots;  // slots: of a block, of a tile's 16 rows
+    int32_t adapters, rank, padded, splits, chunks;  // chunks: of 256 columns of a block
 };
 
-// The adapter of the lane's row (lane % 16) of the tile; -1: none, or no row.
-template <typename T>
-__device__ __forceinline__ int32_t adapter_of(const AdapterArgs<T> &a, int64_t row) {
-    const int32_t id = row < a.rows ? a.ids[row] : -1;
-    return id >= 0 && id < a.adapters ? id : -1;
-}
-// Whether slot `s` of the tile is the first row of its adapter; the adapter.
-__device__ __forceinline__ bool leads(int32_t id, int s, int32_t &adapter) {
-    adapter = __builtin_amdgcn_readlane(id, s);
-    return adapter >= 0 && __builtin_ctzll(__ballot(id == adapter)) == s;
-}
+// The adapters that occur in a tile of up to 64 rows, one after the other in the order of their first rows: every `step`th from number `first` on.
+struct Occurring {
+    int32_t id;     // of row `lane` of the tile; -1: none, or no row
+    uint64_t left;  // rows whose adapters are still to come
+    int step;
+    template <typename T>
+    __device__ __forceinline__ Occurring(const AdapterArgs<T> &a, int64_t row0, int rows, int first, int every) {
+        const int lane = threadIdx.x & 63;
+        id = lane < rows && row0 + lane < a.rows ? a.ids[row0 + lane] : -1;
+        id = id >= 0 && id < a.adapters ? id : -1;
+        left = __ballot(id >= 0), step = every;
+        for (int i = 0; i < first && left != 0; i++) skip();
+    }
+    __device__ __forceinline__ void skip() { left &= ~__ballot(id == __builtin_amdgcn_readlane(id, __builtin_ctzll(left))); }
+    __device__ __forceinline__ bool any() const { return left != 0; }
+    __device__ __forceinline__ int32_t now() const { return __builtin_amdgcn_readlane(id, __builtin_ctzll(left)); }
+    __device__ __forceinline__ void next() {
+        for (int i = 0; i < step && left != 0; i++) skip();
+    }
+    // The adapter of row `row` of the tile.
+    __device__ __forceinline__ int32_t of(int row) const { return __shfl(id, row); }
+};
 
-// RT tiles of 16 ranks at a time.
-template <typename T, int RT>
-__global__ void __launch_bounds__(64 * kAdapterWaves) adapters_down_kernel(const AdapterArgs<T> a) {
-    __shared__ acc4_t shares[kAdapterWaves][RT][64];
+template <int N>
+struct Count {
+    static constexpr int value = N;
+};
+
+// RW tiles of 16 rows, RT tiles of 16 ranks at a time.
+template <typename T, int RW, int RT>
+__global__ void __launch_bounds__(64 * kDownWaves) adapters_down_kernel(const AdapterArgs<T> a) {
+    __shared__ acc4_t shares[kDownWaves][RW * RT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, quarter = lane >> 4;
-    const int64_t row = (int64_t)blockIdx.x * kTileRows + col;
-    const int32_t id = adapter_of(a, row);
-    const int64_t steps = (a.inputs + kFragStep<T> - 1) / kFragStep<T>, whole = a.inputs / kFragStep<T>;
-    const int64_t per = (steps + a.splits * kAdapterWaves - 1) / (a.splits * kAdapterWaves);
-    const int64_t from = ((int64_t)blockIdx.y * kAdapterWaves + wave) * per, to = from + per < steps ? from + per : steps, to_whole = to < whole ? to : whole;
-    const T *x = a.x + (row < a.rows ? row : a.rows - 1) * a.x_stride + quarter * kFragRun<T>;
-    for (int s = blockIdx.z * a.slots; s < (int)(blockIdx.z + 1) * a.slots; s++) {
-        int32_t adapter;
-        if (!leads(id, s, adapter)) continue;
+    const int64_t row0 = (int64_t)blockIdx.x * (16 * RW);
+    const int32_t steps = (int32_t)((a.inputs + kFragStep<T> - 1) / kFragStep<T>), whole = (int32_t)(a.inputs / kFragStep<T>);
+    const int32_t per = (steps + a.splits * kDownWaves - 1) / (a.splits * kDownWaves);
+    const int32_t from = ((int32_t)blockIdx.y * kDownWaves + wave) * per, to = from + per < steps ? from + per : steps, to_whole = to < whole ? to : whole;
+    const T *x[RW];
+#pragma unroll
+    for (int i = 0; i < RW; i++) {
+        const int64_t row = row0 + 16 * i + col;
+        x[i] = a.x + (row < a.rows ? row : a.rows - 1) * a.x_stride + quarter * kFragRun<T>;
+    }
+    for (Occurring at(a, row0, 16 * RW, blockIdx.z, gridDim.z); at.any(); at.next()) {
+        const int32_t adapter = at.now();
         for (int t0 = 0; t0 < a.padded; t0 += 16 * RT) {
             const T *down[RT];
-            acc4_t acc[RT];
+            acc4_t acc[RW][RT];
 #pragma unroll
             for (int t = 0; t < RT; t++) {
                 const int r = t0 + 16 * t + col;
                 down[t] = a.down + ((int64_t)adapter * a.rank + (r < a.rank ? r : a.rank - 1)) * a.inputs + quarter * kFragRun<T>;
-                acc[t] = acc4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            }
-#pragma unroll 4
-            for (int64_t k = from; k < to_whole; k++) {
-                const uint4 xf = load_run(x + k * kFragStep<T>);
 #pragma unroll
-                for (int t = 0; t < RT; t++) acc[t] = product16<T>(load_run(down[t] + k * kFragStep<T>), xf, acc[t]);
+                for (int i = 0; i < RW; i++) acc[i][t] = acc4_t{0.0f, 0.0f, 0.0f, 0.0f};
             }
+            auto some = [&](int32_t k, auto count) __attribute__((always_inline)) {  // that many steps' loads under way at a time
+                constexpr int U = decltype(count)::value;
+                uint4 xf[U][RW], df[U][RT];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+#pragma unroll
+                    for (int i = 0; i < RW; i++) xf[u][i] = load_run(x[i] + (int64_t)(k + u) * kFragStep<T>);
+#pragma unroll
+                    for (int t = 0; t < RT; t++) df[u][t] = load_run(down[t] + (int64_t)(k + u) * kFragStep<T>);
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int t = 0; t < RT; t++)
+#pragma unroll
+                        for (int i = 0; i < RW; i++) acc[i][t] = product16<T>(df[u][t], xf[u][i], acc[i][t]);
+            };
+            int32_t k = from;
+            for (; k + 4 <= to_whole; k += 4) some(k, Count<4>{});
+            for (; k < to_whole; k++) some(k, Count<1>{});
             if (from < to && to > whole) {  // the last, ragged step
-                const int64_t at = whole * kFragStep<T>, left = a.inputs - at - quarter * kFragRun<T>;
-                const uint4 xf = load_run(x + at, left);
+                const int64_t k = (int64_t)whole * kFragStep<T>, left = a.inputs - k - quarter * kFragRun<T>;
 #pragma unroll
-                for (int t = 0; t < RT; t++) acc[t] = product16<T>(load_run(down[t] + at, left), xf, acc[t]);
+                for (int i = 0; i < RW; i++) {
+                    const uint4 xf = load_run(x[i] + k, left);
+#pragma unroll
+                    for (int t = 0; t < RT; t++) acc[i][t] = product16<T>(load_run(down[t] + k, left), xf, acc[i][t]);
+                }
             }
 #pragma unroll
-            for (int t = 0; t < RT; t++) shares[wave][t][lane] = acc[t];
-            __syncthreads();
-            for (int t = wave; t < RT; t += kAdapterWaves) {
-                const int r = t0 + 16 * t + 4 * quarter;
-                acc4_t sum = shares[0][t][lane];
+            for (int i = 0; i < RW; i++)
 #pragma unroll
-                for (int w = 1; w < kAdapterWaves; w++) sum += shares[w][t][lane];
+                for (int t = 0; t < RT; t++) shares[wave][i * RT + t][lane] = acc[i][t];
+            __syncthreads();
+            for (int s = wave; s < RW * RT; s += kDownWaves) {
+                const int tile = s / RT, r = t0 + 16 * (s % RT) + 4 * quarter;
+                acc4_t sum = shares[0][s][lane];
+#pragma unroll
+                for (int w = 1; w < kDownWaves; w++) sum += shares[w][s][lane];
 #pragma unroll
                 for (int i = 0; i < 4; i++) sum[i] = r + i < a.rank ? sum[i] : 0.0f;
-                if (id == adapter && r < a.padded) *reinterpret_cast<acc4_t *>(a.low + (blockIdx.y * a.rows + row) * a.padded + r) = sum;
+                const int64_t row = row0 + 16 * tile + col;
+                if (at.of(16 * tile + col) == adapter && r < a.padded) *reinterpret_cast<acc4_t *>(a.low + (blockIdx.y * a.rows + row) * a.padded + r) = sum;
             }
             __syncthreads();
         }
     }
 }
 
-// 16 consecutive values of a row, of which `left` lie in it.
+// Eight consecutive values of a row, of which `left` lie in it.
 template <typename T>
-__device__ __forceinline__ void load_sixteen(const T *p, int64_t left, float (&v)[16]) {
-    if (left >= 16) {
-        struct __attribute__((packed)) Run { T t[16]; };
-        const Run run = *reinterpret_cast<const Run *>(p);
+struct __attribute__((packed)) Eight {
+    T t[8];
+};
+template <typename T>
+__device__ __forceinline__ void load_eight(const T *p, int64_t left, float *v) {
+    if (left >= 8) {
+        const Eight<T> e = *reinterpret_cast<const Eight<T> *>(p);
 #pragma unroll
-        for (int i = 0; i < 16; i++) v[i] = Elem<T>::load(run.t, i);
+        for (int i = 0; i < 8; i++) v[i] = Elem<T>::load(e.t, i);
     } else {
 #pragma unroll
-        for (int i = 0; i < 16; i++) v[i] = i < left ? Elem<T>::load(p, i) : 0.0f;
+        for (int i = 0; i < 8; i++) v[i] = i < left ? Elem<T>::load(p, i) : 0.0f;
     }
 }
 template <typename T>
-__device__ __forceinline__ void store_sixteen(T *p, int64_t left, const float (&v)[16]) {
-    if (left >= 16) {
-        struct __attribute__((packed)) Run { T t[16]; };
-        Run run;
+__device__ __forceinline__ void store_eight(T *p, int64_t left, const float *v) {
+    if (left >= 8) {
+        Eight<T> e;
 #pragma unroll
-        for (int i = 0; i < 16; i++) Elem<T>::store(run.t, i, v[i]);
-        *reinterpret_cast<Run *>(p) = run;
+        for (int i = 0; i < 8; i++) Elem<T>::store(e.t, i, v[i]);
+        *reinterpret_cast<Eight<T> *>(p) = e;
     } else {
 #pragma unroll
-        for (int i = 0; i < 16; i++)
+        for (int i = 0; i < 8; i++)
             if (i < left) Elem<T>::store(p, i, v[i]);
     }
 }
 
-// A lane's share of 16 ranks of t as an operand: float32, ranks 4 quarter .. + 3; else the terms of ranks 8 (quarter % 2) .. + 7, the high ones in
-// the first two quarters and the low ones in the others.
-template <typename T> constexpr int kLowRun = sizeof(T) == 4 ? 4 : 8;
+// The rows' own t as operands of 16 ranks, a kilobyte a tile of rows and block of ranks.  float32: lane (row, quarter) holds ranks 4 quarter .. + 3; else the terms
+// of ranks 8 (quarter % 2) .. + 7, the high ones in the first two quarters and the low ones in the others.  Eight ranks of a row are a thread's at a time.  (Of a
+// row without an adapter they are whatever the workspace holds, and are not used.)
 template <typename T>
-__device__ __forceinline__ uint4 low_terms(const float (&t)[kLowRun<T>], bool low) {
+__device__ __forceinline__ void put_terms(uint4 *block, int row, int run, const float (&t)[8]) {
     if constexpr (sizeof(T) == 4) {
-        return make_uint4(f2u(t[0]), f2u(t[1]), f2u(t[2]), f2u(t[3]));
+        block[row + 32 * run] = make_uint4(f2u(t[0]), f2u(t[1]), f2u(t[2]), f2u(t[3]));
+        block[row + 32 * run + 16] = make_uint4(f2u(t[4]), f2u(t[5]), f2u(t[6]), f2u(t[7]));
     } else {
-        T terms[8];
+        T high[8], low[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float high = rounded<T>(t[j]), rest = fabsf(high) < INFINITY ? t[j] - high : 0.0f;  // (what has no finite high term has no low one)
-            Elem<T>::store(terms, j, low ? rest : high);
+            const float h = rounded<T>(t[j]);
+            Elem<T>::store(high, j, h);
+            Elem<T>::store(low, j, fabsf(h) < INFINITY ? t[j] - h : 0.0f);  // (what has no finite high term has no low one)
         }
-        uint4 w;
-        __builtin_memcpy(&w, terms, 16);
-        return w;
+        __builtin_memcpy(&block[row + 16 * run], high, 16);
+        __builtin_memcpy(&block[row + 16 * (run + 2)], low, 16);
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(64 * kAdapterWaves) adapters_up_kernel(const AdapterArgs<T> a) {
-    constexpr int R = kLowRun<T>;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, quarter = lane >> 4;
-    const int64_t row = (int64_t)blockIdx.x * kTileRows + col;
-    const int64_t n0 = ((int64_t)blockIdx.y * kAdapterWaves + wave) * kWaveColumns;
-    if (n0 >= a.outputs) return;
-    const int32_t id = adapter_of(a, row);
-    const int rank0 = sizeof(T) == 4 ? 4 * quarter : 8 * (quarter & 1);
-    // Tile c of the columns: line m of the operand is column 16 (m / 4) + 4 c + m % 4, so that a lane's four accumulators are 16 consecutive ones.
-    int64_t column[4];
+// RW tiles of 16 rows.  The products' tile goes through LDS, so that y and out are read and written in runs of 512 bytes a row.
+template <typename T, int RW>
+__global__ void __launch_bounds__(64 * kUpWaves, RW == 2 ? 3 : 4) adapters_up_kernel(const AdapterArgs<T> a) {
+    constexpr bool kScaled = Elem<T>::code == NVQ_F16;
+    extern __shared__ uint4 terms[];  // [RW][padded / 16][64]
+    __shared__ float sums[16 * RW][kBlockColumns + 4];
+    __shared__ uint32_t largest[16 * RW];  // float16: of a row's t, its bits
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quarter = lane >> 4;
+    const int64_t row0 = (int64_t)blockIdx.x * (16 * RW);
+    const Occurring occurring(a, row0, 16 * RW, blockIdx.z, gridDim.z);
+    const int blocks = a.padded / 16;
+    // The rows that this block writes, a bit each: those of its adapters, and the first block's without one.
+    const uint64_t bare = blockIdx.z == 0 ? __ballot(occurring.id < 0 && lane < 16 * RW && row0 + lane < a.rows) : 0;
+    uint64_t mine = bare;
+    for (Occurring at = occurring; at.any(); at.next()) mine |= __ballot(occurring.id == at.now());
+    if (mine == 0) return;
+    // y of 256 columns: eight rows at a time, eight values a thread, requested before the columns in front of them are worked on.
+    const int y_row = tid >> 5, y_col = 8 * (tid & 31);
+    Eight<T> ahead[2 * RW];
+    auto request = [&](int64_t n0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-        const int64_t n = n0 + 16 * (col >> 2) + 4 * c + (col & 3);
-        column[c] = n < a.outputs ? n : a.outputs - 1;
+        for (int i = 0; i < 2 * RW; i++) {
+            const int64_t r = row0 + 8 * i + y_row;
+            ahead[i] = *reinterpret_cast<const Eight<T> *>(a.y + (r < a.rows ? r : a.rows - 1) * a.y_stride + n0 + y_col);
+        }
+    };
+    const int64_t n_first = (int64_t)blockIdx.y * a.chunks * kBlockColumns, n_most = n_first + a.chunks * kBlockColumns, n_end = n_most < a.outputs ? n_most : a.outputs;
+    const int64_t n_whole = n_first + (n_end - n_first) / kBlockColumns * kBlockColumns;
+    if (n_first < n_whole) request(n_first);
+
+    // ── the terms ──
+    auto low_at = [&](int r, int run, float (&t)[8]) __attribute__((always_inline)) {
+        const int64_t row = row0 + r < a.rows ? row0 + r : a.rows - 1, split = a.rows * a.padded;
+        const float *p = a.low + row * a.padded + 8 * run;
+        const int32_t id = a.ids[row];
+        const float scale = a.scales != nullptr && id >= 0 && id < a.adapters ? a.scales[id] : 1.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) t[j] = 0.0f;
+        for (int z = 0; z < a.splits; z += 4) {  // (four splits' loads under way at a time)
+            acc4_t v[4][2];
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) v[s][j] = *reinterpret_cast<const acc4_t *>(p + (z + s < a.splits ? z + s : z) * split + 4 * j);
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) t[j] += z + s < a.splits ? v[s][j >> 2][j & 3] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) t[j] *= scale;
+    };
+    const int runs = 2 * blocks, all = 16 * RW * runs;
+    if constexpr (kScaled) {  // a row's t is scaled by a power of two, so that its largest is between 1 and 2
+        if (tid < 16 * RW) largest[tid] = 0u;
+        __syncthreads();
+        for (int i = tid; i < all; i += 64 * kUpWaves) {
+            float t[8], top = 0.0f;
+            low_at(i % (16 * RW), i / (16 * RW), t);
+#pragma unroll
+            for (int j = 0; j < 8; j++) top = fabsf(t[j]) < INFINITY ? fmaxf(top, fabsf(t[j])) : top;
+            atomicMax(&largest[i % (16 * RW)], f2u(top));
+        }
+        __syncthreads();
     }
-    bool mine = id < 0 && blockIdx.z == 0;  // (a row without an adapter: y as it is)
-    float sum[16];
+    auto exponent_of = [&](int r) __attribute__((always_inline)) { return largest[r] != 0u ? ilogbf(u2f(largest[r])) : 0; };
+    for (int i = tid; i < all; i += 64 * kUpWaves) {
+        const int r = i % (16 * RW), run = i / (16 * RW);
+        float t[8];
+        low_at(r, run, t);
+        if constexpr (kScaled) {
+            const int e = exponent_of(r);
 #pragma unroll
-    for (int i = 0; i < 16; i++) sum[i] = 0.0f;
-    for (int s = blockIdx.z * a.slots; s < (int)(blockIdx.z + 1) * a.slots; s++) {
-        int32_t adapter;
-        if (!leads(id, s, adapter)) continue;
-        const bool match = id == adapter;
-        const float scale = a.scales == nullptr ? 1.0f : a.scales[adapter];
-        const float *low = a.low + (match ? row : (int64_t)blockIdx.x * kTileRows + s) * a.padded + rank0;  // (a row that has been written)
-        auto low_at = [&](int b, float (&t)[R]) __attribute__((always_inline)) {
-#pragma unroll
-            for (int j = 0; j < R; j++) t[j] = 0.0f;
-            for (int z = 0; z < a.splits; z++) {
-                const float *p = low + z * a.rows * a.padded + 16 * b;
-#pragma unroll
-                for (int j = 0; j < R; j += 4) {
-                    const acc4_t v = *reinterpret_cast<const acc4_t *>(p + j);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) t[j + i] += v[i];
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < R; j++) t[j] *= scale;
-        };
-        int exponent = 0;  // of the row's largest t, taken out of float16's terms
-        if constexpr (Elem<T>::code == NVQ_F16) {
-            float top = 0.0f;
-            for (int b = 0; b < a.padded / 16; b++) {
-                float t[R];
-                low_at(b, t);
-#pragma unroll
-                for (int j = 0; j < R; j++) top = fabsf(t[j]) < INFINITY ? fmaxf(top, fabsf(t[j])) : top;
-            }
-            top = fmaxf(top, __shfl_xor(top, 16));
-            exponent = top > 0.0f ? ilogbf(top) : 0;
+            for (int j = 0; j < 8; j++) t[j] = ldexpf(t[j], -e);
         }
-        acc4_t acc[4];
-#pragma unroll
-        for (int c = 0; c < 4; c++) acc[c] = acc4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        const T *up = a.up + (int64_t)adapter * a.outputs * a.rank + rank0;
-        for (int b = 0; b < a.padded / 16; b++) {
-            float t[R];
-            low_at(b, t);
-            if constexpr (Elem<T>::code == NVQ_F16)
-#pragma unroll
-                for (int j = 0; j < R; j++) t[j] = ldexpf(t[j], -exponent);
-            const uint4 tf = low_terms<T>(t, quarter >= 2);
-#pragma unroll
-            for (int c = 0; c < 4; c++) acc[c] = product16<T>(load_run(up + column[c] * a.rank + 16 * b, (int64_t)a.rank - 16 * b - rank0), tf, acc[c]);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            float v = acc[i >> 2][i & 3];
-            if constexpr (Elem<T>::code == NVQ_F16) v = ldexpf(v, exponent);
-            sum[i] = match ? v : sum[i];
-        }
-        mine |= match;
+        put_terms<T>(terms + ((r >> 4) * blocks + (run >> 1)) * 64, r & 15, run & 1, t);
     }
-    const int64_t n = n0 + 16 * quarter, left = a.outputs - n;
-    if (!mine || row >= a.rows || left <= 0) return;
-    float v[16];
-    load_sixteen(a.y + row * a.y_stride + n, left, v);
+    int32_t id[RW];
+    int exponent[RW] = {};
 #pragma unroll
-    for (int i = 0; i < 16; i++) v[i] += sum[i];
-    store_sixteen(a.out + row * a.out_stride + n, left, v);
+    for (int i = 0; i < RW; i++) id[i] = occurring.of(16 * i + col);
+    __syncthreads();
+    if constexpr (kScaled)
+#pragma unroll
+        for (int i = 0; i < RW; i++) exponent[i] = exponent_of(16 * i + col);
+
+    // ── the products ──
+    // Tile c of a wavefront's 64 columns: line m of the operand is column 32 (c / 2) + 8 (m / 4) + 4 (c % 2) + m % 4.
+    const int line = 8 * (col >> 2) + (col & 3), rank0 = sizeof(T) == 4 ? 4 * quarter : 8 * (quarter & 1);
+    const uint32_t from_line = (uint32_t)(line * a.rank + rank0) * (uint32_t)sizeof(T);
+    // From column n0 on.  WHOLE: they and the runs of ranks are whole, so that no load stands under a condition.
+    auto products = [&](int64_t n0, auto whole) __attribute__((always_inline)) {
+        constexpr bool WHOLE = decltype(whole)::value != 0;
+        for (Occurring at = occurring; at.any(); at.next()) {
+            const int32_t adapter = at.now();
+            const T *up = a.up + ((int64_t)adapter * a.outputs + n0) * a.rank;
+            acc4_t acc[RW][4];
+#pragma unroll
+            for (int i = 0; i < RW; i++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) acc[i][c] = acc4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            auto some = [&](int b0, auto count) __attribute__((always_inline)) {
+                constexpr int U = decltype(count)::value;
+                uint4 w[U][4];
+#pragma unroll
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const int shift = 32 * (c >> 1) + 4 * (c & 1), r = 16 * (b0 + u);
+                        const bool in = r + rank0 < a.rank;
+                        if constexpr (WHOLE) {
+                            const T *p = reinterpret_cast<const T *>(reinterpret_cast<const uint8_t *>(up + shift * a.rank + r) + from_line);
+                            const uint4 v = load_run(in ? p : p - rank0);  // (ranks behind the last: read again, not used)
+                            const uint32_t k = in ? ~0u : 0u;
+                            w[u][c] = make_uint4(v.x & k, v.y & k, v.z & k, v.w & k);
+                        } else {
+                            const int64_t n = n0 + shift + line;
+                            w[u][c] = load_run(a.up + ((int64_t)adapter * a.outputs + (n < a.outputs ? n : a.outputs - 1)) * a.rank + (in ? r + rank0 : 0), (int64_t)a.rank - r - rank0);
+                        }
+                    }
+#pragma unroll
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int i = 0; i < RW; i++) {
+                        const uint4 t = terms[(i * blocks + b0 + u) * 64 + lane];
+#pragma unroll
+                        for (int c = 0; c < 4; c++) acc[i][c] = product16<T>(w[u][c], t, acc[i][c]);
+                    }
+            };
+            int b = 0;
+            for (; b + 2 <= blocks; b += 2) some(b, Count<2>{});
+            if (b < blocks) some(b, Count<1>{});
+#pragma unroll
+            for (int i = 0; i < RW; i++) {
+                if constexpr (kScaled)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[i][c][e] = ldexpf(acc[i][c][e], exponent[i]);
+                if (id[i] == adapter)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        *reinterpret_cast<acc4_t *>(&sums[16 * i + col][64 * wave + 32 * (c >> 1) + 8 * quarter + 4 * (c & 1)]) = acc[i][c];
+            }
+        }
+    };
+    const bool whole_ranks = a.rank % kFragRun<T> == 0;
+    for (int64_t n0 = n_first; n0 < n_end; n0 += kBlockColumns) {
+        const int64_t from = n0 + 64 * wave;
+        if (whole_ranks && from + 64 <= a.outputs) products(from, Count<1>{});
+        else if (from < a.outputs) products(from, Count<0>{});
+        __syncthreads();
+        const bool whole = n0 < n_whole;
+#pragma unroll
+        for (int i = 0; i < 2 * RW; i++) {
+            const int r = 8 * i + y_row;
+            const int64_t n = n0 + y_col, left = a.outputs - n;
+            float v[8];
+            if (whole) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = Elem<T>::load(ahead[i].t, e);
+            }
+            if ((mine >> r & 1) == 0) continue;
+            if (!whole) load_eight(a.y + (row0 + r) * a.y_stride + (left > 0 ? n : 0), left, v);
+            if ((bare >> r & 1) == 0) {
+                const acc4_t s0 = *reinterpret_cast<const acc4_t *>(&sums[r][y_col]), s1 = *reinterpret_cast<const acc4_t *>(&sums[r][y_col + 4]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] += s0[e], v[4 + e] += s1[e];
+            }
+            store_eight(a.out + (row0 + r) * a.out_stride + n, whole ? 8 : left, v);
+        }
+        if (whole) request(n0 + kBlockColumns < n_whole ? n0 + kBlockColumns : n0);
+        __syncthreads();
+    }
 }
 
+// How the rows, columns and the contraction are dealt to blocks.
+struct Shape {
+    int32_t wide;          // tiles of 16 rows of a block: 2 where there are many rows, so that the adapters' weights are read half as often
+    int32_t splits, down_slots, up_slots, chunks;
+    int64_t tiles;
+};
+int64_t at_most(int64_t v, int64_t most) { return v < 1 ? 1 : v < most ? v : most; }
+Shape shape_of(const nvq_adapters_desc &d) {
+    Shape s{};
+    const int64_t cus = compute_units();
+    s.wide = d.rows >= 32 * cus / 4 ? 2 : 1;
+    s.tiles = (d.rows + 16 * s.wide - 1) / (16 * s.wide);
+    const int64_t most = d.adapters < 16 * s.wide ? d.adapters : 16 * s.wide, occurring = at_most(most < d.rows ? most : d.rows, 32);
+    const int64_t step = d.dtype == NVQ_F32 ? 16 : 32, steps = (d.inputs + step - 1) / step;
+    // A tile's adapters go to blocks of their own where the tiles alone leave compute units without work, and the contraction is split, four steps a
+    // wavefront at least.
+    s.down_slots = (int32_t)at_most(cus / s.tiles, occurring);
+    s.splits = (int32_t)at_most(2 * cus / (s.tiles * s.down_slots), at_most(steps / (4 * kDownWaves), 16));
+    const int64_t columns = (d.outputs + kBlockColumns - 1) / kBlockColumns;
+    s.up_slots = (int32_t)at_most(4 * cus / (s.tiles * columns), occurring);
+    s.chunks = (int32_t)at_most(s.tiles * columns * s.up_slots / (4 * cus), 4);
+    return s;
+}
 int32_t padded_rank(const nvq_adapters_desc &d) { return (d.rank + 15) / 16 * 16; }
 
-// A tile's adapters go to blocks of their own where the tiles alone leave compute units without work.
-int32_t slots_of_block(const nvq_adapters_desc &d) {
-    const int64_t tiles = (d.rows + kTileRows - 1) / kTileRows;
-    return tiles * kTileRows <= 4 * (int64_t)compute_units() ? 1 : kTileRows;
-}
-int32_t splits_of(const nvq_adapters_desc &d) {
-    const int64_t tiles = (d.rows + kTileRows - 1) / kTileRows, step = d.dtype == NVQ_F32 ? 16 : 32;
-    const int64_t steps = (d.inputs + step - 1) / step, most = steps / (4 * kAdapterWaves);  // (four steps a wavefront at least)
-    const int64_t blocks = slots_of_block(d) == 1 ? (d.rows < kTileRows ? d.rows : d.rows) : tiles;
-    const int64_t want = (4 * (int64_t)compute_units() + blocks - 1) / blocks;
-    const int64_t splits = want < most ? want : most;
-    return (int32_t)(splits < 1 ? 1 : splits < 16 ? splits : 16);
+template <typename T, int RW>
+int32_t run_sized(const AdapterArgs<T> &a, const Shape &shape, hipStream_t s) {
+    const dim3 grid((unsigned)shape.tiles, (unsigned)shape.splits, (unsigned)shape.down_slots), block(64 * kDownWaves);
+    if (a.padded <= 16) hipLaunchKernelGGL((adapters_down_kernel<T, RW, 1>), grid, block, 0, s, a);
+    else if (a.padded <= 32) hipLaunchKernelGGL((adapters_down_kernel<T, RW, 2>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((adapters_down_kernel<T, RW, 4>), grid, block, 0, s, a);
+    NVQ_LAUNCH_CHECK("apply_adapters");
+    const int64_t columns = kBlockColumns * (int64_t)shape.chunks;
+    const dim3 wide((unsigned)shape.tiles, (unsigned)((a.outputs + columns - 1) / columns), (unsigned)shape.up_slots);
+    hipLaunchKernelGGL((adapters_up_kernel<T, RW>), wide, dim3(64 * kUpWaves), (size_t)RW * (a.padded / 16) * 64 * sizeof(uint4), s, a);
+    NVQ_LAUNCH_CHECK("apply_adapters");
+    return NVQ_OK;
 }
 
 template <typename T>
 int32_t run_adapters(const nvq_adapters_desc &d, const void *x, const void *down, const void *up, const float *scales, const int32_t *ids, const void *y,
                      void *out, void *workspace, hipStream_t s) {
+    const Shape shape = shape_of(d);
     AdapterArgs<T> a{};
     a.x = (const T *)x, a.down = (const T *)down, a.up = (const T *)up, a.y = (const T *)y, a.scales = scales, a.ids = ids, a.out = (T *)out;
     a.low = (float *)workspace, a.rows = d.rows, a.inputs = d.inputs, a.outputs = d.outputs;
     a.x_stride = d.x_stride, a.y_stride = d.y_stride, a.out_stride = d.out_stride;
-    a.adapters = (int32_t)d.adapters, a.rank = d.rank, a.padded = padded_rank(d), a.splits = splits_of(d), a.slots = slots_of_block(d);
-    const unsigned tiles = (unsigned)((d.rows + kTileRows - 1) / kTileRows);
-    const unsigned slots = a.slots == 1 ? (unsigned)(d.rows < kTileRows ? d.rows : kTileRows) : 1;
-    const dim3 block(64 * kAdapterWaves), grid(tiles, (unsigned)a.splits, slots);
-    if (a.padded <= 16) hipLaunchKernelGGL((adapters_down_kernel<T, 1>), grid, block, 0, s, a);
-    else if (a.padded <= 32) hipLaunchKernelGGL((adapters_down_kernel<T, 2>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((adapters_down_kernel<T, 4>), grid, block, 0, s, a);
-    NVQ_LAUNCH_CHECK("apply_adapters");
-    const dim3 wide(tiles, (unsigned)((d.outputs + kAdapterWaves * kWaveColumns - 1) / (kAdapterWaves * kWaveColumns)), slots);
-    hipLaunchKernelGGL((adapters_up_kernel<T>), wide, block, 0, s, a);
-    NVQ_LAUNCH_CHECK("apply_adapters");
-    return NVQ_OK;
+    a.adapters = (int32_t)d.adapters, a.rank = d.rank, a.padded = padded_rank(d), a.splits = shape.splits, a.chunks = shape.chunks;
+    return shape.wide == 2 ? run_sized<T, 2>(a, shape, s) : run_sized<T, 1>(a, shape, s);
 }
 
 }  // namespace
 
-size_t adapters_workspace_bytes(const nvq_adapters_desc &d) { return (size_t)splits_of(d) * (size_t)d.rows * (size_t)padded_rank(d) * sizeof(float); }
+size_t adapters_workspace_bytes(const nvq_adapters_desc &d) { return (size_t)shape_of(d).splits * (size_t)d.rows * (size_t)padded_rank(d) * sizeof(float); }
 
 int32_t launch_adapters(const nvq_adapters_desc &d, const void *x, const void *down, const void *up, const float *scales, const int32_t *ids, const void *y,
                         void *out, void *workspace, hipStream_t s) {
