@@ -73,6 +73,13 @@ __global__ void __launch_bounds__(64 * kDownWaves) adapters_down_kernel(const Ad
         const int64_t row = row0 + 16 * i + col;
         x[i] = a.x + (row < a.rows ? row : a.rows - 1) * a.x_stride + quarter * kFragRun<T>;
     }
+    uint4 ahead[4][RW];  // of x, the first four steps, requested before the rows' adapters are known
+    const bool four = from + 4 <= to_whole;
+    if (four)
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int i = 0; i < RW; i++) ahead[u][i] = load_run(x[i] + (int64_t)(from + u) * kFragStep<T>);
     for (Occurring at(a, row0, 16 * RW, blockIdx.z, gridDim.z); at.any(); at.next()) {
         const int32_t adapter = at.now();
         for (int t0 = 0; t0 < a.padded; t0 += 16 * RT) {
@@ -85,13 +92,13 @@ __global__ void __launch_bounds__(64 * kDownWaves) adapters_down_kernel(const Ad
 #pragma unroll
                 for (int i = 0; i < RW; i++) acc[i][t] = acc4_t{0.0f, 0.0f, 0.0f, 0.0f};
             }
-            auto some = [&](int32_t k, auto count) __attribute__((always_inline)) {  // that many steps' loads under way at a time
+            auto some = [&](int32_t k, auto count, bool first) __attribute__((always_inline)) {  // that many steps' loads under way at a time
                 constexpr int U = decltype(count)::value;
                 uint4 xf[U][RW], df[U][RT];
 #pragma unroll
                 for (int u = 0; u < U; u++) {
 #pragma unroll
-                    for (int i = 0; i < RW; i++) xf[u][i] = load_run(x[i] + (int64_t)(k + u) * kFragStep<T>);
+                    for (int i = 0; i < RW; i++) xf[u][i] = first ? ahead[u][i] : load_run(x[i] + (int64_t)(k + u) * kFragStep<T>);
 #pragma unroll
                     for (int t = 0; t < RT; t++) df[u][t] = load_run(down[t] + (int64_t)(k + u) * kFragStep<T>);
                 }
@@ -103,8 +110,9 @@ __global__ void __launch_bounds__(64 * kDownWaves) adapters_down_kernel(const Ad
                         for (int i = 0; i < RW; i++) acc[i][t] = product16<T>(df[u][t], xf[u][i], acc[i][t]);
             };
             int32_t k = from;
-            for (; k + 4 <= to_whole; k += 4) some(k, Count<4>{});
-            for (; k < to_whole; k++) some(k, Count<1>{});
+            if (four) some(k, Count<4>{}, true), k += 4;
+            for (; k + 4 <= to_whole; k += 4) some(k, Count<4>{}, false);
+            for (; k < to_whole; k++) some(k, Count<1>{}, false);
             if (from < to && to > whole) {  // the last, ragged step
                 const int64_t k = (int64_t)whole * kFragStep<T>, left = a.inputs - k - quarter * kFragRun<T>;
 #pragma unroll
@@ -164,14 +172,26 @@ __device__ __forceinline__ void store_eight(T *p, int64_t left, const float *v) 
     }
 }
 
-// The rows' own t as operands of 16 ranks, a kilobyte a tile of rows and block of ranks.  float32: lane (row, quarter) holds ranks 4 quarter .. + 3; else the terms
-// of ranks 8 (quarter % 2) .. + 7, the high ones in the first two quarters and the low ones in the others.  Eight ranks of a row are a thread's at a time.  (Of a
-// row without an adapter they are whatever the workspace holds, and are not used.)
+// Runs of ranks, as long as a lane's 16 bytes of up.  The last one of a rank that is no whole number of them begins as much earlier, so that it is read as the
+// others are; what it has in common with the one in front of it is taken for zeros, of t and of up.  (Ranks shorter than a run are read value by value.)
+struct RankRun {
+    int from, skip;  // the first rank; how many of the run are not its own
+    bool any;
+};
 template <typename T>
-__device__ __forceinline__ void put_terms(uint4 *block, int row, int run, const float (&t)[8]) {
+__device__ __forceinline__ RankRun rank_run(int rank, int run) {
+    constexpr int L = kFragRun<T>;
+    const int first = L * run, last = rank > L ? rank - L : 0;
+    return RankRun{first < last ? first : last, first < last ? 0 : first - last, first < rank};
+}
+
+// The rows' own t as operands of 16 ranks, a kilobyte a tile of rows and block of ranks.  float32: lane (row, quarter) holds the block's run `quarter`; else
+// the terms of its run quarter % 2, the high ones in the first two quarters and the low ones in the others.  (Of a row without an adapter they are whatever
+// the workspace holds, and are not used.)
+template <typename T>
+__device__ __forceinline__ void put_terms(uint4 *block, int row, int run, const float (&t)[kFragRun<T>]) {
     if constexpr (sizeof(T) == 4) {
-        block[row + 32 * run] = make_uint4(f2u(t[0]), f2u(t[1]), f2u(t[2]), f2u(t[3]));
-        block[row + 32 * run + 16] = make_uint4(f2u(t[4]), f2u(t[5]), f2u(t[6]), f2u(t[7]));
+        block[row + 16 * run] = make_uint4(f2u(t[0]), f2u(t[1]), f2u(t[2]), f2u(t[3]));
     } else {
         T high[8], low[8];
 #pragma unroll
@@ -194,8 +214,9 @@ __global__ void __launch_bounds__(64 * kUpWaves, RW == 2 ? 3 : 4) adapters_up_ke
     __shared__ uint32_t largest[16 * RW];  // float16: of a row's t, its bits
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quarter = lane >> 4;
     const int64_t row0 = (int64_t)blockIdx.x * (16 * RW);
-    const Occurring occurring(a, row0, 16 * RW, blockIdx.z, gridDim.z);
     const int blocks = a.padded / 16;
+    constexpr int L = kFragRun<T>, kRuns = 16 / L;  // runs of a block of ranks
+    const Occurring occurring(a, row0, 16 * RW, blockIdx.z, gridDim.z);
     // The rows that this block writes, a bit each: those of its adapters, and the first block's without one.
     const uint64_t bare = blockIdx.z == 0 ? __ballot(occurring.id < 0 && lane < 16 * RW && row0 + lane < a.rows) : 0;
     uint64_t mine = bare;
@@ -215,53 +236,93 @@ __global__ void __launch_bounds__(64 * kUpWaves, RW == 2 ? 3 : 4) adapters_up_ke
     const int64_t n_whole = n_first + (n_end - n_first) / kBlockColumns * kBlockColumns;
     if (n_first < n_whole) request(n_first);
 
-    // ── the terms ──
-    auto low_at = [&](int r, int run, float (&t)[8]) __attribute__((always_inline)) {
-        const int64_t row = row0 + r < a.rows ? row0 + r : a.rows - 1, split = a.rows * a.padded;
-        const float *p = a.low + row * a.padded + 8 * run;
-        const int32_t id = a.ids[row];
-        const float scale = a.scales != nullptr && id >= 0 && id < a.adapters ? a.scales[id] : 1.0f;
+    // ── the weights ──
+    // Tile c of a wavefront's 64 columns: line m of the operand is column 32 (c / 2) + 8 (m / 4) + 4 (c % 2) + m % 4.
+    const int line = 8 * (col >> 2) + (col & 3), run0 = sizeof(T) == 4 ? quarter : quarter & 1;
+    const RankRun last_run = rank_run<T>(a.rank, kRuns * (blocks - 1) + run0);
+    uint32_t last_kept[4];  // what is its own of the last block's run
 #pragma unroll
-        for (int j = 0; j < 8; j++) t[j] = 0.0f;
-        for (int z = 0; z < a.splits; z += 4) {  // (four splits' loads under way at a time)
-            acc4_t v[4][2];
+    for (int j = 0; j < 4; j++) {
+        const uint32_t low = last_run.any && (sizeof(T) == 4 ? j : 2 * j) >= last_run.skip ? (sizeof(T) == 4 ? ~0u : 0xFFFFu) : 0u;
+        last_kept[j] = sizeof(T) == 4 ? low : low | (last_run.any && 2 * j + 1 >= last_run.skip ? 0xFFFF0000u : 0u);
+    }
+    // Of an adapter, `U` blocks of ranks from b0 on, 64 columns from n0 on.  KIND 0: value by value; 1: they are whole and so are the runs, so that no load stands
+    // under a condition; 2: and so are the blocks of ranks.
+    auto weights = [&](int32_t adapter, int64_t n0, int b0, auto &w, auto kind) __attribute__((always_inline)) {
+        constexpr int KIND = decltype(kind)::value;
+        constexpr int U = sizeof(w) / sizeof(w[0]);
+        const T *up = a.up + ((int64_t)adapter * a.outputs + n0) * a.rank;
 #pragma unroll
-            for (int s = 0; s < 4; s++)
+        for (int u = 0; u < U; u++) {
+            const bool last = KIND < 2 && b0 + u == blocks - 1;
+            const int r = last ? last_run.from : 16 * (b0 + u) + L * run0;
 #pragma unroll
-                for (int j = 0; j < 2; j++) v[s][j] = *reinterpret_cast<const acc4_t *>(p + (z + s < a.splits ? z + s : z) * split + 4 * j);
-#pragma unroll
-            for (int s = 0; s < 4; s++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) t[j] += z + s < a.splits ? v[s][j >> 2][j & 3] : 0.0f;
+            for (int c = 0; c < 4; c++) {
+                const int shift = 32 * (c >> 1) + 4 * (c & 1);
+                if constexpr (KIND > 0) {
+                    const uint4 v = load_run(reinterpret_cast<const T *>(reinterpret_cast<const uint8_t *>(up + shift * a.rank) + (uint32_t)(line * a.rank + r) * (uint32_t)sizeof(T)));
+                    w[u][c] = last ? make_uint4(v.x & last_kept[0], v.y & last_kept[1], v.z & last_kept[2], v.w & last_kept[3]) : v;
+                } else {
+                    const int64_t n = n0 + shift + line;
+                    const uint4 v = load_run(a.up + ((int64_t)adapter * a.outputs + (n < a.outputs ? n : a.outputs - 1)) * a.rank + r, (int64_t)a.rank - r);
+                    w[u][c] = last ? make_uint4(v.x & last_kept[0], v.y & last_kept[1], v.z & last_kept[2], v.w & last_kept[3]) : v;
+                }
+            }
         }
-#pragma unroll
-        for (int j = 0; j < 8; j++) t[j] *= scale;
     };
-    const int runs = 2 * blocks, all = 16 * RW * runs;
+    // ── the terms: a thread's runs are all of one row ──
+    static_assert(64 * kUpWaves % (16 * RW) == 0);
+    const int runs = kRuns * blocks, my_row = tid % (16 * RW);
+    const int32_t my_id = occurring.of(my_row);
+    const float my_scale = a.scales != nullptr && my_id >= 0 ? a.scales[my_id] : 1.0f;
+    auto each = [&](auto f) __attribute__((always_inline)) {
+        const int64_t row = row0 + my_row < a.rows ? row0 + my_row : a.rows - 1, split = a.rows * a.padded;
+        for (int run = tid / (16 * RW); run < runs; run += 64 * kUpWaves / (16 * RW)) {
+            const RankRun of = rank_run<T>(a.rank, run);
+            const float *p = a.low + row * a.padded + of.from;
+            float t[L];
+#pragma unroll
+            for (int j = 0; j < L; j++) t[j] = 0.0f;
+            for (int z = 0; z < a.splits; z += 4) {  // (four splits' loads under way at a time)
+                uint4 v[4][L / 4];
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+#pragma unroll
+                    for (int j = 0; j < L / 4; j++) v[s][j] = load_run(p + (z + s < a.splits ? z + s : z) * split + 4 * j);
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+#pragma unroll
+                    for (int j = 0; j < L / 4; j++) {
+                        const float w[4] = {u2f(v[s][j].x), u2f(v[s][j].y), u2f(v[s][j].z), u2f(v[s][j].w)};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) t[4 * j + e] += z + s < a.splits ? w[e] : 0.0f;
+                    }
+            }
+#pragma unroll
+            for (int j = 0; j < L; j++) t[j] = of.any && j >= of.skip ? t[j] * my_scale : 0.0f;
+            f(run, t);
+        }
+    };
     if constexpr (kScaled) {  // a row's t is scaled by a power of two, so that its largest is between 1 and 2
         if (tid < 16 * RW) largest[tid] = 0u;
         __syncthreads();
-        for (int i = tid; i < all; i += 64 * kUpWaves) {
-            float t[8], top = 0.0f;
-            low_at(i % (16 * RW), i / (16 * RW), t);
+        each([&](int, const float (&t)[L]) __attribute__((always_inline)) {
+            float top = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; j++) top = fabsf(t[j]) < INFINITY ? fmaxf(top, fabsf(t[j])) : top;
-            atomicMax(&largest[i % (16 * RW)], f2u(top));
-        }
+            for (int j = 0; j < L; j++) top = fabsf(t[j]) < INFINITY ? fmaxf(top, fabsf(t[j])) : top;
+            atomicMax(&largest[my_row], f2u(top));
+        });
         __syncthreads();
     }
     auto exponent_of = [&](int r) __attribute__((always_inline)) { return largest[r] != 0u ? ilogbf(u2f(largest[r])) : 0; };
-    for (int i = tid; i < all; i += 64 * kUpWaves) {
-        const int r = i % (16 * RW), run = i / (16 * RW);
-        float t[8];
-        low_at(r, run, t);
+    each([&](int run, float (&t)[L]) __attribute__((always_inline)) {
         if constexpr (kScaled) {
-            const int e = exponent_of(r);
+            const int e = exponent_of(my_row);
 #pragma unroll
-            for (int j = 0; j < 8; j++) t[j] = ldexpf(t[j], -e);
+            for (int j = 0; j < L; j++) t[j] = ldexpf(t[j], -e);
         }
-        put_terms<T>(terms + ((r >> 4) * blocks + (run >> 1)) * 64, r & 15, run & 1, t);
-    }
+        put_terms<T>(terms + ((my_row >> 4) * blocks + run / kRuns) * 64, my_row & 15, run % kRuns, t);
+    });
     int32_t id[RW];
     int exponent[RW] = {};
 #pragma unroll
@@ -272,51 +333,33 @@ __global__ void __launch_bounds__(64 * kUpWaves, RW == 2 ? 3 : 4) adapters_up_ke
         for (int i = 0; i < RW; i++) exponent[i] = exponent_of(16 * i + col);
 
     // ── the products ──
-    // Tile c of a wavefront's 64 columns: line m of the operand is column 32 (c / 2) + 8 (m / 4) + 4 (c % 2) + m % 4.
-    const int line = 8 * (col >> 2) + (col & 3), rank0 = sizeof(T) == 4 ? 4 * quarter : 8 * (quarter & 1);
-    const uint32_t from_line = (uint32_t)(line * a.rank + rank0) * (uint32_t)sizeof(T);
-    // From column n0 on.  WHOLE: they and the runs of ranks are whole, so that no load stands under a condition.
-    auto products = [&](int64_t n0, auto whole) __attribute__((always_inline)) {
-        constexpr bool WHOLE = decltype(whole)::value != 0;
+    auto products = [&](int64_t n0, auto kind) __attribute__((always_inline)) {
         for (Occurring at = occurring; at.any(); at.next()) {
             const int32_t adapter = at.now();
-            const T *up = a.up + ((int64_t)adapter * a.outputs + n0) * a.rank;
             acc4_t acc[RW][4];
 #pragma unroll
             for (int i = 0; i < RW; i++)
 #pragma unroll
                 for (int c = 0; c < 4; c++) acc[i][c] = acc4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            auto some = [&](int b0, auto count) __attribute__((always_inline)) {
-                constexpr int U = decltype(count)::value;
-                uint4 w[U][4];
+            auto add = [&](int b, const uint4 (&w)[4]) __attribute__((always_inline)) {
 #pragma unroll
-                for (int u = 0; u < U; u++)
+                for (int i = 0; i < RW; i++) {
+                    const uint4 t = terms[(i * blocks + b) * 64 + lane];
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const int shift = 32 * (c >> 1) + 4 * (c & 1), r = 16 * (b0 + u);
-                        const bool in = r + rank0 < a.rank;
-                        if constexpr (WHOLE) {
-                            const T *p = reinterpret_cast<const T *>(reinterpret_cast<const uint8_t *>(up + shift * a.rank + r) + from_line);
-                            const uint4 v = load_run(in ? p : p - rank0);  // (ranks behind the last: read again, not used)
-                            const uint32_t k = in ? ~0u : 0u;
-                            w[u][c] = make_uint4(v.x & k, v.y & k, v.z & k, v.w & k);
-                        } else {
-                            const int64_t n = n0 + shift + line;
-                            w[u][c] = load_run(a.up + ((int64_t)adapter * a.outputs + (n < a.outputs ? n : a.outputs - 1)) * a.rank + (in ? r + rank0 : 0), (int64_t)a.rank - r - rank0);
-                        }
-                    }
-#pragma unroll
-                for (int u = 0; u < U; u++)
-#pragma unroll
-                    for (int i = 0; i < RW; i++) {
-                        const uint4 t = terms[(i * blocks + b0 + u) * 64 + lane];
-#pragma unroll
-                        for (int c = 0; c < 4; c++) acc[i][c] = product16<T>(w[u][c], t, acc[i][c]);
-                    }
+                    for (int c = 0; c < 4; c++) acc[i][c] = product16<T>(w[c], t, acc[i][c]);
+                }
             };
             int b = 0;
-            for (; b + 2 <= blocks; b += 2) some(b, Count<2>{});
-            if (b < blocks) some(b, Count<1>{});
+            for (; b + 2 <= blocks; b += 2) {
+                uint4 w[2][4];
+                weights(adapter, n0, b, w, kind);
+                add(b, w[0]), add(b + 1, w[1]);
+            }
+            if (b < blocks) {
+                uint4 w[1][4];
+                weights(adapter, n0, b, w, kind);
+                add(b, w[0]);
+            }
 #pragma unroll
             for (int i = 0; i < RW; i++) {
                 if constexpr (kScaled)
@@ -331,10 +374,10 @@ __global__ void __launch_bounds__(64 * kUpWaves, RW == 2 ? 3 : 4) adapters_up_ke
             }
         }
     };
-    const bool whole_ranks = a.rank % kFragRun<T> == 0;
     for (int64_t n0 = n_first; n0 < n_end; n0 += kBlockColumns) {
         const int64_t from = n0 + 64 * wave;
-        if (whole_ranks && from + 64 <= a.outputs) products(from, Count<1>{});
+        if (a.rank % 16 == 0 && from + 64 <= a.outputs) products(from, Count<2>{});
+        else if (a.rank >= L && from + 64 <= a.outputs) products(from, Count<1>{});
         else if (from < a.outputs) products(from, Count<0>{});
         __syncthreads();
         const bool whole = n0 < n_whole;
@@ -377,7 +420,7 @@ Shape shape_of(const nvq_adapters_desc &d) {
     const int64_t step = d.dtype == NVQ_F32 ? 16 : 32, steps = (d.inputs + step - 1) / step;
     // A tile's adapters go to blocks of their own where the tiles alone leave compute units without work, and the contraction is split, four steps a
     // wavefront at least.
-    s.down_slots = (int32_t)at_most(cus / s.tiles, occurring);
+    s.down_slots = s.wide == 2 ? 1 : (int32_t)at_most(cus / s.tiles, occurring);
     s.splits = (int32_t)at_most(2 * cus / (s.tiles * s.down_slots), at_most(steps / (4 * kDownWaves), 16));
     const int64_t columns = (d.outputs + kBlockColumns - 1) / kBlockColumns;
     s.up_slots = (int32_t)at_most(4 * cus / (s.tiles * columns), occurring);
