@@ -3,11 +3,14 @@
 // a group's score is the sum of its one or two largest c, the best groups stay, the k largest c of their experts are chosen, and their
 // weights are p, divided by (their sum + 1e-20) where asked, times a scale.
 //
-// What is chosen is decided on 64 bits: two values of c that float32 makes one, or turns round, are an expert of difference.  Without a bias
-// (and groups by their best alone) c's order is the logits', and nothing is computed to find it.  Values are compared as whole numbers of the
-// same order, 0 for what is not to be chosen, 1 for a NaN.
+// What is chosen is decided as by real numbers.  Without a bias (and groups by their best alone) c's order is the logits', and nothing is computed to find it.
+// Otherwise c is computed in float32, off by less than kNear: where two values that follow one another among the chosen, or at the border of what is chosen,
+// are further apart than that their order is certain, and where they are not (or a value is not finite) the row is decided again in 64 bits.  The
+// weights are computed in 64 bits, for the chosen alone.
 //
-// One wavefront a row, a lane holding V consecutive experts; the maximum over the lanes by data-parallel moves, its place by a ballot.
+// One wavefront a row.  A group has a power of two of the lanes, a lane V consecutive experts, so that (lane, place) is the experts' order and a group's
+// score a few exchanges among its lanes.  Values are compared as whole numbers of the same order, 0 for what is not to be chosen; a round's maximum is found
+// by data-parallel moves, its place by ballots, whose masks stay in scalar registers.
 #include "heads.h"
 #include "nvq_internal.h"
 #include "wave_reduce.h"
@@ -23,7 +26,7 @@ struct SelectArgs {
     int32_t *indices;
     void *weights;
     int64_t rows;
-    int32_t experts, k, groups, top_groups, group_best, normalize, sigmoid;
+    int32_t experts, k, groups, top_groups, group_best, normalize, sigmoid, lanes_shift;  // lanes of a group: a power of two
     double scale;
 };
 
@@ -51,6 +54,11 @@ __device__ __forceinline__ uint64_t ordered(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v + 0.0);
     return v != v ? 1u : b >> 63 ? ~b : b | 1ull << 63;
 }
+__device__ __forceinline__ uint32_t ordered_number(float v) {  // (of what is a number)
+    const uint32_t b = f2u(v + 0.0f);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t key) { return u2f(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key); }
 
 __device__ __forceinline__ double from_lane(double v, int lane) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
@@ -58,128 +66,259 @@ __device__ __forceinline__ double from_lane(double v, int lane) {
     return __builtin_bit_cast(double, (uint64_t)lo | (uint64_t)hi << 32);
 }
 
-// WIDE: c is computed, and compared in 64 bits; else the logits are compared.
-template <typename T, int V, bool WIDE>
-__global__ void __launch_bounds__(64 * kSelectWaves) moe_select_kernel(const SelectArgs a) {
-    __shared__ double held[WIDE ? kSelectWaves : 1][WIDE ? 64 * V : 1];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row = (int64_t)blockIdx.x * kSelectWaves + wave;
-    if (row >= a.rows) return;
-    const int n = a.experts, first = lane * V;
-    const T *logits = (const T *)a.logits + row * n;
-    float l[V];
-    if (n % V == 0 && first < n) {
-        struct __attribute__((packed)) Run { T t[V]; };
-        const Run run = *reinterpret_cast<const Run *>(logits + first);
-#pragma unroll
-        for (int j = 0; j < V; j++) l[j] = Elem<T>::load(run.t, j);
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; j++) l[j] = first + j < n ? Elem<T>::load(logits, first + j) : 0.0f;
-    }
-    // p = e / total
-    double e[V], total = 1.0;
+// exp(x) with the product's rounding put back: off by a step of float32.
+__device__ __forceinline__ float exponential(float x) {
+    constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+    const float y = x * kLog2e, e = __builtin_amdgcn_exp2f(y);
+    return fabsf(y) < 200.0f ? __builtin_fmaf(e, __builtin_fmaf(x, kLog2e, -y) * kLn2, e) : e;  // (0, infinite or not a number as it is)
+}
+
+// The lane's place: of the group `group` of `each` experts the expert `first` and those behind it, `count` of the V.
+struct Place {
+    int group, first, count;
+};
+
+// The row decided in 64 bits: lane r's round r, its expert.
+template <int V>
+__device__ __forceinline__ int select_wide(const SelectArgs &a, const float (&l)[V], const Place &at_place, double *held) {
+    const int lane = threadIdx.x & 63, each = a.experts / a.groups;
+    double c[V];
     if (a.sigmoid) {
 #pragma unroll
-        for (int j = 0; j < V; j++) e[j] = 1.0 / (1.0 + exp(-(double)l[j]));
+        for (int j = 0; j < V; j++) c[j] = 1.0 / (1.0 + exp(-(double)l[j]));
     } else {
         float top = -INFINITY;
         bool wild = false;
 #pragma unroll
         for (int j = 0; j < V; j++)
-            if (first + j < n) top = fmaxf(top, l[j]), wild |= l[j] != l[j];
+            if (j < at_place.count) top = fmaxf(top, l[j]), wild |= l[j] != l[j];
         top = across<64>(top, [](float x, float y) { return fmaxf(x, y); });
         const bool none = top == -INFINITY && !__any(wild);  // (a row of -inf alone: zeros)
         double sum = 0.0;
 #pragma unroll
         for (int j = 0; j < V; j++) {
-            e[j] = none ? 0.0 : exp((double)l[j] - (double)top);
-            if (first + j < n) sum += e[j];
+            c[j] = none ? 0.0 : exp((double)l[j] - (double)top);
+            if (j < at_place.count) sum += c[j];
         }
         sum = across<64>(sum, [](double x, double y) { return x + y; });
-        total = none ? 1.0 : sum;
 #pragma unroll
-        for (int j = 0; j < V; j++) e[j] = e[j] / total;
+        for (int j = 0; j < V; j++) c[j] = none ? 0.0 : c[j] / sum;
     }
+    const bool by_logits = a.bias == nullptr && (a.groups == 1 || a.group_best == 1);
     uint32_t hi[V], lo[V];
 #pragma unroll
     for (int j = 0; j < V; j++) {
-        const bool real = first + j < n;
-        if (WIDE) {
-            const double c = a.bias != nullptr && real ? e[j] + (double)a.bias[first + j] : e[j];
-            const uint64_t b = real ? ordered(c) : 0;
-            hi[j] = (uint32_t)(b >> 32), lo[j] = (uint32_t)b;
-            held[wave][first + j] = c != c ? -INFINITY : c;
-        } else {
-            hi[j] = real ? ordered(l[j]) : 0, lo[j] = 0;
-        }
+        const bool real = j < at_place.count;
+        if (a.bias != nullptr && real) c[j] += (double)a.bias[at_place.first + j];
+        if (by_logits) c[j] = (double)l[j];
+        const uint64_t b = real ? ordered(c[j]) : 0;
+        hi[j] = (uint32_t)(b >> 32), lo[j] = (uint32_t)b;
+        if (real) held[at_place.first + j] = c[j] != c[j] ? -INFINITY : c[j];
     }
     if (a.groups > 1) {
-        const int each = n / a.groups;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         uint32_t group_hi = 0, group_lo = 0;
-        if constexpr (WIDE) {
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            if (lane < a.groups) {
-                double best = -INFINITY, second = -INFINITY;
-                for (int i = 0; i < each; i++) {
-                    const double c = held[wave][lane * each + i];
-                    second = c > best ? best : c > second ? c : second, best = c > best ? c : best;
-                }
-                const uint64_t b = ordered(a.group_best == 2 && each > 1 ? best + second : best);
-                group_hi = (uint32_t)(b >> 32), group_lo = (uint32_t)b;
+        if (lane < a.groups) {
+            double best = -INFINITY, second = -INFINITY;
+            for (int i = 0; i < each; i++) {
+                const double v = held[lane * each + i];
+                second = v > best ? best : v > second ? v : second, best = v > best ? v : best;
             }
-        } else {
-            for (int g = 0; g < a.groups; g++) {
-                uint32_t best = 0;
-#pragma unroll
-                for (int j = 0; j < V; j++) best = (first + j) / each == g && hi[j] > best ? hi[j] : best;
-                best = wave_largest(best);
-                if (lane == g) group_hi = best;
-            }
+            const uint64_t b = ordered(a.group_best == 2 && each > 1 ? best + second : best);
+            group_hi = (uint32_t)(b >> 32), group_lo = (uint32_t)b;
         }
         uint64_t kept = 0;
         for (int i = 0; i < a.top_groups; i++) {
-            const uint32_t h = wave_largest(group_hi), w = WIDE ? wave_largest(group_hi == h ? group_lo : 0) : 0;
+            const uint32_t h = wave_largest(group_hi), w = wave_largest(group_hi == h ? group_lo : 0);
             const int at = __builtin_ctzll(__ballot(group_hi == h && group_lo == w));
             kept |= 1ull << at;
             if (lane == at) group_hi = 0, group_lo = 0;
         }
+        if ((kept >> at_place.group & 1) == 0)
 #pragma unroll
-        for (int j = 0; j < V; j++)
-            if (first + j < n && (kept >> ((first + j) / each) & 1) == 0) hi[j] = 0, lo[j] = 0;
+            for (int j = 0; j < V; j++) hi[j] = 0, lo[j] = 0;
     }
-    // round r's choice and its weight: lane r's
     int chosen = 0;
-    double weight = 0.0, sum = 0.0;
     for (int r = 0; r < a.k; r++) {
-        uint32_t best = 0;
+        uint32_t best = 0, w = 0;
 #pragma unroll
         for (int j = 0; j < V; j++) best = hi[j] > best ? hi[j] : best;
         const uint32_t h = wave_largest(best);
-        uint32_t w = 0;
-        if (WIDE) {
 #pragma unroll
-            for (int j = 0; j < V; j++) w = hi[j] == h && lo[j] > w ? lo[j] : w;
-            w = wave_largest(w);
-        }
+        for (int j = 0; j < V; j++) w = hi[j] == h && lo[j] > w ? lo[j] : w;
+        w = wave_largest(w);
         int mine = V;
-        double p = 0.0;
 #pragma unroll
         for (int j = V - 1; j >= 0; j--)
-            if (hi[j] == h && lo[j] == w) mine = j, p = e[j];
+            if (hi[j] == h && lo[j] == w) mine = j;
         const int at = __builtin_ctzll(__ballot(mine < V));
 #pragma unroll
         for (int j = 0; j < V; j++)
             if (lane == at && j == mine) hi[j] = 0, lo[j] = 0;
-        const int index = __builtin_amdgcn_readlane(first + mine, at);
-        p = from_lane(p, at);
-        sum += p;
-        if (lane == r) chosen = index, weight = p;
+        const int expert = __builtin_amdgcn_readlane(at_place.first + mine, at);
+        if (lane == r) chosen = expert;
+    }
+    return chosen;
+}
+
+// Float32's error of c, relative to 1 and to c: sigmoids and softmaxes (at most 1) are off by 2^-21 at most, products with 64 lanes' sums among it, and the sum
+// with the bias by half a step; a group's two twice that.  What is as near as this is decided again.
+constexpr float kNear = 1.0f / (1 << 19);
+
+// BIASED: c is computed; else the logits are compared, and nothing is in doubt but what is not a number.
+template <typename T, int V, bool BIASED>
+__global__ void __launch_bounds__(64 * kSelectWaves) moe_select_kernel(const SelectArgs a) {
+    __shared__ double held[kSelectWaves][64 * V];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = (int64_t)blockIdx.x * kSelectWaves + wave;
+    if (row >= a.rows) return;
+    const int each = a.experts / a.groups, per = 1 << a.lanes_shift;  // lanes of a group
+    Place place;
+    place.group = lane >> a.lanes_shift;
+    const int within = (lane & (per - 1)) * V;
+    place.first = place.group * each + within;
+    place.count = place.group < a.groups ? each - within : 0;
+    place.count = place.count < 0 ? 0 : place.count < V ? place.count : V;
+    const T *logits = (const T *)a.logits + row * a.experts;
+    const bool biased = BIASED && a.bias != nullptr;
+    float l[V], bias[V];
+    if (each % V == 0) {  // a lane's are all there or none
+        struct __attribute__((packed)) Run { T t[V]; };
+        struct __attribute__((packed)) Biases { float t[V]; };
+        const int from = place.count > 0 ? place.first : 0;
+        const Run run = *reinterpret_cast<const Run *>(logits + from);
+        Biases b{};
+        if (biased) b = *reinterpret_cast<const Biases *>(a.bias + from);
+#pragma unroll
+        for (int j = 0; j < V; j++) l[j] = Elem<T>::load(run.t, j), bias[j] = b.t[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const int from = j < place.count ? place.first + j : 0;
+            l[j] = Elem<T>::load(logits, from), bias[j] = biased ? a.bias[from] : 0.0f;
+        }
+    }
+    constexpr float kLog2e = 1.44269504088896340736f;
+    double total = 1.0;  // softmax: of exp(l - top)
+    bool none = false;   // a row of -inf alone: zeros
+    float top = 0.0f;
+    float c[V];
+    if (!a.sigmoid) {
+        top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < V; j++) top = j < place.count ? fmaxf(top, l[j]) : top;
+        top = across<64>(top, [](float x, float y) { return fmaxf(x, y); });
+        if (top == -INFINITY) {
+            asm volatile("");  // (a branch, the same for all lanes)
+            bool wild = false;
+#pragma unroll
+            for (int j = 0; j < V; j++) wild |= j < place.count && l[j] != l[j];
+            none = !__any(wild);
+        }
+        if (BIASED || !a.normalize) {  // (normalized weights do without the sum, but for what keeps them from 0 / 0)
+            double sum = 0.0;
+#pragma unroll
+            for (int j = 0; j < V; j++) c[j] = exponential(l[j] - top), sum += j < place.count ? (double)c[j] : 0.0;
+            total = across<64>(sum, [](double x, double y) { return x + y; });
+        }
+    }
+    uint32_t key[V];
+    float wild = 0.0f;  // NaN where a value is not finite (not a number)
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        if (BIASED) c[j] = (a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(l[j] * -kLog2e)) : c[j] * __builtin_amdgcn_rcpf((float)total)) + bias[j];
+        else c[j] = l[j];
+        const float v = j < place.count ? c[j] : 0.0f;
+        wild = BIASED ? __builtin_fmaf(v, 0.0f, wild) : v != v ? v : wild;
+        key[j] = j < place.count ? ordered_number(c[j]) : 0u;
+    }
+    bool doubt = wild != wild;
+    if (a.groups > 1) {
+        // a group's two best, among its lanes
+        float best = -INFINITY, second = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const float v = j < place.count ? c[j] : -INFINITY;
+            second = fmaxf(second, fminf(best, v)), best = fmaxf(best, v);
+        }
+        auto meet = [&](float b, float s) __attribute__((always_inline)) { second = fmaxf(fminf(best, b), fmaxf(second, s)), best = fmaxf(best, b); };
+        if (a.lanes_shift > 0) meet(moved<kPairs>(best), moved<kPairs>(second));
+        if (a.lanes_shift > 1) meet(moved<kQuads>(best), moved<kQuads>(second));
+        if (a.lanes_shift > 2) meet(moved<kHalfRow>(best), moved<kHalfRow>(second));
+        if (a.lanes_shift > 3) meet(moved<kRow>(best), moved<kRow>(second));
+        if (a.lanes_shift > 4) meet(__shfl_xor(best, 16), __shfl_xor(second, 16));
+        const float score = a.group_best == 2 && each > 1 ? best + second : best;
+        const bool real = place.group < a.groups;
+        const uint32_t mine = real ? ordered_number(score) : 0u;
+        int before = 0;  // groups that come first
+        for (int g0 = 0; g0 < a.groups; g0 += 4)
+#pragma unroll
+            for (int g = g0; g < g0 + 4; g++) {  // (those behind the last are 0)
+                const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)mine, g << a.lanes_shift);
+                before += other + (g < place.group ? 1u : 0u) > mine ? 1 : 0;  // (no key is the largest number)
+            }
+        const bool kept = before < a.top_groups;
+        if (BIASED && a.top_groups < a.groups) {
+            const float least = value_of((uint32_t)__builtin_amdgcn_readlane((int)mine, __builtin_ctzll(__ballot(before == a.top_groups - 1) | 1ull << 63)));
+            doubt |= !kept && real && !(score < least - 2.0f * kNear * (1.0f + fabsf(least)));
+        }
+#pragma unroll
+        for (int j = 0; j < V; j++) key[j] = kept ? key[j] : 0u;
+    }
+    int chosen = 0, keys = 0;  // lane r's of round r
+    if (!__any(doubt)) {
+        for (int r = 0;; r++) {
+            uint32_t best = key[0];
+#pragma unroll
+            for (int j = 1; j < V; j++) best = key[j] > best ? key[j] : best;
+            const uint32_t h = wave_largest(best);
+            const bool mine = lane == r;
+            keys = mine ? (int)h : keys;
+            if (r == a.k) break;  // (the one behind the last chosen is looked at too)
+            uint64_t has[V], any = 0;
+#pragma unroll
+            for (int j = 0; j < V; j++) has[j] = __ballot(key[j] == h), any |= has[j];
+            const uint64_t at = any & -any;  // the first lane's
+            int place_of = 0;
+            uint64_t open = at;
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                const uint64_t here = open & has[j];
+                place_of = here != 0 ? j : place_of, open &= ~here;
+                key[j] = __builtin_amdgcn_inverse_ballot_w64(here) ? 0u : key[j];
+            }
+            const int expert = __builtin_amdgcn_readlane(place.first, __builtin_ctzll(at)) + place_of;
+            chosen = mine ? expert : chosen;
+            if (BIASED && r == 63) break;
+        }
+        if (BIASED) {  // neighbours among the chosen, and the one behind them
+            const uint32_t behind = (uint32_t)__shfl_down(keys, 1);
+            const float v = value_of((uint32_t)keys), w = value_of(behind);
+            doubt = (lane < a.k && lane < 63 && behind != 0u && !(w < v - kNear * (1.0f + fabsf(v)))) || a.k == 64;
+        }
+    }
+    if (BIASED ? __any(doubt) : __any(wild != wild)) {
+        asm volatile("");  // (a branch, the same for all lanes)
+        chosen = select_wide<V>(a, l, place, held[wave]);
+    }
+    // the weights, lane r's of round r: quotients and sums of 64 bits, over exponentials of float32 for 16-bit results
+    double p = 0.0;
+    if (lane < a.k) {
+        const float x = Elem<T>::load(logits, chosen);
+        const float from = a.sigmoid ? -x : x - top;
+        double e;
+        if constexpr (sizeof(T) == 4) e = exp(a.sigmoid ? -(double)x : (double)x - (double)top);
+        else e = (double)exponential(from);
+        p = a.sigmoid ? 1.0 / (1.0 + e) : none ? 0.0 : e / total;
+    }
+    if (a.normalize) {
+        auto add = [](double x, double y) { return x + y; };
+        const double sum = a.k <= 16 ? across<16>(p, add) : across<64>(p, add);
+        p /= sum + 1e-20;
     }
     if (lane < a.k) {
         a.indices[row * a.k + lane] = chosen;
-        if (a.normalize) weight /= sum + 1e-20;
-        Elem<T>::store((T *)a.weights, row * a.k + lane, (float)(weight * a.scale));
+        Elem<T>::store((T *)a.weights, row * a.k + lane, (float)(p * a.scale));
     }
 }
 
@@ -192,17 +331,19 @@ void run_select(const SelectArgs &a, hipStream_t s) {
 
 template <typename T>
 void run_select_type(const SelectArgs &a, hipStream_t s) {
-    if (a.experts <= 64) run_select<T, 1>(a, s);
-    else if (a.experts <= 128) run_select<T, 2>(a, s);
-    else if (a.experts <= 256) run_select<T, 4>(a, s);
-    else if (a.experts <= 512) run_select<T, 8>(a, s);
+    const int each = a.experts / a.groups, of_lane = (each + (1 << a.lanes_shift) - 1) >> a.lanes_shift;
+    if (of_lane <= 1) run_select<T, 1>(a, s);
+    else if (of_lane <= 2) run_select<T, 2>(a, s);
+    else if (of_lane <= 4) run_select<T, 4>(a, s);
+    else if (of_lane <= 8) run_select<T, 8>(a, s);
     else run_select<T, 16>(a, s);
 }
 
 }  // namespace
 
 int32_t launch_moe_select(const nvq_moe_select_desc &d, const void *logits, const float *bias, int32_t *indices, void *weights, hipStream_t s) {
-    const SelectArgs a{logits, bias, indices, weights, d.rows, d.experts, d.k, d.groups, d.top_groups, d.group_best, d.normalize, d.scores == NVQ_SCORES_SIGMOID, d.scale};
+    SelectArgs a{logits, bias, indices, weights, d.rows, d.experts, d.k, d.groups, d.top_groups, d.group_best, d.normalize, d.scores == NVQ_SCORES_SIGMOID, 0, d.scale};
+    while (a.groups << (a.lanes_shift + 1) <= 64) a.lanes_shift++;
     if (d.dtype == NVQ_F32) run_select_type<float>(a, s);
     else if (d.dtype == NVQ_BF16) run_select_type<bf16_t>(a, s);
     else run_select_type<f16_t>(a, s);
