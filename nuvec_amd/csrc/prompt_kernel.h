@@ -18,6 +18,8 @@
 // are zeros in the tile, so that lines that do not see them stay clean; the lines that do are given them afterwards.
 #pragma once
 
+#include <type_traits>
+
 #include "matrix.h"
 #include "nvq_device.h"
 #include "nvq_internal.h"
@@ -83,8 +85,13 @@ __device__ __forceinline__ uint32_t half_pair(float a, float b) {
     const f32x2_t v = {a, b};
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
 }
-__device__ __forceinline__ float half_of(uint32_t w, int i) {
-    return (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> (16 * i)));
+// v less half I of w.
+template <int I>
+__device__ __forceinline__ float behind(float v, uint32_t w) {
+    float d;
+    if constexpr (I == 0) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(w), "v"(v));
+    else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(w), "v"(v));
+    return d;
 }
 
 // The keys that a block's lines see, from `begin` to `end`, and how its items share them: evenly, `keys` each.  An item that has them all writes the result.
@@ -118,6 +125,7 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
     constexpr int SHARE = Of::kShare;
     __shared__ alignas(16) Stage stages[2];
     __shared__ uint32_t flags[2];             // of a stage: a value that it does not hold
+    __shared__ uint32_t again;                // sums that are not finite
     __shared__ uint32_t most[2][kWaves];      // of a tile that is laid out again: the largest finite value's bits; whether one is not finite
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
     PagedItem item;
@@ -163,23 +171,37 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
         const int at = tid + 64 * kWaves * i;
         row = at / Of::kRuns, run = at % Of::kRuns;
     };
-    auto request_values = [&](int s0) __attribute__((always_inline)) {
+    // A run's offset from its tile's first row is below 2^32 (the entry refuses strides beyond that), so that a load adds it to a scalar address.  It is
+    // worked out from the first run's where the runs of a thread lie whole rows apart.
+    constexpr bool kEven = 64 * kWaves % Of::kRuns == 0;
+    constexpr int kApart = 64 * kWaves / Of::kRuns;  // rows
+    auto offset = [&](int64_t stride, int row, int run) __attribute__((always_inline)) {
+        return ((uint32_t)row * (uint32_t)stride + (uint32_t)(run * RUN < a.dim ? run * RUN : 0)) * (uint32_t)sizeof(T);
+    };
+    uint32_t k_offset[kEven ? 1 : SHARE], v_offset[kEven ? 1 : SHARE];
+#pragma unroll
+    for (int i = 0; i < (kEven ? 1 : SHARE); i++) {
+        int row, run;
+        place(i, row, run);
+        k_offset[i] = offset(a.k_strides[0], row, run), v_offset[i] = offset(a.v_strides[0], row, run);
+    }
+    const bool whole_rows = a.dim == D;
+    // (keys behind the sequence's last are read as the last; loads under a condition would be waited for at its end)
+    auto load_tile = [&](uint4 (&to)[SHARE], const T *from, int64_t stride, uint32_t (&of)[kEven ? 1 : SHARE], int s0) __attribute__((always_inline)) {
+        const uint8_t *first = reinterpret_cast<const uint8_t *>(from + (int64_t)s0 * stride);
+        const uint32_t step = (uint32_t)stride * (uint32_t)sizeof(T), last = (uint32_t)(S - 1 - s0 < KT - 1 ? S - 1 - s0 : KT - 1) * step;
+        asm volatile("" : "+v"(of[0]));  // (what follows from it is not worth a register each)
 #pragma unroll
         for (int i = 0; i < SHARE; i++) {
             int row, run;
-            place(i, row, run);
-            const int64_t key = s0 + row < S ? s0 + row : S - 1;
-            vr[i] = load_run(values + key * a.v_strides[0] + (run * RUN < a.dim ? run * RUN : 0));
+            place(kEven ? 0 : i, row, run);
+            const uint32_t at = kEven ? of[0] + (uint32_t)(i * kApart) * step : of[kEven ? 0 : i], end = last + (uint32_t)(run * RUN < a.dim ? run * RUN : 0) * (uint32_t)sizeof(T);
+            to[i] = load_run(reinterpret_cast<const T *>(first + (at < end ? at : end)));
         }
     };
+    auto request_values = [&](int s0) __attribute__((always_inline)) { load_tile(vr, values, a.v_strides[0], v_offset, s0); };
     auto request = [&](int s0) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < SHARE; i++) {
-            int row, run;
-            place(i, row, run);
-            const int64_t key = s0 + row < S ? s0 + row : S - 1;
-            kr[i] = load_run(keys + key * a.k_strides[0] + (run * RUN < a.dim ? run * RUN : 0));
-        }
+        load_tile(kr, keys, a.k_strides[0], k_offset, s0);
         request_values(s0);
     };
     // What lies behind the head's values and behind the sequence's end: zeros.
@@ -209,28 +231,38 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
         place(i, row, run);
         return reinterpret_cast<uint4 *>(to.values + row * Of::kValueRow + 16 * run);
     };
-    // The tile's rows into a stage; its flag where a value is not finite there.
-    auto lay = [&](Stage &to, uint32_t &flag, int s0) __attribute__((always_inline)) {
+    // The tile's rows into a stage; (CAREFUL) its flag where a value is not finite there.
+    auto lay = [&](auto careful, Stage &to, uint32_t &flag, int s0) __attribute__((always_inline)) {
         typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
         float wild = 0.0f;
         f16x2_t wild2 = {(_Float16)0.0f, (_Float16)0.0f};
+        if (!whole_rows || s0 + KT > S) {
+            asm volatile("");  // (a branch, the same for all; so is the next)
+#pragma unroll
+            for (int i = 0; i < SHARE; i++) {
+                int row, run;
+                place(i, row, run);
+                // (keys behind the head's values meet zeros of the queries, which an infinite value would spoil)
+                const uint32_t k = run * RUN < a.dim ? ~0u : 0u, v = real(s0, i) ? ~0u : 0u;
+                kr[i] = make_uint4(kr[i].x & k, kr[i].y & k, kr[i].z & k, kr[i].w & k), vr[i] = make_uint4(vr[i].x & v, vr[i].y & v, vr[i].z & v, vr[i].w & v);
+            }
+        }
+        if (kBf16 && value_scale != 1.0f) {
+            asm volatile("");
+#pragma unroll
+            for (int i = 0; i < SHARE; i++) vr[i] = operand(vr[i], true);
+        } else {
+#pragma unroll
+            for (int i = 0; i < SHARE; i++) vr[i] = operand(vr[i], false);
+        }
 #pragma unroll
         for (int i = 0; i < SHARE; i++) {
             int row, run;
             place(i, row, run);
-            const bool used = real(s0, i);
-            const uint32_t k = used ? ~0u : 0u;
-            // (keys behind the head's values meet zeros of the queries, which an infinite value would spoil)
-            const uint32_t in = run * RUN < a.dim ? ~0u : 0u;
-            *reinterpret_cast<uint4 *>(to.keys + row * Of::kKeyRow + 16 * run) = make_uint4(kr[i].x & in, kr[i].y & in, kr[i].z & in, kr[i].w & in);
-            uint4 w = make_uint4(vr[i].x & k, vr[i].y & k, vr[i].z & k, vr[i].w & k);
-            if (kBf16 && value_scale != 1.0f) {
-                asm volatile("");  // (a branch, the same for all)
-                w = operand(w, true);
-            } else {
-                w = operand(w, false);
-            }
-            *value_place(to, i) = w;
+            *reinterpret_cast<uint4 *>(to.keys + row * Of::kKeyRow + 16 * run) = kr[i];
+            *value_place(to, i) = vr[i];
+            if constexpr (!decltype(careful)::value) continue;
+            const uint4 w = vr[i];
             if constexpr (kWide) {  // x 0 is NaN of what is not finite
                 wild = __builtin_fmaf(u2f(w.x), 0.0f, wild), wild = __builtin_fmaf(u2f(w.y), 0.0f, wild);
                 wild = __builtin_fmaf(u2f(w.z), 0.0f, wild), wild = __builtin_fmaf(u2f(w.w), 0.0f, wild);
@@ -243,7 +275,7 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
             }
         }
         if constexpr (!kWide) wild = (float)wild2[0] + (float)wild2[1];
-        if (wild != wild) flag = 1u;
+        if (decltype(careful)::value && wild != wild) flag = 1u;
     };
 
     acc16_t o[ND];
@@ -282,7 +314,7 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
                 if constexpr (!kBf16) {
                     uint32_t q[4];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) q[j] = half_pair(e[2 * j] - half_of(p[j], 0), e[2 * j + 1] - half_of(p[j], 1));
+                    for (int j = 0; j < 4; j++) q[j] = half_pair(behind<0>(e[2 * j], p[j]), behind<1>(e[2 * j + 1], p[j]));
                     low = __builtin_bit_cast(half8_t, make_uint4(q[0], q[1], q[2], q[3]));
                 }
 #pragma unroll
@@ -473,8 +505,40 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
         }
     };
 
-    if (tid < 2) flags[tid] = 0u;
-    __syncthreads();
+    // The keys of the item.  First without a look at what the values hold: where one is not finite, or has left float16's range, the sums of some line are
+    // not finite, and the block walks its keys again with care.  (In one loop the rare paths' loads would be waited for in every tile.)
+    auto walk = [&](auto careful) __attribute__((always_inline)) {
+        constexpr bool kCareful = decltype(careful)::value;
+        lay(careful, stages[0], flags[0], s_begin);
+        __syncthreads();
+        int at = 0;
+        for (int s0 = s_begin; s0 < s_end; s0 += KT) {
+            const bool more = s0 + KT < s_end;
+            bool flagged = false, wild = false;
+            if constexpr (kCareful) {
+                flagged = uniform((int32_t)flags[at]) != 0;
+                if (flagged) {
+                    asm volatile("");
+                    __syncthreads();
+                    if (tid == 0) flags[at] = 0u;
+                    lay_again(stages[at], s0, wild);
+                }
+            }
+            if (more) request(s0 + KT);
+            uint32_t seen = 0;
+            if (s0 <= any_last && s0 + KT > any_first) tile(stages[at], s0, flagged, seen);  // (uniform in the wavefront)
+            if constexpr (kCareful) {
+                if (wild) {
+                    add_wild(stages[at], s0, seen);
+                    if (more) request(s0 + KT);
+                }
+            }
+            if (more) lay(careful, stages[at ^ 1], flags[at ^ 1], s0 + KT);
+            __syncthreads();
+            at ^= 1;
+        }
+    };
+    if (tid < 3) (tid < 2 ? flags[tid] : again) = 0u;
     if (s_begin < s_end) {
         request(s_begin);
         if constexpr (kBf16) {
@@ -483,30 +547,24 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
             survey(s_begin, top, wild);
             value_scale = scale_for(top);
         }
-        lay(stages[0], flags[0], s_begin);
-    }
-    __syncthreads();
-    int at = 0;
-    for (int s0 = s_begin; s0 < s_end; s0 += KT) {
-        const bool more = s0 + KT < s_end;
-        const bool flagged = uniform((int32_t)flags[at]) != 0;
-        bool wild = false;
-        if (flagged) {
-            asm volatile("");
-            __syncthreads();
-            if (tid == 0) flags[at] = 0u;
-            lay_again(stages[at], s0, wild);
-        }
-        if (more) request(s0 + KT);
-        uint32_t seen = 0;
-        if (s0 <= any_last && s0 + KT > any_first) tile(stages[at], s0, flagged, seen);  // (uniform in the wavefront)
-        if (wild) {
-            add_wild(stages[at], s0, seen);
-            if (more) request(s0 + KT);
-        }
-        if (more) lay(stages[at ^ 1], flags[at ^ 1], s0 + KT);
+        const float first_scale = value_scale;
+        walk(std::false_type{});
+        float odd = l * 0.0f;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) odd = __builtin_fmaf(o[d][i], 0.0f, odd);
+        if (__any(odd != odd) && lane == 0) again = 1u;
         __syncthreads();
-        at ^= 1;
+        if (uniform((int32_t)again) != 0) {
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+            m = kLowest, l = 0.0f, value_scale = first_scale;
+            request(s_begin);
+            walk(std::true_type{});
+        }
     }
     l += __shfl_xor(l, 32);
     if (!live) return;

@@ -30,6 +30,8 @@ static int32_t check_prompt(const nvq_prompt_attention_desc *d) {
         return fail(NVQ_UNSUPPORTED, "%s: 2^30 rows and heads, 2^30 keys or 2^20 sequences", op);
     for (int i = 0; i < 2; i++)
         if (d->q_strides[i] < 0 || d->k_strides[i] < 0 || d->v_strides[i] < 0 || d->out_strides[i] < 0) return fail(NVQ_INVALID_ARGUMENT, "%s: negative stride", op);
+    if (d->keys > 1 && (d->k_strides[0] >= 1 << 24 || d->v_strides[0] >= 1 << 24))  // (offsets within a tile are of 32 bits)
+        return fail(NVQ_UNSUPPORTED, "%s: keys %lld and values %lld elements apart (less than 2^24)", op, (long long)d->k_strides[0], (long long)d->v_strides[0]);
     if (!prompt_attention_launchable(*d)) return fail(NVQ_UNSUPPORTED, "%s: %lld rows of %lld sequences, %lld heads each, in one launch", op, (long long)d->rows, (long long)d->sequences, (long long)d->query_heads);
     return NVQ_OK;
 }
