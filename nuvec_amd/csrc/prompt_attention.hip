@@ -9,12 +9,15 @@ namespace {
 constexpr int32_t kLeast = 4;
 
 int32_t target_of(const nvq_prompt_attention_desc &d) { return (prompt::padded_dim(d.head_dim) <= 128 ? 2 : 1) * compute_units(); }
-// (the device decides by the lengths, which are at most all keys)
-bool may_split(const nvq_prompt_attention_desc &d) { return d.keys > 2 * kScheduleKeys * kLeast; }
 // Units at most, whatever the starts on the device say: every sequence's last block of lines may be short.
 int64_t most_units(const nvq_prompt_attention_desc &d) {
     const int64_t lines = d.rows * (d.query_heads / d.key_heads);
     return (lines / prompt::kLines + d.sequences) * d.key_heads;
+}
+// The device decides by the lengths, which are at most all keys.  One sequence of all rows is as the host sees it: its blocks of lines are split where
+// they are fewer than the target.
+bool may_split(const nvq_prompt_attention_desc &d, bool starts) {
+    return d.keys > 2 * kScheduleKeys * kLeast && (starts || (d.rows * (d.query_heads / d.key_heads) + prompt::kLines - 1) / prompt::kLines * d.key_heads < target_of(d));
 }
 // Items of sequences that are split: at most twice the target (paged_schedule.h), and no more than their units have.
 int64_t most_states(const nvq_prompt_attention_desc &d) {
@@ -27,21 +30,22 @@ int64_t most_states(const nvq_prompt_attention_desc &d) {
 bool prompt_attention_launchable(const nvq_prompt_attention_desc &d) { return launchable(most_units(d) + (1 << 12), 256); }
 
 size_t prompt_attention_workspace_bytes(const nvq_prompt_attention_desc &d) {
-    if (!may_split(d) || d.rows == 0) return 0;
+    if (!may_split(d, true) || d.rows == 0) return 0;
     return prompt::kPlanBytes + (size_t)(most_states(d) * prompt::kLines * (prompt::padded_dim(d.head_dim) + 4)) * sizeof(float);
 }
 
 int32_t launch_prompt_attention(const nvq_prompt_attention_desc &d, const PromptAttentionOperands &o, hipStream_t s) {
+    const bool split = may_split(d, o.query_starts != nullptr || o.key_starts != nullptr);
     prompt::PromptLaunch r{};
     prompt::PromptBatch &b = r.batch;
     b.starts = o.query_starts, b.key_starts = o.key_starts, b.rows = d.rows, b.keys = d.keys;
     b.window = d.window < 1LL << 30 ? d.window : 1LL << 30;  // (as good as any larger one, and sums with it stay far from 64 bits)
     b.sequences = (int32_t)d.sequences, b.key_heads = (int32_t)d.key_heads, b.rep = (int32_t)(d.query_heads / d.key_heads), b.causal = d.causal != 0;
-    b.few = -1, b.target = target_of(d), b.least = may_split(d) ? kLeast : 1 << 26;
-    const int64_t units = most_units(d), least = (int64_t)kScheduleKeys * kLeast, splits = may_split(d) ? (d.keys + least - 1) / least : 1;
+    b.few = -1, b.target = target_of(d), b.least = split ? kLeast : 1 << 26;
+    const int64_t units = most_units(d), least = (int64_t)kScheduleKeys * kLeast, splits = split ? (d.keys + least - 1) / least : 1;
     const int64_t full = b.target, spare = full / 2 + units, items = full > spare ? full : spare;
     r.grid = (uint32_t)(units * splits < items ? units * splits : items);
-    r.merge_units = may_split(d) ? (uint32_t)(units < full ? units : full) : 0;
+    r.merge_units = split ? (uint32_t)(units < full ? units : full) : 0;
     if (d.dtype == NVQ_F32) return prompt::launch_f32(d, o, r, s);
     return d.dtype == NVQ_BF16 ? prompt::launch_bf16(d, o, r, s) : prompt::launch_f16(d, o, r, s);
 }

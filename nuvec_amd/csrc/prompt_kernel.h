@@ -29,6 +29,7 @@ namespace nvq {
 namespace prompt {
 
 constexpr int kWaves = 4;
+constexpr int kMatrix = 8, kLdsRead = 0x100;  // kinds of instructions, of an order that the compiler is told to keep
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLowest = -3.4e38f;  // where maxima start (paged_rows_kernel.h says why it is finite)
 
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
         typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
         float wild = 0.0f;
         f16x2_t wild2 = {(_Float16)0.0f, (_Float16)0.0f};
-        if (!whole_rows || s0 + KT > S) {
+        if (__builtin_expect(!whole_rows || s0 + KT > S, 0)) {
             asm volatile("");  // (a branch, the same for all; so is the next)
 #pragma unroll
             for (int i = 0; i < SHARE; i++) {
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
                 kr[i] = make_uint4(kr[i].x & k, kr[i].y & k, kr[i].z & k, kr[i].w & k), vr[i] = make_uint4(vr[i].x & v, vr[i].y & v, vr[i].z & v, vr[i].w & v);
             }
         }
-        if (kBf16 && value_scale != 1.0f) {
+        if (kBf16 && __builtin_expect(value_scale != 1.0f, 0)) {
             asm volatile("");
 #pragma unroll
             for (int i = 0; i < SHARE; i++) vr[i] = operand(vr[i], true);
@@ -296,40 +297,57 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
     auto value_at = [&](const Stage &from, int i, int d) __attribute__((always_inline)) {
         return reinterpret_cast<const float *>(from.values + (8 * (i >> 2) + 4 * half + (i & 3)) * Of::kValueRow)[32 * d + col];
     };
-    auto weighted = [&](const Stage &from, const float (&x)[TB][16]) __attribute__((always_inline)) {
+    // Exponentials, sums and products.  16-bit types: the weights of 16 keys are worked out, and the values of the next 16 read, between the products of the
+    // 16 before them (in the order written: products wait for neither, and the vector unit works beside them).
+    auto weigh = [&](const Stage &from, float (&x)[TB][16], auto careful, uint32_t &seen) __attribute__((always_inline)) {
+        auto weight = [&](int i) __attribute__((always_inline)) {
+            const float e = __builtin_amdgcn_exp2f(x[i >> 4][i & 15]);
+            l += e;
+            if constexpr (decltype(careful)::value) seen |= (e == 0.0f ? 0u : 1u) << i;
+            return e;
+        };
         if constexpr (kWide) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[0][i] = weight(i);
 #pragma unroll
             for (int i = 0; i < 16; i++)
 #pragma unroll
                 for (int d = 0; d < ND; d++) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(value_at(from, i, d), x[0][i], o[d], 0, 0, 0);
         } else {
+            constexpr int NC = KT / 16;
+            uint32_t high[2][4], low[2][4];
+            half8_t v[2][ND];
+            auto prepare = [&](int c, int j) __attribute__((always_inline)) {
+                const float e0 = weight(8 * c + 2 * j), e1 = weight(8 * c + 2 * j + 1);
+                high[c & 1][j] = half_pair(e0, e1);
+                if constexpr (!kBf16) low[c & 1][j] = half_pair(behind<0>(e0, high[c & 1][j]), behind<1>(e1, high[c & 1][j]));
+            };
+            auto operand_of = [&](const uint32_t (&w)[4]) __attribute__((always_inline)) { return __builtin_bit_cast(half8_t, make_uint4(w[0], w[1], w[2], w[3])); };
 #pragma unroll
-            for (int c = 0; c < KT / 16; c++) {
-                const float *e = &x[c >> 1][8 * (c & 1)];
-                uint32_t p[4];
+            for (int d = 0; d < ND; d++) v[0][d] = value_run(from, 0, d);
 #pragma unroll
-                for (int j = 0; j < 4; j++) p[j] = half_pair(e[2 * j], e[2 * j + 1]);
-                const half8_t high = __builtin_bit_cast(half8_t, make_uint4(p[0], p[1], p[2], p[3]));
-                half8_t low;
-                if constexpr (!kBf16) {
-                    uint32_t q[4];
+            for (int j = 0; j < 4; j++) prepare(0, j);
+            __builtin_amdgcn_s_setprio(1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) q[j] = half_pair(behind<0>(e[2 * j], p[j]), behind<1>(e[2 * j + 1], p[j]));
-                    low = __builtin_bit_cast(half8_t, make_uint4(q[0], q[1], q[2], q[3]));
-                }
+            for (int c = 0; c < NC; c++)
 #pragma unroll
                 for (int d = 0; d < ND; d++) {
-                    const half8_t v = value_run(from, c, d);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, high, o[d], 0, 0, 0);
-                    if constexpr (!kBf16) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, low, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[c & 1][d], operand_of(high[c & 1]), o[d], 0, 0, 0);
+                    if (c + 1 < NC) v[(c + 1) & 1][d] = value_run(from, c + 1, d);
+                    if constexpr (!kBf16) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[c & 1][d], operand_of(low[c & 1]), o[d], 0, 0, 0);
+                    if (c + 1 < NC)
+#pragma unroll
+                        for (int j = 4 * d / ND; j < 4 * (d + 1) / ND; j++) prepare(c + 1, j);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-            }
         }
     };
-    // One tile: the scores, one look at their maximum, the weights and their products.  x[t][i]: key 32 t + 8 (i / 4) + 4 half + i % 4.  `seen`, where the
-    // tile is flagged: a bit for each of these keys that has a weight.
-    auto tile = [&](const Stage &from, int s0, bool flagged, uint32_t &seen) __attribute__((always_inline)) {
+    // One tile: the scores, one look at their maximum, the weights and their products.  x[t][i]: key 32 t + 8 (i / 4) + 4 half + i % 4.  `seen` (CAREFUL): a bit
+    // for each of these keys that has a weight.
+    auto tile = [&](const Stage &from, int s0, auto careful, uint32_t &seen) __attribute__((always_inline)) {
         float x[TB][16];
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int t = 0; t < TB; t++) {
             acc16_t s;
@@ -341,7 +359,18 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
 #pragma unroll
             for (int i = 0; i < 16; i++) x[t][i] = s[i];
         }
-        if (s0 + KT - 1 > all_last || s0 < all_first || s0 + KT > s_end) {
+        if constexpr (!kWide) {  // the rows' reads KS products ahead of them
+            constexpr int kAhead = KS < TB * KS ? KS : KS / 2;
+            __builtin_amdgcn_sched_group_barrier(kLdsRead, kAhead, 0);
+#pragma unroll
+            for (int k = kAhead; k < TB * KS; k++) {
+                __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kLdsRead, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(kMatrix, kAhead, 0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        if (__builtin_expect(s0 + KT - 1 > all_last || s0 < all_first || s0 + KT > s_end, 0)) {
             asm volatile("");  // (a branch: as selects it would cost every tile)
 #pragma unroll
             for (int t = 0; t < TB; t++)
@@ -356,7 +385,7 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
         for (int i = 1; i < 16 * TB; i++) top = fmaxf(top, x[i >> 4][i & 15]);
         top *= scale;
         // Rescaled only when a maximum has grown by more than 2^8: until then the weights are at most 2^8.
-        if (__any(top > m + 8.0f)) {
+        if (__builtin_expect(__any(top > m + 8.0f), 0)) {
             top = fmaxf(top, __shfl_xor(top, 32));
             const float m_new = fmaxf(m, top), f = exp2f(m - m_new);
             m = m_new, l *= f;
@@ -367,7 +396,7 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
         }
         // The maximum is a rounded product, which the fused one is not: the difference is a factor that all weights of a line share, but one that grows
         // with the scores' size.  From 2^20 on both are rounded.
-        if (__any(fabsf(m) > 1048576.0f)) {
+        if (__builtin_expect(__any(fabsf(m) > 1048576.0f), 0)) {
             asm volatile("");
 #pragma unroll
             for (int t = 0; t < TB; t++)
@@ -379,18 +408,8 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
 #pragma unroll
                 for (int i = 0; i < 16; i++) x[t][i] = __builtin_fmaf(x[t][i], scale, -m);
         }
-#pragma unroll
-        for (int t = 0; t < TB; t++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) x[t][i] = __builtin_amdgcn_exp2f(x[t][i]), l += x[t][i];
-        if (flagged) {
-            asm volatile("");
-#pragma unroll
-            for (int t = 0; t < TB; t++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) seen |= (x[t][i] == 0.0f ? 0u : 1u) << (16 * t + i);
-        }
-        weighted(from, x);
+        weigh(from, x, careful, seen);
+        __builtin_amdgcn_s_setprio(0);
     };
 
     // The largest finite value of the tile in vr (its bits as a positive number) and whether one is not finite, for all of the block.
@@ -514,26 +533,25 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
         int at = 0;
         for (int s0 = s_begin; s0 < s_end; s0 += KT) {
             const bool more = s0 + KT < s_end;
-            bool flagged = false, wild = false;
+            bool wild = false;
             if constexpr (kCareful) {
-                flagged = uniform((int32_t)flags[at]) != 0;
-                if (flagged) {
+                if (uniform((int32_t)flags[at]) != 0) {
                     asm volatile("");
                     __syncthreads();
                     if (tid == 0) flags[at] = 0u;
                     lay_again(stages[at], s0, wild);
                 }
             }
-            if (more) request(s0 + KT);
+            if (__builtin_expect(more, 1)) request(s0 + KT);
             uint32_t seen = 0;
-            if (s0 <= any_last && s0 + KT > any_first) tile(stages[at], s0, flagged, seen);  // (uniform in the wavefront)
+            if (__builtin_expect(s0 <= any_last && s0 + KT > any_first, 1)) tile(stages[at], s0, careful, seen);  // (uniform in the wavefront)
             if constexpr (kCareful) {
                 if (wild) {
                     add_wild(stages[at], s0, seen);
                     if (more) request(s0 + KT);
                 }
             }
-            if (more) lay(careful, stages[at ^ 1], flags[at ^ 1], s0 + KT);
+            if (__builtin_expect(more, 1)) lay(careful, stages[at ^ 1], flags[at ^ 1], s0 + KT);
             __syncthreads();
             at ^= 1;
         }
@@ -556,7 +574,7 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
             for (int i = 0; i < 16; i++) odd = __builtin_fmaf(o[d][i], 0.0f, odd);
         if (__any(odd != odd) && lane == 0) again = 1u;
         __syncthreads();
-        if (uniform((int32_t)again) != 0) {
+        if (__builtin_expect(uniform((int32_t)again) != 0, 0)) {
 #pragma unroll
             for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -607,15 +625,11 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
 
 // The splits' states merged: D / 4 threads a line, four splits' loads under way at a time.
 template <int D> constexpr int kMergeLines = 256 / (D / 4);  // of a block
+constexpr uint32_t kMergeBlocks = 2048;
 template <typename T, int D>
-__global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptArgs<T> a, uint32_t units) {
-    constexpr int kThreads = D / 4;
-    PagedItem item;
-    if (!paged_item<kLines, 1, true>(a.batch, threadIdx.x & 63, blockIdx.x % units, a.length, item)) return;
-    const int rep = a.batch.rep, ln = (int)(blockIdx.x / units) * kMergeLines<D> + (int)threadIdx.x / kThreads, at = (int)threadIdx.x % kThreads * 4;
-    const int part = item.s.parts - 1 - item.part, line = part * kLines + ln;  // (items count the parts from the last)
-    const Span span = span_of(a.batch, item, part);
-    if ((int)threadIdx.x >= kMergeLines<D> * kThreads || ln >= kLines || line >= item.s.rows * rep || span.items == 1 || at >= a.dim) return;
+__device__ __forceinline__ void merge_line(const PromptArgs<T> &a, const PagedItem &item, const Span &span, int part, int ln, int at) {
+    const int rep = a.batch.rep, line = part * kLines + ln;
+    if (ln >= kLines || line >= item.s.rows * rep) return;
     const int64_t stride = (int64_t)a.batch.key_heads * kLines * kState<D>;  // of a split's states
     const float *src = a.states + ((int64_t)item.slot * kLines + ln) * kState<D>;
     float top = kLowest, total = 0.0f, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -662,11 +676,26 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptArgs<T> a
 }
 
 template <typename T, int D>
+__global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptArgs<T> a, uint32_t units) {
+    constexpr int kThreads = D / 4;
+    PagedItem item;
+    if (!paged_item<kLines, 1, true>(a.batch, threadIdx.x & 63, blockIdx.x % units, a.length, item)) return;
+    const int at = (int)threadIdx.x % kThreads * 4;
+    const int part = item.s.parts - 1 - item.part;  // (items count the parts from the last)
+    const Span span = span_of(a.batch, item, part);
+    if ((int)threadIdx.x >= kMergeLines<D> * kThreads || span.items == 1 || at >= a.dim) return;
+    for (int first = (int)(blockIdx.x / units) * kMergeLines<D>; first < kLines; first += (int)(gridDim.x / units) * kMergeLines<D>)
+        merge_line<T, D>(a, item, span, part, first + (int)threadIdx.x / kThreads, at);
+}
+
+template <typename T, int D>
 int32_t launch_sized(const PromptArgs<T> &a, const PromptLaunch &r, hipStream_t s) {
     hipLaunchKernelGGL((prompt_kernel<T, D>), dim3(r.grid), dim3(64 * kWaves), 0, s, a);
     NVQ_LAUNCH_CHECK("prompt_attention");
     if (r.merge_units == 0) return NVQ_OK;
-    hipLaunchKernelGGL((prompt_merge_kernel<T, D>), dim3(r.merge_units * ((kLines + kMergeLines<D> - 1) / kMergeLines<D>)), dim3(256), 0, s, a, r.merge_units);
+    // (blocks of several passes over a unit's lines from where they would be more than the chip holds: often nothing is split)
+    const uint32_t all = (kLines + kMergeLines<D> - 1) / kMergeLines<D>, some = kMergeBlocks / r.merge_units, blocks = some < 1 ? 1 : some < all ? some : all;
+    hipLaunchKernelGGL((prompt_merge_kernel<T, D>), dim3(r.merge_units * blocks), dim3(256), 0, s, a, r.merge_units);
     NVQ_LAUNCH_CHECK("prompt_attention merge");
     return NVQ_OK;
 }
