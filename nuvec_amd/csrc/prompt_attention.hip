@@ -8,7 +8,8 @@ namespace {
 // Tiles of 32 keys of an item at least, where a block's keys are shared.
 constexpr int32_t kLeast = 4;
 
-int32_t target_of(const nvq_prompt_attention_desc &d) { return (prompt::padded_dim(d.head_dim) <= 128 ? 2 : 1) * compute_units(); }
+// Blocks that the chip holds.
+int32_t target_of(const nvq_prompt_attention_desc &d) { return prompt::blocks_of((int)dtype_size(d.dtype), prompt::padded_dim(d.head_dim)) * compute_units(); }
 // Units at most, whatever the starts on the device say: every sequence's last block of lines may be short.
 int64_t most_units(const nvq_prompt_attention_desc &d) {
     const int64_t lines = d.rows * (d.query_heads / d.key_heads);

@@ -28,8 +28,6 @@
 namespace nvq {
 namespace prompt {
 
-constexpr int kWaves = 4;
-constexpr int kMatrix = 8, kLdsRead = 0x100;  // kinds of instructions, of an order that the compiler is told to keep
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLowest = -3.4e38f;  // where maxima start (paged_rows_kernel.h says why it is finite)
 
@@ -117,7 +115,7 @@ __device__ __forceinline__ Span span_of(const PromptBatch &a, const PagedItem &i
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(const PromptArgs<T> a) {
+__global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) prompt_kernel(const PromptArgs<T> a) {
     using Of = Tile<T, D>;
     using Stage = typename Of::Stage;
     constexpr bool kWide = sizeof(T) == 4, kBf16 = Elem<T>::code == NVQ_BF16;
@@ -212,16 +210,19 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
         return s0 + row < S && run * RUN < a.dim;
     };
     float value_scale = 1.0f;  // (bfloat16; a power of two)
+    // A run of bfloat16 values times the scale, in bfloat16 (what falls below its normal range is far below float16's).
+    auto scaled = [&](uint4 w) __attribute__((always_inline)) {
+        uint32_t in[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) in[j] = f2u(u2f(in[j] << 16) * value_scale) >> 16 | (f2u(u2f(in[j] & 0xFFFF0000u) * value_scale) & 0xFFFF0000u);
+        return make_uint4(in[0], in[1], in[2], in[3]);
+    };
     // A run of values as operands: float16 for both 16-bit types.
-    auto operand = [&](uint4 w, bool scaled) __attribute__((always_inline)) {
+    auto operand = [&](uint4 w) __attribute__((always_inline)) {
         if constexpr (kBf16) {
             uint32_t in[4] = {w.x, w.y, w.z, w.w}, out[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                float x = u2f(in[j] << 16), y = u2f(in[j] & 0xFFFF0000u);
-                if (scaled) x *= value_scale, y *= value_scale;
-                out[j] = half_pair(x, y);
-            }
+            for (int j = 0; j < 4; j++) out[j] = half_pair(u2f(in[j] << 16), u2f(in[j] & 0xFFFF0000u));
             return make_uint4(out[0], out[1], out[2], out[3]);
         } else {
             return w;
@@ -232,13 +233,15 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
         place(i, row, run);
         return reinterpret_cast<uint4 *>(to.values + row * Of::kValueRow + 16 * run);
     };
-    // The tile's rows into a stage; (CAREFUL) its flag where a value is not finite there.
-    auto lay = [&](auto careful, Stage &to, uint32_t &flag, int s0) __attribute__((always_inline)) {
-        typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
-        float wild = 0.0f;
-        f16x2_t wild2 = {(_Float16)0.0f, (_Float16)0.0f};
+    // The tile's rows into a stage, in pieces: run i of the values and of the keys by turns.  First what takes a branch; last (CAREFUL) the stage's flag where a
+    // value is not finite there.
+    typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+    float wild;
+    f16x2_t wild2;
+    auto lay_first = [&](int s0) __attribute__((always_inline)) {
+        wild = 0.0f, wild2 = f16x2_t{(_Float16)0.0f, (_Float16)0.0f};
         if (__builtin_expect(!whole_rows || s0 + KT > S, 0)) {
-            asm volatile("");  // (a branch, the same for all; so is the next)
+            asm volatile("");  // (a branch, the same for all)
 #pragma unroll
             for (int i = 0; i < SHARE; i++) {
                 int row, run;
@@ -251,40 +254,46 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
         if (kBf16 && __builtin_expect(value_scale != 1.0f, 0)) {
             asm volatile("");
 #pragma unroll
-            for (int i = 0; i < SHARE; i++) vr[i] = operand(vr[i], true);
-        } else {
-#pragma unroll
-            for (int i = 0; i < SHARE; i++) vr[i] = operand(vr[i], false);
+            for (int i = 0; i < SHARE; i++) vr[i] = scaled(vr[i]);
         }
-#pragma unroll
-        for (int i = 0; i < SHARE; i++) {
-            int row, run;
-            place(i, row, run);
+    };
+    auto lay_piece = [&](auto careful, Stage &to, int piece) __attribute__((always_inline)) {
+        const int i = piece >> 1;
+        int row, run;
+        place(i, row, run);
+        if (piece & 1) {
             *reinterpret_cast<uint4 *>(to.keys + row * Of::kKeyRow + 16 * run) = kr[i];
-            *value_place(to, i) = vr[i];
-            if constexpr (!decltype(careful)::value) continue;
-            const uint4 w = vr[i];
-            if constexpr (kWide) {  // x 0 is NaN of what is not finite
-                wild = __builtin_fmaf(u2f(w.x), 0.0f, wild), wild = __builtin_fmaf(u2f(w.y), 0.0f, wild);
-                wild = __builtin_fmaf(u2f(w.z), 0.0f, wild), wild = __builtin_fmaf(u2f(w.w), 0.0f, wild);
-            } else {
-                const f16x2_t zero = {(_Float16)0.0f, (_Float16)0.0f};
-                wild2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, w.x), zero, wild2);
-                wild2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, w.y), zero, wild2);
-                wild2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, w.z), zero, wild2);
-                wild2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, w.w), zero, wild2);
-            }
+            return;
         }
+        const uint4 w = operand(vr[i]);
+        *value_place(to, i) = w;
+        if constexpr (!decltype(careful)::value) return;
+        if constexpr (kWide) {  // x 0 is NaN of what is not finite
+            wild = __builtin_fmaf(u2f(w.x), 0.0f, wild), wild = __builtin_fmaf(u2f(w.y), 0.0f, wild);
+            wild = __builtin_fmaf(u2f(w.z), 0.0f, wild), wild = __builtin_fmaf(u2f(w.w), 0.0f, wild);
+        } else {
+            const f16x2_t zero = {(_Float16)0.0f, (_Float16)0.0f};
+            wild2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, w.x), zero, wild2);
+            wild2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, w.y), zero, wild2);
+            wild2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, w.z), zero, wild2);
+            wild2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, w.w), zero, wild2);
+        }
+    };
+    auto lay_last = [&](auto careful, uint32_t &flag) __attribute__((always_inline)) {
+        if constexpr (!decltype(careful)::value) return;
         if constexpr (!kWide) wild = (float)wild2[0] + (float)wild2[1];
-        if (decltype(careful)::value && wild != wild) flag = 1u;
+        if (wild != wild) flag = 1u;
     };
 
     acc16_t o[ND];
+    float m, l;
+    auto clear = [&]() __attribute__((always_inline)) {
+        m = kLowest, l = 0.0f;
 #pragma unroll
-    for (int d = 0; d < ND; d++)
+        for (int d = 0; d < ND; d++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-    float m = kLowest, l = 0.0f;
+            for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+    };
 
     // V^T . P^T of 16 keys (float32: of two), their weights in `p` as the scores' accumulators hold them.
     auto value_run = [&](const Stage &from, int c, int d) __attribute__((always_inline)) {
@@ -319,8 +328,9 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
             half8_t v[2][ND];
             auto prepare = [&](int c, int j) __attribute__((always_inline)) {
                 const float e0 = weight(8 * c + 2 * j), e1 = weight(8 * c + 2 * j + 1);
-                high[c & 1][j] = half_pair(e0, e1);
-                if constexpr (!kBf16) low[c & 1][j] = half_pair(behind<0>(e0, high[c & 1][j]), behind<1>(e1, high[c & 1][j]));
+                uint32_t &h = high[c & 1][j];
+                h = half_pair(e0, e1);
+                if constexpr (!kBf16) low[c & 1][j] = half_pair(behind<0>(e0, h), behind<1>(e1, h));
             };
             auto operand_of = [&](const uint32_t (&w)[4]) __attribute__((always_inline)) { return __builtin_bit_cast(half8_t, make_uint4(w[0], w[1], w[2], w[3])); };
 #pragma unroll
@@ -343,31 +353,38 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
                 }
         }
     };
-    // One tile: the scores, one look at their maximum, the weights and their products.  x[t][i]: key 32 t + 8 (i / 4) + 4 half + i % 4.  `seen` (CAREFUL): a bit
-    // for each of these keys that has a weight.
-    auto tile = [&](const Stage &from, int s0, auto careful, uint32_t &seen) __attribute__((always_inline)) {
+    // One tile: the scores, one look at their maximum, the weights and their products.  x[t][i]: key 32 t + 8 (i / 4) + 4 half + i % 4 of the lane's line.
+    // The next tile is laid between the scores' products, whose keys are read kAhead products before them.  `seen` (CAREFUL): a bit for each of these
+    // keys that has a weight.
+    auto tile = [&](const Stage &from, Stage &next, int s0, auto careful, uint32_t &seen) __attribute__((always_inline)) {
+        constexpr int STEPS = TB * KS, PIECES = 2 * SHARE, kAhead = 8;
         float x[TB][16];
-        __builtin_amdgcn_s_setprio(1);
+        {
+            acc16_t s[TB];
 #pragma unroll
-        for (int t = 0; t < TB; t++) {
-            acc16_t s;
+            for (int t = 0; t < TB; t++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[i] = 0.0f;
-            const uint8_t *row = from.keys + (32 * t + col) * Of::kKeyRow + 16 * half;
+                for (int i = 0; i < 16; i++) s[t][i] = 0.0f;
+            uint4 k[STEPS];
+            auto read = [&](int step) __attribute__((always_inline)) {
+                k[step] = *reinterpret_cast<const uint4 *>(from.keys + (32 * (step / KS) + col) * Of::kKeyRow + 16 * half + 32 * (step % KS));
+            };
 #pragma unroll
-            for (int k = 0; k < KS; k++) s = scores32<T>(*reinterpret_cast<const uint4 *>(row + 32 * k), qf[k], s);
+            for (int step = 0; step < kAhead && step < STEPS; step++) read(step);
+            __builtin_amdgcn_s_setprio(1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < 16; i++) x[t][i] = s[i];
-        }
-        if constexpr (!kWide) {  // the rows' reads KS products ahead of them
-            constexpr int kAhead = KS < TB * KS ? KS : KS / 2;
-            __builtin_amdgcn_sched_group_barrier(kLdsRead, kAhead, 0);
+            for (int step = 0; step < STEPS; step++) {
+                s[step / KS] = scores32<T>(k[step], qf[step % KS], s[step / KS]);
+                if (step + kAhead < STEPS) read(step + kAhead);
 #pragma unroll
-            for (int k = kAhead; k < TB * KS; k++) {
-                __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(kLdsRead, 1, 0);
+                for (int piece = (PIECES * step + STEPS - 1) / STEPS; piece < (PIECES * (step + 1) + STEPS - 1) / STEPS; piece++) lay_piece(careful, next, piece);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_group_barrier(kMatrix, kAhead, 0);
+#pragma unroll
+            for (int t = 0; t < TB; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[t][i] = s[t][i];
         }
         __builtin_amdgcn_s_setprio(0);
         if (__builtin_expect(s0 + KT - 1 > all_last || s0 < all_first || s0 + KT > s_end, 0)) {
@@ -399,14 +416,10 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
         if (__builtin_expect(__any(fabsf(m) > 1048576.0f), 0)) {
             asm volatile("");
 #pragma unroll
-            for (int t = 0; t < TB; t++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) x[t][i] = x[t][i] * scale - m;
+            for (int i = 0; i < 16 * TB; i++) x[i >> 4][i & 15] = x[i >> 4][i & 15] * scale - m;
         } else {
 #pragma unroll
-            for (int t = 0; t < TB; t++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) x[t][i] = __builtin_fmaf(x[t][i], scale, -m);
+            for (int i = 0; i < 16 * TB; i++) x[i >> 4][i & 15] = __builtin_fmaf(x[i >> 4][i & 15], scale, -m);
         }
         weigh(from, x, careful, seen);
         __builtin_amdgcn_s_setprio(0);
@@ -474,12 +487,12 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
                 if (!used || !(fabsf(Elem<T>::load(t, j)) < INFINITY)) Elem<T>::store(t, j, 0.0f);
             uint4 w;
             __builtin_memcpy(&w, t, 16);
-            *value_place(to, i) = operand(w, true);
+            *value_place(to, i) = operand(kBf16 ? scaled(w) : w);
         }
         __syncthreads();
     };
     // What is not finite, to the lines that see it: by a product of ones at the places of one kind with ones at the keys that are seen.
-    auto add_wild = [&](Stage &to, int s0, uint32_t seen) __attribute__((always_inline)) {
+    auto add_wild = [&](Stage &to, int s0, const uint32_t &seen) __attribute__((always_inline)) {
         request_values(s0);
         for (int kind = 0; kind < 3; kind++) {
             __syncthreads();
@@ -526,36 +539,48 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
 
     // The keys of the item.  First without a look at what the values hold: where one is not finite, or has left float16's range, the sums of some line are
     // not finite, and the block walks its keys again with care.  (In one loop the rare paths' loads would be waited for in every tile.)
+    // Tile s lies in a stage while tile s + 1 is on its way through registers and tile s + 2 is requested; behind the item's last tile
+    // that one again (loads under a condition cost registers that spilled: 5% of the time).
     auto walk = [&](auto careful) __attribute__((always_inline)) {
         constexpr bool kCareful = decltype(careful)::value;
-        lay(careful, stages[0], flags[0], s_begin);
+        auto behind_of = [&](int s0) { return s0 + KT < s_end ? s0 + KT : s0; };
+        lay_first(s_begin);
+#pragma unroll
+        for (int piece = 0; piece < 2 * SHARE; piece++) lay_piece(careful, stages[0], piece);
+        lay_last(careful, flags[0]);
+        request(behind_of(s_begin));
         __syncthreads();
         int at = 0;
         for (int s0 = s_begin; s0 < s_end; s0 += KT) {
-            const bool more = s0 + KT < s_end;
-            bool wild = false;
+            const int next = behind_of(s0);
+            bool wild_tile = false;
             if constexpr (kCareful) {
                 if (uniform((int32_t)flags[at]) != 0) {
                     asm volatile("");
                     __syncthreads();
                     if (tid == 0) flags[at] = 0u;
-                    lay_again(stages[at], s0, wild);
+                    lay_again(stages[at], s0, wild_tile);
+                    request_values(next);
                 }
             }
-            if (__builtin_expect(more, 1)) request(s0 + KT);
             uint32_t seen = 0;
-            if (__builtin_expect(s0 <= any_last && s0 + KT > any_first, 1)) tile(stages[at], s0, careful, seen);  // (uniform in the wavefront)
-            if constexpr (kCareful) {
-                if (wild) {
-                    add_wild(stages[at], s0, seen);
-                    if (more) request(s0 + KT);
-                }
+            lay_first(next);
+            if (__builtin_expect(s0 <= any_last && s0 + KT > any_first, 1)) {  // (uniform in the wavefront)
+                tile(stages[at], stages[at ^ 1], s0, careful, seen);
+            } else {
+#pragma unroll
+                for (int piece = 0; piece < 2 * SHARE; piece++) lay_piece(careful, stages[at ^ 1], piece);
             }
-            if (__builtin_expect(more, 1)) lay(careful, stages[at ^ 1], flags[at ^ 1], s0 + KT);
+            lay_last(careful, flags[at ^ 1]);
+            if constexpr (kCareful) {
+                if (wild_tile) add_wild(stages[at], s0, seen);
+            }
+            request(behind_of(next));
             __syncthreads();
             at ^= 1;
         }
     };
+    clear();
     if (tid < 3) (tid < 2 ? flags[tid] : again) = 0u;
     if (s_begin < s_end) {
         request(s_begin);
@@ -567,7 +592,8 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
         }
         const float first_scale = value_scale;
         walk(std::false_type{});
-        float odd = l * 0.0f;
+        float odd = 0.0f;
+        odd = __builtin_fmaf(l, 0.0f, odd);
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -575,11 +601,8 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) prompt_kernel(c
         if (__any(odd != odd) && lane == 0) again = 1u;
         __syncthreads();
         if (__builtin_expect(uniform((int32_t)again) != 0, 0)) {
-#pragma unroll
-            for (int d = 0; d < ND; d++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-            m = kLowest, l = 0.0f, value_scale = first_scale;
+            clear();
+            value_scale = first_scale;
             request(s_begin);
             walk(std::true_type{});
         }
