@@ -147,21 +147,6 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
     const int all_last = uniform(last_of(w_first)), all_first = uniform(first_of(w_last));                    // keys up to / from which all of them see
     const int any_last = uniform(r0 < lines ? last_of(w_last) : -1), any_first = uniform(first_of(w_first));  // and any does
 
-    // Scores are kept positive multiples of the product: a negative scale's sign goes to the queries, and of a scale of 0 they are zeros.
-    const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
-    uint4 qf[KS];
-    {
-        const T *query = a.q + (int64_t)(item.s.start + my_row) * a.q_strides[0] + (int64_t)my_head * a.q_strides[1];
-        const uint32_t sign = a.scale < 0.0f ? (kWide ? 0x80000000u : 0x80008000u) : 0u, keep = a.scale == 0.0f ? 0u : ~0u;
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const int d = (2 * s + half) * RUN;
-            const uint4 w = load_run(query + (d < a.dim ? d : 0));
-            const uint32_t k = d < a.dim ? keep : 0u;
-            qf[s] = make_uint4((w.x ^ sign) & k, (w.y ^ sign) & k, (w.z ^ sign) & k, (w.w ^ sign) & k);
-        }
-    }
-
     // ── staging: run i of a thread is run tid + 256 i of the tile ──
     const int64_t first_key = a.batch.first_key(item.b);
     const T *keys = a.k + first_key * a.k_strides[0] + (int64_t)hk * a.k_strides[1], *values = a.v + first_key * a.v_strides[0] + (int64_t)hk * a.v_strides[1];
@@ -203,6 +188,21 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
         load_tile(kr, keys, a.k_strides[0], k_offset, s0);
         request_values(s0);
     };
+    if (s_begin < s_end) request(s_begin);  // (the queries come behind it)
+    // Scores are kept positive multiples of the product: a negative scale's sign goes to the queries, and of a scale of 0 they are zeros.
+    const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
+    uint4 qf[KS];
+    {
+        const T *query = a.q + (int64_t)(item.s.start + my_row) * a.q_strides[0] + (int64_t)my_head * a.q_strides[1];
+        const uint32_t sign = a.scale < 0.0f ? (kWide ? 0x80000000u : 0x80008000u) : 0u, keep = a.scale == 0.0f ? 0u : ~0u;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const int d = (2 * s + half) * RUN;
+            const uint4 w = load_run(query + (d < a.dim ? d : 0));
+            const uint32_t k = d < a.dim ? keep : 0u;
+            qf[s] = make_uint4((w.x ^ sign) & k, (w.y ^ sign) & k, (w.z ^ sign) & k, (w.w ^ sign) & k);
+        }
+    }
     // What lies behind the head's values and behind the sequence's end: zeros.
     auto real = [&](int s0, int i) __attribute__((always_inline)) {
         int row, run;
@@ -583,7 +583,6 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
     clear();
     if (tid < 3) (tid < 2 ? flags[tid] : again) = 0u;
     if (s_begin < s_end) {
-        request(s_begin);
         if constexpr (kBf16) {
             uint32_t top;
             bool wild;
