@@ -11,6 +11,8 @@
 // One wavefront a row.  A group has a power of two of the lanes, a lane V consecutive experts, so that (lane, place) is the experts' order and a group's
 // score a few exchanges among its lanes.  Values are compared as whole numbers of the same order, 0 for what is not to be chosen; a round's maximum is found
 // by data-parallel moves, its place by ballots, whose masks stay in scalar registers.
+#include <type_traits>
+
 #include "heads.h"
 #include "nvq_internal.h"
 #include "wave_reduce.h"
@@ -165,6 +167,24 @@ __device__ __forceinline__ int select_wide(const SelectArgs &a, const float (&l)
 // with the bias by half a step; a group's two twice that.  What is as near as this is decided again.
 constexpr float kNear = 1.0f / (1 << 19);
 
+// The weight of the expert that lane r of k has, from its logit.
+template <typename Real>
+__device__ __forceinline__ float weight_of(const SelectArgs &a, float x, float top, bool none, double total) {
+    constexpr bool kWide = sizeof(Real) == 8;
+    Real p = 0;
+    if ((int)(threadIdx.x & 63) < a.k) {
+        if constexpr (kWide) p = a.sigmoid ? 1.0 / (1.0 + exp(-(double)x)) : none ? 0.0 : exp((double)x - (double)top) / total;
+        else p = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exponential(-x)) : none ? 0.0f : exponential(x - top) * __builtin_amdgcn_rcpf((float)total);
+    }
+    if (a.normalize) {
+        auto add = [](Real x, Real y) { return x + y; };
+        const Real sum = (a.k <= 16 ? across<16>(p, add) : across<64>(p, add)) + (Real)1e-20;
+        if constexpr (kWide) p /= sum;
+        else p *= __builtin_amdgcn_rcpf(sum);
+    }
+    return (float)(p * (Real)a.scale);
+}
+
 // BIASED: c is computed; else the logits are compared, and nothing is in doubt but what is not a number.
 template <typename T, int V, bool BIASED>
 __global__ void __launch_bounds__(64 * kSelectWaves) moe_select_kernel(const SelectArgs a) {
@@ -265,60 +285,49 @@ __global__ void __launch_bounds__(64 * kSelectWaves) moe_select_kernel(const Sel
 #pragma unroll
         for (int j = 0; j < V; j++) key[j] = kept ? key[j] : 0u;
     }
-    int chosen = 0, keys = 0;  // lane r's of round r
-    if (!__any(doubt)) {
-        for (int r = 0;; r++) {
-            uint32_t best = key[0];
+    // A value's place among the wavefront's (V a lane, in the experts' order) replaces its key's low bits, the first the largest: a round is the largest key
+    // below the last one's, and holds its place.  Keys that have come wrap round to less than all others when the last is taken off.
+    constexpr uint32_t kPlaces = 64 * V - 1;
+    constexpr bool kWhole = !BIASED && sizeof(T) == 2;  // no key has lost a bit that it had
 #pragma unroll
-            for (int j = 1; j < V; j++) best = key[j] > best ? key[j] : best;
-            const uint32_t h = wave_largest(best);
-            const bool mine = lane == r;
-            keys = mine ? (int)h : keys;
-            if (r == a.k) break;  // (the one behind the last chosen is looked at too)
-            uint64_t has[V], any = 0;
+    for (int j = 0; j < V; j++) key[j] = key[j] == 0u ? 0u : (key[j] & ~kPlaces) | (kPlaces - (uint32_t)(lane * V + j));
+    int slot = 0;  // lane r's of round r
+    uint32_t h = 0;
+    auto round = [&]() __attribute__((always_inline)) {
+        uint32_t best = key[0] - h;
 #pragma unroll
-            for (int j = 0; j < V; j++) has[j] = __ballot(key[j] == h), any |= has[j];
-            const uint64_t at = any & -any;  // the first lane's
-            int place_of = 0;
-            uint64_t open = at;
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                const uint64_t here = open & has[j];
-                place_of = here != 0 ? j : place_of, open &= ~here;
-                key[j] = __builtin_amdgcn_inverse_ballot_w64(here) ? 0u : key[j];
-            }
-            const int expert = __builtin_amdgcn_readlane(place.first, __builtin_ctzll(at)) + place_of;
-            chosen = mine ? expert : chosen;
-            if (BIASED && r == 63) break;
-        }
-        if (BIASED) {  // neighbours among the chosen, and the one behind them
-            const uint32_t behind = (uint32_t)__shfl_down(keys, 1);
-            const float v = value_of((uint32_t)keys), w = value_of(behind);
-            doubt = (lane < a.k && lane < 63 && behind != 0u && !(w < v - kNear * (1.0f + fabsf(v)))) || a.k == 64;
-        }
+        for (int j = 1; j < V; j++) best = key[j] - h > best ? key[j] - h : best;
+        h += wave_largest(best);
+    };
+    for (int r = 0; r < a.k; r++) {
+        round();
+        slot = lane == r ? (int)(kPlaces - (h & kPlaces)) : slot;
     }
-    if (BIASED ? __any(doubt) : __any(wild != wild)) {
+    float2 *both = reinterpret_cast<float2 *>(held[wave]);  // logits, and what decided
+#pragma unroll
+    for (int j = 0; j < V; j++) both[lane * V + j] = make_float2(l[j], c[j]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const float2 mine_of = both[slot];
+    int chosen = __shfl(place.first, slot / V) + slot % V;
+    if (!kWhole) {
+        // What the keys have lost: those chosen have to be in order by themselves, and the last of them in front of all that the key behind it can stand for.
+        round();
+        const float v = mine_of.y, next = __shfl_down(v, 1), w = lane == a.k - 1 ? value_of(h | kPlaces) : next;
+        const bool last = lane == a.k - 1, sure = BIASED ? w < v - kNear * (1.0f + fabsf(v)) : last ? w < v : w <= v;
+        doubt |= lane < a.k && !sure && !(last && (h & ~kPlaces) == 0u);
+    }
+    float x = mine_of.x;
+    if (__any(doubt)) {
         asm volatile("");  // (a branch, the same for all lanes)
         chosen = select_wide<V>(a, l, place, held[wave]);
+        x = lane < a.k ? Elem<T>::load(logits, chosen) : 0.0f;
     }
-    // the weights, lane r's of round r: quotients and sums of 64 bits, over exponentials of float32 for 16-bit results
-    double p = 0.0;
-    if (lane < a.k) {
-        const float x = Elem<T>::load(logits, chosen);
-        const float from = a.sigmoid ? -x : x - top;
-        double e;
-        if constexpr (sizeof(T) == 4) e = exp(a.sigmoid ? -(double)x : (double)x - (double)top);
-        else e = (double)exponential(from);
-        p = a.sigmoid ? 1.0 / (1.0 + e) : none ? 0.0 : e / total;
-    }
-    if (a.normalize) {
-        auto add = [](double x, double y) { return x + y; };
-        const double sum = a.k <= 16 ? across<16>(p, add) : across<64>(p, add);
-        p /= sum + 1e-20;
-    }
+    // Results of 16 bits from float32, off by less than 2^-20, but where an exponential would leave its normal range; of 32 from 64 bits.
+    const bool far = lane < a.k && (a.sigmoid ? -x : top - x) > 80.0f;
+    const float weight = sizeof(T) == 4 || __builtin_expect(__any(far), 0) ? weight_of<double>(a, x, top, none, total) : weight_of<float>(a, x, top, none, total);
     if (lane < a.k) {
         a.indices[row * a.k + lane] = chosen;
-        Elem<T>::store((T *)a.weights, row * a.k + lane, (float)(p * a.scale));
+        Elem<T>::store((T *)a.weights, row * a.k + lane, weight);
     }
 }
 

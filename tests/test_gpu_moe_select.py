@@ -41,10 +41,12 @@ def check(logits, k, *args, **more):
     want, w = expected(logits, k, *args, **more)
     assert experts.dtype == torch.int32 and weights.dtype == logits.dtype and experts.shape == want.shape == weights.shape
     assert torch.equal(experts.cpu().long(), want)
-    # exp, the quotients and the sums are 64 bits wide; then float32's rounding and the type's
+    # Float32: exp, the quotients and the sums are 64 bits wide; then float32's rounding and the scale's.  16 bits: an exponential (2^-23, and the product with
+    # log2 e put back), a reciprocal twice (2^-23 each), a tree of six sums, three products and the rounding of the scale (2^-24 each): 8 steps of 2^-23 at
+    # most, 2^-20; then the type's rounding.
     got, t = weights.double().cpu(), logits.dtype
     both = got.isnan() & w.isnan()
-    assert (both | ((got - w).abs() <= (HALF[t] + 2.0 ** -23) * w.abs() + TINY[t])).all()
+    assert (both | ((got - w).abs() <= (HALF[t] + (2.0 ** -23 if t == torch.float32 else 2.0 ** -20)) * w.abs() + TINY[t])).all()
     return experts, weights
 
 
@@ -100,6 +102,54 @@ def test_neighbours_that_float32_does_not_tell_apart():
     x = torch.full((1, 8), 60.0, device="cuda")  # (beyond 64 bits' reach the logits themselves tell)
     x[0, 3] = 61.0
     assert nv.moe_select(x, 1, "sigmoid")[0].tolist() == [[3]]
+
+
+@pytest.mark.parametrize("e", [60, 128, 256, 512])
+def test_logits_a_few_steps_apart(e):
+    """Float32 logits that differ in their last bits alone, in any order, and pairs of equal ones among them."""
+    order = torch.randperm(e, generator=torch.Generator().manual_seed(e)).to("cuda").float()
+    for step in (2.0 ** -23, 2.0 ** -20, 2.0 ** -16):
+        x = torch.stack([1 + order * step, -1 - order * step, 1 + (order // 2) * step])
+        for k in (8, 33, min(e, 64)):
+            check(x, k)
+            check(x, k, "sigmoid")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_biases_that_all_but_meet(dtype, scores):
+    """Sums with the bias a part of a float32 step to many steps apart: among those chosen, behind the last of them, between groups."""
+    order = torch.randperm(256, generator=torch.Generator().manual_seed(7)).to("cuda").float()
+    x = normal(9, 256, dtype=dtype) * 0
+    for step in (2.0 ** -24, 2.0 ** -21, 2.0 ** -18, 2.0 ** -15):
+        bias = 0.25 + order * step
+        for k, groups, top in ((8, 1, 1), (64, 1, 1), (8, 8, 4), (8, 64, 9), (64, 4, 1)):
+            check(x, k, scores, bias, groups, top)
+            check(x, k, scores, bias, groups, top, 1)
+            check(normal(9, 256, dtype=dtype, seed=3, size=1e-6), k, scores, bias, groups, top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_biases_without_end(dtype):
+    """A bias of -inf masks an expert, one of inf brings it to the front."""
+    x, bias = normal(5, 64, dtype=dtype), normal(64, size=0.1)
+    bias[::3] = float("-inf")
+    check(x, 8, "sigmoid", bias)
+    check(x, 8, "softmax", bias, 4, 2)
+    bias[50] = float("inf")
+    experts, _ = nv.moe_select(x, 8, "sigmoid", bias)
+    assert (experts[:, 0] == 50).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_scores_far_from_one(dtype, scores):
+    """Weights of scores near and below the smallest normal number."""
+    x = normal(6, 32, dtype=dtype, size=2.0) - 88
+    x[3:, 7] = 40.0
+    for normalize in (True, False):
+        check(x, 6, scores, normalize=normalize)
+        check(x, 6, scores, torch.zeros(32, device="cuda"), normalize=normalize)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
