@@ -141,12 +141,15 @@ struct PairAxes {
             rows[i] = table + (p < 0 ? 0 : p < table_rows ? p : table_rows - 1) * half;
         }
         Turn t;
+        // Four pairs of a run where both of a pair lie in it, else eight.
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int j = j0 + i;
             t.c[i] = 1.0f, t.n[i] = 0.0f;
-            if (j < 2 * half) {
-                const bool second = interleaved ? (j & 1) != 0 : j >= half;
+            if (interleaved && (i & 1) != 0) {
+                t.c[i] = t.c[i - 1], t.n[i] = -t.n[i - 1];
+            } else if (j < 2 * half) {
+                const bool second = !interleaved && j >= half;
                 const int pair = interleaved ? j >> 1 : second ? j - half : j;
                 const uint32_t axis = axes.of_pairs[pair >> 4] >> (2 * (pair & 15)) & 3u;
                 const float2 a = (axis & 2u ? (axis & 1u ? rows[3] : rows[2]) : axis & 1u ? rows[1] : rows[0])[pair];
