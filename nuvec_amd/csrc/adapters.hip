@@ -10,7 +10,10 @@
 // Terms: x, down and up are exact operands.  t is two terms of the element type, high and low (16 bits in bfloat16, 22 in float16, there scaled by
 // a power of two into its range), side by side in one contraction of 32 beside 16 values of up twice; float32 runs on the float32 instruction.
 //
-// Both are bound by memory: the adapters' weights where there are few rows, x and y where there are many.
+// Both are bound by memory: the adapters' weights where there are few rows, x and y where there are many; a call of one row is two launches, 7.4 us.
+// Measured (bfloat16, us): 64 rows of 64 adapters of rank 16 beside [4096, 4096] 12.4 (kernels 5.6 and 7.8; the weights alone, 17 MB, at the rate of a large copy
+// 3.4); 4096 rows of four of rank 32 beside [14336, 4096] 90 (21 and 72; x, y and out, 268 MB, 55); float16, 517 rows of nine of rank 12 beside [2880, 2880] 14.5.
+// A product's tile goes through LDS so that y and out are moved in runs of 512 bytes a row: 64 bytes a row and wavefront took 140 us in the second of these.
 #include "matrix.h"
 #include "nvq_internal.h"
 
@@ -406,7 +409,9 @@ __global__ void __launch_bounds__(64 * kUpWaves, RW == 2 ? 3 : 4) adapters_up_ke
 
 // How the rows, columns and the contraction are dealt to blocks.
 struct Shape {
-    int32_t wide;          // tiles of 16 rows of a block: 2 where there are many rows, so that the adapters' weights are read half as often
+    // Tiles of 16 rows of a block: 2 where there are many rows, so that the adapters' weights are read half as often.  (4096 rows beside [14336, 4096] 90 us,
+    // with 1 113; 2048 beside [4096, 4096] 24.9 and 23.9, where the rule changes; 1024 23.4 with 2, 18.8 with 1; 64 rows 63 with 2, 12.4 with 1.)
+    int32_t wide;
     int32_t splits, down_slots, up_slots, chunks;
     int64_t tiles;
 };
@@ -419,10 +424,13 @@ Shape shape_of(const nvq_adapters_desc &d) {
     const int64_t most = d.adapters < 16 * s.wide ? d.adapters : 16 * s.wide, occurring = at_most(most < d.rows ? most : d.rows, 32);
     const int64_t step = d.dtype == NVQ_F32 ? 16 : 32, steps = (d.inputs + step - 1) / step;
     // A tile's adapters go to blocks of their own where the tiles alone leave compute units without work, and the contraction is split, four steps a
-    // wavefront at least.
+    // wavefront at least.  (The 64 rows: one block for all adapters 34 us, four 17, sixteen 12.6; one split 17.9, two 14.4, four 12.7, eight 12.7.  4096 rows:
+    // slots of 1, 4 and 8 89, 96 and 110, splits of 1, 2, 4 and 8 110, 92, 89 and 98.)
     s.down_slots = s.wide == 2 ? 1 : (int32_t)at_most(cus / s.tiles, occurring);
     s.splits = (int32_t)at_most(2 * cus / (s.tiles * s.down_slots), at_most(steps / (4 * kDownWaves), 16));
     const int64_t columns = (d.outputs + kBlockColumns - 1) / kBlockColumns;
+    // The second kernel: slots in the same way (the 64 rows: 1, 4, 8 and 16 21, 13.8, 12.5 and 12.7), and several times 256 columns a block, whose terms are then
+    // worked out once, where blocks are many (4096 rows: 1, 2 and 4 104, 90 and 90; the 64 rows: 2 and 4 13.4 and 17.3).
     s.up_slots = (int32_t)at_most(4 * cus / (s.tiles * columns), occurring);
     s.chunks = (int32_t)at_most(s.tiles * columns * s.up_slots / (4 * cus), 4);
     return s;

@@ -117,7 +117,8 @@ __device__ __forceinline__ Turn read_turn(const float2 *__restrict__ angles, int
 }
 
 // Rotations whose pairs belong to axes (time, height, width, ...): each axis has a position a token, pair i turns by the angle of its axis's.
-// A token's positions are a handful of words, the angles are gathered pair by pair, once for all heads that a block walks.
+// A token's positions are a handful of words, the angles are gathered pair by pair, once for all heads that a block walks.  (bfloat16, 2 x 2049 tokens, 40
+// heads of 128 with norms, three axes: 21.6 us, one position a token 20.2; float16, 3 x 1025 tokens, 16 heads of 80, neighbouring pairs, two axes: 7.4.)
 struct NoAxes {
     static constexpr bool kAny = false;
 };

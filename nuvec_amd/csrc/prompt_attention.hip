@@ -5,7 +5,9 @@ namespace nvq {
 
 namespace {
 
-// Tiles of 32 keys of an item at least, where a block's keys are shared.
+// Tiles of 32 keys of an item at least, where a block's keys are shared.  (bfloat16, 32 heads of 128 over 8 key heads: 61 rows over 512 keys 15.5 us, with eight
+// tiles 19.2, not shared 19.2; 300 rows over 1000 keys 27.9, 27.0 with eight, 30.4 with sixteen; one row over 32768 keys 39 us, not shared 640.  A target
+// of twice the blocks that the chip holds: 15.5, 34.7 and 54.)
 constexpr int32_t kLeast = 4;
 
 // Blocks that the chip holds.

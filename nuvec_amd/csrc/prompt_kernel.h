@@ -12,10 +12,26 @@
 // are exact in float16 within its range, below), in float16 two terms (22 bits), in float32 themselves.  Scores, maxima, sums and accumulators are float32.
 //
 // bfloat16 values as float16: a block's first tile tells their size; where it is far from 1 they are scaled by a power of two.  A later tile
-// that leaves float16's range is laid out again with the scale it needs, and the accumulators follow.
+// that leaves float16's range is laid out again with the scale it needs, and the accumulators follow.  Values far smaller than the first tile's keep the
+// step that the scale leaves them: at most 2^-21 of its largest.
 //
 // Masked keys (behind the sequence's end, in front of a row or outside its window) have no weight whatever their keys hold.  Values that are not finite
 // are zeros in the tile, so that lines that do not see them stay clean; the lines that do are given them afterwards.
+//
+// The bound is the instructions beside the products: 32 fused multiply-adds, exponentials (eight cycles each, others five and eight beside the other
+// wavefront's products), additions, 16 maxima and conversions a lane for 64 keys of a line, and as many again for the tile's way into LDS, whose conversion
+// four wavefronts share.  Two wavefronts a SIMD take turns on the matrix cores (three of heads of 64 values); what is
+// written between the products runs beside them: the next tile's way into LDS in those of the scores, the next keys' weights in those of the values.
+//
+// Measured (us; a large product of the types runs at 1235 and 1183 TFLOP/s): 8192 rows of 32 heads of 128 over 8 key heads in bfloat16 576 to 600, 916 to
+// 954 TFLOP/s; nine ragged prompts of up to 1500 rows in float16, 20 heads of 64, sinks and a window 67, 383 TFLOP/s; seven prompts of up to 61 rows 10.9,
+// a chain of first loads.  4096 rows of 16 heads over 4 (shorter, so that the last blocks weigh more): bfloat16 heads of 64 442 TFLOP/s, 128 640, 256 592;
+// float16 397, 537, 550; float32 87, 91, 70 (of 154).  One row over 32768 keys 39 us, 3.45 TB/s.
+//
+// Timed without its parts, the first of these: the tile's way into LDS 23 % (half of it the loads), the products of the values 15 %.  Tried and not kept: 64 lines a
+// wavefront at one a SIMD (690 us: one wavefront issues no more than an instruction in five cycles), blocks of eight wavefronts (3 % faster here, half
+// of the blocks empty in short prompts), tiles of 32 keys (652, at three wavefronts a SIMD 700 with spills), the branches of the rare cases in the loop
+// (714: their loads made every tile wait for its successor's).
 #pragma once
 
 #include <type_traits>

@@ -6,11 +6,15 @@
 // What is chosen is decided as by real numbers.  Without a bias (and groups by their best alone) c's order is the logits', and nothing is computed to find it.
 // Otherwise c is computed in float32, off by less than kNear: where two values that follow one another among the chosen, or at the border of what is chosen,
 // are further apart than that their order is certain, and where they are not (or a value is not finite) the row is decided again in 64 bits.  The
-// weights are computed in 64 bits, for the chosen alone.
+// weights are computed for the chosen alone, in 64 bits for float32 results.
 //
 // One wavefront a row.  A group has a power of two of the lanes, a lane V consecutive experts, so that (lane, place) is the experts' order and a group's
-// score a few exchanges among its lanes.  Values are compared as whole numbers of the same order, 0 for what is not to be chosen; a round's maximum is found
-// by data-parallel moves, its place by ballots, whose masks stay in scalar registers.
+// score a few exchanges among its lanes.  Values are compared as whole numbers of the same order, 0 for what is not to be chosen, whose low bits are their
+// places: a round is one maximum over the wavefront, by data-parallel moves, and knows whose it is.
+//
+// Bound by the vector unit's instructions, several hundred a row of 256 experts; memory would allow 1.9 us for the first of these.  Measured (us): 16384 rows of
+// 256 in eight groups, bfloat16, sigmoid, a bias 16.5 (all of it in 64 bits 35; ballots for a maximum's place, and weights of 64 bits 19.6; every lane's
+// values sorted beforehand 21.5); 1333 rows of 60 in float16 4.9 and eight rows of 256 4.6, a launch.
 #include <type_traits>
 
 #include "heads.h"

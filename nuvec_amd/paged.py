@@ -4,6 +4,7 @@
     cache = PagedCache.new(pages=4096, key_heads=8, page_size=64, head_dim=128)
     q = append_paged(cache, k, v, page_table, positions, sequences, rotation, q=q)
     y = paged_attention(q, cache, page_table, lengths, 128 ** -0.5)  # one row per sequence
+    y = prompt_attention(q, k, v, 128 ** -0.5, starts)               # whole prompts over their own keys and values, as the projections leave them
 
 A pool's pages are shared by all sequences: position p of sequence b lies in page `page_table[b, p // page_size]`.  Page tables, positions
 and lengths stay on the device and may change between replays of a captured graph.  All of it computes in libnuvec_hip.so.
@@ -468,7 +469,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     Rows that see nothing are zeros; rows of no sequence are left as they were in `out` (and undefined in a new result).  Keys and values that a row does
     not see may hold anything.
 
-    The softmax's weights hold 11 bits beside the 8 of a bfloat16 result (float16: 22, float32: 24), everything else is float32."""
+    The softmax's weights hold 11 bits beside the 8 of a bfloat16 result (float16: 22, float32: 24), everything else is float32.  Values of a bfloat16 sequence that
+    are far smaller than its others are taken to 2^-21 of the largest among the first 64 that a block of rows sees.  Keys and values of one head less than
+    2^24 elements apart.  Two calls at once have a workspace each."""
     y = (_lib._native or _lib.native()).prompt_attention(q, k, v, scale, query_starts, key_starts, sinks, causal, window, out)
     if y is not None:
         return y if out is None else out
@@ -501,6 +504,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     if window < 0 or (window > 0 and not causal):
         raise InvalidArgument(f"{op}: a window of {window}{'' if causal else ' without the causal mask'}")
     q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
+    if k.shape[0] > 1 and max(k.stride(0), v.stride(0)) >= 1 << 24:
+        raise Unsupported(f"{op}: keys {k.stride(0)} and values {v.stride(0)} elements apart (less than 2^24)")
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     elif out.dtype != q.dtype or out.shape != q.shape or out.stride(2) != 1:

@@ -315,6 +315,42 @@ def test_two_streams_at_once():
     assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
 
 
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.float16, 64), (torch.bfloat16, 96), (torch.float32, 72), (torch.float16, 200)])
+def test_keys_as_far_apart_as_they_may_be(dtype, dim):
+    """2^24 - 8 values between two keys: offsets within a tile need all of 32 bits."""
+    keys, step = 70, (1 << 24) - 8
+    room = torch.empty(keys * step, device="cuda", dtype=dtype)
+    q, k, v = make(30, keys, 4, 2, dim, dtype)
+    far = [room[1000 * i:].as_strided(t.shape, (step, dim, 1)).copy_(t) for i, t in enumerate((k, v))]
+    assert torch.equal(nv.prompt_attention(q, *far, 0.1), nv.prompt_attention(q, k, v, 0.1))
+    one = [room.as_strided((1, 2, dim), (1 << 30, dim, 1)) for _ in range(2)]  # (a single key may be as far from the next as it likes)
+    assert torch.equal(nv.prompt_attention(q[:1], *one, 0.1), nv.prompt_attention(q[:1], *(t.contiguous() for t in one), 0.1))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_values_without_end_in_shared_keys(dtype):
+    """Few rows over many keys, which several blocks share: one of them meets values that are not finite, seen by some rows alone."""
+    rows, length = 12, 4000
+    q, k, v = make(rows, length, 4, 1, 128, dtype)
+    plain = nv.prompt_attention(q, k, v, 0.05, window=3000)
+    v[-5, 0, 7], v[990, 0, 3], v[2000, 0, 9] = float("inf"), float("nan"), float("-inf")
+    got = nv.prompt_attention(q, k, v, 0.05, window=3000)
+    # row i sees the keys 989 + i to 3988 + i
+    last = length - rows + torch.arange(rows, device="cuda")
+    sees = {7: last >= length - 5, 3: (last >= 990) & (last - 3000 < 990), 9: last >= 2000}
+    for column, value in ((7, float("inf")), (3, float("nan")), (9, float("-inf"))):
+        of = got[..., column]
+        is_it = of.isnan() if value != value else of == value
+        assert torch.equal(is_it, sees[column][:, None].expand_as(is_it))
+    rest = torch.ones_like(got, dtype=torch.bool)
+    for column, seen in sees.items():
+        rest[..., column] &= ~seen[:, None]
+    clean = v.clone()
+    clean[-5, 0, 7], clean[990, 0, 3], clean[2000, 0, 9] = 0, 0, 0
+    want, bound = expected(q, k, clean, 0.05, [rows], [length], window=3000)
+    assert ((got.double() - want).abs() <= bound)[rest].all() and plain.isfinite().all()
+
+
 def test_offsets_beyond_32_bits():
     """Rows so far apart that the last ones lie beyond 2^32 values."""
     rows, step = 1100, 1 << 22

@@ -104,7 +104,8 @@ def test_no_cpu_path():
 
 @pytest.mark.parametrize("call", [
     lambda: prompt(q=Z(4, 2, 4), k=Z(4, 1, 4), v=Z(4, 1, 4)), lambda: prompt(q=Z(4, 2, 100), k=Z(4, 1, 100), v=Z(4, 1, 100)),
-    lambda: prompt(q=Z(4, 2, 264), k=Z(4, 1, 264), v=Z(4, 1, 264)), lambda: nv.moe_select(F(2, 2000), 2), lambda: nv.moe_select(F(2, 256), 65), lambda: nv.moe_select(F(2, 256), 2, groups=128)])
+    lambda: prompt(q=Z(4, 2, 264), k=Z(4, 1, 264), v=Z(4, 1, 264)), lambda: nv.moe_select(F(2, 2000), 2), lambda: nv.moe_select(F(2, 256), 65), lambda: nv.moe_select(F(2, 256), 2, groups=128),
+    lambda: prompt(k=Z((1 << 24) + 64).as_strided((2, 1, 64), (1 << 24, 64, 1)), v=Z(2, 1, 64), query_starts=ints(2), key_starts=ints(2))])
 def test_unsupported(call):
     with pytest.raises(nv.Unsupported):
         call()
@@ -161,6 +162,11 @@ def test_entry_points():
     d = t(rows=4)
     d.k_strides[0] = -1
     assert lib.nvq_prompt_attention(C.byref(d), one, one, one, None, None, None, one, one, None) == bad and "stride" in _lib.last_error()
+    d = t()
+    d.v_strides[0] = 1 << 24
+    assert lib.nvq_prompt_attention(C.byref(d), *none * 9) == un and "apart" in _lib.last_error()
+    d.keys = 1
+    assert lib.nvq_prompt_attention(C.byref(d), *none * 9) == ok
 
     axes = _lib.RotaryAxesC(3)
     r = _lib.HeadRopeDescC(_lib.BF16, 64, 32, 0, 0, 8, 0, 1)
