@@ -18,9 +18,10 @@
 // Masked keys (behind the sequence's end, in front of a row or outside its window) have no weight whatever their keys hold.  Values that are not finite
 // are zeros in the tile, so that lines that do not see them stay clean; the lines that do are given them afterwards.
 //
-// The bound is the instructions beside the products: 32 fused multiply-adds, exponentials (eight cycles each, others five and eight beside the other
-// wavefront's products), additions, 16 maxima and conversions a lane for 64 keys of a line, and as many again for the tile's way into LDS, whose conversion
-// four wavefronts share.  Two wavefronts a SIMD take turns on the matrix cores (three of heads of 64 values); what is
+// The bound of long prompts in bfloat16 is the chip's power limit, as it is a large product's: 1.7 GHz of 2.4 at matrix cores busy for 52 % of the cycles (a form that took 29 %
+// more cycles ran at 2.06 GHz and took 7 % longer).  That of small heads is the instructions beside the products: 32 fused multiply-adds, exponentials
+// (eight cycles each, others five, and eight beside the other wavefront's products), additions, 16 maxima and conversions a lane for 64 keys of a line, in
+// float16 48 more for the weights' second terms.  Two wavefronts a SIMD take turns on the matrix cores (three of heads of 64 values); what is
 // written between the products runs beside them: the next tile's way into LDS in those of the scores, the next keys' weights in those of the values.
 //
 // Measured (us; a large product of the types runs at 1235 and 1183 TFLOP/s): 8192 rows of 32 heads of 128 over 8 key heads in bfloat16 576 to 600, 916 to
