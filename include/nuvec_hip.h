@@ -462,7 +462,7 @@ NVQ_API int32_t nvq_paged_attention(const nvq_paged_attention_desc *desc, const 
  * query_starts[b] .. query_starts[b + 1] - 1 and keys key_starts[b] .. key_starts[b + 1] - 1 (i32 [sequences + 1], ascending); query_starts
  * NULL: one sequence of all rows; key_starts NULL: those of the rows, or one sequence's all keys.  Rows outside every sequence are left as
  * they were; starts outside the operands are clamped to them.  Keys and values of one head lie less than 2^24 elements apart.  `workspace`: the
- * size query's bytes (float32 states of splits of the keys), one call's at a time, NULL where it says 0. */
+ * size query's bytes (float32 states of splits of the keys), one call's at a time, NULL where it says 0.  out may be q. */
 NVQ_API size_t nvq_prompt_attention_workspace_bytes(const nvq_prompt_attention_desc *desc);
 NVQ_API int32_t nvq_prompt_attention(const nvq_prompt_attention_desc *desc, const void *q, const void *k, const void *v, const int32_t *query_starts,
                              const int32_t *key_starts, const void *sinks, void *out, void *workspace, void *stream);

@@ -28,6 +28,7 @@ struct PromptBatch {
 struct PromptLaunch {
     PromptBatch batch;
     uint32_t grid, merge_units;  // merge_units 0: nothing can be split
+    int32_t slots;               // states that the workspace holds
 };
 
 int32_t launch_bf16(const nvq_prompt_attention_desc &d, const PromptAttentionOperands &o, const PromptLaunch &r, hipStream_t s);

@@ -56,7 +56,7 @@ struct PromptArgs {
     int32_t *length;  // of the plan, for the merge; NULL: no merge
     float *states;    // [slots][kLines][D + 4]: maximum of the base-2 scores, denominator, two unused, D weighted means
     int64_t q_strides[2], k_strides[2], v_strides[2], out_strides[2];
-    int32_t dim;
+    int32_t dim, slots;  // (starts that are not ascending may ask for more states than there are: those are left out)
     float scale;
 };
 
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
     auto last_of = [&](int i) { return a.batch.causal ? S - n + i : S - 1; };
     auto first_of = [&](int i) { return window > 0 && a.batch.causal ? last_of(i) - window + 1 : 0; };
     const Span span = span_of(a.batch, item, part);
-    if (item.split >= span.items) return;
+    if (item.split >= span.items || (span.items > 1 && item.slot >= a.slots)) return;
     const int s_begin = uniform(span.begin + item.split * span.keys), s_end = uniform(span.end < s_begin + span.keys ? span.end : s_begin + span.keys);
     // the wavefront's lines
     const int r0 = part * kLines + wave * 32, r = r0 + col;
@@ -722,7 +722,9 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptArgs<T> a
     const int at = (int)threadIdx.x % kThreads * 4;
     const int part = item.s.parts - 1 - item.part;  // (items count the parts from the last)
     const Span span = span_of(a.batch, item, part);
-    if ((int)threadIdx.x >= kMergeLines<D> * kThreads || span.items == 1 || at >= a.dim) return;
+    if ((int)threadIdx.x >= kMergeLines<D> * kThreads || span.items == 1 || at >= a.dim ||
+        item.slot + (span.items - 1) * a.batch.key_heads >= a.slots)
+        return;
     for (int first = (int)(blockIdx.x / units) * kMergeLines<D>; first < kLines; first += (int)(gridDim.x / units) * kMergeLines<D>)
         merge_line<T, D>(a, item, span, part, first + (int)threadIdx.x / kThreads, at);
 }
@@ -748,7 +750,7 @@ int32_t launch_type(const nvq_prompt_attention_desc &d, const PromptAttentionOpe
     a.states = o.workspace == nullptr ? nullptr : (float *)((uint8_t *)o.workspace + kPlanBytes);
     for (int i = 0; i < 2; i++)
         a.q_strides[i] = d.q_strides[i], a.k_strides[i] = d.k_strides[i], a.v_strides[i] = d.v_strides[i], a.out_strides[i] = d.out_strides[i];
-    a.dim = d.head_dim, a.scale = d.scale;
+    a.dim = d.head_dim, a.slots = r.slots, a.scale = d.scale;
     switch (padded_dim(d.head_dim)) {
     case 64: return launch_sized<T, 64>(a, r, s);
     case 96: return launch_sized<T, 96>(a, r, s);

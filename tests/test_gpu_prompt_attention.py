@@ -1,8 +1,11 @@
 """Attention of whole prompts over dense keys and values (csrc/prompt_kernel.h) against 64 bits."""
+import ctypes as C
+
 import pytest
 import torch
 
 import nuvec_amd as nv
+from nuvec_amd import _lib
 from tests.paged_reference import HALF, TINY
 
 pytestmark = pytest.mark.gpu
@@ -299,6 +302,34 @@ def test_captured_calls_follow_their_starts():
         assert torch.equal(outs[0][:n], outs[2][:n]) and torch.equal(outs[1][:n], outs[2][:n])
         want, bound = expected(q, k, v, 0.1, rows, lengths)
         assert ((outs[2].double() - want).abs() <= bound)[:n].all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_results_in_place_of_the_queries(dtype):
+    for rows, lengths in (([150, 1, 70], [150, 1, 70]), ([20], [3000]), ([130], [0])):
+        q, k, v = make(sum(rows), sum(lengths), 6, 2, 128, dtype)
+        starts = ints(starts_of(rows)), ints(starts_of(lengths))
+        want = nv.prompt_attention(q, k, v, 0.1, *starts)
+        assert nv.prompt_attention(q, k, v, 0.1, *starts, out=q) is q and torch.equal(q, want)
+
+
+def test_starts_that_are_not_ascending_stay_in_the_workspace():
+    """Sequences that cover the same rows again and again, split over their keys: more states than the workspace has room for."""
+    rows, keys, sequences = 300, 5000, 41
+    q, k, v = make(rows, keys, 8, 2, 128, torch.bfloat16)
+    starts, key_starts = (ints([n * (i % 2) for i in range(sequences + 1)]) for n in (rows, keys))
+    d = _lib.PromptAttentionDescC(_lib.BF16, 128, rows, keys, 8, 2, sequences)
+    for i in range(2):
+        d.q_strides[i], d.k_strides[i], d.v_strides[i], d.out_strides[i] = q.stride(i), k.stride(i), v.stride(i), q.stride(i)
+    d.causal, d.scale = 1, 0.1
+    lib = _lib.load()
+    need = lib.nvq_prompt_attention_workspace_bytes(C.byref(d))
+    room = torch.full((need + (64 << 20),), 77, dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(q)
+    p = lambda t: C.c_void_p(t.data_ptr())
+    _lib.check(lib.nvq_prompt_attention(C.byref(d), p(q), p(k), p(v), p(starts), p(key_starts), None, p(out), p(room), C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    torch.cuda.synchronize()
+    assert need > 0 and (room[need:] == 77).all()
 
 
 def test_two_streams_at_once():
