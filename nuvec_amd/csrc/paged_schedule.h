@@ -161,6 +161,17 @@ __device__ __forceinline__ bool paged_find(const Batch &a, const PagedPlan &p, i
     return false;
 }
 
+// Item or unit `at` of a plan.
+template <int LINES, int KIND, bool UNITS, typename Batch>
+__device__ __forceinline__ bool paged_item_of(const Batch &a, const PagedPlan &plan, int lane, const PagedSequence &first, int32_t at, PagedItem &item) {
+    const bool found = at < plan.items && paged_find<LINES, KIND, UNITS>(a, plan, lane, first, at, item);
+    if (uniform(found) == 0) return false;
+    const PagedSequence &s = item.s;
+    item = PagedItem{{uniform(s.start), uniform(s.rows), uniform(s.length), uniform(s.base), uniform(s.tiles), uniform(s.parts)},
+                     uniform(item.b), uniform(item.splits), uniform(item.per), uniform(item.part), uniform(item.split), uniform(item.head), uniform(item.slot)};
+    return true;
+}
+
 // Item (or unit, which comes after the items) `at` of the whole plan; false behind the last.  `length`: where the first block of the items leaves the
 // plan's length for the units'; NULL: nothing is split.
 template <int LINES, int KIND, bool UNITS, typename Batch>
@@ -173,12 +184,7 @@ __device__ __forceinline__ bool paged_item(const Batch &a, int lane, int32_t at,
         plan = paged_plan<LINES, KIND>(a, lane, first);
         if (at == 0 && threadIdx.x == 0 && length != nullptr) *length = plan.per;
     }
-    const bool found = at < plan.items && paged_find<LINES, KIND, UNITS>(a, plan, lane, first, at, item);
-    if (uniform(found) == 0) return false;
-    const PagedSequence &s = item.s;
-    item = PagedItem{{uniform(s.start), uniform(s.rows), uniform(s.length), uniform(s.base), uniform(s.tiles), uniform(s.parts)},
-                     uniform(item.b), uniform(item.splits), uniform(item.per), uniform(item.part), uniform(item.split), uniform(item.head), uniform(item.slot)};
-    return true;
+    return paged_item_of<LINES, KIND, UNITS>(a, plan, lane, first, at, item);
 }
 
 }  // namespace

@@ -25,7 +25,7 @@
 // written between the products runs beside them: the next tile's way into LDS in those of the scores, the next keys' weights in those of the values.
 //
 // Measured (us; a large product of the types runs at 1235 and 1183 TFLOP/s): 8192 rows of 32 heads of 128 over 8 key heads in bfloat16 576 to 600, 916 to
-// 954 TFLOP/s; nine ragged prompts of up to 1500 rows in float16, 20 heads of 64, sinks and a window 67, 383 TFLOP/s; seven prompts of up to 61 rows 10.9,
+// 954 TFLOP/s; nine ragged prompts of up to 1500 rows in float16, 20 heads of 64, sinks and a window 67, 383 TFLOP/s; seven prompts of up to 61 rows 9.5,
 // a chain of first loads.  4096 rows of 16 heads over 4 (shorter, so that the last blocks weigh more): bfloat16 heads of 64 442 TFLOP/s, 128 640, 256 592;
 // float16 397, 537, 550; float32 87, 91, 70 (of 154).  One row over 32768 keys 39 us, 3.45 TB/s.
 //
@@ -41,6 +41,7 @@
 #include "nvq_device.h"
 #include "nvq_internal.h"
 #include "prompt_attention.h"
+#include "wave_reduce.h"
 
 namespace nvq {
 namespace prompt {
@@ -145,7 +146,11 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
     __shared__ uint32_t most[2][kWaves];      // of a tile that is laid out again: the largest finite value's bits; whether one is not finite
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
     PagedItem item;
-    if (!paged_item<kLines, 1, false>(a.batch, lane, blockIdx.x, a.length, item)) return;
+    if (a.length != nullptr) {
+        if (!paged_item<kLines, 1, false>(a.batch, lane, blockIdx.x, a.length, item)) return;
+    } else if (!paged_item_of<kLines, 1, false>(a.batch, PagedPlan{1 << 26, INT32_MAX}, lane, paged_sequence<kLines, 1>(a.batch, lane), blockIdx.x, item)) {
+        return;  // (nothing is split: no plan to work out)
+    }
     const int rep = a.batch.rep, hk = item.head, S = item.s.length, n = item.s.rows;
     const int part = item.s.parts - 1 - item.part;  // (the lines that see most first)
     const int lines = n * rep;
@@ -601,9 +606,27 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
     if (tid < 3) (tid < 2 ? flags[tid] : again) = 0u;
     if (s_begin < s_end) {
         if constexpr (kBf16) {
-            uint32_t top;
-            bool wild;
-            survey(s_begin, top, wild);
+            // The largest value, two at a time; what lies behind the keys or the head is a copy of others.  (With one that is not finite: in full.)
+            typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+            u16x2_t largest = {0, 0};
+#pragma unroll
+            for (int i = 0; i < SHARE; i++) {
+                const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2_t, w[j] & 0x7FFF7FFFu));
+            }
+            uint32_t top = wave_largest(largest[0] > largest[1] ? largest[0] : largest[1]);
+            if (lane == 0) most[0][wave] = top;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) top = most[0][w] > top ? most[0][w] : top;
+            top = (uint32_t)uniform((int32_t)top) << 16;
+            if (top >= 0x7F800000u) {
+                asm volatile("");
+                bool wild;
+                __syncthreads();
+                survey(s_begin, top, wild);
+            }
             value_scale = scale_for(top);
         }
         const float first_scale = value_scale;

@@ -36,21 +36,6 @@ struct SelectArgs {
     double scale;
 };
 
-// The larger of own and moved whole numbers; 0 from lanes that feed nothing.
-template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t larger(uint32_t v) {
-    const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, true);
-    return v > other ? v : other;
-}
-__device__ __forceinline__ uint32_t wave_largest(uint32_t v) {
-    v = larger<0x111, 0xF>(v);
-    v = larger<0x112, 0xF>(v);
-    v = larger<0x114, 0xF>(v);
-    v = larger<0x118, 0xF>(v);
-    v = larger<0x142, 0xA>(v);
-    v = larger<0x143, 0xC>(v);
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
-}
-
 // Whole numbers in the values' order, above 1; a NaN is 1.
 __device__ __forceinline__ uint32_t ordered(float v) {
     const uint32_t b = f2u(v + 0.0f);  // (-0 is 0)

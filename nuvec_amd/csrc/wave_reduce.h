@@ -39,6 +39,20 @@ __device__ __forceinline__ float wave_max_lane63(float v) {
     v = dpp_max<0x142, 0xA>(v);
     return dpp_max<0x143, 0xC>(v);
 }
+// The larger of own and moved whole numbers; 0 from lanes that feed nothing.
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t larger(uint32_t v) {
+    const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, true);
+    return v > other ? v : other;
+}
+__device__ __forceinline__ uint32_t wave_largest(uint32_t v) {
+    v = larger<0x111, 0xF>(v);
+    v = larger<0x112, 0xF>(v);
+    v = larger<0x114, 0xF>(v);
+    v = larger<0x118, 0xF>(v);
+    v = larger<0x142, 0xA>(v);
+    v = larger<0x143, 0xC>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
 __device__ __forceinline__ float from_lane(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
 
 }  // namespace
