@@ -12,7 +12,7 @@
 //
 // Both are bound by memory: the adapters' weights where there are few rows, x and y where there are many; a call of one row is two launches, 7.4 us.
 // Measured (bfloat16, us): 64 rows of 64 adapters of rank 16 beside [4096, 4096] 12.4 (kernels 5.6 and 7.8; the weights alone, 17 MB, at the rate of a large copy
-// 3.4); 4096 rows of four of rank 32 beside [14336, 4096] 90 (21 and 72; x, y and out, 268 MB, 55); float16, 517 rows of nine of rank 12 beside [2880, 2880] 14.5.
+// 3.4); 4096 rows of four of rank 32 beside [14336, 4096] 88 (19 and 70; x, y and out, 268 MB, 55); float16, 517 rows of nine of rank 12 beside [2880, 2880] 14.5.
 // A product's tile goes through LDS so that y and out are moved in runs of 512 bytes a row: 64 bytes a row and wavefront took 140 us in the second of these.
 #include "matrix.h"
 #include "nvq_internal.h"
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(64 * kUpWaves, RW == 2 ? 3 : 4) adapters_up_ke
 // How the rows, columns and the contraction are dealt to blocks.
 struct Shape {
     // Tiles of 16 rows of a block: 2 where there are many rows, so that the adapters' weights are read half as often.  (4096 rows beside [14336, 4096] 90 us,
-    // with 1 113; 2048 beside [4096, 4096] 24.9 and 23.9, where the rule changes; 1024 23.4 with 2, 18.8 with 1; 64 rows 63 with 2, 12.4 with 1.)
+    // with 1 113; 2048 beside [4096, 4096] 21.7 and 23.6, where the rule changes; 1024 23.4 with 2, 18.8 with 1; 64 rows 63 with 2, 12.4 with 1.)
     int32_t wide;
     int32_t splits, down_slots, up_slots, chunks;
     int64_t tiles;
@@ -429,10 +429,11 @@ Shape shape_of(const nvq_adapters_desc &d) {
     s.down_slots = s.wide == 2 ? 1 : (int32_t)at_most(cus / s.tiles, occurring);
     s.splits = (int32_t)at_most(2 * cus / (s.tiles * s.down_slots), at_most(steps / (4 * kDownWaves), 16));
     const int64_t columns = (d.outputs + kBlockColumns - 1) / kBlockColumns;
-    // The second kernel: slots in the same way (the 64 rows: 1, 4, 8 and 16 21, 13.8, 12.5 and 12.7), and several times 256 columns a block, whose terms are then
-    // worked out once, where blocks are many (4096 rows: 1, 2 and 4 104, 90 and 90; the 64 rows: 2 and 4 13.4 and 17.3).
+    // The second kernel: slots in the same way (the 64 rows: 1, 4, 8 and 16 21, 13.8, 12.5 and 12.7), and two or three times 256 columns a block, whose terms are
+    // then worked out once, where blocks are several times what the chip holds (4096 rows beside [14336, 4096]: 1, 2, 3, 4 and 6 times 103, 90.8, 87.5, 89.4 and
+    // 92.5; 2048 beside [4096, 4096] 24.6, 21.6, 24.8 and 26.4; 1024, in blocks of 16 rows, 18.9, 20.2 and 23; the 64 rows 12.5, 13.3 and 15.5).
     s.up_slots = (int32_t)at_most(4 * cus / (s.tiles * columns), occurring);
-    s.chunks = (int32_t)at_most(s.tiles * columns * s.up_slots / (4 * cus), 4);
+    s.chunks = (int32_t)at_most(s.tiles * columns * s.up_slots / ((s.wide == 2 ? 2 : 4) * cus), 3);
     return s;
 }
 int32_t padded_rank(const nvq_adapters_desc &d) { return (d.rank + 15) / 16 * 16; }

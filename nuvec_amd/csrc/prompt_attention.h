@@ -29,6 +29,7 @@ struct PromptLaunch {
     PromptBatch batch;
     uint32_t grid, merge_units;  // merge_units 0: nothing can be split
     int32_t slots;               // states that the workspace holds
+    int32_t turn, back;          // where the order of blocks turns back (turned), and for how many: eights
 };
 
 int32_t launch_bf16(const nvq_prompt_attention_desc &d, const PromptAttentionOperands &o, const PromptLaunch &r, hipStream_t s);

@@ -49,6 +49,9 @@ int32_t launch_prompt_attention(const nvq_prompt_attention_desc &d, const Prompt
     const int64_t full = b.target, spare = full / 2 + units, items = full > spare ? full : spare;
     r.grid = (uint32_t)(units * splits < items ? units * splits : items);
     r.slots = split ? (int32_t)most_states(d) : 0;
+    // (the last of the units that short sequences might have are seldom there)
+    const int32_t cus = compute_units() & ~7;
+    if (full > cus && units > cus && units <= full + cus / 4) r.turn = cus, r.back = (int32_t)(units < 2 * cus ? units : 2 * cus) - cus & ~7;
     r.merge_units = split ? (uint32_t)(units < full ? units : full) : 0;
     if (d.dtype == NVQ_F32) return prompt::launch_f32(d, o, r, s);
     return d.dtype == NVQ_BF16 ? prompt::launch_bf16(d, o, r, s) : prompt::launch_f16(d, o, r, s);

@@ -26,8 +26,8 @@
 //
 // Measured (us; a large product of the types runs at 1235 and 1183 TFLOP/s): 8192 rows of 32 heads of 128 over 8 key heads in bfloat16 576 to 600, 916 to
 // 954 TFLOP/s; nine ragged prompts of up to 1500 rows in float16, 20 heads of 64, sinks and a window 67, 383 TFLOP/s; seven prompts of up to 61 rows 9.5,
-// a chain of first loads.  4096 rows of 16 heads over 4 (shorter, so that the last blocks weigh more): bfloat16 heads of 64 442 TFLOP/s, 128 640, 256 592;
-// float16 397, 537, 550; float32 87, 91, 70 (of 154).  One row over 32768 keys 39 us, 3.45 TB/s.
+// a chain of first loads.  4096 rows of 16 heads over 4 (512 blocks, all on the chip at once): bfloat16 heads of 64 454 TFLOP/s, 128 669, 256 611;
+// float16 425, 573, 558; float32 112, 125, 71 (of 154).  One row over 32768 keys 39 us, 3.45 TB/s.
 //
 // Timed without its parts, the first of these: the tile's way into LDS 23 % (half of it the loads), the products of the values 15 %.  Tried and not kept: 64 lines a
 // wavefront at one a SIMD (690 us: one wavefront issues no more than an instruction in five cycles), blocks of eight wavefronts (3 % faster here, half
@@ -57,7 +57,7 @@ struct PromptArgs {
     int32_t *length;  // of the plan, for the merge; NULL: no merge
     float *states;    // [slots][kLines][D + 4]: maximum of the base-2 scores, denominator, two unused, D weighted means
     int64_t q_strides[2], k_strides[2], v_strides[2], out_strides[2];
-    int32_t dim, slots;  // (starts that are not ascending may ask for more states than there are: those are left out)
+    int32_t dim, turn, back, slots;  // (starts that are not ascending may ask for more states than there are: those are left out)
     float scale;
 };
 
@@ -132,6 +132,15 @@ __device__ __forceinline__ Span span_of(const PromptBatch &a, const PagedItem &i
     return s;
 }
 
+// The item of a block.  Items come with the longest of a sequence first, a block on each compute unit in turn, and where they are all on the chip at once the unit
+// that has the longest would have the longest of the second turn too: the second turn goes back, eight at a time, so that a key head stays with its XCD.
+// (4096 rows of 16 heads over 4: float32, 128 values 742 -> 549 us, bfloat16 104.3 -> 100.6, float16, 64 values 83.0 -> 76.9; where more blocks follow, which
+// go where one has ended, it is of no use: 3000 rows of 32 heads over 8 93.2 and 94.1.)
+__device__ __forceinline__ int32_t turned(uint32_t block, int32_t turn, int32_t back) {
+    const int32_t r = (int32_t)block - turn;
+    return r >= 0 && r < back ? turn + back - 8 - (r & ~7) + (r & 7) : (int32_t)block;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) prompt_kernel(const PromptArgs<T> a) {
     using Of = Tile<T, D>;
@@ -146,9 +155,10 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
     __shared__ uint32_t most[2][kWaves];      // of a tile that is laid out again: the largest finite value's bits; whether one is not finite
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
     PagedItem item;
+    const int32_t at_item = turned(blockIdx.x, a.turn, a.back);
     if (a.length != nullptr) {
-        if (!paged_item<kLines, 1, false>(a.batch, lane, blockIdx.x, a.length, item)) return;
-    } else if (!paged_item_of<kLines, 1, false>(a.batch, PagedPlan{1 << 26, INT32_MAX}, lane, paged_sequence<kLines, 1>(a.batch, lane), blockIdx.x, item)) {
+        if (!paged_item<kLines, 1, false>(a.batch, lane, at_item, a.length, item)) return;
+    } else if (!paged_item_of<kLines, 1, false>(a.batch, PagedPlan{1 << 26, INT32_MAX}, lane, paged_sequence<kLines, 1>(a.batch, lane), at_item, item)) {
         return;  // (nothing is split: no plan to work out)
     }
     const int rep = a.batch.rep, hk = item.head, S = item.s.length, n = item.s.rows;
@@ -773,7 +783,7 @@ int32_t launch_type(const nvq_prompt_attention_desc &d, const PromptAttentionOpe
     a.states = o.workspace == nullptr ? nullptr : (float *)((uint8_t *)o.workspace + kPlanBytes);
     for (int i = 0; i < 2; i++)
         a.q_strides[i] = d.q_strides[i], a.k_strides[i] = d.k_strides[i], a.v_strides[i] = d.v_strides[i], a.out_strides[i] = d.out_strides[i];
-    a.dim = d.head_dim, a.slots = r.slots, a.scale = d.scale;
+    a.dim = d.head_dim, a.turn = r.turn, a.back = r.back, a.slots = r.slots, a.scale = d.scale;
     switch (padded_dim(d.head_dim)) {
     case 64: return launch_sized<T, 64>(a, r, s);
     case 96: return launch_sized<T, 96>(a, r, s);
