@@ -51,12 +51,6 @@ __device__ __forceinline__ uint32_t ordered_number(float v) {  // (of what is a 
 }
 __device__ __forceinline__ float value_of(uint32_t key) { return u2f(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key); }
 
-__device__ __forceinline__ double from_lane(double v, int lane) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
-    return __builtin_bit_cast(double, (uint64_t)lo | (uint64_t)hi << 32);
-}
-
 // exp(x) with the product's rounding put back: off by a step of float32.
 __device__ __forceinline__ float exponential(float x) {
     constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
