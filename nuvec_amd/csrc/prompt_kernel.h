@@ -8,15 +8,14 @@
 // O^T = V^T . P^T, whose V is read from LDS through the transposing read in the order in which the lanes hold the keys.  float32 runs the same way on
 // v_mfma_f32_32x32x2_f32.
 //
-// Terms.  Queries and keys are exact operands.  The weights: in bfloat16 one term of float16 (11 bits beside the result's 8; the values, 8 bits,
-// are exact in float16 within its range, below), in float16 two terms (22 bits), in float32 themselves.  Scores, maxima, sums and accumulators are float32.
+// Terms.  Queries, keys and values are exact operands in their own type.  The weights are two terms of it, 16 bits in bfloat16 and 22 in float16 (one term
+// leaves an error beside the result's own rounding), in float32 themselves.  Scores, maxima, sums and accumulators are float32.  bfloat16 values as float16
+// operands would take one term, but a power of two that brings a tile's values into float16's range is one for lines that see the largest of them and for
+// lines that do not, whose own would be lost.
 //
-// bfloat16 values as float16: a block's first tile tells their size; where it is far from 1 they are scaled by a power of two.  A later tile
-// that leaves float16's range is laid out again with the scale it needs, and the accumulators follow.  Values far smaller than the first tile's keep the
-// step that the scale leaves them: at most 2^-21 of its largest.
-//
-// Masked keys (behind the sequence's end, in front of a row or outside its window) have no weight whatever their keys hold.  Values that are not finite
-// are zeros in the tile, so that lines that do not see them stay clean; the lines that do are given them afterwards.
+// Masked keys (behind the sequence's end, in front of a row or outside its window) have no weight whatever their keys hold.  A block whose sums are not finite
+// walks its keys again: values that are not finite are zeros in the tile then, so that lines that do not see them stay clean, and the lines that do are given them
+// afterwards; and the weights are 2^-32 at most, so that sums of the largest finite values stay finite.
 //
 // The bound of long prompts in bfloat16 is the chip's power limit, as it is a large product's: 1.7 GHz of 2.4 at matrix cores busy for 52 % of the cycles (a form that took 29 %
 // more cycles ran at 2.06 GHz and took 7 % longer).  That of small heads is the instructions beside the products: 32 fused multiply-adds, exponentials
@@ -41,7 +40,6 @@
 #include "nvq_device.h"
 #include "nvq_internal.h"
 #include "prompt_attention.h"
-#include "wave_reduce.h"
 
 namespace nvq {
 namespace prompt {
@@ -83,7 +81,7 @@ struct Tile {
 };
 
 template <typename T>
-__device__ __forceinline__ acc16_t scores32(uint4 k, uint4 q, acc16_t c) {
+__device__ __forceinline__ acc16_t product32(uint4 k, uint4 q, acc16_t c) {
     if constexpr (Elem<T>::code == NVQ_BF16) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, k), __builtin_bit_cast(bf16x8_t, q), c, 0, 0, 0);
     } else if constexpr (Elem<T>::code == NVQ_F16) {
@@ -96,15 +94,20 @@ __device__ __forceinline__ acc16_t scores32(uint4 k, uint4 q, acc16_t c) {
     }
 }
 
-__device__ __forceinline__ uint32_t half_pair(float a, float b) {
+// Two values as a pair of the (16-bit) element type.
+template <typename T>
+__device__ __forceinline__ uint32_t pair_of(float a, float b) {
     typedef float f32x2_t __attribute__((ext_vector_type(2)));
     typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
     const f32x2_t v = {a, b};
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
+    if constexpr (Elem<T>::code == NVQ_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
 }
-// v less half I of w.
-template <int I>
+// v less half I of the pair w.
+template <typename T, int I>
 __device__ __forceinline__ float behind(float v, uint32_t w) {
+    if constexpr (Elem<T>::code == NVQ_BF16) return v - u2f(I == 0 ? w << 16 : w & 0xFFFF0000u);
     float d;
     if constexpr (I == 0) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(w), "v"(v));
     else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(w), "v"(v));
@@ -145,14 +148,15 @@ template <typename T, int D>
 __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) prompt_kernel(const PromptArgs<T> a) {
     using Of = Tile<T, D>;
     using Stage = typename Of::Stage;
-    constexpr bool kWide = sizeof(T) == 4, kBf16 = Elem<T>::code == NVQ_BF16;
+    constexpr bool kWide = sizeof(T) == 4;
     constexpr int KT = Of::kKeys, TB = KT / 32, RUN = kFragRun<T>;      // keys of a tile, blocks of 32; values of a run
     constexpr int KS = D / (2 * RUN), ND = D / 32;                     // steps of a score (a run of both halves of the wavefront), blocks of D
     constexpr int SHARE = Of::kShare;
+    // With care maxima stand 2^kLift above the scores' own, as far as the terms of a weight reach (float16's sums stay in float32's range anyway).
+    constexpr float kLift = Elem<T>::code == NVQ_F16 ? 0.0f : 40.0f;
     __shared__ alignas(16) Stage stages[2];
-    __shared__ uint32_t flags[2];             // of a stage: a value that it does not hold
+    __shared__ uint32_t flags[2];             // of a stage: a value that is not finite
     __shared__ uint32_t again;                // sums that are not finite
-    __shared__ uint32_t most[2][kWaves];      // of a tile that is laid out again: the largest finite value's bits; whether one is not finite
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
     PagedItem item;
     const int32_t at_item = turned(blockIdx.x, a.turn, a.back);
@@ -241,25 +245,6 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
         place(i, row, run);
         return s0 + row < S && run * RUN < a.dim;
     };
-    float value_scale = 1.0f;  // (bfloat16; a power of two)
-    // A run of bfloat16 values times the scale, in bfloat16 (what falls below its normal range is far below float16's).
-    auto scaled = [&](uint4 w) __attribute__((always_inline)) {
-        uint32_t in[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int j = 0; j < 4; j++) in[j] = f2u(u2f(in[j] << 16) * value_scale) >> 16 | (f2u(u2f(in[j] & 0xFFFF0000u) * value_scale) & 0xFFFF0000u);
-        return make_uint4(in[0], in[1], in[2], in[3]);
-    };
-    // A run of values as operands: float16 for both 16-bit types.
-    auto operand = [&](uint4 w) __attribute__((always_inline)) {
-        if constexpr (kBf16) {
-            uint32_t in[4] = {w.x, w.y, w.z, w.w}, out[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) out[j] = half_pair(u2f(in[j] << 16), u2f(in[j] & 0xFFFF0000u));
-            return make_uint4(out[0], out[1], out[2], out[3]);
-        } else {
-            return w;
-        }
-    };
     auto value_place = [&](Stage &to, int i) __attribute__((always_inline)) {
         int row, run;
         place(i, row, run);
@@ -267,11 +252,9 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
     };
     // The tile's rows into a stage, in pieces: run i of the values and of the keys by turns.  First what takes a branch; last (CAREFUL) the stage's flag where a
     // value is not finite there.
-    typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
     float wild;
-    f16x2_t wild2;
     auto lay_first = [&](int s0) __attribute__((always_inline)) {
-        wild = 0.0f, wild2 = f16x2_t{(_Float16)0.0f, (_Float16)0.0f};
+        wild = 0.0f;
         if (__builtin_expect(!whole_rows || s0 + KT > S, 0)) {
             asm volatile("");  // (a branch, the same for all)
 #pragma unroll
@@ -283,11 +266,6 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
                 kr[i] = make_uint4(kr[i].x & k, kr[i].y & k, kr[i].z & k, kr[i].w & k), vr[i] = make_uint4(vr[i].x & v, vr[i].y & v, vr[i].z & v, vr[i].w & v);
             }
         }
-        if (kBf16 && __builtin_expect(value_scale != 1.0f, 0)) {
-            asm volatile("");
-#pragma unroll
-            for (int i = 0; i < SHARE; i++) vr[i] = scaled(vr[i]);
-        }
     };
     auto lay_piece = [&](auto careful, Stage &to, int piece) __attribute__((always_inline)) {
         const int i = piece >> 1;
@@ -297,23 +275,15 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
             *reinterpret_cast<uint4 *>(to.keys + row * Of::kKeyRow + 16 * run) = kr[i];
             return;
         }
-        const uint4 w = operand(vr[i]);
-        *value_place(to, i) = w;
+        *value_place(to, i) = vr[i];
         if constexpr (!decltype(careful)::value) return;
-        if constexpr (kWide) {  // x 0 is NaN of what is not finite
-            wild = __builtin_fmaf(u2f(w.x), 0.0f, wild), wild = __builtin_fmaf(u2f(w.y), 0.0f, wild);
-            wild = __builtin_fmaf(u2f(w.z), 0.0f, wild), wild = __builtin_fmaf(u2f(w.w), 0.0f, wild);
-        } else {
-            const f16x2_t zero = {(_Float16)0.0f, (_Float16)0.0f};
-            wild2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, w.x), zero, wild2);
-            wild2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, w.y), zero, wild2);
-            wild2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, w.z), zero, wild2);
-            wild2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, w.w), zero, wild2);
-        }
+        T t[RUN];
+        __builtin_memcpy(t, &vr[i], 16);
+#pragma unroll
+        for (int j = 0; j < RUN; j++) wild = __builtin_fmaf(Elem<T>::load(t, j), 0.0f, wild);  // (x 0 is NaN of what is not finite)
     };
     auto lay_last = [&](auto careful, uint32_t &flag) __attribute__((always_inline)) {
         if constexpr (!decltype(careful)::value) return;
-        if constexpr (!kWide) wild = (float)wild2[0] + (float)wild2[1];
         if (wild != wild) flag = 1u;
     };
 
@@ -333,7 +303,7 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
         typedef __attribute__((address_space(3))) short4_t *Lds;
         const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(uintptr_t)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(uintptr_t)(at + 8 * Of::kValueRow));
         struct { short4_t v[2]; } both = {{lo, hi}};
-        return __builtin_bit_cast(half8_t, both);
+        return __builtin_bit_cast(uint4, both);
     };
     auto value_at = [&](const Stage &from, int i, int d) __attribute__((always_inline)) {
         return reinterpret_cast<const float *>(from.values + (8 * (i >> 2) + 4 * half + (i & 3)) * Of::kValueRow)[32 * d + col];
@@ -344,7 +314,7 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
         auto weight = [&](int i) __attribute__((always_inline)) {
             const float e = __builtin_amdgcn_exp2f(x[i >> 4][i & 15]);
             l += e;
-            if constexpr (decltype(careful)::value) seen |= (e == 0.0f ? 0u : 1u) << i;
+            if constexpr (decltype(careful)::value) seen |= (x[i >> 4][i & 15] < -126.0f - kLift ? 0u : 1u) << i;  // (as without the lift)
             return e;
         };
         if constexpr (kWide) {
@@ -357,14 +327,14 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
         } else {
             constexpr int NC = KT / 16;
             uint32_t high[2][4], low[2][4];
-            half8_t v[2][ND];
+            uint4 v[2][ND];
             auto prepare = [&](int c, int j) __attribute__((always_inline)) {
                 const float e0 = weight(8 * c + 2 * j), e1 = weight(8 * c + 2 * j + 1);
                 uint32_t &h = high[c & 1][j];
-                h = half_pair(e0, e1);
-                if constexpr (!kBf16) low[c & 1][j] = half_pair(behind<0>(e0, h), behind<1>(e1, h));
+                h = pair_of<T>(e0, e1);
+                low[c & 1][j] = pair_of<T>(behind<T, 0>(e0, h), behind<T, 1>(e1, h));
             };
-            auto operand_of = [&](const uint32_t (&w)[4]) __attribute__((always_inline)) { return __builtin_bit_cast(half8_t, make_uint4(w[0], w[1], w[2], w[3])); };
+            auto operand_of = [&](const uint32_t (&w)[4]) __attribute__((always_inline)) { return make_uint4(w[0], w[1], w[2], w[3]); };
 #pragma unroll
             for (int d = 0; d < ND; d++) v[0][d] = value_run(from, 0, d);
 #pragma unroll
@@ -375,9 +345,9 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
             for (int c = 0; c < NC; c++)
 #pragma unroll
                 for (int d = 0; d < ND; d++) {
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[c & 1][d], operand_of(high[c & 1]), o[d], 0, 0, 0);
+                    o[d] = product32<T>(v[c & 1][d], operand_of(high[c & 1]), o[d]);
                     if (c + 1 < NC) v[(c + 1) & 1][d] = value_run(from, c + 1, d);
-                    if constexpr (!kBf16) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[c & 1][d], operand_of(low[c & 1]), o[d], 0, 0, 0);
+                    o[d] = product32<T>(v[c & 1][d], operand_of(low[c & 1]), o[d]);
                     if (c + 1 < NC)
 #pragma unroll
                         for (int j = 4 * d / ND; j < 4 * (d + 1) / ND; j++) prepare(c + 1, j);
@@ -407,7 +377,7 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int step = 0; step < STEPS; step++) {
-                s[step / KS] = scores32<T>(k[step], qf[step % KS], s[step / KS]);
+                s[step / KS] = product32<T>(k[step], qf[step % KS], s[step / KS]);
                 if (step + kAhead < STEPS) read(step + kAhead);
 #pragma unroll
                 for (int piece = (PIECES * step + STEPS - 1) / STEPS; piece < (PIECES * (step + 1) + STEPS - 1) / STEPS; piece++) lay_piece(careful, next, piece);
@@ -433,10 +403,11 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
 #pragma unroll
         for (int i = 1; i < 16 * TB; i++) top = fmaxf(top, x[i >> 4][i & 15]);
         top *= scale;
-        // Rescaled only when a maximum has grown by more than 2^8: until then the weights are at most 2^8.
-        if (__builtin_expect(__any(top > m + 8.0f), 0)) {
+        // Rescaled only when a maximum has grown by more than 2^8: until then the weights are at most 2^8 (with care 2^8 less the lift).
+        constexpr float kUp = decltype(careful)::value ? kLift : 0.0f;
+        if (__builtin_expect(__any(top > m + (8.0f - kUp)), 0)) {
             top = fmaxf(top, __shfl_xor(top, 32));
-            const float m_new = fmaxf(m, top), f = exp2f(m - m_new);
+            const float m_new = fmaxf(m, top + kUp), f = exp2f(m - m_new);
             m = m_new, l *= f;
 #pragma unroll
             for (int d = 0; d < ND; d++)
@@ -457,58 +428,9 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
         __builtin_amdgcn_s_setprio(0);
     };
 
-    // The largest finite value of the tile in vr (its bits as a positive number) and whether one is not finite, for all of the block.
-    auto survey = [&](int s0, uint32_t &top, bool &wild) __attribute__((always_inline)) {
-        uint32_t mine = 0, odd = 0;
-#pragma unroll
-        for (int i = 0; i < SHARE; i++) {
-            const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-            const bool used = real(s0, i);
-#pragma unroll
-            for (int j = 0; j < RUN; j++) {
-                T t[RUN];
-                __builtin_memcpy(t, w, 16);
-                const uint32_t b = f2u(Elem<T>::load(t, j)) & 0x7FFFFFFFu;
-                if (used && b < 0x7F800000u && b > mine) mine = b;
-                odd |= used && b >= 0x7F800000u ? 1u : 0u;
-            }
-        }
-        for (int i = 1; i < 64; i <<= 1) {
-            const uint32_t other = (uint32_t)__shfl_xor((int)mine, i);
-            mine = other > mine ? other : mine, odd |= (uint32_t)__shfl_xor((int)odd, i);
-        }
-        if (lane == 0) most[0][wave] = mine, most[1][wave] = odd;
-        __syncthreads();
-        top = 0, wild = false;
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) top = most[0][w] > top ? most[0][w] : top, wild |= most[1][w] != 0;
-        __syncthreads();
-    };
-    // A scale that brings the largest value to 16 .. 32, 2^11 below what float16 holds, where it is outside 2^-3 .. 2^9: the smallest step is then 2^-29 of
-    // it, and at most 2^-21 in between.
-    auto scale_for = [&](uint32_t top) {
-        const int exponent = (int)(top >> 23);  // (of bfloat16's subnormals 0: as 2^-127)
-        if (top == 0 || (exponent >= 127 - 3 && exponent < 127 + 9)) return 1.0f;
-        const int e = 127 + 4 - (exponent - 127);
-        return u2f((uint32_t)(e < 1 ? 1 : e > 254 ? 254 : e) << 23);
-    };
-    // A flagged tile laid out again: the values that are not finite as zeros, the others with the scale they need.
-    auto lay_again = [&](Stage &to, int s0, bool &wild) __attribute__((always_inline)) {
+    // A flagged tile laid out again: the values that are not finite as zeros.
+    auto lay_again = [&](Stage &to, int s0) __attribute__((always_inline)) {
         request_values(s0);
-        uint32_t top;
-        survey(s0, top, wild);
-        if constexpr (kBf16) {
-            const float before = value_scale;
-            // (down only: what has been added up keeps its precision)
-            const float now = scale_for(top);
-            if (u2f(top) * value_scale >= 32768.0f && now < value_scale) value_scale = now;
-            const float f = value_scale / before;
-            if (f != 1.0f)
-#pragma unroll
-                for (int d = 0; d < ND; d++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) o[d][i] *= f;
-        }
 #pragma unroll
         for (int i = 0; i < SHARE; i++) {
             T t[RUN];
@@ -519,12 +441,13 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
                 if (!used || !(fabsf(Elem<T>::load(t, j)) < INFINITY)) Elem<T>::store(t, j, 0.0f);
             uint4 w;
             __builtin_memcpy(&w, t, 16);
-            *value_place(to, i) = operand(kBf16 ? scaled(w) : w);
+            *value_place(to, i) = w;
         }
         __syncthreads();
     };
     // What is not finite, to the lines that see it: by a product of ones at the places of one kind with ones at the keys that are seen.
     auto add_wild = [&](Stage &to, int s0, const uint32_t &seen) __attribute__((always_inline)) {
+        constexpr uint32_t kOne = Elem<T>::code == NVQ_BF16 ? 0x3F80u : 0x3C00u;
         request_values(s0);
         for (int kind = 0; kind < 3; kind++) {
             __syncthreads();
@@ -539,7 +462,7 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
                     const float v = Elem<T>::load(t, j);
                     const bool is = used && (kind == 0 ? v == INFINITY : kind == 1 ? v == -INFINITY : v != v);
                     if constexpr (kWide) w[j] = is ? f2u(1.0f) : 0u;
-                    else w[j >> 1] |= (is ? 0x3C00u : 0u) << (16 * (j & 1));
+                    else w[j >> 1] |= (is ? kOne : 0u) << (16 * (j & 1));
                 }
                 *value_place(to, i) = make_uint4(w[0], w[1], w[2], w[3]);
             }
@@ -558,8 +481,8 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
                     for (int c = 0; c < KT / 16; c++) {
                         uint32_t p[4];
 #pragma unroll
-                        for (int j = 0; j < 4; j++) p[j] = (seen >> (8 * c + 2 * j) & 1u) * 0x3C00u | (seen >> (8 * c + 2 * j + 1) & 1u) * 0x3C000000u;
-                        count = __builtin_amdgcn_mfma_f32_32x32x16_f16(value_run(to, c, d), __builtin_bit_cast(half8_t, make_uint4(p[0], p[1], p[2], p[3])), count, 0, 0, 0);
+                        for (int j = 0; j < 4; j++) p[j] = (seen >> (8 * c + 2 * j) & 1u) * kOne | (seen >> (8 * c + 2 * j + 1) & 1u) * (kOne << 16);
+                        count = product32<T>(value_run(to, c, d), make_uint4(p[0], p[1], p[2], p[3]), count);
                     }
                 }
 #pragma unroll
@@ -569,7 +492,7 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
         }
     };
 
-    // The keys of the item.  First without a look at what the values hold: where one is not finite, or has left float16's range, the sums of some line are
+    // The keys of the item.  First without a look at what the values hold: where one is not finite, or sums leave float32's range, those of some line are
     // not finite, and the block walks its keys again with care.  (In one loop the rare paths' loads would be waited for in every tile.)
     // Tile s lies in a stage while tile s + 1 is on its way through registers and tile s + 2 is requested; behind the item's last tile
     // that one again (loads under a condition cost registers that spilled: 5% of the time).
@@ -591,7 +514,8 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
                     asm volatile("");
                     __syncthreads();
                     if (tid == 0) flags[at] = 0u;
-                    lay_again(stages[at], s0, wild_tile);
+                    wild_tile = true;
+                    lay_again(stages[at], s0);
                     request_values(next);
                 }
             }
@@ -615,31 +539,6 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
     clear();
     if (tid < 3) (tid < 2 ? flags[tid] : again) = 0u;
     if (s_begin < s_end) {
-        if constexpr (kBf16) {
-            // The largest value, two at a time; what lies behind the keys or the head is a copy of others.  (With one that is not finite: in full.)
-            typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
-            u16x2_t largest = {0, 0};
-#pragma unroll
-            for (int i = 0; i < SHARE; i++) {
-                const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-#pragma unroll
-                for (int j = 0; j < 4; j++) largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2_t, w[j] & 0x7FFF7FFFu));
-            }
-            uint32_t top = wave_largest(largest[0] > largest[1] ? largest[0] : largest[1]);
-            if (lane == 0) most[0][wave] = top;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) top = most[0][w] > top ? most[0][w] : top;
-            top = (uint32_t)uniform((int32_t)top) << 16;
-            if (top >= 0x7F800000u) {
-                asm volatile("");
-                bool wild;
-                __syncthreads();
-                survey(s_begin, top, wild);
-            }
-            value_scale = scale_for(top);
-        }
-        const float first_scale = value_scale;
         walk(std::false_type{});
         float odd = 0.0f;
         odd = __builtin_fmaf(l, 0.0f, odd);
@@ -651,7 +550,6 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
         __syncthreads();
         if (__builtin_expect(uniform((int32_t)again) != 0, 0)) {
             clear();
-            value_scale = first_scale;
             request(s_begin);
             walk(std::true_type{});
         }
@@ -660,7 +558,6 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
     if (!live) return;
     const bool whole = span.items == 1;
     float factor = 1.0f;
-    const float back = 1.0f / value_scale;  // (by itself: times the factor it may leave float32's normal range)
     float *state = nullptr;  // of this line and split: maximum, denominator, weighted means
     if (whole) {
         float denom = l, f = 1.0f;
@@ -682,7 +579,7 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
             const int c = 32 * d + 8 * g + 4 * half;
             float v[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = o[d][4 * g + i] * factor * back;
+            for (int i = 0; i < 4; i++) v[i] = o[d][4 * g + i] * factor;
             if (!whole) {
                 *reinterpret_cast<float4 *>(state + 4 + c) = make_float4(v[0], v[1], v[2], v[3]);
             } else if (c < a.dim) {

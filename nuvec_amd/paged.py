@@ -469,8 +469,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     Rows that see nothing are zeros; rows of no sequence are left as they were in `out` (and undefined in a new result).  Keys and values that a row does
     not see may hold anything.
 
-    The softmax's weights hold 11 bits beside the 8 of a bfloat16 result (float16: 22, float32: 24), everything else is float32.  Values of a bfloat16 sequence that
-    are far smaller than its others are taken to 2^-21 of the largest among the first 64 that a block of rows sees.  Keys and values of one head less than
+    The softmax's weights hold 16 bits beside the 8 of a bfloat16 result (float16: 22, float32: 24), everything else is float32.  Keys and values of one head less than
     2^24 elements apart.  `out` may be `q` itself and shares no memory with the keys and values."""
     y = (_lib._native or _lib.native()).prompt_attention(q, k, v, scale, query_starts, key_starts, sinks, causal, window, out)
     if y is not None:
