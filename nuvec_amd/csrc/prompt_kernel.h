@@ -9,7 +9,8 @@
 // v_mfma_f32_32x32x2_f32.
 //
 // Terms.  Queries, keys and values are exact operands in their own type.  The weights are two terms of it, 16 bits in bfloat16 and 22 in float16 (one term
-// leaves an error beside the result's own rounding), in float32 themselves.  Scores, maxima, sums and accumulators are float32.  bfloat16 values as float16
+// leaves an error beside the result's own rounding; float16's are relative to a reference that follows the tiles' maxima up and down, so that small ones have
+// them too: a weight is off by 2^-22 of itself or 2^-21 of its tile's largest), in float32 themselves.  Scores, maxima, sums and accumulators are float32.  bfloat16 values as float16
 // operands would take one term, but a power of two that brings a tile's values into float16's range is one for lines that see the largest of them and for
 // lines that do not, whose own would be lost.
 //
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
     constexpr int KT = Of::kKeys, TB = KT / 32, RUN = kFragRun<T>;      // keys of a tile, blocks of 32; values of a run
     constexpr int KS = D / (2 * RUN), ND = D / 32;                     // steps of a score (a run of both halves of the wavefront), blocks of D
     constexpr int SHARE = Of::kShare;
-    // With care maxima stand 2^kLift above the scores' own, as far as the terms of a weight reach (float16's sums stay in float32's range anyway).
+    // With care maxima stand 2^kLift above the scores' own (not float16's, whose sums stay in float32's range anyway).
     constexpr float kLift = Elem<T>::code == NVQ_F16 ? 0.0f : 40.0f;
     __shared__ alignas(16) Stage stages[2];
     __shared__ uint32_t flags[2];             // of a stage: a value that is not finite
@@ -404,10 +405,21 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
         for (int i = 1; i < 16 * TB; i++) top = fmaxf(top, x[i >> 4][i & 15]);
         top *= scale;
         // Rescaled only when a maximum has grown by more than 2^8: until then the weights are at most 2^8 (with care 2^8 less the lift).
-        constexpr float kUp = decltype(careful)::value ? kLift : 0.0f;
-        if (__builtin_expect(__any(top > m + (8.0f - kUp)), 0)) {
+        // float16: weights of a tile have to lie high in its range, 2^-24 to 2^16, to keep their bits however many small ones there are.  `m` is 11 below the tile's
+        // maximum then, rises where a weight would leave 2^15, and falls where the tile's largest would be below 2^-4 (not for a score that is masked, and only as
+        // far as the sums, which grow by that much, stay below 2^60).
+        constexpr bool kFalls = Elem<T>::code == NVQ_F16;
+        constexpr float kBelow = kFalls ? 11.0f : decltype(careful)::value ? -kLift : 0.0f, kMost = kFalls ? 15.0f : 8.0f + kBelow;
+        bool moves = top > m + kMost;
+        if constexpr (kFalls) moves |= top < m - 4.0f && top > kLowest;
+        if (__builtin_expect(__any(moves), 0)) {
             top = fmaxf(top, __shfl_xor(top, 32));
-            const float m_new = fmaxf(m, top + kUp), f = exp2f(m - m_new);
+            float m_new = fmaxf(m, top - kBelow);
+            if constexpr (kFalls) {
+                const float sum = l + __shfl_xor(l, 32), least = sum > 0.0f ? m + __builtin_amdgcn_logf(sum) - 60.0f : kLowest;  // (the same in both halves)
+                m_new = top > m + kMost || (top < m - 4.0f && top > kLowest) ? fmaxf(top - kBelow, least) : m;
+            }
+            const float f = exp2f(m - m_new);
             m = m_new, l *= f;
 #pragma unroll
             for (int d = 0; d < ND; d++)

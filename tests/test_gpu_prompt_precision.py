@@ -146,3 +146,30 @@ def many_small_weights(dtype, dim, length):
         got = nv.prompt_attention(q, k.expand(-1, heads, -1), v.expand(-1, heads, -1), 1.0)
         want, bound = expected(q, k, v, 1.0)
         within(got, want, bound, heavy)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("length", [4000, 131073])
+def test_many_small_weights_in_float16(dim, length):
+    many_small_weights(torch.float16, dim, length)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,heads,window", [(300, 8, 0), (300, 8, 500), (3, 800, 0), (3, 2, 0)])
+def test_weights_that_rise_and_fall(dtype, rows, heads, window):
+    """Stretches of keys whose scores lie up to 24 apart, in any order; those of the upper ones have values of 0, so that the result is the others'."""
+    length, dim = 3000, 64
+    g = torch.Generator(device="cuda").manual_seed(rows + heads + window)
+    put = lambda *s: torch.randn(s, generator=g, device="cuda")
+    level = (24 * torch.rand(length // 50 + 1, generator=g, device="cuda")).repeat_interleave(torch.randint(1, 120, (length // 50 + 1,), generator=g, device="cuda"))
+    level = torch.cat([level, torch.zeros(length, device="cuda")])[:length]
+    q, k, v = 0.3 * put(rows, heads, dim), 0.3 * put(length, 1, dim), 1 + 0.25 * put(length, 1, dim)
+    q[..., 0] = torch.linspace(0.2, 1.0, heads, device="cuda")
+    k[:, 0, 0] = level
+    v[level > 4] = 0.0
+    q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+    sinks = torch.linspace(-5.0, 30.0, heads, device="cuda").to(dtype)
+    for s in (None, sinks):
+        got = nv.prompt_attention(q, k.expand(-1, heads, -1), v.expand(-1, heads, -1), 1.0, sinks=s, window=window)
+        want, bound = expected(q, k, v, 1.0, s, window=window)
+        within(got, want, bound)
