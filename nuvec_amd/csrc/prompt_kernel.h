@@ -312,9 +312,10 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
     // Exponentials, sums and products.  16-bit types: the weights of 16 keys are worked out, and the values of the next 16 read, between the products of the
     // 16 before them (in the order written: products wait for neither, and the vector unit works beside them).
     auto weigh = [&](const Stage &from, float (&x)[TB][16], auto careful, uint32_t &seen) __attribute__((always_inline)) {
+        float sum = 0.0f;  // (a tile's by itself: beside a large sum many small weights would be lost one by one)
         auto weight = [&](int i) __attribute__((always_inline)) {
             const float e = __builtin_amdgcn_exp2f(x[i >> 4][i & 15]);
-            l += e;
+            sum += e;
             if constexpr (decltype(careful)::value) seen |= (x[i >> 4][i & 15] < -126.0f - kLift ? 0u : 1u) << i;  // (as without the lift)
             return e;
         };
@@ -355,6 +356,7 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
                     __builtin_amdgcn_sched_barrier(0);
                 }
         }
+        l += sum;
     };
     // One tile: the scores, one look at their maximum, the weights and their products.  x[t][i]: key 32 t + 8 (i / 4) + 4 half + i % 4 of the lane's line.
     // The next tile is laid between the scores' products, whose keys are read kAhead products before them.  `seen` (CAREFUL): a bit for each of these

@@ -129,17 +129,18 @@ def test_many_small_weights(dtype, dim, length):
     many_small_weights(dtype, dim, length)
 
 
-def many_small_weights(dtype, dim, length):
+def many_small_weights(dtype, dim, length, apart=0, spread=0.3):
     """One key, of value 0, that takes nearly all of the weight, first, in the middle or last: the result is the others' alone.  (More heads than the chip has
-    places for blocks, so that no block has a part of the keys; all share their keys and values.)"""
+    places for blocks, so that no block has a part of the keys; all share their keys and values.)  `apart`: a second key like it that far behind."""
     heads = 800
     g = torch.Generator(device="cuda").manual_seed(length + dim)
     put = lambda *s: torch.randn(s, generator=g, device="cuda")
-    for heavy in (0, length // 2, length - 1):
-        q, k, v = 0.3 * put(1, heads, dim), 0.3 * put(length, 1, dim), 1 + 0.25 * put(length, 1, dim)
+    for heavy in (0, length // 2, length - 1 - apart):
+        q, k, v = spread * put(1, heads, dim), spread * put(length, 1, dim), 1 + 0.25 * put(length, 1, dim)
         # (from a half of the weight to all but 6e-6 of it)
         share = torch.linspace(0.0, 12.0, heads, device="cuda")
         q[0, :, 0] = (share + torch.log(torch.tensor(float(length)))) / 8
+        heavy = [heavy, heavy + apart]
         k[:, 0, 0], k[heavy, 0], v[heavy] = 0.0, 0.0, 0.0
         k[heavy, 0, 0] = 8.0
         q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
@@ -152,6 +153,12 @@ def many_small_weights(dtype, dim, length):
 @pytest.mark.parametrize("length", [4000, 131073])
 def test_many_small_weights_in_float16(dim, length):
     many_small_weights(torch.float16, dim, length)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sums_of_many_small_weights(dtype):
+    """Two keys that take nearly all of the weight, in either half of the keys that a line's two lanes add up: the others count beside both."""
+    many_small_weights(dtype, 64, (1 << 19) + 1, apart=4, spread=0.0)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
