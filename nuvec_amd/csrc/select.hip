@@ -271,7 +271,8 @@ __global__ void __launch_bounds__(64 * kSelectWaves) moe_select_kernel(const Sel
     // A value's place among the wavefront's (V a lane, in the experts' order) replaces its key's low bits, the first the largest: a round is the largest key
     // below the last one's, and holds its place.  Keys that have come wrap round to less than all others when the last is taken off.
     constexpr uint32_t kPlaces = 64 * V - 1;
-    constexpr bool kWhole = !BIASED && sizeof(T) == 2;  // no key has lost a bit that it had
+    constexpr bool kWhole = !BIASED && sizeof(T) == 2;  // no key has lost a bit that it had (the 13 lowest are alike in all of float16's, 16 in bfloat16's)
+    static_assert(kPlaces < 1u << 13);
 #pragma unroll
     for (int j = 0; j < V; j++) key[j] = key[j] == 0u ? 0u : (key[j] & ~kPlaces) | (kPlaces - (uint32_t)(lane * V + j));
     int slot = 0;  // lane r's of round r
@@ -328,7 +329,8 @@ void run_select_type(const SelectArgs &a, hipStream_t s) {
     else if (of_lane <= 2) run_select<T, 2>(a, s);
     else if (of_lane <= 4) run_select<T, 4>(a, s);
     else if (of_lane <= 8) run_select<T, 8>(a, s);
-    else run_select<T, 16>(a, s);
+    else if (of_lane <= 16) run_select<T, 16>(a, s);
+    else run_select<T, 32>(a, s);  // (31 at most: 1024 experts over the more than 32 lanes that the groups have together)
 }
 
 }  // namespace

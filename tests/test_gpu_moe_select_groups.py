@@ -1,0 +1,21 @@
+"""The choice of experts (csrc/select.hip): numbers of groups that are no powers of two, groups whose two best all but cancel, NaN and the last bits of weights."""
+import pytest
+import torch
+
+import nuvec_amd as nv
+from tests.test_gpu_moe_select import HALF, TINY, TYPES, check, expected, normal
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e,groups,top", [(1000, 5, 2), (960, 3, 2), (720, 10, 3), (561, 17, 4), (1023, 33, 9), (1020, 60, 60), (1024, 32, 5), (1023, 3, 1)])
+def test_more_than_sixteen_experts_of_a_lane(dtype, scores, e, groups, top):
+    """Groups whose power of two of lanes is little more than half of the wavefront: up to 31 experts a lane."""
+    x, bias = normal(19, e, dtype=dtype, seed=e), normal(e, seed=2, size=0.2)
+    for k in (1, 16):
+        check(x, k, scores, bias, groups, top, scale=1.5)
+        check(x, k, scores, None, groups, top, normalize=False)
+        check(x, k, scores, None, groups, top, 2)
+    check(x, e // groups * top if e // groups * top < 64 else 64, scores, bias, groups, top)
