@@ -147,7 +147,7 @@ __device__ __forceinline__ int select_wide(const SelectArgs &a, const float (&l)
 }
 
 // Float32's error of c, relative to 1 and to c: sigmoids and softmaxes (at most 1) are off by 2^-21 at most, products with 64 lanes' sums among it, and the sum
-// with the bias by half a step; a group's two twice that.  What is as near as this is decided again.
+// with the bias by half a step; a group's score by that of its two and another half step of their sum.  What is as near as this is decided again.
 constexpr float kNear = 1.0f / (1 << 19);
 
 // The weight of the expert that lane r of k has, from its logit.
@@ -250,7 +250,9 @@ __global__ void __launch_bounds__(64 * kSelectWaves) moe_select_kernel(const Sel
         if (a.lanes_shift > 2) meet(moved<kHalfRow>(best), moved<kHalfRow>(second));
         if (a.lanes_shift > 3) meet(moved<kRow>(best), moved<kRow>(second));
         if (a.lanes_shift > 4) meet(__shfl_xor(best, 16), __shfl_xor(second, 16));
-        const float score = a.group_best == 2 && each > 1 ? best + second : best;
+        const bool two = a.group_best == 2 && each > 1;
+        const float score = two ? best + second : best;
+        const float off = kNear * (1.0f + fabsf(best) + (two ? fabsf(second) : 0.0f));  // (of what is added up: the sum may be far smaller)
         const bool real = place.group < a.groups;
         const uint32_t mine = real ? ordered_number(score) : 0u;
         int before = 0;  // groups that come first
@@ -262,8 +264,9 @@ __global__ void __launch_bounds__(64 * kSelectWaves) moe_select_kernel(const Sel
             }
         const bool kept = before < a.top_groups;
         if (BIASED && a.top_groups < a.groups) {
-            const float least = value_of((uint32_t)__builtin_amdgcn_readlane((int)mine, __builtin_ctzll(__ballot(before == a.top_groups - 1) | 1ull << 63)));
-            doubt |= !kept && real && !(score < least - 2.0f * kNear * (1.0f + fabsf(least)));
+            const int last = __builtin_ctzll(__ballot(before == a.top_groups - 1) | 1ull << 63);
+            const float least = value_of((uint32_t)__builtin_amdgcn_readlane((int)mine, last)), least_off = from_lane(off, last);
+            doubt |= !kept && real && !(score < least - (off + least_off));
         }
 #pragma unroll
         for (int j = 0; j < V; j++) key[j] = kept ? key[j] : 0u;
@@ -303,6 +306,7 @@ __global__ void __launch_bounds__(64 * kSelectWaves) moe_select_kernel(const Sel
     float x = mine_of.x;
     if (__any(doubt)) {
         asm volatile("");  // (a branch, the same for all lanes)
+        if (!BIASED && __any(wild != wild)) total = NAN;  // (the sum that was not needed: a softmax with a NaN is NaN)
         chosen = select_wide<V>(a, l, place, held[wave]);
         x = lane < a.k ? Elem<T>::load(logits, chosen) : 0.0f;
     }
