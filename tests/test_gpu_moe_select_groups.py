@@ -19,3 +19,18 @@ def test_more_than_sixteen_experts_of_a_lane(dtype, scores, e, groups, top):
         check(x, k, scores, None, groups, top, normalize=False)
         check(x, k, scores, None, groups, top, 2)
     check(x, e // groups * top if e // groups * top < 64 else 64, scores, bias, groups, top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [1.0, 64.0, 300.0, 1e5])
+def test_groups_whose_two_best_cancel(dtype, size):
+    """Biases of either sign: a group's score is small beside its two values, which are what float32 rounds."""
+    for e, groups, top in ((64, 32, 16), (128, 64, 9), (256, 8, 3)):
+        each = e // groups
+        x = normal(200, e, dtype=dtype, seed=e, size=1e-4 if dtype == torch.float32 else 1e-2)
+        bias = torch.full((e,), -2 * size, device="cuda")
+        bias[::each] = size * (1 + normal(groups, seed=3, size=0.1))
+        bias[1::each] = -bias[::each]
+        for scores in ("sigmoid", "softmax"):
+            check(x, 4, scores, bias, groups, top)
+            check(x, 4, scores, bias, groups, top, 1)
