@@ -477,7 +477,8 @@ NVQ_API int32_t nvq_apply_adapters(const nvq_adapters_desc *desc, const void *x,
 /* Per row p = softmax or sigmoid of the logits, c = p + bias (f32 [experts], or NULL); a group's score is the sum of its group_best largest
  * c, the top_groups best groups stay, and of their experts the k with the largest c are chosen, largest first (ties, of groups too: the
  * lowest index; a NaN below everything).  Without a bias c's order is the logits' own.  indices i32 [rows, k]; weights dtype [rows, k]: p of
- * the chosen, with `normalize` divided by (their sum + 1e-20), times scale, rounded once.  A softmax of nothing but -inf is zeros. */
+ * the chosen, with `normalize` divided by (their sum + 1e-20), times scale, rounded once.  A softmax of nothing but -inf is
+ * zeros, one with a NaN is NaN. */
 NVQ_API int32_t nvq_moe_select(const nvq_moe_select_desc *desc, const void *logits, const float *bias, int32_t *indices, void *weights, void *stream);
 
 /* GpuEval::sorted_offsets (gpu.rs:6732-6756); kernels::sorted_offsets (kernels.rs:873-892):

@@ -306,6 +306,7 @@ __global__ void __launch_bounds__(64 * kSelectWaves) moe_select_kernel(const Sel
     float x = mine_of.x;
     if (__any(doubt)) {
         asm volatile("");  // (a branch, the same for all lanes)
+        if (!BIASED && __any(wild != wild)) total = NAN;  // (the sum that was not needed: a softmax with a NaN is NaN)
         chosen = select_wide<V>(a, l, place, held[wave]);
         x = lane < a.k ? Elem<T>::load(logits, chosen) : 0.0f;
     }

@@ -671,7 +671,7 @@ def moe_select(logits: torch.Tensor, k: int, scores: str = "softmax", bias: Opti
     consecutive experts the `top_groups` best stay (None: all), by the sum of their `group_best` largest c (1 or 2; None: 2 with a bias, else 1), and of their
     experts the k with the largest c are chosen, largest first; ties, of groups too, go to the lowest index, a NaN is below everything.  The weights are the p of the chosen, with
     `normalize` divided by (their sum + 1e-20), times `scale`, rounded once.  Without a bias c has the logits' order; with one it is compared in 64 bits.  A softmax of
-    nothing but -inf is zeros."""
+    nothing but -inf is zeros, one with a NaN is NaN."""
     if bias is None or isinstance(bias, torch.Tensor):
         done = (_lib._native or _lib.native()).moe_select(logits, k, scores == "sigmoid" if scores in MOE_SCORES else None, bias, groups, top_groups, group_best, normalize, scale)
         if done is not None:

@@ -34,3 +34,23 @@ def test_groups_whose_two_best_cancel(dtype, size):
         for scores in ("sigmoid", "softmax"):
             check(x, 4, scores, bias, groups, top)
             check(x, 4, scores, bias, groups, top, 1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_nan_among_the_logits_reaches_every_weight_of_its_softmax(dtype):
+    """Chosen or not; the experts are those of the others, and a sigmoid's weights too."""
+    x, zeros = normal(6, 64, dtype=dtype), torch.zeros(64, device="cuda")
+    x[1, 5], x[2, 60], x[3, ::2] = float("nan"), float("nan"), float("nan")
+    x[4] = -float("inf")
+    x[4, 7] = float("nan")
+    for normalize in (True, False):
+        for more in ({}, {"groups": 8, "top_groups": 2}, {"groups": 8, "top_groups": 8, "group_best": 2}):
+            for bias in (None, zeros):
+                experts, weights = nv.moe_select(x, 3, "softmax", bias, normalize=normalize, **more)
+                assert weights[1:5].isnan().all() and weights[[0, 5]].isfinite().all()
+                clean = expected(x[[0, 5]], 3, "softmax", bias, normalize=normalize, **more)[0]
+                assert torch.equal(experts[[0, 5]].cpu().long(), clean)
+            experts, weights = nv.moe_select(x[1:4], 3, "softmax", None, normalize=normalize)
+            assert (experts[0] != 5).all() and (experts[1] != 60).all() and (experts[2] % 2 == 1).all()
+            experts, weights = nv.moe_select(x[1:4], 3, "sigmoid", None, normalize=normalize, **more)
+            assert weights.isfinite().all()
