@@ -6,7 +6,7 @@
 // What is chosen is decided as by real numbers.  Without a bias (and groups by their best alone) c's order is the logits', and nothing is computed to find it.
 // Otherwise c is computed in float32, off by less than kNear: where two values that follow one another among the chosen, or at the border of what is chosen,
 // are further apart than that their order is certain, and where they are not (or a value is not finite) the row is decided again in 64 bits.  The
-// weights are computed for the chosen alone, in 64 bits for float32 results.
+// weights are computed for the chosen alone, for float32 results in 64 bits, as a softmax's sum is.
 //
 // One wavefront a row.  A group has a power of two of the lanes, a lane V consecutive experts, so that (lane, place) is the experts' order and a group's
 // score a few exchanges among its lanes.  Values are compared as whole numbers of the same order, 0 for what is not to be chosen, whose low bits are their
@@ -221,7 +221,10 @@ __global__ void __launch_bounds__(64 * kSelectWaves) moe_select_kernel(const Sel
         if (BIASED || !a.normalize) {  // (normalized weights do without the sum, but for what keeps them from 0 / 0)
             double sum = 0.0;
 #pragma unroll
-            for (int j = 0; j < V; j++) c[j] = exponential(l[j] - top), sum += j < place.count ? (double)c[j] : 0.0;
+            for (int j = 0; j < V; j++) {
+                c[j] = exponential(l[j] - top);
+                sum += j >= place.count ? 0.0 : sizeof(T) == 4 ? exp((double)l[j] - (double)top) : (double)c[j];
+            }
             total = across<64>(sum, [](double x, double y) { return x + y; });
         }
     }

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import nuvec_amd as nv
-from tests.test_gpu_moe_select import HALF, TINY, TYPES, check, expected, normal
+from tests.test_gpu_moe_select import HALF, TYPES, check, expected, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +54,16 @@ def test_a_nan_among_the_logits_reaches_every_weight_of_its_softmax(dtype):
             assert (experts[0] != 5).all() and (experts[1] != 60).all() and (experts[2] % 2 == 1).all()
             experts, weights = nv.moe_select(x[1:4], 3, "sigmoid", None, normalize=normalize, **more)
             assert weights.isfinite().all()
+
+
+@pytest.mark.parametrize("e,k,groups,top", [(1024, 40, 1, 1), (256, 8, 8, 3), (60, 12, 1, 1), (17, 17, 1, 1)])
+def test_float32_weights_of_a_softmax_are_rounded_once(e, k, groups, top):
+    """Against 64 bits: half a step of float32, and what 64 bits lose of it (2^-50 for the sum of up to 1024 terms and the quotients)."""
+    x = normal(300, e, seed=e, size=3.0)
+    bias = normal(e, seed=1, size=0.1)
+    for more in ({"normalize": False}, {"normalize": False, "scale": 2.5}, {"normalize": True}):
+        for b in (None, bias):
+            experts, weights = nv.moe_select(x, k, "softmax", b, groups, top, **more)
+            want, w = expected(x, k, "softmax", b, groups, top, **more)
+            assert torch.equal(experts.cpu().long(), want)
+            assert ((weights.double().cpu() - w).abs() <= (HALF[torch.float32] + 2.0 ** -50) * w).all()
