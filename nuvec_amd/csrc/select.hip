@@ -123,6 +123,12 @@ __device__ __forceinline__ int select_wide(const SelectArgs &a, const float (&l)
 #pragma unroll
             for (int j = 0; j < V; j++) hi[j] = 0, lo[j] = 0;
     }
+    if (a.bias == nullptr && !by_logits)  // (groups by c, but their experts by the logits, whose order c's is as far as 64 bits hold it)
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const uint64_t b = (hi[j] | lo[j]) != 0 ? ordered((double)l[j]) : 0;
+            hi[j] = (uint32_t)(b >> 32), lo[j] = (uint32_t)b;
+        }
     int chosen = 0;
     for (int r = 0; r < a.k; r++) {
         uint32_t best = 0, w = 0;

@@ -67,3 +67,21 @@ def test_float32_weights_of_a_softmax_are_rounded_once(e, k, groups, top):
             want, w = expected(x, k, "softmax", b, groups, top, **more)
             assert torch.equal(experts.cpu().long(), want)
             assert ((weights.double().cpu() - w).abs() <= (HALF[torch.float32] + 2.0 ** -50) * w).all()
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_groups_by_two_without_a_bias_keep_the_order_of_the_logits(scores):
+    """Scores that 64 bits do not tell apart, near 1 or 0: the larger logit first all the same."""
+    g = torch.Generator().manual_seed(5)
+    for base in (40.0, -900.0):
+        x = base + torch.rand(20, 64, generator=g) * 8
+        x[:, ::8] = 0.0 if scores == "sigmoid" else 50.0  # (one of each group: groups are as good as each other, or alike)
+        x[:, 1::8] = 0.0 if scores == "sigmoid" else 50.0
+        x = x.cuda()
+        experts, _ = nv.moe_select(x, 40, scores, None, 8, 8, 2)
+        want = sorted_experts(x, 40)
+        assert torch.equal(experts.cpu().long(), want)
+
+
+def sorted_experts(x, k):
+    return torch.tensor([sorted(range(x.shape[1]), key=lambda i: (-row[i], i))[:k] for row in x.tolist()])
