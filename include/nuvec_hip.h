@@ -469,7 +469,7 @@ NVQ_API int32_t nvq_prompt_attention(const nvq_prompt_attention_desc *desc, cons
 
 /* out[r] = y[r] + scales[a] (x[r] . down[a]^T) . up[a]^T with a = ids[r] (i32 [rows]), rounded once; out[r] = y[r] where a is no adapter
  * (negative, or `adapters` and more).  scales f32 [adapters], NULL: ones.  out may be y itself.  `workspace`: the size query's bytes (float32
- * x . down^T), one call's at a time. */
+ * x . down^T), one call's at a time.  Without adapters x, down, up and the workspace may be NULL. */
 NVQ_API size_t nvq_apply_adapters_workspace_bytes(const nvq_adapters_desc *desc);
 NVQ_API int32_t nvq_apply_adapters(const nvq_adapters_desc *desc, const void *x, const void *down, const void *up, const float *scales,
                            const int32_t *ids, const void *y, void *out, void *workspace, void *stream);

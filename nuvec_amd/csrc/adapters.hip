@@ -436,15 +436,17 @@ Shape shape_of(const nvq_adapters_desc &d) {
     s.chunks = (int32_t)at_most(s.tiles * columns * s.up_slots / ((s.wide == 2 ? 2 : 4) * cus), 3);
     return s;
 }
-int32_t padded_rank(const nvq_adapters_desc &d) { return (d.rank + 15) / 16 * 16; }
+int32_t padded_rank(const nvq_adapters_desc &d) { return d.adapters == 0 ? 0 : (d.rank + 15) / 16 * 16; }
 
 template <typename T, int RW>
 int32_t run_sized(const AdapterArgs<T> &a, const Shape &shape, hipStream_t s) {
     const dim3 grid((unsigned)shape.tiles, (unsigned)shape.splits, (unsigned)shape.down_slots), block(64 * kDownWaves);
-    if (a.padded <= 16) hipLaunchKernelGGL((adapters_down_kernel<T, RW, 1>), grid, block, 0, s, a);
-    else if (a.padded <= 32) hipLaunchKernelGGL((adapters_down_kernel<T, RW, 2>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((adapters_down_kernel<T, RW, 4>), grid, block, 0, s, a);
-    NVQ_LAUNCH_CHECK("apply_adapters");
+    if (a.padded > 0) {  // (without adapters there are no shares, nor need there be an x)
+        if (a.padded <= 16) hipLaunchKernelGGL((adapters_down_kernel<T, RW, 1>), grid, block, 0, s, a);
+        else if (a.padded <= 32) hipLaunchKernelGGL((adapters_down_kernel<T, RW, 2>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((adapters_down_kernel<T, RW, 4>), grid, block, 0, s, a);
+        NVQ_LAUNCH_CHECK("apply_adapters");
+    }
     const int64_t columns = kBlockColumns * (int64_t)shape.chunks;
     const dim3 wide((unsigned)shape.tiles, (unsigned)((a.outputs + columns - 1) / columns), (unsigned)shape.up_slots);
     hipLaunchKernelGGL((adapters_up_kernel<T, RW>), wide, dim3(64 * kUpWaves), (size_t)RW * (a.padded / 16) * 64 * sizeof(uint4), s, a);
@@ -460,7 +462,7 @@ int32_t run_adapters(const nvq_adapters_desc &d, const void *x, const void *down
     a.x = (const T *)x, a.down = (const T *)down, a.up = (const T *)up, a.y = (const T *)y, a.scales = scales, a.ids = ids, a.out = (T *)out;
     a.low = (float *)workspace, a.rows = d.rows, a.inputs = d.inputs, a.outputs = d.outputs;
     a.x_stride = d.x_stride, a.y_stride = d.y_stride, a.out_stride = d.out_stride;
-    a.adapters = (int32_t)d.adapters, a.rank = d.rank, a.padded = padded_rank(d), a.splits = shape.splits, a.chunks = shape.chunks;
+    a.adapters = (int32_t)d.adapters, a.rank = d.adapters == 0 ? 0 : d.rank, a.padded = padded_rank(d), a.splits = shape.splits, a.chunks = shape.chunks;
     return shape.wide == 2 ? run_sized<T, 2>(a, shape, s) : run_sized<T, 1>(a, shape, s);
 }
 
