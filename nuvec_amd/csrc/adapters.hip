@@ -449,7 +449,13 @@ int32_t run_sized(const AdapterArgs<T> &a, const Shape &shape, hipStream_t s) {
     }
     const int64_t columns = kBlockColumns * (int64_t)shape.chunks;
     const dim3 wide((unsigned)shape.tiles, (unsigned)((a.outputs + columns - 1) / columns), (unsigned)shape.up_slots);
-    hipLaunchKernelGGL((adapters_up_kernel<T, RW>), wide, dim3(64 * kUpWaves), (size_t)RW * (a.padded / 16) * 64 * sizeof(uint4), s, a);
+    const size_t terms = (size_t)RW * (a.padded / 16) * 64 * sizeof(uint4), sums = 16 * RW * (kBlockColumns + 5) * sizeof(float);
+    static std::atomic<bool> configured = false;
+    if (terms + sums > 64 * 1024 && !configured) {  // (32 rows and ranks from 241 on)
+        NVQ_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(adapters_up_kernel<T, RW>), hipFuncAttributeMaxDynamicSharedMemorySize, RW * 16 * 1024));
+        configured = true;
+    }
+    hipLaunchKernelGGL((adapters_up_kernel<T, RW>), wide, dim3(64 * kUpWaves), terms, s, a);
     NVQ_LAUNCH_CHECK("apply_adapters");
     return NVQ_OK;
 }
