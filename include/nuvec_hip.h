@@ -438,7 +438,8 @@ NVQ_API int32_t nvq_append_paged(const nvq_paged_append_desc *desc, const int32_
                          uint32_t *k_w, void *k_s, void *k_b, uint32_t *v_w, void *v_s, void *v_b, void *stream);
 
 /* The same where the angles are not those of the places in the cache (images take fewer positions than tokens): rotary_positions i32
- * [axes->count, tokens].  A token with one of them outside the table writes no row of the cache. */
+ * [axes->count, tokens].  A token with one of them outside the table writes no row of the cache; with rotary_dims 0 that is all that they are
+ * for (keys and queries that have been rotated; table_rows 0: not that either). */
 NVQ_API int32_t nvq_append_paged_axes(const nvq_paged_append_desc *desc, const nvq_rotary_axes *axes, const int32_t *page_table,
                               const int32_t *sequences, const int32_t *positions, const int32_t *rotary_positions, const float *table,
                               const void *q, const void *q_weight, void *q_out, const void *k, const void *k_weight, const void *v,

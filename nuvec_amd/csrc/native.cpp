@@ -729,11 +729,11 @@ struct Angles {
     Tensor table;
     bool interleaved = false;
     nvq_rotary_axes axes{};  // count 0: none; else one more than the largest of the pairs'
-    int64_t pairs = 0;       // that have an axis
+    int64_t pairs = -1;      // that have an axis
     int32_t dims() const { return table.defined() ? (int32_t)(2 * table.size(1)) : 0; }
     int64_t rows() const { return table.defined() ? table.size(0) : 0; }
-    bool fits(const Place &at, int64_t dim) const {
-        return !table.defined() || (table.scalar_type() == at::kFloat && table.dim() == 3 && table.size(2) == 2 && table.size(0) > 0 && table.size(1) > 0 &&
+    bool fits(const Place &at, int64_t dim, int64_t least = 1) const {  // least: pairs
+        return !table.defined() || (table.scalar_type() == at::kFloat && table.dim() == 3 && table.size(2) == 2 && table.size(0) > 0 && table.size(1) >= least &&
                                     2 * table.size(1) <= dim && at.holds(table));
     }
 };
@@ -759,7 +759,7 @@ bool read_angles(PyObject *o, Angles &a) {
 // The axes for positions of `count` of them.
 bool axes_fit(const Angles &a, int64_t count, nvq_rotary_axes &axes) {
     axes = a.axes, axes.count = (int32_t)count;
-    return a.table.defined() && a.pairs > 0 && a.pairs == a.table.size(1) && count >= a.axes.count && count <= 4;
+    return a.table.defined() && a.pairs == a.table.size(1) && count >= a.axes.count && count <= 4;
 }
 
 bool weight_fits(const Tensor &w, const Place &at, at::ScalarType type, int64_t dim) {
@@ -920,7 +920,7 @@ PyObject *py_append_paged(PyObject *, PyObject *const *args, Py_ssize_t n) {
         const int64_t tokens = k.size(0), dim = k.size(2);
         if (!p.fits(at, type) || p.d.head_dim != dim || !is_rows(k, at, type, tokens, dim) || !is_rows(v, at, type, tokens, dim) ||
             k.size(1) != p.d.key_heads || v.size(1) != p.d.key_heads || !is_index(positions, at, tokens) ||
-            (sequences.defined() ? !is_index(sequences, at, tokens) : p.d.sequences != tokens) || !angles.fits(at, dim) ||
+            (sequences.defined() ? !is_index(sequences, at, tokens) : p.d.sequences != tokens) || !angles.fits(at, dim, 0) ||
             !weight_fits(k_weight, at, type, dim) || (q.defined() && (!is_rows(q, at, type, tokens, dim) || !weight_fits(q_weight, at, type, dim))))
             return none();
         nvq_paged_append_desc d{};

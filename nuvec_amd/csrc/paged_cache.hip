@@ -101,8 +101,10 @@ __global__ void __launch_bounds__(kHeadBlock) append_paged_kernel(const AppendAr
     int64_t row = row_of<T>(a.place, a.sequences, a.positions, token, a.key_heads, a.half > 0 && !Axes::kAny ? a.table_rows : INT64_MAX);
     Turn turn{};
     if constexpr (Axes::kAny) {
-        if (a.half > 0) {
+        if (a.half > 0 || a.table_rows > 0) {  // (a table of no pairs: its length counts all the same)
             if (!axes.inside(token, a.tokens, a.table_rows)) row = -1;
+        }
+        if (a.half > 0) {
             turn = axes.turn(a.table, a.table_rows, token, a.tokens, j0, a.half, interleaved);
         }
     } else if (a.half > 0) {

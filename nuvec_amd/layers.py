@@ -429,7 +429,10 @@ class PagedAttention:
             if self.rotation is not None or self.q_norm is not None or self.k_norm is not None:
                 at = positions[None] if rotary_positions is None else rotary_positions[None] if rotary_positions.ndim == 1 else rotary_positions[:, None]
                 q, k = (y[0].transpose(0, 1) for y in paged.head_norm_rope(q.transpose(0, 1)[None], k.transpose(0, 1)[None], self.q_norm, self.k_norm, self.rotation, at, self.eps))
-            paged.append_paged(cache, k, v, page_table, positions, sequences)
+            # (what has a position without angles is left out as otherwise: a rotation of no pairs, whose table is as long)
+            table = None if self.rotation is None else paged.Rotation(self.rotation.table[:, :0], axes=())
+            at = None if table is None else positions if rotary_positions is None else rotary_positions
+            paged.append_paged(cache, k, v, page_table, positions, sequences, table, rotary_positions=at)
             y = paged.prompt_attention(q, k, v, scale, query_starts, query_starts, self.sinks, True, self.window)
             return _adapted(self.o_proj, y.flatten(1), adapter_ids)
         q = paged.append_paged(cache, k, v, page_table, positions, sequences, self.rotation, self.k_norm, q, self.q_norm, self.eps, rotary_positions)

@@ -330,7 +330,7 @@ def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table
     stored, those of `quantize` to the unrounded ones.)
 
     `rotary_positions` int32 `[tokens]`, or `[axes, tokens]` with a rotation of several `axes`: the positions whose angles the heads are turned by, where they
-    are not the places in the cache (an image's tokens); outside the rotation's table they are like positions outside it."""
+    are not the places in the cache (an image's tokens); outside the rotation's table they are like positions outside it, also that of a rotation of no pairs."""
     done = (_lib._native or _lib.native()).append_paged(cache, k, v, page_table, positions, sequences, rotation, k_weight, q, q_weight, eps, rotary_positions)
     if done is not None:
         return None if done is True else done
