@@ -420,6 +420,8 @@ class PagedAttention:
             raise ops.InvalidArgument("paged_attention: sequences and query starts go together")
         if x.ndim != 2:
             raise ops.InvalidArgument(f"paged_attention: tokens must be [tokens, dims], got {list(x.shape)}")
+        if rotary_positions is not None and self.rotation is None:
+            raise ops.InvalidArgument("paged_attention: rotary positions without a rotation")
         q, k, v = (self._heads(_adapted(p, x, adapter_ids), n)
                    for p, n in ((self.q_proj, self.query_heads), (self.k_proj, self.key_heads), (self.v_proj, self.key_heads)))
         scale = q.shape[2] ** -0.5 if self.scale is None else self.scale
