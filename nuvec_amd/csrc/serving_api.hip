@@ -93,7 +93,7 @@ int32_t nvq_moe_select(const nvq_moe_select_desc *d, const void *logits, const f
     if (d->k < 1 || d->k > open) return fail(NVQ_INVALID_ARGUMENT, "%s: k must be in 1..=%d, got %d", op, open, d->k);
     if (d->experts > 1024 || d->k > 64 || d->groups > 64)
         return fail(NVQ_UNSUPPORTED, "%s: %d experts in %d groups, k = %d: up to 1024, 64 and 64", op, d->experts, d->groups, d->k);
-    if (d->rows >= 1LL << 26) return fail(NVQ_UNSUPPORTED, "%s: %lld rows (fewer than 2^26)", op, (long long)d->rows);
+    if (d->rows >= 1LL << 26 || !launchable((d->rows + 3) / 4, 256)) return fail(NVQ_UNSUPPORTED, "%s: %lld rows (2^26 - 4 at most)", op, (long long)d->rows);
     if (d->rows == 0) return NVQ_OK;
     if (logits == nullptr || indices == nullptr || weights == nullptr) return fail(NVQ_INVALID_ARGUMENT, "%s: null operand", op);
     for (const void *p : {logits, (const void *)weights}) NVQ_TRY(check_aligned(op, "an operand", p, (size_t)dtype_size(d->dtype)));
