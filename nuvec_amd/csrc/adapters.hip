@@ -12,7 +12,7 @@
 //
 // Both are bound by memory: the adapters' weights where there are few rows, x and y where there are many; a call of one row is two launches, 7.4 us.
 // Measured (bfloat16, us): 64 rows of 64 adapters of rank 16 beside [4096, 4096] 12.4 (kernels 5.6 and 7.8; the weights alone, 17 MB, at the rate of a large copy
-// 3.4); 4096 rows of four of rank 32 beside [14336, 4096] 88 (19 and 70; x, y and out, 268 MB, 55); float16, 517 rows of nine of rank 12 beside [2880, 2880] 14.5.
+// 3.4); 4096 rows of four of rank 32 beside [14336, 4096] 87 to 94 (19 and 70; x, y and out, 268 MB, 55); float16, 517 rows of nine of rank 12 beside [2880, 2880] 14.7.
 // A product's tile goes through LDS so that y and out are moved in runs of 512 bytes a row: 64 bytes a row and wavefront took 140 us in the second of these.
 #include "matrix.h"
 #include "nvq_internal.h"

@@ -39,8 +39,8 @@ int32_t launch_f32(const nvq_prompt_attention_desc &d, const PromptAttentionOper
 // The head sizes that kernels are made for: a head lies in the next of them, with zeros behind it.
 constexpr int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256; }
 
-// Blocks of a compute unit: three where the accumulators of 64 values leave room for them (8192 rows of 32 heads of 64 in bfloat16: 399 us with two,
-// 361 with three), two of heads up to 128, one behind that.
+// Blocks of a compute unit: three where the accumulators of 64 values leave room for them (8192 rows of 32 heads of 64 over 8: bfloat16 441 us
+// with two, 433 with three, float16 457 and 448), two of heads up to 128, one behind that.
 constexpr int blocks_of(int bytes, int padded) { return bytes == 2 && padded == 64 ? 3 : padded <= 128 ? 2 : 1; }
 
 }  // namespace prompt

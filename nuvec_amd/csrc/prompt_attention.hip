@@ -5,9 +5,9 @@ namespace nvq {
 
 namespace {
 
-// Tiles of 32 keys of an item at least, where a block's keys are shared.  (bfloat16, 32 heads of 128 over 8 key heads: 61 rows over 512 keys 15.5 us, with eight
-// tiles 19.2, not shared 19.2; 300 rows over 1000 keys 27.9, 27.0 with eight, 30.4 with sixteen; one row over 32768 keys 39 us, not shared 640.  A target
-// of twice the blocks that the chip holds: 15.5, 34.7 and 54.)
+// Tiles of 32 keys of an item at least, where a block's keys are shared.  (bfloat16, 32 heads of 128 over 8 key heads: 61 rows over 512 keys 16.4 us, with eight
+// tiles 18.8, not shared 18.9; 300 rows over 1000 keys 29.2, 28.8 with eight, 31.4 with sixteen; one row over 32768 keys 41 us, not shared 703.  In an
+// earlier form a target of twice the blocks that the chip holds took 1.0, 1.25 and 1.4 times as long.)
 constexpr int32_t kLeast = 4;
 
 // Blocks that the chip holds.

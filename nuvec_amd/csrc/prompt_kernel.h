@@ -18,21 +18,24 @@
 // walks its keys again: values that are not finite are zeros in the tile then, so that lines that do not see them stay clean, and the lines that do are given them
 // afterwards; and the weights are 2^-32 at most, so that sums of the largest finite values stay finite.
 //
-// The bound of long prompts in bfloat16 is the chip's power limit, as it is a large product's: 1.7 GHz of 2.4 at matrix cores busy for 52 % of the cycles (a form that took 29 %
-// more cycles ran at 2.06 GHz and took 7 % longer).  That of small heads is the instructions beside the products: 32 fused multiply-adds, exponentials
-// (eight cycles each, others five, and eight beside the other wavefront's products), additions, 16 maxima and conversions a lane for 64 keys of a line, in
-// float16 48 more for the weights' second terms.  Two wavefronts a SIMD take turns on the matrix cores (three of heads of 64 values); what is
+// The bound of long prompts of 128 values is the matrix cores at the clock that the chip's power leaves them: busy for 60 % of the cycles that a compute unit is,
+// vector instructions for as many, at 1.70 GHz (GRBM_GUI_ACTIVE over the time; launches that are short or wait more run at 2.05 and more).  That of small heads
+// is the instructions beside the products: 32 fused multiply-adds, exponentials (eight cycles each, others five, and eight beside the other wavefront's
+// products), additions, 16 maxima and conversions a lane for 64 keys of a line, and 48 more for the weights' second terms (64 in bfloat16, which has no
+// instruction that takes a pair's half off).  Two wavefronts a SIMD take turns on the matrix cores (three of heads of 64 values); what is
 // written between the products runs beside them: the next tile's way into LDS in those of the scores, the next keys' weights in those of the values.
 //
-// Measured (us; a large product of the types runs at 1235 and 1183 TFLOP/s): 8192 rows of 32 heads of 128 over 8 key heads in bfloat16 576 to 600, 916 to
-// 954 TFLOP/s; nine ragged prompts of up to 1500 rows in float16, 20 heads of 64, sinks and a window 67, 383 TFLOP/s; seven prompts of up to 61 rows 9.5,
-// a chain of first loads.  4096 rows of 16 heads over 4 (512 blocks, all on the chip at once): bfloat16 heads of 64 454 TFLOP/s, 128 669, 256 611;
-// float16 425, 573, 558; float32 112, 125, 71 (of 154).  One row over 32768 keys 39 us, 3.45 TB/s.
+// Measured (us; a large product of the types runs at 1235 and 1183 TFLOP/s; boxes differ by 3 to 5 %): 8192 rows of 32 heads of 128 over 8 key heads in bfloat16
+// 701 to 737, 746 to 784 TFLOP/s; nine ragged prompts of up to 1500 rows in float16, 20 heads of 64, sinks and a window 69 to 70, 370 TFLOP/s: vector
+// instructions for 61 % of a busy compute unit's cycles, and a fifth of the launch in which it is not busy (920 blocks on 768 places); seven prompts of up to 61
+// rows 9.5, a chain of first loads.  4096 rows of 16 heads over 4 (512 blocks, all on the chip at once): bfloat16 heads of 64 423 TFLOP/s, 128 557 to 585, 256 561;
+// float16 426, 560, 539; float32 110, 123, 67 (of 154).  One row over 32768 keys 39 to 41 us, 3.3 to 3.5 TB/s.
 //
-// Timed without its parts, the first of these: the tile's way into LDS 23 % (half of it the loads), the products of the values 15 %.  Tried and not kept: 64 lines a
-// wavefront at one a SIMD (690 us: one wavefront issues no more than an instruction in five cycles), blocks of eight wavefronts (3 % faster here, half
-// of the blocks empty in short prompts), tiles of 32 keys (652, at three wavefronts a SIMD 700 with spills), the branches of the rare cases in the loop
-// (714: their loads made every tile wait for its successor's).
+// Weights of one float16 term over values taken as float16 were 576 to 605 us in the first of these, and wrong where a row does not see the largest values
+// (paragraph on terms).  Timed without its parts in that form: the tile's way into LDS 23 % (half of it the loads), the products of the values 15 %.  Tried with it
+// and not kept: 64 lines a wavefront at one a SIMD (690 us: one wavefront issues no more than an instruction in five cycles), blocks of eight wavefronts (3 %
+// faster, half of the blocks empty in short prompts), tiles of 32 keys (652, at three wavefronts a SIMD 700 with spills), the branches of the rare cases in
+// the loop (714: their loads made every tile wait for its successor's).
 #pragma once
 
 #include <type_traits>
@@ -138,8 +141,8 @@ __device__ __forceinline__ Span span_of(const PromptBatch &a, const PagedItem &i
 
 // The item of a block.  Items come with the longest of a sequence first, a block on each compute unit in turn, and where they are all on the chip at once the unit
 // that has the longest would have the longest of the second turn too: the second turn goes back, eight at a time, so that a key head stays with its XCD.
-// (4096 rows of 16 heads over 4: float32, 128 values 742 -> 549 us, bfloat16 104.3 -> 100.6, float16, 64 values 83.0 -> 76.9; where more blocks follow, which
-// go where one has ended, it is of no use: 3000 rows of 32 heads over 8 93.2 and 94.1.)
+// (4096 rows of 16 heads over 4: float32, 128 values 754 -> 556 us, bfloat16 130 -> 123, float16, 64 values 87.0 -> 80.5; where more blocks follow, which
+// go where one has ended, it is of no use: 3000 rows of 32 heads over 8 114.4 and 114.5.)
 __device__ __forceinline__ int32_t turned(uint32_t block, int32_t turn, int32_t back) {
     const int32_t r = (int32_t)block - turn;
     return r >= 0 && r < back ? turn + back - 8 - (r & ~7) + (r & 7) : (int32_t)block;

@@ -12,9 +12,9 @@
 // score a few exchanges among its lanes.  Values are compared as whole numbers of the same order, 0 for what is not to be chosen, whose low bits are their
 // places: a round is one maximum over the wavefront, by data-parallel moves, and knows whose it is.
 //
-// Bound by the vector unit's instructions, 425 a row of 256 experts; memory would allow 1.9 us for the first of these.  Measured (us): 16384 rows of
+// Bound by the vector unit's instructions, 427 a row of 256 experts; memory would allow 1.9 us for the first of these.  Measured (us): 16384 rows of
 // 256 in eight groups, bfloat16, sigmoid, a bias 16.5 (all of it in 64 bits 35; ballots for a maximum's place, and weights of 64 bits 19.6; every lane's
-// values sorted beforehand 21.5); 1333 rows of 60 in float16 4.9 and eight rows of 256 4.6, a launch.
+// values sorted beforehand 21.5); 1333 rows of 60 in float16 5.0 and eight rows of 256 4.6 to 5.4, a launch.
 #include <type_traits>
 
 #include "heads.h"

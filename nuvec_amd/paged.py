@@ -464,7 +464,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     `k` and `v` `[keys, key_heads, dim]`, heads of a multiple of 8 values up to 256, any strides with consecutive values of a head.
 
     Sequence b has the rows `query_starts[b]` to `query_starts[b + 1] - 1` and the keys `key_starts[b]` to `key_starts[b + 1] - 1` (int32 `[sequences + 1]`,
-    ascending, on the device).  `query_starts` None: one sequence; `key_starts` None: the rows' own keys, or all keys of one sequence.  With `causal` row i of n
+    ascending, on the device).  `query_starts` None: one sequence; `key_starts` None: of several sequences the rows' own keys, of one all keys.  With `causal` row i of n
     sees the keys up to number keys - n + i of its sequence, with `window` the last `window` of those alone.  `sinks` `[query_heads]` join each head's softmax.
     Rows that see nothing are zeros; rows of no sequence are left as they were in `out` (and undefined in a new result).  Keys and values that a row does
     not see may hold anything.
