@@ -410,19 +410,23 @@ __global__ void __launch_bounds__(64 * kWaves, blocks_of((int)sizeof(T), D)) pro
         for (int i = 1; i < 16 * TB; i++) top = fmaxf(top, x[i >> 4][i & 15]);
         top *= scale;
         // Rescaled only when a maximum has grown by more than 2^8: until then the weights are at most 2^8 (with care 2^8 less the lift).
-        // float16: weights of a tile have to lie high in its range, 2^-24 to 2^16, to keep their bits however many small ones there are.  `m` is 11 below the tile's
+        // float16: weights of a tile have to lie high in its range, 2^-24 to 2^16, to keep their bits however many small ones there are.  `m` is 7 below the tile's
         // maximum then, rises where a weight would leave 2^15, and falls where the tile's largest would be below 2^-4 (not for a score that is masked, and only as
-        // far as the sums, which grow by that much, stay below 2^60).
+        // far as the sums, which grow by that much, stay below 2^60).  Scores that are multiples of 16 and more have weights of at most 1 so: 7 is rounded to 0, and
+        // differences are exact where sums are not.
         constexpr bool kFalls = Elem<T>::code == NVQ_F16;
-        constexpr float kBelow = kFalls ? 11.0f : decltype(careful)::value ? -kLift : 0.0f, kMost = kFalls ? 15.0f : 8.0f + kBelow;
-        bool moves = top > m + kMost;
-        if constexpr (kFalls) moves |= top < m - 4.0f && top > kLowest;
+        constexpr float kBelow = kFalls ? 7.0f : decltype(careful)::value ? -kLift : 0.0f, kMost = kFalls ? 15.0f : 8.0f + kBelow;
+        auto leaves = [&]() __attribute__((always_inline)) {
+            const float above = top - m;
+            return above > kMost || (kFalls && above < -4.0f && top > kLowest);
+        };
+        const bool moves = leaves();
         if (__builtin_expect(__any(moves), 0)) {
             top = fmaxf(top, __shfl_xor(top, 32));
             float m_new = fmaxf(m, top - kBelow);
             if constexpr (kFalls) {
                 const float sum = l + __shfl_xor(l, 32), least = sum > 0.0f ? m + __builtin_amdgcn_logf(sum) - 60.0f : kLowest;  // (the same in both halves)
-                m_new = top > m + kMost || (top < m - 4.0f && top > kLowest) ? fmaxf(top - kBelow, least) : m;
+                m_new = leaves() ? fmaxf(top - kBelow, least) : m;
             }
             const float f = exp2f(m - m_new);
             m = m_new, l *= f;

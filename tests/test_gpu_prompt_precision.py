@@ -180,3 +180,24 @@ def test_weights_that_rise_and_fall(dtype, rows, heads, window):
         got = nv.prompt_attention(q, k.expand(-1, heads, -1), v.expand(-1, heads, -1), 1.0, sinks=s, window=window)
         want, bound = expected(q, k, v, 1.0, s, window=window)
         within(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("power", [20, 24, 25, 26, 27, 28, 30])
+def test_scores_far_from_zero(dtype, power):
+    """Scores that are multiples of a step of float32 near 2^power: no sum with a maximum may round a weight out of its type's range."""
+    step, heads, dim = 2.0 ** (power - 23), 4, 64
+    for length, rows in ((40, 1), (300, 1), (5000, 1), (300, 90)):
+        place = torch.randperm(length, generator=torch.Generator().manual_seed(power + length)).to("cuda").double()
+        q, k = torch.zeros(rows, heads, dim, device="cuda"), torch.zeros(length, 1, dim, device="cuda")
+        _, _, v = make(1, length, 1, 1, dim, dtype)
+        # score = 2^power + step x place, in parts that every type holds; log2 e times this scale is 1 in float32, so that scores and their distances are exact
+        q[..., 0], k[..., 0], q[..., 1:4] = 2.0 ** (power // 2), 2.0 ** (power - power // 2), step
+        k[:, 0, 1], k[:, 0, 2], k[:, 0, 3] = place % 64, place // 64 % 64 * 64, place // 4096 * 4096
+        assert all(torch.equal(t, t.to(dtype).float()) for t in (q, k))
+        got = nv.prompt_attention(q.to(dtype), k.to(dtype), v, 0.6931471805599453, causal=False).double()
+        p = torch.exp2(step * (place - place.max()))
+        p, values = p / p.sum(), v[:, 0].double()
+        y, size = p @ values, p @ values.abs()
+        bound = (TERM[dtype] + 2.0 ** -20) * size + (2.0 ** -20 + HALF[dtype]) * y.abs() + TINY[dtype]
+        assert got.isfinite().all() and ((got - y).abs() <= bound).all(), (length, rows, ((got - y).abs() / bound).max().item())
