@@ -267,8 +267,8 @@ __global__ void __launch_bounds__(64 * kSelectWaves) moe_select_kernel(const Sel
         int before = 0;  // groups that come first
         for (int g0 = 0; g0 < a.groups; g0 += 4)
 #pragma unroll
-            for (int g = g0; g < g0 + 4; g++) {  // (those behind the last are 0)
-                const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)mine, g << a.lanes_shift);
+            for (int g = g0; g < g0 + 4; g++) {  // (of two groups those behind the last would be lanes 64 and 96)
+                const uint32_t other = g < a.groups ? (uint32_t)__builtin_amdgcn_readlane((int)mine, g << a.lanes_shift) : 0u;
                 before += other + (g < place.group ? 1u : 0u) > mine ? 1 : 0;  // (no key is the largest number)
             }
         const bool kept = before < a.top_groups;

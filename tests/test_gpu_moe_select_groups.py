@@ -85,3 +85,16 @@ def test_groups_by_two_without_a_bias_keep_the_order_of_the_logits(scores):
 
 def sorted_experts(x, k):
     return torch.tensor([sorted(range(x.shape[1]), key=lambda i: (-row[i], i))[:k] for row in x.tolist()])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("groups", [2, 3, 4, 5, 6, 7, 8, 9, 13, 16, 17, 31, 32, 33, 47, 61, 64])
+def test_every_number_of_groups_that_stay(dtype, groups):
+    for each in (1, 2, 5):
+        for top in sorted({1, 2, groups // 2, groups - 1, groups}):
+            x, bias = normal(20, groups * each, dtype=dtype, seed=top, size=10.0), normal(groups * each, seed=each, size=0.3)
+            k = min(64, top * each)
+            for scores in ("softmax", "sigmoid"):
+                check(x, k, scores, None, groups, top, normalize=False)
+                check(x, k, scores, bias, groups, top)
+                check(x, 1, scores, bias, groups, top, 1)
