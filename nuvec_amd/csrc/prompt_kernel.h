@@ -21,7 +21,7 @@
 // The bound of long prompts of 128 values is the matrix cores at the clock that the chip's power leaves them: busy for 60 % of the cycles that a compute unit is,
 // vector instructions for as many, at 1.70 GHz (GRBM_GUI_ACTIVE over the time; launches that are short or wait more run at 2.05 and more).  That of small heads
 // is the instructions beside the products: 32 fused multiply-adds, exponentials (eight cycles each, others five, and eight beside the other wavefront's
-// products), additions, 16 maxima and conversions a lane for 64 keys of a line, and 48 more for the weights' second terms (64 in bfloat16, which has no
+// products), additions, 16 maxima and conversions a lane for 64 keys of a line, and 48 more for the weights' second terms (80 in bfloat16, which has no
 // instruction that takes a pair's half off).  Two wavefronts a SIMD take turns on the matrix cores (three of heads of 64 values); what is
 // written between the products runs beside them: the next tile's way into LDS in those of the scores, the next keys' weights in those of the values.
 //
