@@ -45,3 +45,33 @@ def test_positions_outside_the_table_write_nothing(dtype, native, monkeypatch):
         assert all(torch.equal(f, o) for f, o in zip(fresh, other))
         missing = {None: 11, 1: 4, 2: 4}[None if rotary is None else rotary.ndim] if layer is not bare else 1
         assert fresh[0].sum().item() == (60 - missing) * KEY_HEADS
+
+
+def test_captured_fresh_sequences_follow_their_inputs():
+    """One graph of a batch with padding behind its sequences, replayed with other starts and positions, against the eager layer on a second pool."""
+    torch.manual_seed(5)
+    a, _ = block(torch.bfloat16)
+    caches = [nv.PagedCache.new(16, KEY_HEADS, 16, DIM) for _ in range(2)]
+    page_table = torch.randperm(16, device="cuda").to(torch.int32).reshape(2, 8)
+    x = torch.randn(70, DIMS, device="cuda").bfloat16()
+    positions, sequences, starts = ints([-1] * 70), ints([0] * 70), ints([0, 0, 0])
+    rotary, ids, lengths = torch.zeros(3, 70, dtype=torch.int32, device="cuda"), ints([-1] * 70), ints([0, 0])
+    run = lambda cache: a(x, cache, page_table, positions, lengths, sequences, starts, 70, rotary, ids, True)
+    run(caches[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = run(caches[0])
+    for rows in ([40, 20], [1, 69], [0, 33], [70, 0], [5, 5]):
+        n = sum(rows)
+        x.normal_()
+        positions.copy_(ints([*range(rows[0]), *range(rows[1]), *[-1] * (70 - n)]))
+        sequences.copy_(ints([0] * rows[0] + [1] * (70 - rows[0])))
+        starts.copy_(ints([0, rows[0], n]))
+        rotary.copy_(torch.randint(0, 140, (3, 70)).to(torch.int32))  # (some outside the table of 128)
+        ids.copy_((torch.arange(70) % 4 - 1).to(torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = run(caches[1])
+        assert torch.equal(y[:n], want[:n])
+        for one, other in zip((caches[0].keys, caches[0].values), (caches[1].keys, caches[1].values)):
+            assert torch.equal(one.weight.view(torch.int32), other.weight.view(torch.int32)) and torch.equal(one.scales, other.scales)
